@@ -1075,7 +1075,7 @@ std::string resultKind(const Func &f, bool *hasMatmul, bool *hasRWI, bool *hasRe
   *hasMatmul = *hasRWI = *hasReduce = false;
   for (const Op *op : f.ops) {
     if (op->name == "linalg.matmul" || op->name == "linalg.matmul_transpose_b" || op->name == "hivm.hir.matmul" ||
-        op->name == "hfusion.matmul_mx")
+        op->name == "hfusion.matmul_mx" || op->name == "hfusion.linear_mx")
       *hasMatmul = true;
     if (op->name == "hfusion.reduce_with_index") *hasRWI = true;
     if (op->name == "linalg.reduce") *hasReduce = true;
@@ -2475,6 +2475,11 @@ constexpr int MK_BF16_CODE = 1; // hf::MK_BF16
 // (256x128) against 46.1 (128x128 and 256x256); M = 5000 103 (256x256) against
 // 125 (128x128).  bf16, M = 5000, N = 1024, K = 4096: 60 (256x128) against 65
 // (256x256) and 93 (128x64).
+int mxFormatOf(const Op *op, const char *attr);
+void checkCodes(const Op *op, const Value *v, int fmt, std::vector<int64_t> shape, size_t axis);
+void checkScales(const Op *op, const Value *v, const std::vector<int64_t> &shape);
+const char *mxFormatName(int fmt);
+
 struct TileTime {
   double fixed, queued, one, second, more, part1, part, tall;
 };
@@ -2555,15 +2560,33 @@ ContractionTile pickTile(int64_t M, int64_t N, int64_t Kb, bool bT, int mk) {
   return *best;
 }
 
+// linear_mx of few rows: rows up to `top` take 16 mt x 16 nt tiles whose nw
+// waves split K
+struct WxTile {
+  int64_t top;
+  int mt, nt, nw;
+  int64_t blocksPerRow(int64_t N) const { return (N + 16 * nt - 1) / (16 * nt); }
+};
+const WxTile kWxTiles[] = {{16, 1, 1, 8}, {32, 2, 1, 8}, {64, 4, 1, 8}};
+constexpr int64_t kWxRows = 64;
+const WxTile &wxTile(int64_t M) {
+  for (const WxTile &t : kWxTiles)
+    if (M <= t.top) return t;
+  throw CompileError("internal: linear_mx tile");
+}
+
 KernelPlan lowerMatmul(Analysis &A, const std::string &kname, const LowerOptions &opt) {
   Func &f = *A.f;
   const Op *mm = findOp(f, [](const Op *o) {
     return o->name == "linalg.matmul" || o->name == "linalg.matmul_transpose_b" || o->name == "hivm.hir.matmul" ||
-           o->name == "hfusion.matmul_mx";
+           o->name == "hfusion.matmul_mx" || o->name == "hfusion.linear_mx";
   });
   const bool hivm = mm->name == "hivm.hir.matmul";
   const bool mx = mm->name == "hfusion.matmul_mx";
-  const bool bT = hivm ? mm->attrs.count("b_transpose") != 0 : mm->name == "linalg.matmul_transpose_b";
+  // linear_mx: A [M, K] bf16, W [N, K] fp8 codes or [N, K/2] bytes of two e2m1
+  // codes, scales [N, K/32] e8m0
+  const bool wx = mm->name == "hfusion.linear_mx";
+  const bool bT = hivm ? mm->attrs.count("b_transpose") != 0 : wx || mm->name == "linalg.matmul_transpose_b";
   const bool aT = hivm && mm->attrs.count("a_transpose") != 0;
   // matmul_mx (HFusionOps.td:1233-1291): A [M, K], B [K, N] fp8 (or bytes
   // reinterpreted by hfusion.bitcast or by lhsFormat / rhsFormat), scales
@@ -2583,9 +2606,9 @@ KernelPlan lowerMatmul(Analysis &A, const std::string &kname, const LowerOptions
   if (a->type.shape.size() != 2 || b->type.shape.size() != 2) unsupported(mm, "matmul operands must be rank 2");
   int64_t M = aT ? a->type.shape[1] : a->type.shape[0], K = aT ? a->type.shape[0] : a->type.shape[1];
   int64_t N = bT ? b->type.shape[0] : b->type.shape[1];
-  if ((bT ? b->type.shape[1] : b->type.shape[0]) != K) unsupported(mm, "matmul shapes");
+  if (!wx && (bT ? b->type.shape[1] : b->type.shape[0]) != K) unsupported(mm, "matmul shapes");
   Elem ae = a->type.elem, be = b->type.elem;
-  int mk = -1;
+  int mk = -1, wfmt = -1;
   bool fp4 = false;
   int64_t Kl = K; // logical K (fp4 packs two values per byte)
   const Value *sa = nullptr, *sb = nullptr;
@@ -2632,12 +2655,24 @@ KernelPlan lowerMatmul(Analysis &A, const std::string &kname, const LowerOptions
     if (N % 16 != 0) unsupported(mm, "matmul_mx N must be a multiple of 16");
     if (mm->results[0]->type.elem != Elem::F32) unsupported(mm, "matmul_mx accumulates in f32");
     ae = be = Elem::I8; // bytes from here on
+  } else if (wx) {
+    if (mm->ins.size() != 3) unsupported(mm, "linear_mx takes A, W and its scales");
+    sb = mm->ins[2];
+    if (sb->argIdx < 0) unsupported(mm, "linear_mx scales must be a group argument");
+    wfmt = mxFormatOf(mm, "rhsFormat");
+    if (wfmt < 0) unsupported(mm, "linear_mx without rhsFormat");
+    if (ae != Elem::BF16) unsupported(mm, "linear_mx rows of another type than bf16");
+    if (M < 0 || N < 1 || K < 32 || K % 32 != 0) unsupported(mm, "linear_mx K must be a multiple of 32 (N at least 1)");
+    checkCodes(mm, b, wfmt, {N, K}, 1);
+    checkScales(mm, sb, {N, K / 32});
+    if (mm->results[0]->type.elem != Elem::F32) unsupported(mm, "linear_mx accumulates in f32");
+    mk = 1;
   } else if (ae == Elem::I8 && be == Elem::I8) mk = 0;
   else if (ae == Elem::BF16 && be == Elem::BF16) mk = 1;
   else if (ae == Elem::F16 && be == Elem::F16) mk = 2;
   if (mk < 0) unsupported(mm, "matmul element types (supported: i8 x i8, bf16 x bf16, f16 x f16, matmul_mx fp8 / fp4)");
   const bool i8 = mk == 0;
-  if (!hivm && !mx) {
+  if (!hivm && !mx && !wx) {
     Elem ce = mm->results[0]->type.elem;
     if (ce != (i8 ? Elem::I32 : Elem::F32)) unsupported(mm, "matmul accumulator type (i32 for i8, f32 for bf16/f16)");
   }
@@ -2668,6 +2703,7 @@ KernelPlan lowerMatmul(Analysis &A, const std::string &kname, const LowerOptions
   // smaller tiles where 256x256 ones would leave CUs idle (these take any K
   // spanning a multiple of 64 bytes, and a B [K, N] as it is)
   const bool tiles = !aT && dma0 != 0 && kmajOk && offs32 && !(mx && opt.mxExact);
+  if (wx && !tiles) unsupported(mm, "linear_mx with K above 2^23");
   // (a runtime row count: the tile for the largest; the others below)
   const ContractionTile tile = tiles ? pickTile(M, N, K * esz, bT, mk) : kRing256;
   const bool ring = tile.kind == 'r';
@@ -2692,14 +2728,14 @@ KernelPlan lowerMatmul(Analysis &A, const std::string &kname, const LowerOptions
   // matmul_mx accumulates onto its `outs`: a tensor.empty (taken as zero) or
   // a constant fill, added after the contraction
   std::string accInit;
-  if (mx) {
+  if (mx || wx) {
     const Value *acc0 = mm->outs.empty() ? nullptr : mm->outs[0];
-    if (!acc0 || !acc0->def) unsupported(mm, "matmul_mx accumulator must be a tensor.empty or a constant linalg.fill");
+    if (!acc0 || !acc0->def) unsupported(mm, "block-scaled accumulator must be a tensor.empty or a constant linalg.fill");
     if (acc0->def->name == "linalg.fill") {
-      if (!acc0->def->ins[0]->isConst) unsupported(mm, "matmul_mx accumulator fill must be a constant");
+      if (!acc0->def->ins[0]->isConst) unsupported(mm, "block-scaled accumulator fill must be a constant");
       if (acc0->def->ins[0]->fconst != 0.0) accInit = constExpr(acc0->def->ins[0], Elem::F32);
     } else if (acc0->def->name != "tensor.empty") {
-      unsupported(mm, "matmul_mx accumulator must be a tensor.empty or a constant linalg.fill");
+      unsupported(mm, "block-scaled accumulator must be a tensor.empty or a constant linalg.fill");
     }
   } else if (!hivm) {
     const Value *acc0 = mm->outs[0];
@@ -2711,6 +2747,7 @@ KernelPlan lowerMatmul(Analysis &A, const std::string &kname, const LowerOptions
   // epilogue over D = [M, N] with the matmul result as the accumulator
   std::set<const Value *> excl = {a, b};
   if (mx) excl.insert({sa, sb, mm->ins[0], mm->ins[1]});
+  if (wx) excl.insert(sb);
   A.D = {M, N};
   if (!hivm) inferMaps(A, excl);
   // per-element code, plus the operand loads split by their index: [m] once
@@ -2780,6 +2817,8 @@ KernelPlan lowerMatmul(Analysis &A, const std::string &kname, const LowerOptions
   if (f.returns.size() != 1) unsupported(mm, "matmul groups must return exactly one tensor");
   const Value *outv = f.returns[0];
   if (outv->type.shape != std::vector<int64_t>{M, N}) unsupported(mm, "matmul group result shape");
+  if (wx && A.resultTied[0] >= 0 && A.params[A.resultTied[0]].shape != outv->type.shape)
+    unsupported(mm, "linear_mx destination of another shape than its result");
   if (hivm) name[outv] = hivmOut;
   else ensure(outv);
   Elem oe = outv->type.elem;
@@ -2787,7 +2826,10 @@ KernelPlan lowerMatmul(Analysis &A, const std::string &kname, const LowerOptions
   p.kernelName = kname;
   p.kind = "SINGLE_CUBE";
   std::ostringstream k;
-  std::string params = kernelParamList(A, p.kargs, preA || preB || mxExact);
+  // linear_mx: up to kWxRows rows straight from the codes (hf_mmwx.h), more
+  // through the weight as bf16 in the workspace and the bf16 contraction
+  const bool wxPre = wx && (A.rowsDyn || M > kWxRows);
+  std::string params = kernelParamList(A, p.kargs, preA || preB || mxExact || wxPre);
   // epilogue functor receives all kernel pointer arguments
   k << "namespace {\nstruct " << kname << "_args {";
   for (size_t i = 0; i < A.params.size(); ++i)
@@ -2815,7 +2857,7 @@ KernelPlan lowerMatmul(Analysis &A, const std::string &kname, const LowerOptions
   };
   const std::string et = i8 ? "int8_t" : "uint16_t";
   const std::string aPtr = preA ? "(const " + et + "*)((char*)ws + " + std::to_string(wsB) + ")" : "(const " + et + "*)p" + std::to_string(a->argIdx);
-  const std::string bPtr = preB ? "(const " + et + "*)ws" : "(const " + et + "*)p" + std::to_string(b->argIdx);
+  const std::string bPtr = preB || wxPre ? "(const " + et + "*)ws" : "(const " + et + "*)p" + std::to_string(b->argIdx);
   auto tileCall = [&](const ContractionTile &t) {
     const std::string tt = mx ? "uint8_t" : et;
     k << "  hf::" << (mx ? "mmad_mx<" : t.kind == 's' ? "mmad_skinny<" : "mmad_tile<") << mk << ", " << kname << "_epi, "
@@ -2825,7 +2867,9 @@ KernelPlan lowerMatmul(Analysis &A, const std::string &kname, const LowerOptions
       k << t.tm << ", " << t.tn << ", " << t.a << ", " << t.b << ", " << t.s;
       if (!mx) k << ", " << t.kg;
     }
-    k << ">((const " << tt << "*)p" << a->argIdx << ", (const " << tt << "*)p" << b->argIdx;
+    k << ">((const " << tt << "*)p" << a->argIdx << ", ";
+    if (wx) k << bPtr;
+    else k << "(const " << tt << "*)p" << b->argIdx;
     if (mx) k << ", (const uint8_t*)p" << sa->argIdx << ", (const uint8_t*)p" << sb->argIdx;
     k << ", (" << mtype(oe) << "*)" << resultPtr(A, 0) << ", " << Mx << ", " << N << "ll, " << K << "ll, P);\n}\n";
   };
@@ -2836,9 +2880,44 @@ KernelPlan lowerMatmul(Analysis &A, const std::string &kname, const LowerOptions
         << ", (const uint8_t*)p" << sa->argIdx << ", (const uint8_t*)p" << sb->argIdx;
     else
       k << "  hf::mmad<" << mk << ", " << kname << "_epi, false, " << (bT ? "true, 3" : "false, 4") << ">((const " << et << "*)p"
-        << a->argIdx << ", (const " << et << "*)p" << b->argIdx;
+        << a->argIdx << ", " << bPtr;
     k << ", (" << mtype(oe) << "*)" << resultPtr(A, 0) << ", " << Mx << ", " << N << "ll, " << K << "ll, P);\n}\n";
   };
+  // linear_mx of few rows
+  auto wxCall = [&](const WxTile &t) {
+    k << "  hf::linear_wx<" << wfmt << ", " << kname << "_epi, " << t.mt << ", " << t.nt << ", " << t.nw << ", " << K << "ll>((const uint16_t*)p"
+      << a->argIdx << ", (const uint8_t*)p" << b->argIdx << ", (const uint8_t*)p" << sb->argIdx << ", (" << mtype(oe) << "*)"
+      << resultPtr(A, 0) << ", " << Mx << ", " << N << "ll, P);\n}\n";
+  };
+  if (wx && A.rowsDyn)
+    for (const WxTile &t : kWxTiles) {
+      const std::string nm = altName(kname, "wx" + std::to_string(t.top));
+      kernelHead(nm, 64 * t.nw);
+      wxCall(t);
+      p.alts.push_back({nm, t.top, 16 * t.mt, t.blocksPerRow(N), (unsigned)(64 * t.nw)});
+    }
+  if (wx) {
+    p.algoOps = 2.0 * (double)M * (double)N * (double)K;
+    if (!wxPre) {
+      const WxTile &t = wxTile(M);
+      kernelHead(kname, 64 * t.nw);
+      wxCall(t);
+      p.source = k.str();
+      p.grid[0] = (unsigned)std::max<int64_t>(1, (M + 16 * t.mt - 1) / (16 * t.mt) * t.blocksPerRow(N));
+      p.block[0] = (unsigned)(64 * t.nw);
+      p.variant = std::string("bf16 rows x ") + mxFormatName(wfmt) + " weight, K split over " + std::to_string(t.nw) + " waves";
+      return p;
+    }
+    KernelPlan::PreKernel pk;
+    pk.name = kname + "_weight";
+    pk.grid = (unsigned)std::min<int64_t>((N * K / 8 + 255) / 256, 65536);
+    pk.block = 256;
+    pk.kargs = {"param:" + std::to_string(b->argIdx), "param:" + std::to_string(sb->argIdx), "ws"};
+    k << "extern \"C\" __global__ __launch_bounds__(256) void " << pk.name
+      << "(const void* __restrict__ w, const void* __restrict__ s, void* __restrict__ ws) {\n"
+      << "  hf::mx_dequantize_rows<hf::EL_BF16, " << wfmt << ", " << K << "ll>(w, s, ws, " << N << "ll);\n}\n";
+    p.pre.push_back(pk);
+  }
   // a runtime row count: the tile that each count would be given, up to the
   // last that differs from the main kernel's
   if (A.rowsDyn && tiles) {
@@ -2853,6 +2932,7 @@ KernelPlan lowerMatmul(Analysis &A, const std::string &kname, const LowerOptions
     if (seq.back() == tile) seq.pop_back();
     for (size_t i = 0; i < seq.size(); ++i) {
       const ContractionTile &t = seq[i];
+      if (wx && top[i] <= kWxRows) continue;
       const bool main = ring && t == tile;
       const std::string nm = main ? kname : altName(kname, std::to_string(t.tm) + "x" + std::to_string(t.tn) + (t.kg > 1 ? "k" + std::to_string(t.kg) : ""));
       if (!main && std::find(emitted.begin(), emitted.end(), t) == emitted.end()) {
@@ -2861,7 +2941,7 @@ KernelPlan lowerMatmul(Analysis &A, const std::string &kname, const LowerOptions
         if (t.kind == 'r') ringCall();
         else tileCall(t);
       }
-      p.alts.push_back({nm, top[i], t.tm, t.blocksPerRow(N), (unsigned)t.threads()});
+      p.alts.push_back({nm, top[i], t.tm, t.blocksPerRow(N), (unsigned)t.threads(), wx});
     }
   }
   kernelHead(kname, threads);
@@ -2890,7 +2970,7 @@ KernelPlan lowerMatmul(Analysis &A, const std::string &kname, const LowerOptions
   };
   if (preB) preKernel("_relayout_b", b, N, 0);
   if (preA) preKernel("_relayout_a", a, M, wsB);
-  p.workspaceBytes = wsB + wsA;
+  p.workspaceBytes = wsB + wsA + (wx ? align256((uint64_t)(N * K * 2)) : 0);
   if (mxExact) {
     auto mxPre = [&](const char *suffix, const Value *src, const Value *scl, int fmt, bool rowScale, int64_t R, int64_t Cc,
                      uint64_t off) {
@@ -2920,10 +3000,11 @@ KernelPlan lowerMatmul(Analysis &A, const std::string &kname, const LowerOptions
     p.rowsC = tile.blocksPerRow(N);
   }
   p.block[0] = (unsigned)threads;
-  static const char *mxName[5] = {"e4m3 x e4m3", "e4m3 x e5m2", "e5m2 x e4m3", "e5m2 x e5m2", "e2m1 x e2m1, fp4 two per byte"};
+  const char *mxName[5] = {"e4m3 x e4m3", "e4m3 x e5m2", "e5m2 x e4m3", "e5m2 x e5m2", "e2m1 x e2m1, fp4 two per byte"};
   p.variant = std::string(mxExact ? std::string("exact matmul_mx: ") + mxName[mk - 3] +
                                          " with e8m0 scales per 32 k, scaled into bf16 by pre kernels, mfma_f32_32x32x16_bf16"
                           : mx ? std::string("mfma_scale_f32_32x32x64_f8f6f4 (") + mxName[mk - 3] + ", e8m0 scales per 32 k)"
+                          : wx ? std::string("bf16 rows x ") + mxFormatName(wfmt) + " weight as bf16 in the workspace, mfma_f32_32x32x16_bf16"
                           : mk == 0 ? "mfma_i32_32x32x32_i8" : mk == 1 ? "mfma_f32_32x32x16_bf16" : "mfma_f32_32x32x16_f16") +
               (aT ? ", A [K,M]" : "") + (bT ? ", B [N,K]" : ", B [K,N]") +
               (preA || preB ? " (re-laid K-contiguous by a transpose kernel)" : "") +
@@ -2943,7 +3024,8 @@ KernelPlan lowerMatmul(Analysis &A, const std::string &kname, const LowerOptions
 bool isSingleOpKernel(const std::string &n) {
   return n == "hfusion.cumsum" || n == "hfusion.cumprod" || n == "hfusion.cummax" || n == "hfusion.cummin" ||
          n == "hfusion.histogram" || n == "hfusion.deinterleave" || n == "hfusion.interleave" || n == "hfusion.flip" ||
-         n == "hfusion.mulext" || n == "hfusion.mulextui" || n == "hfusion.arange" || n == "hfusion.gather" || n == "hfusion.sort";
+         n == "hfusion.mulext" || n == "hfusion.mulextui" || n == "hfusion.arange" || n == "hfusion.gather" || n == "hfusion.sort" ||
+         n == "hfusion.quantize_mx" || n == "hfusion.dequantize_mx" || n == "hfusion.layer_norm" || n == "hfusion.layer_norm_grad";
 }
 
 static std::vector<int64_t> intList(const std::string &s) {
@@ -2954,10 +3036,286 @@ static std::vector<int64_t> intList(const std::string &s) {
   return v;
 }
 
+// ---- block-scaled codes and layer norm (hf_mx.h, hf_ln.h): ops of this
+// backend, with no counterpart in the reference's dialect
+
+namespace {
+// The matrix core's number of a `format` / `rhsFormat` attribute (1 e5m2,
+// 2 e4m3, 3 e2m1, as matmul_mx's lhsFormat), -1 without one.
+int mxFormatOf(const Op *op, const char *attr) {
+  auto it = op->attrs.find(attr);
+  if (it == op->attrs.end()) return -1;
+  int code = 0;
+  try { code = std::stoi(it->second); } catch (const std::exception &) {}
+  if (code < 1 || code > 3) unsupported(op, std::string(attr) + " other than 1 (e5m2), 2 (e4m3) or 3 (e2m1)");
+  return code == 1 ? 1 : code == 2 ? 0 : 4;
+}
+
+// the codes' tensor: bytes, or the 8-bit type of the format
+void checkCodes(const Op *op, const Value *v, int fmt, std::vector<int64_t> shape, size_t axis) {
+  if (fmt == 4) {
+    if (shape[axis] % 2) unsupported(op, "an odd number of 4-bit codes along the blocks' axis (two share a byte)");
+    shape[axis] /= 2;
+  }
+  if (v->type.elem != Elem::I8 && v->type.elem != (fmt == 0 ? Elem::F8E4M3FN : fmt == 1 ? Elem::F8E5M2 : Elem::I8))
+    unsupported(op, "codes of another type than the format's (or bytes)");
+  if (v->type.shape != shape) unsupported(op, "codes shape " + v->type.str());
+}
+void checkScales(const Op *op, const Value *v, const std::vector<int64_t> &shape) {
+  if (v->type.elem != Elem::I8) unsupported(op, "scales that are not ui8 / i8 (e8m0)");
+  if (v->type.shape != shape) unsupported(op, "scales shape " + v->type.str() + " (one byte per block of 32, the last may be short)");
+}
+const char *mxFormatName(int fmt) { return fmt == 0 ? "e4m3" : fmt == 1 ? "e5m2" : "e2m1"; }
+} // namespace
+
+// hf::MxElem of a value type
+static std::string mxElem(const Op *op, const Value *v) {
+  switch (v->type.elem) {
+  case Elem::F32: return "hf::EL_F32";
+  case Elem::BF16: return "hf::EL_BF16";
+  case Elem::F16: return "hf::EL_F16";
+  default: unsupported(op, std::string("values of type ") + elemName(v->type.elem) + " (f32, bf16 or f16)");
+  }
+}
+// operands are group arguments and no destination is one of them
+static void checkOwnOperands(const Op *op, size_t nins, size_t nouts) {
+  if (op->ins.size() != nins || op->outs.size() != nouts || op->results.size() != nouts) unsupported(op, "number of operands or results");
+  for (const Value *v : op->ins) {
+    if (v->argIdx < 0) unsupported(op, "operand that is not a group argument");
+    for (const Value *o : op->outs)
+      if (tiedArgOf(o) == v->argIdx) unsupported(op, "operand that is also a destination");
+  }
+  for (size_t i = 0; i < op->outs.size(); ++i)
+    for (size_t j = 0; j < i; ++j)
+      if (tiedArgOf(op->outs[i]) >= 0 && tiedArgOf(op->outs[i]) == tiedArgOf(op->outs[j])) unsupported(op, "one destination of two results");
+  for (size_t i = 0; i < op->outs.size(); ++i)
+    if (op->outs[i]->type.elem != op->results[i]->type.elem || op->outs[i]->type.shape != op->results[i]->type.shape)
+      unsupported(op, "destination " + op->outs[i]->type.str() + " of a result " + op->results[i]->type.str());
+}
+// rows (all dims but the last), as the kernels are told them and as a grid's
+// rows per launch-time row
+static std::string leadRows(const Analysis &A, const Op *op, const std::vector<int64_t> &shape, int64_t &R, int64_t &perRow) {
+  if (shape.size() < 2) unsupported(op, "rank below 2");
+  R = perRow = 1;
+  for (size_t i = 0; i + 1 < shape.size(); ++i) {
+    R *= shape[i];
+    if (i > 0 || !A.rowsDyn) perRow *= shape[i];
+  }
+  if (shape.back() < 1) unsupported(op, "rows of no elements");
+  if (!A.rowsDyn) return std::to_string(R) + "ll";
+  if (shape[0] != kRuntimeRows) unsupported(op, "a runtime row count other than the rows of the first operand");
+  return perRow == 1 ? "hf_rows" : "hf_rows * " + std::to_string(perRow) + "ll";
+}
+// blocks = ceil(rows * perRow * num / den) up to cap
+static void rowGrid(const Analysis &A, KernelPlan &p, int64_t R, int64_t perRow, int64_t num, int64_t den, int64_t cap) {
+  if (A.rowsDyn) {
+    p.rowsDyn = true;
+    p.rowsA = perRow * num;
+    p.rowsB = den;
+    p.rowsCap = cap;
+    return;
+  }
+  const int64_t blocks = (R * num + den - 1) / den;
+  p.grid[0] = (unsigned)std::max<int64_t>(1, std::min(cap, blocks));
+}
+static KernelPlan lowerMxCodes(Analysis &A, const std::string &kname, const Op *op, const std::vector<std::string> &outPtr) {
+  const bool de = op->name == "hfusion.dequantize_mx";
+  checkOwnOperands(op, de ? 2 : 1, de ? 1 : 2);
+  const Value *x = de ? op->results[0] : op->ins[0], *codes = de ? op->ins[0] : op->results[0],
+              *scales = de ? op->ins[1] : op->results[1];
+  const int fmt = mxFormatOf(op, "format");
+  if (fmt < 0) unsupported(op, "a missing format");
+  const auto &sh = x->type.shape;
+  if (sh.size() < 2) unsupported(op, "rank below 2");
+  int64_t axis = (int64_t)sh.size() - 1;
+  if (op->attrs.count("axis")) {
+    try { axis = std::stoll(op->attr("axis")); } catch (const std::exception &) { unsupported(op, "axis"); }
+    if (axis == -1) axis = (int64_t)sh.size() - 1;
+  }
+  const bool cols = axis == 0 && sh.size() == 2;
+  if (!cols && axis != (int64_t)sh.size() - 1) unsupported(op, "axis other than the last, or 0 of a matrix");
+  if (cols && A.rowsDyn) unsupported(op, "a runtime row count with blocks down the columns (compile per size)");
+  for (auto d : sh) if (d < 1) unsupported(op, "an empty tensor");
+  checkCodes(op, codes, fmt, sh, (size_t)axis);
+  std::vector<int64_t> ssh = sh;
+  if (cols) ssh = {sh[1], (sh[0] + 31) / 32};
+  else ssh.back() = (sh.back() + 31) / 32;
+  checkScales(op, scales, ssh);
+  const std::string el = mxElem(op, x);
+  KernelPlan p;
+  p.kernelName = kname;
+  p.kind = de ? "DEQUANTIZE_MX" : "QUANTIZE_MX";
+  p.variant = std::string(mxFormatName(fmt)) + (cols ? ", blocks down the columns" : ", blocks along the rows");
+  auto in = [&](size_t i) { return "p" + std::to_string(op->ins[i]->argIdx); };
+  std::ostringstream k;
+  int threads = 256;
+  std::string call;
+  if (cols) {
+    threads = 512; // one wave per block of 32 k-rows, eight blocks
+    call = std::string("hf::mx_") + (de ? "de" : "") + "quantize_cols<" + el + ", " + std::to_string(fmt) + ", " + std::to_string(sh[0]) +
+           "ll, " + std::to_string(sh[1]) + "ll>(";
+    const int64_t blocks = ((sh[1] + 255) / 256) * ((ssh[1] + 7) / 8);
+    if (blocks > (int64_t(1) << 22)) unsupported(op, "a matrix of more than 2^22 tiles of 256 columns by 256 rows");
+    p.grid[0] = (unsigned)blocks;
+  } else {
+    int64_t R, per;
+    const std::string rows = leadRows(A, op, sh, R, per);
+    call = std::string("hf::mx_") + (de ? "de" : "") + "quantize_rows<" + el + ", " + std::to_string(fmt) + ", " + std::to_string(sh.back()) + "ll>(";
+    rowGrid(A, p, R, per, ssh.back() * 4, threads, 65536);
+    call += in(0) + ", " + (de ? in(1) + ", " + outPtr[0] : outPtr[0] + ", " + outPtr[1]) + ", " + rows;
+  }
+  if (cols) call += in(0) + ", " + (de ? in(1) + ", " + outPtr[0] : outPtr[0] + ", " + outPtr[1]);
+  k << "extern \"C\" __global__ __launch_bounds__(" << threads << ") void " << kname << "(" << kernelParamList(A, p.kargs, false) << ") {\n  "
+    << call << ");\n}\n";
+  p.block[0] = (unsigned)threads;
+  p.source = k.str();
+  return p;
+}
+
+// Layer norm and its gradient.  Threads of a row group, chunks of eight
+// elements a thread and row groups a workgroup by the row's length.
+struct LnShape { int64_t T, NCH, RPB; };
+static LnShape lnForwardShape(int64_t D) {
+  if (D <= 1024) return {64, (D + 511) / 512, 4};
+  const int64_t T = std::min<int64_t>(1024, (D + 1023) / 1024 * 64);
+  return {T, (D + 8 * T - 1) / (8 * T), 1};
+}
+static LnShape lnGradShape(int64_t D) {
+  if (D <= 512) return {64, 1, 4};
+  const int64_t T = std::min<int64_t>(1024, (D + 511) / 512 * 64);
+  return {T, (D + 8 * T - 1) / (8 * T), 1};
+}
+
+static KernelPlan lowerLayerNorm(Analysis &A, const std::string &kname, const Op *op, const std::vector<std::string> &outPtr) {
+  const bool grad = op->name == "hfusion.layer_norm_grad";
+  const int ck = mxFormatOf(op, "format");
+  if (ck == 4) unsupported(op, "a 4-bit checkpoint");
+  // forward: x [gamma [beta]] -> y mean rstd [codes scales]
+  // gradient: dy x|codes scales [gamma] mean rstd -> dx [dgamma [dbeta]]
+  size_t aff;
+  if (grad) {
+    const size_t base = ck >= 0 ? 5 : 4;
+    aff = op->outs.size() - 1;
+    if (op->outs.empty() || aff > 2) unsupported(op, "number of results");
+    checkOwnOperands(op, base + (aff > 0 ? 1 : 0), 1 + aff);
+  } else {
+    if (op->ins.empty() || op->ins.size() > 3) unsupported(op, "number of operands");
+    aff = op->ins.size() - 1;
+    checkOwnOperands(op, 1 + aff, ck >= 0 ? 5 : 3);
+  }
+  const Value *y = op->results[0];
+  const auto &sh = y->type.shape;
+  int64_t R, per;
+  const std::string rows = leadRows(A, op, sh, R, per);
+  const int64_t D = sh.back();
+  if (D > 16384) unsupported(op, "rows of more than 16384 elements (one workgroup keeps a row)");
+  const std::vector<int64_t> lead(sh.begin(), sh.end() - 1);
+  std::vector<int64_t> ssh = sh;
+  ssh.back() = (D + 31) / 32;
+  const std::string el = mxElem(op, y);
+  auto same = [&](const Value *v) {
+    if (v->type.shape != sh || v->type.elem != y->type.elem) unsupported(op, "operand " + v->type.str() + " beside " + y->type.str());
+  };
+  auto stat = [&](const Value *v) {
+    if (v->type.shape != lead || v->type.elem != Elem::F32) unsupported(op, "mean and 1/std must be f32, one per row");
+  };
+  const Value *param = nullptr;
+  auto affine = [&](const Value *v) {
+    if (v->type.shape != std::vector<int64_t>{D}) unsupported(op, "weight, bias and their gradients have one element per column");
+    if (param && v->type.elem != param->type.elem) unsupported(op, "weight, bias and their gradients of different types");
+    if (v->type.elem != Elem::F32 && v->type.elem != y->type.elem) unsupported(op, "weight and bias of another type than f32 or the rows'");
+    param = v;
+  };
+  auto in = [&](size_t i) { return "p" + std::to_string(op->ins[i]->argIdx); };
+  KernelPlan p;
+  p.kernelName = kname;
+  std::ostringstream k;
+  const LnShape s = grad ? lnGradShape(D) : lnForwardShape(D);
+  const int64_t threads = s.T * s.RPB;
+  auto targs = [&](const std::string &pel) {
+    return "<" + el + ", " + pel + ", " + std::to_string(aff) + ", " + std::to_string(ck) + ", " + std::to_string(s.T) + ", " +
+           std::to_string(s.NCH) + ", " + std::to_string(s.RPB) + ", " + std::to_string(D) + "ll>(";
+  };
+  p.block[0] = (unsigned)threads;
+  p.variant = std::to_string(s.T) + " threads a row" + (ck >= 0 ? std::string(", 8-bit checkpoint ") + mxFormatName(ck) : "");
+  if (!grad) {
+    same(op->ins[0]);
+    for (size_t i = 1; i <= aff; ++i) affine(op->ins[i]);
+    stat(op->results[1]);
+    stat(op->results[2]);
+    if (ck >= 0) {
+      checkCodes(op, op->results[3], ck, sh, sh.size() - 1);
+      checkScales(op, op->results[4], ssh);
+    }
+    float eps = 0;
+    try { eps = std::stof(op->attr("eps", "")); } catch (const std::exception &) { unsupported(op, "a missing eps"); }
+    if (!(eps >= 0) || std::isinf(eps)) unsupported(op, "eps that is negative or no number");
+    p.kind = "LAYER_NORM";
+    k << "extern \"C\" __global__ __launch_bounds__(" << threads << ") void " << kname << "(" << kernelParamList(A, p.kargs, false) << ") {\n"
+      << "  hf::ln_forward" << targs(param ? mxElem(op, param) : el) << in(0) << ", " << (aff > 0 ? in(1) : "nullptr") << ", "
+      << (aff > 1 ? in(2) : "nullptr") << ", " << outPtr[0] << ", (float *)" << outPtr[1] << ", (float *)" << outPtr[2] << ", "
+      << (ck >= 0 ? outPtr[3] + ", " + outPtr[4] : "nullptr, nullptr") << ", " << rows << ", " << floatLit(eps) << ");\n}\n";
+    rowGrid(A, p, R, per, 1, s.RPB, 256 * std::max<int64_t>(1, 2048 / threads));
+    p.source = k.str();
+    return p;
+  }
+  same(op->ins[0]);
+  size_t at = 2;
+  if (ck >= 0) {
+    checkCodes(op, op->ins[1], ck, sh, sh.size() - 1);
+    checkScales(op, op->ins[2], ssh);
+    at = 3;
+  } else {
+    same(op->ins[1]);
+  }
+  if (aff > 0) affine(op->ins[at++]);
+  stat(op->ins[at]);
+  stat(op->ins[at + 1]);
+  for (size_t i = 1; i <= aff; ++i) affine(op->results[i]);
+  p.kind = "LAYER_NORM_GRAD";
+  // row groups that walk the rows, each leaving one row of partial sums
+  const int64_t cap = 512, groups = cap * s.RPB;
+  const std::string call = "  hf::ln_grad_rows" + targs(param ? mxElem(op, param) : el);
+  // the row kernel's arguments by name: dy x scales gamma mean rstd dx ws
+  auto body = [&](const std::vector<std::string> &a) {
+    return call + a[0] + ", " + a[1] + ", " + a[2] + ", " + a[3] + ", (const float *)" + a[4] + ", (const float *)" + a[5] + ", " + a[6] +
+           ", (float *)" + a[7] + ", " + rows + ");\n}\n";
+  };
+  const std::string scl = ck >= 0 ? in(2) : "nullptr", gam = aff > 0 ? in(at - 1) : "nullptr";
+  if (aff == 0) {
+    k << "extern \"C\" __global__ __launch_bounds__(" << threads << ") void " << kname << "(" << kernelParamList(A, p.kargs, false) << ") {\n"
+      << body({in(0), in(1), scl, gam, in(at), in(at + 1), outPtr[0], "nullptr"});
+    rowGrid(A, p, R, per, 1, s.RPB, cap);
+    p.source = k.str();
+    return p;
+  }
+  KernelPlan::PreKernel pk;
+  pk.name = kname + "_rows";
+  std::vector<std::string> none;
+  const std::string params = kernelParamList(A, pk.kargs, true);
+  pk.grid = (unsigned)(A.rowsDyn ? cap : std::max<int64_t>(1, std::min<int64_t>(cap, (R + s.RPB - 1) / s.RPB)));
+  pk.block = (unsigned)threads;
+  k << "extern \"C\" __global__ __launch_bounds__(" << threads << ") void " << pk.name << "(" << params << ") {\n"
+    << body({in(0), in(1), scl, gam, in(at), in(at + 1), outPtr[0], "ws"});
+  p.pre.push_back(pk);
+  const int64_t used = pk.grid * s.RPB; // row groups of a full launch
+  k << "extern \"C\" __global__ __launch_bounds__(1024) void " << kname << "(" << kernelParamList(A, p.kargs, true) << ") {\n"
+    << "  const int64_t R = " << rows << ";\n"
+    << "  hf::ln_grad_columns<" << mxElem(op, param) << ", " << aff << ", 16, " << D << "ll>((const float *)ws, R < " << used << "ll ? R : "
+    << used << "ll, " << outPtr[1] << ", " << (aff > 1 ? outPtr[2] : "nullptr") << ");\n}\n";
+  p.grid[0] = (unsigned)(((int64_t)aff * D + 63) / 64);
+  p.block[0] = 1024;
+  p.rowsDyn = A.rowsDyn;
+  p.rowsZero = A.rowsDyn; // no rows: the weight's gradients are zeros
+  p.workspaceBytes = (uint64_t)std::min<int64_t>(groups, used) * aff * D * 4;
+  p.source = k.str();
+  return p;
+}
+
 static KernelPlan lowerSingleOp(Analysis &A, const std::string &kname, const Op *op) {
   Func &f = *A.f;
   for (const Op *o : f.ops)
-    if (o != op && o->name != "tensor.empty" && o->name != "arith.constant" && o->name.rfind("arith.index", 0) != 0)
+    if (o != op && o->name != "tensor.empty" && o->name != "arith.constant" && o->name != "tensor.dim" && o->name.rfind("arith.index", 0) != 0)
       unsupported(o, "op in a group with " + op->name);
   if (op->name == "hfusion.gather" || op->name == "hfusion.sort")
     for (const Value *v : op->ins)
@@ -2971,6 +3329,10 @@ static KernelPlan lowerSingleOp(Analysis &A, const std::string &kname, const Op 
     if (v->def != op) unsupported(op, "group returns a value other than the op's results");
     outPtr[v->resultIdx] = resultPtr(A, i);
   }
+  // (layer_norm: a caller with no gradient to take leaves mean and 1/std)
+  if (op->name == "hfusion.layer_norm")
+    for (size_t i = 1; i < outPtr.size() && i < 3; ++i)
+      if (outPtr[i].empty()) outPtr[i] = "nullptr";
   for (auto &s : outPtr) if (s.empty()) unsupported(op, "a result the group does not return");
   auto inPtr = [&](size_t i) { return "p" + std::to_string(op->operands.at(i)->argIdx); };
   for (const Value *v : op->operands)
@@ -2982,6 +3344,8 @@ static KernelPlan lowerSingleOp(Analysis &A, const std::string &kname, const Op 
   KernelPlan p;
   p.kernelName = kname;
   std::ostringstream k;
+  if (n == "quantize_mx" || n == "dequantize_mx") return lowerMxCodes(A, kname, op, outPtr);
+  if (n == "layer_norm" || n == "layer_norm_grad") return lowerLayerNorm(A, kname, op, outPtr);
   if (n == "cumsum" || n == "cumprod" || n == "cummax" || n == "cummin") {
     // CPU meaning (cumprod: ConvertHFusionToUpstream.cpp:385-450): along the
     // cumulation dim, in index order (reverse: from the end), acc_0 = x_0 and
@@ -4346,9 +4710,12 @@ std::vector<KernelPlan> lowerModule(Module &m, const LowerOptions &opt) {
         for (Value *b : written) f.returns.push_back(latest[b]);
     }
     splitGenericReductions(m, f);
-    // ui8 is read as raw bytes: only matmul_mx's e8m0 scales may be ui8
+    // ui8 is read as raw bytes: only the e8m0 scales of block-scaled ops may be ui8
     for (const Op *op : f.ops) {
-      if (op->name == "hfusion.matmul_mx" || op->name == "func.return") continue;
+      if (op->name == "hfusion.matmul_mx" || op->name == "hfusion.linear_mx" || op->name == "hfusion.quantize_mx" ||
+          op->name == "hfusion.dequantize_mx" || op->name == "hfusion.layer_norm" || op->name == "hfusion.layer_norm_grad" ||
+          op->name == "func.return")
+        continue;
       for (const Value *v : op->ins)
         if (v->type.uns) unsupported(op, "ui8 operand outside matmul_mx scales");
       for (const Value *v : op->operands)
@@ -4495,7 +4862,7 @@ std::string emitTranslationUnit(const std::vector<KernelPlan> &plans) {
   std::ostringstream s;
   s << "// Generated by bishengir-compile --target=mi355x (ConvertHFusionToHIP).\n"
     << "#include \"hf_ops.h\"\n#include \"hf_row.h\"\n#include \"hf_argmax.h\"\n#include \"hf_mmad.h\"\n#include \"hf_mmsk.h\"\n#include \"hf_mmtl.h\"\n#include \"hf_misc.h\"\n"
-    << "#include \"hf_rmsq.h\"\n#include \"hf_rmsn.h\"\n#include \"hf_sort.h\"\n\n";
+    << "#include \"hf_rmsq.h\"\n#include \"hf_rmsn.h\"\n#include \"hf_sort.h\"\n#include \"hf_mx.h\"\n#include \"hf_mmwx.h\"\n#include \"hf_ln.h\"\n\n";
   for (auto &p : plans) s << "// group @" << p.funcName << ": " << p.kind << " (" << p.variant << ")\n" << p.source << "\n";
   return s.str();
 }
@@ -4514,6 +4881,7 @@ std::string emitManifest(const KernelPlan &p, const std::string &hsacoName) {
     << "algo_bytes " << (uint64_t)p.algoBytes << "\n"
     << "algo_ops " << (uint64_t)p.algoOps << "\n";
   if (p.rowsDyn) s << "rows_dyn " << p.rowsA << " " << p.rowsB << " " << p.rowsC << " " << p.rowsCap << "\n";
+  if (p.rowsZero) s << "rows_zero 1\n";
   auto shp = [](const std::vector<int64_t> &v) {
     std::string r = std::to_string(v.size());
     for (auto d : v) r += " " + std::to_string(d);
@@ -4530,7 +4898,7 @@ std::string emitManifest(const KernelPlan &p, const std::string &hsacoName) {
     s << "\n";
   }
   for (auto &a : p.alts)
-    s << "alt " << a.name << " " << a.maxRows << " " << a.rowsB << " " << a.rowsC << " " << a.block << "\n";
+    s << "alt " << a.name << " " << a.maxRows << " " << a.rowsB << " " << a.rowsC << " " << a.block << (a.pre ? " pre" : "") << "\n";
   s << "variant " << p.variant << "\n";
   return s.str();
 }

@@ -48,11 +48,13 @@ struct KernelPlan {
   std::vector<PreKernel> pre;
   // other kernels of the group for small runtime row counts, by ascending
   // maxRows: a launch of R <= maxRows rows runs the first that fits, without
-  // the pre kernels, on ceil(R / rowsB) * rowsC blocks, instead of the main one
+  // the pre kernels (unless `pre`), on ceil(R / rowsB) * rowsC blocks, instead
+  // of the main one
   struct RowAlt {
     std::string name;
     int64_t maxRows = 0, rowsB = 1, rowsC = 1;
     unsigned block = 256;
+    bool pre = false;
   };
   std::vector<RowAlt> alts;
   // runtime row count (compiler option dyn=runtime): the kernel takes the
@@ -62,6 +64,7 @@ struct KernelPlan {
   // algoBytes is per row.
   bool rowsDyn = false;
   int64_t rowsA = 0, rowsB = 1, rowsC = 1, rowsCap = 0;
+  bool rowsZero = false; // a launch of no rows has results to write
 };
 
 struct LowerOptions {

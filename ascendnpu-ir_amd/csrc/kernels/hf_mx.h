@@ -1,0 +1,472 @@
+// Block-scaled (microscaling) codes: hfusion.quantize_mx and its inverse.
+//
+// 32 consecutive elements along the blocked axis share the scale 2^E, held as
+// the byte E + 127 (e8m0); a code stands for code * 2^E.
+//   E    = floor(log2 max|x|) - EMAX, at least -127   (EMAX: the exponent of
+//          the format's largest binade, so the block's largest element lands
+//          in it; a block of zeros has the byte 0)
+//   code = x * 2^-E rounded to the nearest code, ties to even, values past the
+//          largest finite code becoming that code
+// A block that holds an infinity or a NaN has the byte 255 (its values are
+// NaN whatever the codes) and codes 0.
+// floor(log2 max|x|) is the exponent field of the largest magnitude, which
+// integer maxima of the bits without the sign find (NaN and infinity compare
+// above every number), and x * 2^-E is exact or far below the smallest code,
+// so the only rounding is the conversion's own.
+#pragma once
+#include "hf_row.h"
+
+namespace hf {
+
+// element types of the values
+enum MxElem : int { EL_F32 = 0, EL_BF16 = 1, EL_F16 = 2 };
+// formats of the codes (the matrix core's numbers)
+enum MxFormat : int { MX_E4M3 = 0, MX_E5M2 = 1, MX_E2M1 = 4 };
+template <int EL> constexpr int el_bytes = EL == EL_F32 ? 4 : 2;
+template <int FMT> constexpr int mx_emax = FMT == MX_E4M3 ? 8 : FMT == MX_E5M2 ? 15 : 2;
+template <int FMT> constexpr float mx_top = FMT == MX_E4M3 ? 448.0f : FMT == MX_E5M2 ? 57344.0f : 6.0f;
+// bytes of eight codes
+template <int FMT> constexpr int mx_oct = FMT == MX_E2M1 ? 4 : 8;
+
+// ---------------------------------------------------------------- eight values
+template <int EL> struct Oct { uint32_t w[2 * el_bytes<EL>]; };
+
+// (16-byte accesses at any element: rows of odd lengths start anywhere)
+typedef u32x4 u32x4_any __attribute__((aligned(1)));
+typedef u32x2 u32x2_any __attribute__((aligned(1)));
+typedef uint32_t u32_any __attribute__((aligned(1)));
+
+template <int EL> __device__ __forceinline__ Oct<EL> oct_load(const void *p) {
+  Oct<EL> o;
+  const u32x4_any *q = reinterpret_cast<const u32x4_any *>(p);
+#pragma unroll
+  for (int i = 0; i < el_bytes<EL> / 2; ++i) {
+    const u32x4 v = __builtin_nontemporal_load(q + i);
+    o.w[4 * i] = v.x, o.w[4 * i + 1] = v.y, o.w[4 * i + 2] = v.z, o.w[4 * i + 3] = v.w;
+  }
+  return o;
+}
+// the first n of eight values, zeros behind them
+template <int EL> __device__ __forceinline__ Oct<EL> oct_load_part(const void *p, int n) {
+  Oct<EL> o{};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (i >= n) break;
+    if constexpr (EL == EL_F32) o.w[i] = reinterpret_cast<const uint32_t *>(p)[i];
+    else o.w[i / 2] |= (uint32_t)reinterpret_cast<const uint16_t *>(p)[i] << (16 * (i % 2));
+  }
+  return o;
+}
+template <int EL> __device__ __forceinline__ void oct_store(void *p, const Oct<EL> &o) {
+  u32x4_any *q = reinterpret_cast<u32x4_any *>(p);
+#pragma unroll
+  for (int i = 0; i < el_bytes<EL> / 2; ++i) {
+    const u32x4 v = {o.w[4 * i], o.w[4 * i + 1], o.w[4 * i + 2], o.w[4 * i + 3]};
+    __builtin_nontemporal_store(v, q + i);
+  }
+}
+template <int EL> __device__ __forceinline__ void oct_store_part(void *p, const Oct<EL> &o, int n) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (i >= n) break;
+    if constexpr (EL == EL_F32) reinterpret_cast<uint32_t *>(p)[i] = o.w[i];
+    else reinterpret_cast<uint16_t *>(p)[i] = (uint16_t)(o.w[i / 2] >> (16 * (i % 2)));
+  }
+}
+template <int EL> __device__ __forceinline__ float oct_get(const Oct<EL> &o, int i) {
+  if constexpr (EL == EL_F32) return u2f(o.w[i]);
+  else if constexpr (EL == EL_BF16) return u2f(i % 2 ? o.w[i / 2] & 0xFFFF0000u : o.w[i / 2] << 16);
+  else return f16_to_f32((uint16_t)(o.w[i / 2] >> (16 * (i % 2))));
+}
+// two neighbouring values rounded to nearest even
+template <int EL> __device__ __forceinline__ void oct_set2(Oct<EL> &o, int i, float a, float b) {
+  if constexpr (EL == EL_F32) o.w[i] = f2u(a), o.w[i + 1] = f2u(b);
+  else if constexpr (EL == EL_BF16) o.w[i / 2] = (uint32_t)f32_to_bf16_rne(a) | (uint32_t)f32_to_bf16_rne(b) << 16;
+  else {
+    // (a product and its conversion would become one multiply-add with +0,
+    // which loses the sign of a product that is -0)
+    asm("" : "+v"(a), "+v"(b));
+    o.w[i / 2] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)a) | (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)b) << 16;
+  }
+}
+
+// ---------------------------------------------------------------- magnitudes
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+}
+__device__ __forceinline__ uint32_t max_u32(uint32_t a, uint32_t b) { return a > b ? a : b; }
+// f32 bits of a 16-bit magnitude (bits without the sign)
+template <int EL> __device__ __forceinline__ uint32_t mag_f32(uint32_t half) {
+  if constexpr (EL == EL_BF16) return half << 16;
+  else return f2u(f16_to_f32((uint16_t)half));
+}
+// f32 bits of the largest of eight magnitudes
+template <int EL> __device__ __forceinline__ uint32_t oct_amax(const Oct<EL> &o) {
+  if constexpr (EL == EL_F32) {
+    uint32_t m = o.w[0] & 0x7FFFFFFFu;
+#pragma unroll
+    for (int i = 1; i < 8; ++i) m = max_u32(m, o.w[i] & 0x7FFFFFFFu);
+    return m;
+  } else {
+    uint32_t m = o.w[0] & 0x7FFF7FFFu;
+#pragma unroll
+    for (int i = 1; i < 4; ++i) m = max_u16x2(m, o.w[i] & 0x7FFF7FFFu);
+    return mag_f32<EL>(max_u32(m & 0xFFFFu, m >> 16));
+  }
+}
+// over the four lanes of a quad (they share a block)
+__device__ __forceinline__ uint32_t quad_max(uint32_t m) {
+  m = max_u32(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xF, 0xF, true));        // lanes 1 0 3 2
+  return max_u32(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xF, 0xF, true));     // lanes 2 3 0 1
+}
+
+// ---------------------------------------------------------------- codes
+// the scale byte of a block whose largest magnitude has these f32 bits
+template <int FMT> __device__ __forceinline__ uint32_t mx_scale_byte(uint32_t amax) {
+  const int e = (int)(amax >> 23);
+  return e == 255 ? 255u : (uint32_t)(e > mx_emax<FMT> ? e - mx_emax<FMT> : 0);
+}
+// 2^-E of a scale byte (any number for 255, whose codes are zeros)
+__device__ __forceinline__ float mx_inverse(uint32_t byte) { return u2f((254u - (byte > 253u ? 253u : byte)) << 23); }
+// 2^E; the byte 0 is a subnormal, 255 NaN
+__device__ __forceinline__ float mx_scale(uint32_t byte) {
+  return u2f(byte == 0 ? 0x00400000u : byte == 255 ? 0x7FC00000u : byte << 23);
+}
+template <int FMT> __device__ __forceinline__ float mx_clamp(float v) {
+  return __builtin_amdgcn_fmed3f(v, -mx_top<FMT>, mx_top<FMT>);
+}
+// two codes into half h (16 bits) of w
+template <int FMT> __device__ __forceinline__ uint32_t mx_pair8(float a, float b, uint32_t w, bool hi) {
+  static_assert(FMT != MX_E2M1);
+  a = mx_clamp<FMT>(a), b = mx_clamp<FMT>(b);
+  if constexpr (FMT == MX_E4M3) return (uint32_t)(hi ? __builtin_amdgcn_cvt_pk_fp8_f32(a, b, (int)w, true) : __builtin_amdgcn_cvt_pk_fp8_f32(a, b, (int)w, false));
+  else return (uint32_t)(hi ? __builtin_amdgcn_cvt_pk_bf8_f32(a, b, (int)w, true) : __builtin_amdgcn_cvt_pk_bf8_f32(a, b, (int)w, false));
+}
+// two e2m1 codes into byte B of w, a in the low half
+template <int B> __device__ __forceinline__ uint32_t mx_pair4(float a, float b, uint32_t w) {
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, mx_clamp<MX_E2M1>(a), mx_clamp<MX_E2M1>(b), 1.0f, B);
+}
+// eight codes: one word of e2m1, two of the 8-bit formats
+template <int EL, int FMT> __device__ __forceinline__ u32x2 mx_encode(const Oct<EL> &o, float inv, bool finite) {
+  u32x2 c = {0, 0};
+  auto v = [&](int i) { return oct_get<EL>(o, i) * inv; };
+  if constexpr (FMT == MX_E2M1) {
+    c.x = mx_pair4<0>(v(0), v(1), c.x);
+    c.x = mx_pair4<1>(v(2), v(3), c.x);
+    c.x = mx_pair4<2>(v(4), v(5), c.x);
+    c.x = mx_pair4<3>(v(6), v(7), c.x);
+  } else {
+    c.x = mx_pair8<FMT>(v(0), v(1), c.x, false);
+    c.x = mx_pair8<FMT>(v(2), v(3), c.x, true);
+    c.y = mx_pair8<FMT>(v(4), v(5), c.y, false);
+    c.y = mx_pair8<FMT>(v(6), v(7), c.y, true);
+  }
+  return finite ? c : u32x2{0, 0};
+}
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+// codes 2 i, 2 i + 1 of a word
+template <int FMT> __device__ __forceinline__ f32x2 mx_decode2(uint32_t w, int i) {
+  if constexpr (FMT == MX_E4M3) return i ? __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true) : __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
+  else if constexpr (FMT == MX_E5M2) return i ? __builtin_amdgcn_cvt_pk_f32_bf8((int)w, true) : __builtin_amdgcn_cvt_pk_f32_bf8((int)w, false);
+  else
+    return i == 0   ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 0)
+           : i == 1 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 1)
+           : i == 2 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 2)
+                    : __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 3);
+}
+template <int FMT> __device__ __forceinline__ void mx_decode(u32x2 c, float scale, float (&f)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const f32x2 v = FMT == MX_E2M1 ? mx_decode2<FMT>(c.x, i) : mx_decode2<FMT>(i < 2 ? c.x : c.y, i % 2);
+    f[2 * i] = v.x * scale, f[2 * i + 1] = v.y * scale;
+  }
+}
+template <int FMT> __device__ __forceinline__ void codes_store(void *p, u32x2 c) {
+  if constexpr (FMT == MX_E2M1) __builtin_nontemporal_store(c.x, reinterpret_cast<u32_any *>(p));
+  else __builtin_nontemporal_store(c, reinterpret_cast<u32x2_any *>(p));
+}
+// the codes of the first n of eight values (n even for e2m1)
+template <int FMT> __device__ __forceinline__ void codes_store_part(uint8_t *p, u32x2 c, int n) {
+  const int bytes = FMT == MX_E2M1 ? n / 2 : n;
+#pragma unroll
+  for (int i = 0; i < mx_oct<FMT>; ++i) {
+    if (i >= bytes) break;
+    p[i] = (uint8_t)((i < 4 ? c.x : c.y) >> (8 * (i % 4)));
+  }
+}
+template <int FMT> __device__ __forceinline__ u32x2 codes_load(const void *p) {
+  if constexpr (FMT == MX_E2M1) return u32x2{__builtin_nontemporal_load(reinterpret_cast<const u32_any *>(p)), 0};
+  else return __builtin_nontemporal_load(reinterpret_cast<const u32x2_any *>(p));
+}
+template <int FMT> __device__ __forceinline__ u32x2 codes_load_part(const uint8_t *p, int n) {
+  const int bytes = FMT == MX_E2M1 ? (n + 1) / 2 : n;
+  u32x2 c = {0, 0};
+#pragma unroll
+  for (int i = 0; i < mx_oct<FMT>; ++i) {
+    if (i >= bytes) break;
+    if (i < 4) c.x |= (uint32_t)p[i] << (8 * i);
+    else c.y |= (uint32_t)p[i] << (8 * (i - 4));
+  }
+  return c;
+}
+
+// The scale bytes of the blocks of this row of 16 lanes (lanes 4 j hold block
+// j of `blk` + j): one four-byte store where all four blocks exist.
+__device__ __forceinline__ void scales_store(uint8_t *__restrict__ scales, int64_t blk, int64_t nblk, uint32_t byte) {
+  const int lane = threadIdx.x & 15;
+  if ((blk | 3) < nblk) { // (blk counts up by one every four lanes, from a multiple of 4)
+    uint32_t w = byte;
+    w |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)byte, 0x104, 0xF, 0xF, true) << 8;  // lane + 4
+    w |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)byte, 0x108, 0xF, 0xF, true) << 16; // lane + 8
+    w |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)byte, 0x10C, 0xF, 0xF, true) << 24; // lane + 12
+    if (lane == 0) *reinterpret_cast<u32_any *>(scales + blk) = w;
+  } else if ((lane & 3) == 0) {
+    scales[blk] = (uint8_t)byte;
+  }
+}
+
+// ---------------------------------------------------------------- blocks along a row
+// x [R, K] -> codes [R, K] (e2m1: [R, K/2]), scales [R, ceil(K/32)].  Four
+// lanes share a block, eight elements (one 16-byte access of a 16-bit type)
+// each; a workgroup's accesses are consecutive.
+template <int EL, int FMT, int64_t K>
+__device__ __forceinline__ void mx_quantize_rows(const void *__restrict__ x, void *__restrict__ codes, void *__restrict__ scales,
+                                                 int64_t R) {
+  constexpr int64_t NB = (K + 31) / 32;
+  const int64_t nblk = R * NB, n = nblk * 4;
+  for (int64_t it = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; it < n; it += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t blk = it >> 2;
+    int64_t e = it * 8; // first element, flat
+    int cnt = 8;
+    if constexpr (K % 32 != 0) {
+      const int64_t r = blk / NB, c = (blk - r * NB) * 32 + (it & 3) * 8;
+      e = r * K + c;
+      cnt = (int)(K - c < 0 ? 0 : K - c < 8 ? K - c : 8);
+    }
+    const char *src = (const char *)x + e * el_bytes<EL>;
+    const Oct<EL> o = cnt == 8 ? oct_load<EL>(src) : oct_load_part<EL>(src, cnt);
+    const uint32_t byte = mx_scale_byte<FMT>(quad_max(oct_amax<EL>(o)));
+    const u32x2 c = mx_encode<EL, FMT>(o, mx_inverse(byte), byte != 255);
+    uint8_t *dst = (uint8_t *)codes + (FMT == MX_E2M1 ? e / 2 : e);
+    if (cnt == 8) codes_store<FMT>(dst, c);
+    else codes_store_part<FMT>(dst, c, cnt);
+    scales_store((uint8_t *)scales, blk, nblk, byte);
+  }
+}
+
+// codes -> values, the same layout; f32 products are exact, the one rounding
+// is to the result's type
+template <int EL, int FMT, int64_t K>
+__device__ __forceinline__ void mx_dequantize_rows(const void *__restrict__ codes, const void *__restrict__ scales, void *__restrict__ out,
+                                                   int64_t R) {
+  constexpr int64_t NB = (K + 31) / 32;
+  const int64_t n = R * NB * 4;
+  for (int64_t it = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; it < n; it += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t blk = it >> 2;
+    int64_t e = it * 8;
+    int cnt = 8;
+    if constexpr (K % 32 != 0) {
+      const int64_t r = blk / NB, c = (blk - r * NB) * 32 + (it & 3) * 8;
+      e = r * K + c;
+      cnt = (int)(K - c < 0 ? 0 : K - c < 8 ? K - c : 8);
+    }
+    const uint8_t *src = (const uint8_t *)codes + (FMT == MX_E2M1 ? e / 2 : e);
+    const u32x2 c = cnt == 8 ? codes_load<FMT>(src) : codes_load_part<FMT>(src, cnt);
+    float f[8];
+    mx_decode<FMT>(c, mx_scale(((const uint8_t *)scales)[blk]), f);
+    Oct<EL> o;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) oct_set2<EL>(o, i, f[i], f[i + 1]);
+    char *dst = (char *)out + e * el_bytes<EL>;
+    if (cnt == 8) oct_store<EL>(dst, o);
+    else oct_store_part<EL>(dst, o, cnt);
+  }
+}
+
+// ---------------------------------------------------------------- blocks down a column
+// x [K, N] -> codes [K, N] (e2m1: [K/2, N], two k a byte), scales
+// [N, ceil(K/32)].  A lane owns four columns of one block (32 k-rows), a wave
+// 256 columns, and the eight waves of a workgroup eight blocks, whose scale
+// bytes leave together: eight consecutive bytes of every column.
+constexpr int MXC_COLS = 256, MXC_BLOCKS = 8;
+
+template <int EL> struct Quad4 { uint32_t w[el_bytes<EL>]; }; // four values of a k-row
+template <int EL> __device__ __forceinline__ Quad4<EL> quad_load(const char *p, int n) {
+  Quad4<EL> q{};
+  if (n == 4) {
+    if constexpr (EL == EL_F32) {
+      const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any *>(p));
+      q.w[0] = v.x, q.w[1] = v.y, q.w[2] = v.z, q.w[3] = v.w;
+    } else {
+      const u32x2 v = __builtin_nontemporal_load(reinterpret_cast<const u32x2_any *>(p));
+      q.w[0] = v.x, q.w[1] = v.y;
+    }
+    return q;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (i >= n) break;
+    if constexpr (EL == EL_F32) q.w[i] = reinterpret_cast<const uint32_t *>(p)[i];
+    else q.w[i / 2] |= (uint32_t)reinterpret_cast<const uint16_t *>(p)[i] << (16 * (i % 2));
+  }
+  return q;
+}
+template <int EL> __device__ __forceinline__ float quad_get(const Quad4<EL> &q, int i) {
+  if constexpr (EL == EL_F32) return u2f(q.w[i]);
+  else if constexpr (EL == EL_BF16) return u2f(i % 2 ? q.w[i / 2] & 0xFFFF0000u : q.w[i / 2] << 16);
+  else return f16_to_f32((uint16_t)(q.w[i / 2] >> (16 * (i % 2))));
+}
+__device__ __forceinline__ void bytes_store(uint8_t *p, uint32_t w, int n) {
+  if (n == 4) {
+    __builtin_nontemporal_store(w, reinterpret_cast<u32_any *>(p));
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (i < n) p[i] = (uint8_t)(w >> (8 * i));
+}
+
+template <int EL, int FMT, int64_t K, int64_t N>
+__device__ __forceinline__ void mx_quantize_cols(const void *__restrict__ x, void *__restrict__ codes, void *__restrict__ scales) {
+  constexpr int64_t NB = (K + 31) / 32, CT = (N + MXC_COLS - 1) / MXC_COLS;
+  __shared__ uint8_t sc[MXC_COLS][MXC_BLOCKS];
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const int64_t n0 = (int64_t)(blockIdx.x % CT) * MXC_COLS, n = n0 + 4 * lane;
+  const int64_t kb0 = (int64_t)(blockIdx.x / CT) * MXC_BLOCKS, kb = kb0 + wave, k0 = kb * 32;
+  const int cols = (int)(N - n <= 0 ? 0 : N - n < 4 ? N - n : 4);
+  if (kb < NB && cols > 0) {
+    const int rows = (int)(K - k0 < 32 ? K - k0 : 32);
+    Quad4<EL> q[32];
+    const char *src = (const char *)x + (k0 * N + n) * el_bytes<EL>;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) q[i] = i < rows ? quad_load<EL>(src + (int64_t)i * N * el_bytes<EL>, cols) : Quad4<EL>{};
+    uint32_t m[4];
+    if constexpr (EL == EL_F32) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        m[j] = 0;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) m[j] = max_u32(m[j], q[i].w[j] & 0x7FFFFFFFu);
+      }
+    } else {
+      uint32_t a = 0, b = 0;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) a = max_u16x2(a, q[i].w[0] & 0x7FFF7FFFu), b = max_u16x2(b, q[i].w[1] & 0x7FFF7FFFu);
+      m[0] = mag_f32<EL>(a & 0xFFFFu), m[1] = mag_f32<EL>(a >> 16);
+      m[2] = mag_f32<EL>(b & 0xFFFFu), m[3] = mag_f32<EL>(b >> 16);
+    }
+    float inv[4];
+    uint32_t keep = 0; // bytes of the columns whose block is finite
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t byte = mx_scale_byte<FMT>(m[j]);
+      inv[j] = mx_inverse(byte);
+      keep |= byte == 255 ? 0u : 0xFFu << (8 * j);
+      sc[4 * lane + j][wave] = (uint8_t)byte;
+    }
+    if constexpr (FMT == MX_E2M1) {
+      uint8_t *dst = (uint8_t *)codes + (k0 / 2) * N + n;
+#pragma unroll
+      for (int i = 0; i < 32; i += 2) {
+        uint32_t w = 0;
+        auto v = [&](int d, int j) { return quad_get<EL>(q[i + d], j) * inv[j]; };
+        w = mx_pair4<0>(v(0, 0), v(1, 0), w);
+        w = mx_pair4<1>(v(0, 1), v(1, 1), w);
+        w = mx_pair4<2>(v(0, 2), v(1, 2), w);
+        w = mx_pair4<3>(v(0, 3), v(1, 3), w);
+        if (i < rows) bytes_store(dst + (int64_t)(i / 2) * N, w & keep, cols);
+      }
+    } else {
+      uint8_t *dst = (uint8_t *)codes + k0 * N + n;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        auto v = [&](int j) { return quad_get<EL>(q[i], j) * inv[j]; };
+        uint32_t w = mx_pair8<FMT>(v(0), v(1), 0, false);
+        w = mx_pair8<FMT>(v(2), v(3), w, true);
+        if (i < rows) bytes_store(dst + (int64_t)i * N, w & keep, cols);
+      }
+    }
+  }
+  __syncthreads();
+  const int64_t col = n0 + threadIdx.x;
+  if (threadIdx.x < MXC_COLS && col < N) {
+    uint8_t *dst = (uint8_t *)scales + col * NB + kb0;
+    const u32x2 v = *reinterpret_cast<const u32x2 *>(sc[threadIdx.x]);
+    if (kb0 + MXC_BLOCKS <= NB) {
+      *reinterpret_cast<u32x2_any *>(dst) = v;
+    } else {
+      for (int i = 0; i < (int)(NB - kb0); ++i) dst[i] = (uint8_t)((i < 4 ? v.x : v.y) >> (8 * (i % 4)));
+    }
+  }
+}
+
+template <int EL, int FMT, int64_t K, int64_t N>
+__device__ __forceinline__ void mx_dequantize_cols(const void *__restrict__ codes, const void *__restrict__ scales, void *__restrict__ out) {
+  constexpr int64_t NB = (K + 31) / 32, CT = (N + MXC_COLS - 1) / MXC_COLS;
+  __shared__ uint8_t sc[MXC_COLS][MXC_BLOCKS];
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const int64_t n0 = (int64_t)(blockIdx.x % CT) * MXC_COLS, n = n0 + 4 * lane;
+  const int64_t kb0 = (int64_t)(blockIdx.x / CT) * MXC_BLOCKS, kb = kb0 + wave, k0 = kb * 32;
+  const int64_t col = n0 + threadIdx.x;
+  if (threadIdx.x < MXC_COLS && col < N) {
+    const uint8_t *src = (const uint8_t *)scales + col * NB + kb0;
+    u32x2 v = {0, 0};
+    if (kb0 + MXC_BLOCKS <= NB) v = *reinterpret_cast<const u32x2_any *>(src);
+    else
+      for (int i = 0; i < (int)(NB - kb0); ++i) {
+        if (i < 4) v.x |= (uint32_t)src[i] << (8 * i);
+        else v.y |= (uint32_t)src[i] << (8 * (i - 4));
+      }
+    *reinterpret_cast<u32x2 *>(sc[threadIdx.x]) = v;
+  }
+  __syncthreads();
+  const int cols = (int)(N - n <= 0 ? 0 : N - n < 4 ? N - n : 4);
+  if (kb >= NB || cols == 0) return;
+  const int rows = (int)(K - k0 < 32 ? K - k0 : 32);
+  float s[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) s[j] = mx_scale(sc[4 * lane + j][wave]);
+  constexpr int P = FMT == MX_E2M1 ? 2 : 1; // k-rows a byte
+  const uint8_t *src = (const uint8_t *)codes + (k0 / P) * N + n;
+  char *dst = (char *)out + (k0 * N + n) * el_bytes<EL>;
+  uint32_t w[32 / P];
+#pragma unroll
+  for (int i = 0; i < 32 / P; ++i) {
+    w[i] = 0;
+    if (i * P >= rows) continue;
+    const uint8_t *p = src + (int64_t)i * N;
+    if (cols == 4) w[i] = __builtin_nontemporal_load(reinterpret_cast<const u32_any *>(p));
+    else
+      for (int j = 0; j < cols; ++j) w[i] |= (uint32_t)p[j] << (8 * j);
+  }
+  auto put = [&](int k, float a, float b, float c, float d) {
+    if (k >= rows) return;
+    a *= s[0], b *= s[1], c *= s[2], d *= s[3];
+    char *p = dst + (int64_t)k * N * el_bytes<EL>;
+    Oct<EL> o{};
+    oct_set2<EL>(o, 0, a, b);
+    oct_set2<EL>(o, 2, c, d);
+    if (cols < 4) {
+      oct_store_part<EL>(p, o, cols);
+    } else if constexpr (EL == EL_F32) {
+      __builtin_nontemporal_store(u32x4{o.w[0], o.w[1], o.w[2], o.w[3]}, reinterpret_cast<u32x4_any *>(p));
+    } else {
+      __builtin_nontemporal_store(u32x2{o.w[0], o.w[1]}, reinterpret_cast<u32x2_any *>(p));
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < 32 / P; ++i) {
+    if constexpr (FMT == MX_E2M1) {
+      // byte j of the word is column j's two k
+      const f32x2 a = mx_decode2<FMT>(w[i], 0), b = mx_decode2<FMT>(w[i], 1), c = mx_decode2<FMT>(w[i], 2), d = mx_decode2<FMT>(w[i], 3);
+      put(2 * i, a.x, b.x, c.x, d.x);
+      put(2 * i + 1, a.y, b.y, c.y, d.y);
+    } else {
+      const f32x2 a = mx_decode2<FMT>(w[i], 0), b = mx_decode2<FMT>(w[i], 1);
+      put(i, a.x, a.y, b.x, b.y);
+    }
+  }
+}
+
+} // namespace hf

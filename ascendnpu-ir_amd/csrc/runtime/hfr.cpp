@@ -63,6 +63,7 @@ struct RowAlt {
   hipFunction_t fn = nullptr;
   int64_t maxRows = 0, rowsB = 1, rowsC = 1;
   unsigned block = 0;
+  bool pre = false; // after the group's pre kernels
 };
 
 struct hfr_group {
@@ -79,6 +80,9 @@ struct hfr_group {
   // min(ceil(R * a / b) * c, cap) (cap 0: none), or the static grid when a is 0
   bool rowsDyn = false;
   int64_t rowsA = 0, rowsB = 1, rowsC = 1, rowsCap = 0;
+  // a launch of no rows has results to write (manifest `rows_zero 1`); its
+  // tensors of no rows may be null
+  bool rowsZero = false;
   std::vector<std::string> paramRoles;
   std::vector<Buf> paramBufs, resultBufs;
   std::vector<int> resultTied;
@@ -166,6 +170,11 @@ int parseBlock(const std::vector<std::string> &lines, hfr_group &g) {
       if (g.rowsA < 0 || g.rowsB <= 0 || g.rowsC <= 0 || g.rowsCap < 0)
         return fail(HFR_ERR_MANIFEST, "bad rows_dyn line: " + ln);
     }
+    else if (key == "rows_zero") {
+      int z = 0;
+      is >> z;
+      g.rowsZero = z != 0;
+    }
     else if (key == "param" || key == "result") {
       int i, tied = -1, rank = 0;
       std::string role;
@@ -202,9 +211,16 @@ int parseBlock(const std::vector<std::string> &lines, hfr_group &g) {
       g.pre.push_back(pl);
     }
     else if (key == "alt") {
-      // alt <kernel> <max rows> <rows per block row> <blocks per block row> <threads>
+      // alt <kernel> <max rows> <rows per block row> <blocks per block row> <threads> [pre]
       RowAlt ra;
       is >> ra.kernel >> ra.maxRows >> ra.rowsB >> ra.rowsC >> ra.block;
+      if (is.fail()) return fail(HFR_ERR_MANIFEST, "malformed manifest line: " + ln);
+      std::string more;
+      if (is >> more) {
+        if (more != "pre") return fail(HFR_ERR_MANIFEST, "bad alt line: " + ln);
+        ra.pre = true;
+      }
+      is.clear();
       if (ra.maxRows <= 0 || ra.rowsB <= 0 || ra.rowsC <= 0 || !ra.block || (!g.alts.empty() && g.alts.back().maxRows >= ra.maxRows))
         return fail(HFR_ERR_MANIFEST, "bad alt line: " + ln);
       g.alts.push_back(ra);
@@ -276,7 +292,8 @@ int launchRaw(hipFunction_t fn, const hfr_launch_cfg &cfg, const uint64_t *args,
 }
 
 // Checks a group launch's arguments (counts, null pointers).
-int checkGroupArgs(const hfr_group *g, const uint64_t *params, size_t nparams, void *const *results, size_t nresults) {
+int checkGroupArgs(const hfr_group *g, const uint64_t *params, size_t nparams, void *const *results, size_t nresults,
+                   int64_t rows = -1) {
   if (!g) return fail(HFR_ERR_INVALID, "null group");
   if (nparams != g->paramRoles.size())
     return fail(HFR_ERR_INVALID, "group @" + g->func + " takes " + std::to_string(g->paramRoles.size()) +
@@ -285,11 +302,14 @@ int checkGroupArgs(const hfr_group *g, const uint64_t *params, size_t nparams, v
     return fail(HFR_ERR_INVALID, "group @" + g->func + " has " + std::to_string(g->resultTied.size()) +
                                      " results, got " + std::to_string(nresults));
   if (nparams && !params) return fail(HFR_ERR_INVALID, "null params array");
+  auto empty = [&](const std::vector<Buf> &bufs, size_t i) {
+    return g->rowsZero && rows == 0 && i < bufs.size() && std::count(bufs[i].shape.begin(), bufs[i].shape.end(), int64_t(-1)) != 0;
+  };
   for (size_t i = 0; i < nparams; ++i)
-    if (g->paramRoles[i] != "scalar" && params[i] == 0)
+    if (g->paramRoles[i] != "scalar" && params[i] == 0 && !empty(g->paramBufs, i))
       return fail(HFR_ERR_INVALID, "null device pointer for argument " + std::to_string(i));
   for (size_t i = 0; i < nresults; ++i)
-    if (g->resultTied[i] < 0 && (!results || !results[i]))
+    if (g->resultTied[i] < 0 && (!results || (!results[i] && !empty(g->resultBufs, i))))
       return fail(HFR_ERR_INVALID, "null device pointer for result " + std::to_string(i));
   return HFR_OK;
 }
@@ -321,18 +341,26 @@ int launchGroup(const hfr_group *g, const uint64_t *params, void *const *results
     }
     return launchRaw(fn, cfg, args, n, stream);
   };
+  auto runPre = [&]() {
+    for (auto &pl : g->pre) {
+      const int rc = launch(pl.fn, pl.cfg, pl.kargs);
+      if (rc) return rc;
+    }
+    return (int)HFR_OK;
+  };
   for (auto &alt : g->alts)
     if (rows <= alt.maxRows) {
+      if (alt.pre) {
+        const int rc = runPre();
+        if (rc) return rc;
+      }
       hfr_launch_cfg cfg{};
       cfg.grid[0] = (unsigned)((rows + alt.rowsB - 1) / alt.rowsB * alt.rowsC);
       cfg.grid[1] = cfg.grid[2] = cfg.block[1] = cfg.block[2] = 1;
       cfg.block[0] = alt.block;
       return launch(alt.fn, cfg, g->kargs);
     }
-  for (auto &pl : g->pre) {
-    const int rc = launch(pl.fn, pl.cfg, pl.kargs);
-    if (rc) return rc;
-  }
+  if (const int rc = runPre()) return rc;
   return launch(g->fn, rowsCfg(g->cfg), g->kargs);
 }
 
@@ -486,9 +514,9 @@ int hfr_group_launch_rows(hfr_group_t g, const uint64_t *params, size_t nparams,
   if (g && !g->rowsDyn && rows != -1)
     return fail(HFR_ERR_INVALID, "group @" + g->func + " has a static row count");
   if (g && g->rowsDyn && rows < 0) return fail(HFR_ERR_INVALID, "negative row count for group @" + g->func);
-  int rc = checkGroupArgs(g, params, nparams, results, nresults);
+  int rc = checkGroupArgs(g, params, nparams, results, nresults, rows);
   if (rc) return rc;
-  if (g->rowsDyn && rows == 0) return HFR_OK; // nothing to do
+  if (g->rowsDyn && rows == 0 && !g->rowsZero) return HFR_OK; // nothing to do
   void *ws = workspace;
   if (g->wsBytes && !ws) {
     int dev = 0;

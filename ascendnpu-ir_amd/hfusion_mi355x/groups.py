@@ -483,3 +483,216 @@ def transpose_cast(rows=4096, cols=8192, src="bf16", dst="f32"):
   }}
 }}
 """
+
+
+# ---- block-scaled codes and layer norm (ops of this backend)
+
+_MX_CODE = {"e5m2": 1, "e4m3": 2, "e2m1": 3}  # the `format` attribute, as matmul_mx's lhsFormat
+_MX_TYPE = {"e5m2": "f8E5M2", "e4m3": "f8E4M3FN", "e2m1": "i8"}
+
+
+def _mx_types(rows, cols, fmt, axis):
+    """Types of the codes (e2m1: bytes of two) and of the e8m0 scales (one per
+    32 elements along `axis`, the last may be short)."""
+    if fmt not in _MX_CODE:
+        raise ValueError(f"format {fmt!r} (e4m3, e5m2 or e2m1)")
+    if axis not in (0, 1):
+        raise ValueError("axis 0 or 1")
+    if fmt == "e2m1" and (cols if axis else rows) % 2:
+        raise ValueError("two 4-bit codes share a byte: the blocks' axis must be even")
+    half = 2 if fmt == "e2m1" else 1
+    shape = [rows, cols // half] if axis else [rows // half, cols]
+    scales = [rows, (cols + 31) // 32] if axis else [cols, (rows + 31) // 32]
+    return _t(shape, _MX_TYPE[fmt]), _t(scales, "ui8")
+
+
+def quantize_mx(rows, cols, src="bf16", fmt="e4m3", axis=1):
+    """Block-scaled codes of x [rows, cols] (hfusion.quantize_mx): 32 elements
+    along `axis` share the e8m0 scale 2^E with E = floor(log2 max|x|) less the
+    exponent of the format's largest binade (at least -127); a code is x * 2^-E
+    rounded to nearest even, saturated.  A block of zeros has the scale byte 0;
+    one that holds an infinity or NaN has 255 (NaN) and codes 0.  axis 1: codes
+    [rows, cols] and scales [rows, ceil(cols/32)], matmul_mx's A; axis 0: codes
+    [rows, cols] and scales [cols, ceil(rows/32)], its B.  e2m1 codes are
+    bytes of two along `axis`, the even one in the low half."""
+    X = _t([rows, cols], src)
+    Q, S = _mx_types(rows, cols, fmt, axis)
+    return f"""module {{
+  func.func @quantize_mx(%x: {X}, %q: {Q}, %s: {S}) -> ({Q}, {S})
+      {_ATTRS.format(kind='ANY_PB')} {{
+    %r:2 = hfusion.quantize_mx {{format = {_MX_CODE[fmt]} : i32, axis = {axis} : i32}} ins(%x : {X}) outs(%q, %s : {Q}, {S}) -> {Q}, {S}
+    return %r#0, %r#1 : {Q}, {S}
+  }}
+}}
+"""
+
+
+def dequantize_mx(rows, cols, dst="bf16", fmt="e4m3", axis=1):
+    """The values of block-scaled codes (hfusion.dequantize_mx): code * 2^E,
+    rounded once to `dst` (f32, bf16 or f16); layouts as quantize_mx."""
+    X = _t([rows, cols], dst)
+    Q, S = _mx_types(rows, cols, fmt, axis)
+    return f"""module {{
+  func.func @dequantize_mx(%q: {Q}, %s: {S}, %x: {X}) -> {X}
+      {_ATTRS.format(kind='ANY_PB')} {{
+    %r = hfusion.dequantize_mx {{format = {_MX_CODE[fmt]} : i32, axis = {axis} : i32}} ins(%q, %s : {Q}, {S}) outs(%x : {X}) -> {X}
+    return %r : {X}
+  }}
+}}
+"""
+
+
+def linear_mx(m, n, k, fmt="e2m1", bias=False, out="bf16"):
+    """bf16 rows times a block-scaled weight (hfusion.linear_mx): out[m, n] =
+    sum_k a[m, k] w[n, k] 2^E[n, k/32] (+ f32 bias[n]), f32 sums, one rounding
+    to `out`.  w is [n, k] fp8 or [n, k/2] bytes of two e2m1 codes (the layout
+    quantize_mx gives a weight [n, k] along its rows); k is a multiple of 32.
+    The weight's values are multiplied as bf16: one past its range (2^128,
+    scale bytes above 246) is infinite."""
+    A, O, C = _t([m, k], "bf16"), _t([m, n], out), _t([m, n], "f32")
+    W, S = _mx_types(n, k, fmt, 1)
+    B = _t([n], "f32")
+    args = f"%a: {A}, %w: {W}, %s: {S}" + (f", %bias: {B}" if bias else "") + f", %out: {O}"
+    body = [f"%e0 = tensor.empty() : {C}",
+            f"%c = hfusion.linear_mx {{rhsFormat = {_MX_CODE[fmt]} : i32}} ins(%a, %w, %s : {A}, {W}, {S}) outs(%e0 : {C}) -> {C}"]
+    res = "%c"
+    if bias:
+        dst = "%out" if out == "f32" else "%e2"
+        body += [f"%e1 = tensor.empty() : {C}",
+                 f"%bb = linalg.broadcast ins(%bias : {B}) outs(%e1 : {C}) dimensions = [0]"]
+        if out != "f32":
+            body.append(f"%e2 = tensor.empty() : {C}")
+        body.append(f"%cb = linalg.elemwise_binary {{fun = #linalg.binary_fn<add>}} ins(%c, %bb : {C}, {C}) outs({dst} : {C}) -> {C}")
+        res = "%cb"
+    if out != "f32":
+        body.append(f"%o = hfusion.cast {{round_mode = #hfusion.round_mode<rint>}} ins({res} : {C}) outs(%out : {O}) -> {O}")
+        res = "%o"
+    elif not bias:
+        body[0] = f"%c0 = arith.constant 0.000000e+00 : f32\n    %e0 = linalg.fill ins(%c0 : f32) outs(%out : {C}) -> {C}"
+    body.append(f"return {res} : {O}")
+    lines = "\n".join("    " + x for x in body)
+    return f"""module {{
+  func.func @linear_mx({args}) -> {O}
+      {_ATTRS.format(kind='SINGLE_CUBE')} {{
+{lines}
+  }}
+}}
+"""
+
+
+def _ln_params(cols, elem, params, affine):
+    """Names and type of the weight and bias: affine 2 both, 1 the weight, 0 none."""
+    if affine not in (0, 1, 2):
+        raise ValueError("affine 0, 1 (weight) or 2 (weight and bias)")
+    return ["gamma", "beta"][:affine], _t([cols], params or elem)
+
+
+def layer_norm(rows, cols, elem="bf16", params=None, ckpt=None, eps=1e-5, affine=2):
+    """Layer norm over the last axis (hfusion.layer_norm): y = (x - mean) *
+    rstd * gamma + beta, with mean and rstd = 1 / sqrt(variance + eps) saved
+    in f32 for the gradient.  `params`: type of gamma and beta (`elem`, or
+    f32).  ckpt "e4m3" / "e5m2" also writes x as 8-bit block-scaled codes, as
+    quantize_mx along the rows does: what layer_norm_grad reads in x's place."""
+    X, R = _t([rows, cols], elem), _t([rows], "f32")
+    names, P = _ln_params(cols, elem, params, affine)
+    outs = [("y", X), ("mean", R), ("rstd", R)]
+    fmt = ""
+    if ckpt:
+        outs += list(zip(("q", "s"), _mx_types(rows, cols, ckpt, 1)))
+        fmt = f", format = {_MX_CODE[ckpt]} : i32"
+    ins = [("x", X)] + [(n, P) for n in names]
+    sig = ", ".join(f"%{n}: {t}" for n, t in ins + outs)
+    tys = ", ".join(t for _, t in outs)
+    grp = lambda v: ", ".join("%" + n for n, _ in v) + " : " + ", ".join(t for _, t in v)  # noqa: E731
+    rets = ", ".join(f"%r#{i}" for i in range(len(outs)))
+    return f"""module {{
+  func.func @layer_norm({sig}) -> ({tys})
+      {_ATTRS.format(kind='ANY_PB')} {{
+    %r:{len(outs)} = hfusion.layer_norm {{eps = {eps:.9e} : f32{fmt}}} ins({grp(ins)}) outs({grp(outs)}) -> {tys}
+    return {rets} : {tys}
+  }}
+}}
+"""
+
+
+def layer_norm_grad(rows, cols, elem="bf16", params=None, ckpt=None, affine=2):
+    """Gradient of layer_norm (hfusion.layer_norm_grad): dx, dgamma and dbeta
+    from dy, the saved mean and rstd, and x, or with `ckpt` x's 8-bit codes
+    and scales in its place.  dgamma and dbeta are summed over the rows in
+    f32, in an order that the sizes fix."""
+    X, R = _t([rows, cols], elem), _t([rows], "f32")
+    names, P = _ln_params(cols, elem, params, affine)
+    fmt = ""
+    ins = [("dy", X), ("x", X)]
+    if ckpt:
+        ins = [("dy", X)] + list(zip(("q", "s"), _mx_types(rows, cols, ckpt, 1)))
+        fmt = f" {{format = {_MX_CODE[ckpt]} : i32}}"
+    ins += [(n, P) for n in names[:1]] + [("mean", R), ("rstd", R)]
+    outs = [("dx", X)] + [("d" + n, P) for n in names]
+    sig = ", ".join(f"%{n}: {t}" for n, t in ins + outs)
+    tys = ", ".join(t for _, t in outs)
+    grp = lambda v: ", ".join("%" + n for n, _ in v) + " : " + ", ".join(t for _, t in v)  # noqa: E731
+    lhs = f"%r:{len(outs)}" if len(outs) > 1 else "%r"
+    rets = ", ".join(f"%r#{i}" for i in range(len(outs))) if len(outs) > 1 else "%r"
+    return f"""module {{
+  func.func @layer_norm_grad({sig}) -> ({tys})
+      {_ATTRS.format(kind='ANY_PB')} {{
+    {lhs} = hfusion.layer_norm_grad{fmt} ins({grp(ins)}) outs({grp(outs)}) -> {tys}
+    return {rets} : {tys}
+  }}
+}}
+"""
+
+
+def _layer_norm_stats(m, k, eps):
+    """Statements of a host function's layer norm of %x [m, k] bf16: %ln#0 its
+    result, and the mean and 1/std that a host function's caller does not see."""
+    X, P, R = _t([m, k], "bf16"), _t([k], "bf16"), _t([m], "f32")
+    return [f"%e0 = tensor.empty() : {X}", f"%e1 = tensor.empty() : {R}", f"%e2 = tensor.empty() : {R}",
+            f"%ln:3 = hfusion.layer_norm {{eps = {eps:.9e} : f32}} ins(%x, %gamma, %beta : {X}, {P}, {P}) "
+            f"outs(%e0, %e1, %e2 : {X}, {R}, {R}) -> {X}, {R}, {R}"], X, P, R
+
+
+def layer_norm_matmul_mx(m=4096, n=4096, k=4096, fmt="e4m3", eps=1e-5):
+    """An un-fused host function: layer norm, block-scaled quantisation of its
+    result and the block-scaled contraction with a weight [k, n] in the same
+    format (quantize_mx with axis 0 makes it).  A program of three launches."""
+    body, X, P, _ = _layer_norm_stats(m, k, eps)
+    if fmt == "e2m1":
+        raise ValueError("the program's contraction takes typed fp8 codes (e4m3 or e5m2)")
+    (Q, S), (W, SW) = _mx_types(m, k, fmt, 1), _mx_types(k, n, fmt, 0)
+    C = _t([m, n], "f32")
+    body += [f"%e3 = tensor.empty() : {Q}", f"%e4 = tensor.empty() : {S}",
+             f"%q:2 = hfusion.quantize_mx {{format = {_MX_CODE[fmt]} : i32, axis = 1 : i32}} ins(%ln#0 : {X}) outs(%e3, %e4 : {Q}, {S}) -> {Q}, {S}",
+             f"%e5 = tensor.empty() : {C}",
+             f"%c = hfusion.matmul_mx ins(%q#0, %w, %q#1, %sw : {Q}, {W}, {S}, {SW}) outs(%e5 : {C}) -> {C}",
+             f"return %c : {C}"]
+    lines = "\n".join("    " + x for x in body)
+    return f"""module {{
+  func.func @layer_norm_matmul_mx(%x: {X}, %gamma: {P}, %beta: {P}, %w: {W}, %sw: {SW}) -> {C}
+      {_HOST} {{
+{lines}
+  }}
+}}
+"""
+
+
+def layer_norm_linear_mx(m=16, n=4096, k=4096, fmt="e2m1", eps=1e-5):
+    """An un-fused host function: layer norm and the linear layer with a
+    block-scaled weight [n, k] on its result (a decoding step's pair)."""
+    body, X, P, _ = _layer_norm_stats(m, k, eps)
+    W, S = _mx_types(n, k, fmt, 1)
+    C, O = _t([m, n], "f32"), _t([m, n], "bf16")
+    body += [f"%e3 = tensor.empty() : {C}",
+             f"%c = hfusion.linear_mx {{rhsFormat = {_MX_CODE[fmt]} : i32}} ins(%ln#0, %w, %s : {X}, {W}, {S}) outs(%e3 : {C}) -> {C}",
+             f"%e4 = tensor.empty() : {O}",
+             f"%o = hfusion.cast {{round_mode = #hfusion.round_mode<rint>}} ins(%c : {C}) outs(%e4 : {O}) -> {O}",
+             f"return %o : {O}"]
+    lines = "\n".join("    " + x for x in body)
+    return f"""module {{
+  func.func @layer_norm_linear_mx(%x: {X}, %gamma: {P}, %beta: {P}, %w: {W}, %s: {S}) -> {O}
+      {_HOST} {{
+{lines}
+  }}
+}}
+"""

@@ -27,6 +27,8 @@ import re
 
 import numpy as np
 
+from . import blockscaled as bs
+
 HERE = os.path.dirname(os.path.abspath(__file__))
 _lib = None
 
@@ -391,6 +393,50 @@ def _single_op(op, rest, xs, rtypes):
     out = np.empty(a.shape[:-1] + (2 * a.shape[-1],), a.dtype)
     out[..., 0::2], out[..., 1::2] = a, b
     return [T(out, elem)]
+
+
+def _block_scaled(op, rest, ins, outs):
+    """Block-scaled codes and layer norm (blockscaled.py), results rounded
+    once to their types."""
+    def attr(name):
+        m = re.search(name + r"\s*=\s*([-+.\w]+)", rest)
+        return m.group(1) if m else None
+
+    def f64(v):
+        return to_f32(v).astype(np.float64)
+
+    def rounded(a, o):
+        with np.errstate(over="ignore"):
+            return T(from_f32(np.asarray(a, np.float64).astype(np.float32), o.elem), o.elem)
+
+    def raw(a, o):
+        return T(_contig(a).view(NP[o.elem]), o.elem)
+    fmt = bs.FORMAT.get(int(attr("rhsFormat" if op.endswith("linear_mx") else "format") or 0))
+
+    def quantized(x, axis, qo, so):
+        codes, scales = bs.quantize(x, fmt, axis)
+        return [raw(bs.pack(codes, axis) if fmt == "e2m1" else codes, qo), raw(scales, so)]
+    if op in ("hfusion.quantize_mx", "hfusion.dequantize_mx"):
+        nd = outs[0].a.ndim
+        axis = int(attr("axis") or -1) % nd
+        if op == "hfusion.quantize_mx":
+            return quantized(f64(ins[0]), axis, outs[0], outs[1])
+        return [rounded(bs.dequantize(ins[0].a, ins[1].a, fmt, axis), outs[0])]
+    if op == "hfusion.linear_mx":
+        w = bs.dequantize(ins[1].a, ins[2].a, fmt, 1)
+        with np.errstate(invalid="ignore"):
+            return [rounded(f64(ins[0]) @ w.T + f64(outs[0]), outs[0])]
+    if op == "hfusion.layer_norm":
+        x = f64(ins[0])
+        gb = [f64(v) for v in ins[1:]] + [None] * (3 - len(ins))
+        vals = bs.layer_norm(x, gb[0], gb[1], float(np.float32(attr("eps"))))
+        out = [rounded(v, o) for v, o in zip(vals, outs)]
+        return out + (quantized(x, x.ndim - 1, outs[3], outs[4]) if fmt else [])
+    dy, at = f64(ins[0]), 3 if fmt else 2
+    x = bs.dequantize(ins[1].a, ins[2].a, fmt, dy.ndim - 1) if fmt else f64(ins[1])
+    gamma = f64(ins[at]) if len(outs) > 1 else None
+    mean, rstd = f64(ins[-2]), f64(ins[-1])
+    return [rounded(v, o) for v, o in zip(bs.layer_norm_grad(dy, x, gamma, mean, rstd), outs)]
 
 
 _NON_DPS = ("hfusion.isinf", "hfusion.isnan", "hfusion.isfinite", "hfusion.nextafter", "hfusion.hypot",
@@ -857,6 +903,13 @@ class Interp:
             return
         if op == "hfusion.reduce_with_index":
             self._reduce_with_index(res, rest, ins, outs, env)
+            return
+        if op in ("hfusion.quantize_mx", "hfusion.dequantize_mx", "hfusion.linear_mx", "hfusion.layer_norm",
+                  "hfusion.layer_norm_grad"):
+            vals = _block_scaled(op, rest, [get(n) for n in ins], [get(n) for n in outs])
+            names = [res] + more if more else [res] if len(vals) == 1 else [f"{res}#{i}" for i in range(len(vals))]
+            env.update(zip(names, vals))
+            env.setdefault(res, vals[0])
             return
         if op == "hfusion.matmul_mx":
             # fp8 A [M, K], B [K, N]; lhsFormat / rhsFormat (1 e5m2, 2 e4m3,

@@ -1349,6 +1349,8 @@ def entries():
     e["prog_scores_softmax"] = g.scores_softmax(128, 1024, 128)
     e["prog_scores_softmax_ragged"] = g.scores_softmax(72, 1000, 64)
     e["prog_exp_cumsum_scale"] = g.exp_cumsum_scale(64, 1000)
+    import norm_mx_catalog
+    e.update(norm_mx_catalog.entries())
     return e
 
 

@@ -1,0 +1,85 @@
+"""The layer-norm and block-scaled groups the tests prebuild: every format,
+element type, schedule and ragged end of each operator."""
+from hfusion_mi355x import groups as g
+
+_ANY = 7919
+
+# rows, cols, element type, format, axis
+QUANT = [
+    (37, 128, "bf16", "e4m3", 1), (5, 1, "f32", "e5m2", 1), (33, 101, "f16", "e4m3", 1), (3, 4096, "bf16", "e2m1", 1),
+    (7, 98, "f32", "e2m1", 1), (1, 32, "bf16", "e5m2", 1), (64, 36, "f16", "e2m1", 1), (9, 260, "f32", "e4m3", 1),
+    (32, 256, "bf16", "e4m3", 0), (70, 33, "f32", "e5m2", 0), (300, 261, "f16", "e2m1", 0), (2, 1, "bf16", "e2m1", 0),
+    (1, 7, "f32", "e4m3", 0), (258, 512, "bf16", "e2m1", 0), (513, 258, "f16", "e5m2", 0),
+]
+# rows, cols, element type, type of weight and bias, checkpoint, affine
+NORM = [
+    (3, 1, "f32", "f32", None, 2), (5, 7, "bf16", "f32", None, 2), (9, 64, "f16", "f16", "e4m3", 1), (6, 33, "f32", "f32", "e5m2", 2),
+    (33, 512, "bf16", "bf16", None, 2), (130, 1000, "bf16", "bf16", "e4m3", 2), (40, 1024, "f16", "f32", "e5m2", 0),
+    (7, 1032, "f32", "f32", None, 1), (700, 2001, "bf16", "f32", None, 2), (5, 4096, "bf16", "bf16", "e5m2", 2),
+    (3, 5003, "f32", "f32", "e4m3", 2), (2, 8200, "bf16", "f32", "e4m3", 1), (2, 16384, "f16", "f32", "e4m3", 2),
+    (600, 320, "f32", "f32", None, 2), (1, 16383, "f32", "f32", None, 2), (11, 96, "bf16", "bf16", None, 0),
+]
+# rows, outputs, k, format, bias, result
+LINEAR = [
+    (1, 16, 32, "e2m1", False, "bf16"), (1, 1, 64, "e4m3", True, "f32"), (3, 33, 96, "e5m2", False, "f32"), (16, 40, 288, "e4m3", True, "bf16"),
+    (17, 100, 1024, "e2m1", True, "bf16"), (33, 257, 2080, "e2m1", False, "bf16"), (64, 50, 4096, "e5m2", False, "bf16"), (48, 129, 512, "e4m3", True, "f32"),
+    (65, 100, 544, "e2m1", True, "bf16"), (300, 520, 256, "e4m3", False, "bf16"), (129, 31, 160, "e5m2", True, "f32"),
+]
+# the same at a launch-time row count, and the row counts they are called with
+RT_ROWS = [1, 5, 16, 17, 40, 64, 65, 130, 515]
+
+
+def quant_name(c, kind="quant"):
+    r, n, el, fmt, ax = c
+    return f"{kind}mx_{fmt}_{el}_{r}x{n}_a{ax}"
+
+
+def norm_name(c, kind="ln"):
+    r, n, el, p, ck, aff = c
+    return f"{kind}_{el}_{p}_{ck or 'x'}_{r}x{n}_w{aff}"
+
+
+def linear_name(c):
+    m, n, k, fmt, bias, out = c
+    return f"linmx_{fmt}_{m}x{n}x{k}_{'b' if bias else 'n'}_{out}"
+
+
+def _norm_kw(c):
+    r, n, el, p, ck, aff = c
+    return dict(rows=r, cols=n, elem=el, params=p, ckpt=ck, affine=aff)
+
+
+def norm_rank3():
+    """[2, 3, 64]: the leading dims are the rows."""
+    return g.layer_norm(6, 64, ckpt="e4m3").replace("<6x64x", "<2x3x64x").replace("<6xf32>", "<2x3xf32>").replace("<6x2xui8>", "<2x3x2xui8>")
+
+
+def norm_grad_rank3():
+    return g.layer_norm_grad(6, 64).replace("<6x64x", "<2x3x64x").replace("<6xf32>", "<2x3xf32>")
+
+
+def entries():
+    e = {}
+    for c in QUANT:
+        r, n, el, fmt, ax = c
+        e[quant_name(c)] = g.quantize_mx(r, n, src=el, fmt=fmt, axis=ax)
+        e[quant_name(c, "dequant")] = g.dequantize_mx(r, n, dst=el, fmt=fmt, axis=ax)
+    for c in NORM:
+        e[norm_name(c)] = g.layer_norm(**_norm_kw(c))
+        e[norm_name(c, "lngrad")] = g.layer_norm_grad(**_norm_kw(c))
+    for m, n, k, fmt, bias, out in LINEAR:
+        e[linear_name((m, n, k, fmt, bias, out))] = g.linear_mx(m, n, k, fmt=fmt, bias=bias, out=out)
+    e["ln_rank3"], e["lngrad_rank3"] = norm_rank3(), norm_grad_rank3()
+    rt = lambda ir: g.with_dynamic_rows(ir, _ANY)  # noqa: E731
+    e["quantmx_e4m3_rt"] = rt(g.quantize_mx(_ANY, 100))
+    e["quantmx_e2m1_rt"] = rt(g.quantize_mx(_ANY, 4096, fmt="e2m1"))
+    e["dequantmx_e2m1_rt"] = rt(g.dequantize_mx(_ANY, 4096, fmt="e2m1"))
+    e["ln_rt"] = rt(g.layer_norm(_ANY, 1000, ckpt="e4m3"))
+    e["lngrad_rt"] = rt(g.layer_norm_grad(_ANY, 1000, ckpt="e4m3", params="f32"))
+    e["lngrad_wide_rt"] = rt(g.layer_norm_grad(_ANY, 4096))
+    e["linmx_e2m1_rt"] = rt(g.linear_mx(_ANY, 130, 544, bias=True))
+    e["linmx_e4m3_rt"] = rt(g.linear_mx(_ANY, 1040, 1024, fmt="e4m3"))
+    # the norm, the quantisation of its result and the block-scaled product
+    e["prog_norm_matmul_mx"] = g.layer_norm_matmul_mx(100, 208, 384)
+    e["prog_norm_linear_mx"] = g.layer_norm_linear_mx(20, 208, 384)
+    return e
