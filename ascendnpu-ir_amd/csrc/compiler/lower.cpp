@@ -3161,7 +3161,7 @@ static KernelPlan lowerMxCodes(Analysis &A, const std::string &kname, const Op *
     int64_t R, per;
     const std::string rows = leadRows(A, op, sh, R, per);
     call = std::string("hf::mx_") + (de ? "de" : "") + "quantize_rows<" + el + ", " + std::to_string(fmt) + ", " + std::to_string(sh.back()) + "ll>(";
-    rowGrid(A, p, R, per, ssh.back() * 4, threads, 65536);
+    rowGrid(A, p, R, per, ssh.back() * (x->type.elem == Elem::F32 ? 8 : 4), threads, 65536);
     call += in(0) + ", " + (de ? in(1) + ", " + outPtr[0] : outPtr[0] + ", " + outPtr[1]) + ", " + rows;
   }
   if (cols) call += in(0) + ", " + (de ? in(1) + ", " + outPtr[0] : outPtr[0] + ", " + outPtr[1]);
@@ -3175,15 +3175,30 @@ static KernelPlan lowerMxCodes(Analysis &A, const std::string &kname, const Op *
 // Layer norm and its gradient.  Threads of a row group, chunks of eight
 // elements a thread and row groups a workgroup by the row's length.
 struct LnShape { int64_t T, NCH, RPB; };
-static LnShape lnForwardShape(int64_t D) {
-  if (D <= 1024) return {64, (D + 511) / 512, 4};
-  const int64_t T = std::min<int64_t>(1024, (D + 1023) / 1024 * 64);
-  return {T, (D + 8 * T - 1) / (8 * T), 1};
+// D elements of a row, V to a 16-byte access.  us, bf16 with an 8-bit
+// checkpoint: [8192, 4096] 31.9 with 256 threads of two accesses a row, 33.4
+// with 512 of one, 30.8 with 128 of four, which cost [16, 4096] 4.0 instead of
+// 3.5; [2048, 16384] 30.7 with 512 threads of four, 34.6 with 1024 of two
+// (f32 rows are twice the bytes).  A row of at most 16 accesses has 8 or 16
+// lanes of a wave.
+static LnShape lnForwardShape(int64_t D, int64_t V) {
+  const int64_t acc = (D + V - 1) / V;
+  if (acc <= 16) return {acc <= 8 ? 8 : 16, 1, acc <= 8 ? 32 : 16};
+  const int64_t most = V == 4 || acc > 1024 ? 4 : 2;
+  const int64_t T = (acc + 64 * most - 1) / (64 * most) * 64;
+  return {T, (acc + T - 1) / T, std::max<int64_t>(1, 256 / T)};
 }
-static LnShape lnGradShape(int64_t D) {
-  if (D <= 512) return {64, 1, 4};
-  const int64_t T = std::min<int64_t>(1024, (D + 511) / 512 * 64);
-  return {T, (D + 8 * T - 1) / (8 * T), 1};
+// The gradient: workgroups of 512 threads, one a CU, so that few rows of
+// partial sums are left.  us, [8192, 4096] from an 8-bit checkpoint: 31.8 with
+// two row groups of 256 threads and two accesses, 39.3 of 512 and one (1024
+// threads a workgroup), 68.7 with four row groups of 256; 35.5 with 512
+// workgroups (16.8 MB of partial sums instead of 8.4).  [2048, 16384]: 39.8
+// with 1024 threads of two accesses, 47.7 with 512 of four.
+static LnShape lnGradShape(int64_t D, int64_t V) {
+  const int64_t acc = (D + V - 1) / V;
+  if (acc <= 16) return {acc <= 8 ? 8 : 16, 1, acc <= 8 ? 32 : 16};
+  const int64_t T = std::min<int64_t>(1024, (acc + 127) / 128 * 64);
+  return {T, (acc + T - 1) / T, std::max<int64_t>(1, 512 / T)};
 }
 
 static KernelPlan lowerLayerNorm(Analysis &A, const std::string &kname, const Op *op, const std::vector<std::string> &outPtr) {
@@ -3230,7 +3245,8 @@ static KernelPlan lowerLayerNorm(Analysis &A, const std::string &kname, const Op
   KernelPlan p;
   p.kernelName = kname;
   std::ostringstream k;
-  const LnShape s = grad ? lnGradShape(D) : lnForwardShape(D);
+  const int64_t V = y->type.elem == Elem::F32 ? 4 : 8;
+  const LnShape s = grad ? lnGradShape(D, V) : lnForwardShape(D, V);
   const int64_t threads = s.T * s.RPB;
   auto targs = [&](const std::string &pel) {
     return "<" + el + ", " + pel + ", " + std::to_string(aff) + ", " + std::to_string(ck) + ", " + std::to_string(s.T) + ", " +
@@ -3255,7 +3271,7 @@ static KernelPlan lowerLayerNorm(Analysis &A, const std::string &kname, const Op
       << "  hf::ln_forward" << targs(param ? mxElem(op, param) : el) << in(0) << ", " << (aff > 0 ? in(1) : "nullptr") << ", "
       << (aff > 1 ? in(2) : "nullptr") << ", " << outPtr[0] << ", (float *)" << outPtr[1] << ", (float *)" << outPtr[2] << ", "
       << (ck >= 0 ? outPtr[3] + ", " + outPtr[4] : "nullptr, nullptr") << ", " << rows << ", " << floatLit(eps) << ");\n}\n";
-    rowGrid(A, p, R, per, 1, s.RPB, 256 * std::max<int64_t>(1, 2048 / threads));
+    rowGrid(A, p, R, per, 1, s.RPB, 256 * std::max<int64_t>(1, 1024 / threads));
     p.source = k.str();
     return p;
   }
@@ -3273,8 +3289,8 @@ static KernelPlan lowerLayerNorm(Analysis &A, const std::string &kname, const Op
   stat(op->ins[at + 1]);
   for (size_t i = 1; i <= aff; ++i) affine(op->results[i]);
   p.kind = "LAYER_NORM_GRAD";
-  // row groups that walk the rows, each leaving one row of partial sums
-  const int64_t cap = 512, groups = cap * s.RPB;
+  // workgroups that walk the rows, each leaving one row of partial sums
+  const int64_t cap = 256;
   const std::string call = "  hf::ln_grad_rows" + targs(param ? mxElem(op, param) : el);
   // the row kernel's arguments by name: dy x scales gamma mean rstd dx ws
   auto body = [&](const std::vector<std::string> &a) {
@@ -3291,23 +3307,21 @@ static KernelPlan lowerLayerNorm(Analysis &A, const std::string &kname, const Op
   }
   KernelPlan::PreKernel pk;
   pk.name = kname + "_rows";
-  std::vector<std::string> none;
   const std::string params = kernelParamList(A, pk.kargs, true);
   pk.grid = (unsigned)(A.rowsDyn ? cap : std::max<int64_t>(1, std::min<int64_t>(cap, (R + s.RPB - 1) / s.RPB)));
   pk.block = (unsigned)threads;
   k << "extern \"C\" __global__ __launch_bounds__(" << threads << ") void " << pk.name << "(" << params << ") {\n"
     << body({in(0), in(1), scl, gam, in(at), in(at + 1), outPtr[0], "ws"});
   p.pre.push_back(pk);
-  const int64_t used = pk.grid * s.RPB; // row groups of a full launch
   k << "extern \"C\" __global__ __launch_bounds__(1024) void " << kname << "(" << kernelParamList(A, p.kargs, true) << ") {\n"
-    << "  const int64_t R = " << rows << ";\n"
-    << "  hf::ln_grad_columns<" << mxElem(op, param) << ", " << aff << ", 16, " << D << "ll>((const float *)ws, R < " << used << "ll ? R : "
-    << used << "ll, " << outPtr[1] << ", " << (aff > 1 ? outPtr[2] : "nullptr") << ");\n}\n";
-  p.grid[0] = (unsigned)(((int64_t)aff * D + 63) / 64);
+    << "  const int64_t P = (" << rows << " + " << s.RPB - 1 << ") / " << s.RPB << ";\n"
+    << "  hf::ln_grad_columns<" << mxElem(op, param) << ", " << aff << ", " << D << "ll>((const float *)ws, P < " << pk.grid << " ? P : "
+    << pk.grid << ", " << outPtr[1] << ", " << (aff > 1 ? outPtr[2] : "nullptr") << ");\n}\n";
+  p.grid[0] = (unsigned)(((int64_t)aff * D + 31) / 32);
   p.block[0] = 1024;
   p.rowsDyn = A.rowsDyn;
   p.rowsZero = A.rowsDyn; // no rows: the weight's gradients are zeros
-  p.workspaceBytes = (uint64_t)std::min<int64_t>(groups, used) * aff * D * 4;
+  p.workspaceBytes = (uint64_t)pk.grid * aff * D * 4;
   p.source = k.str();
   return p;
 }

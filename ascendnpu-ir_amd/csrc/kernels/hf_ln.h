@@ -10,33 +10,41 @@
 // An 8-bit checkpoint of x (hf_mx.h's codes along the row) is written by the
 // forward pass and read by the gradient in place of x.
 //
-// A row group of T threads owns a row, NCH chunks of eight consecutive
-// elements a thread (chunk j at column (j T + thread) * 8, so a group's
-// accesses are consecutive and four neighbouring lanes hold a block of 32).
+// A row group of T threads owns a row, NCH 16-byte accesses a thread (access
+// j at column (j T + thread) * V, so a group's accesses are consecutive and
+// neighbouring lanes hold a block of 32).  RPB row groups share a workgroup
+// and take their rows in step; a row is loaded while the one before it is
+// worked on.
 #pragma once
 #include "hf_mx.h"
 
 namespace hf {
 
-// Sum over a wave: 16 lanes by DPP, then the four rows of lanes in order.
-__device__ __forceinline__ float wave_sum(float v) {
+typedef float v4f_ln __attribute__((ext_vector_type(4)));
+
+// Sums over the lanes of a row group, or of the wave where a row has more:
+// up to 16 lanes by DPP, then the four rows of lanes in order.
+template <int T> __device__ __forceinline__ float lane_sum(float v) {
   auto dpp = [](float a, auto ctrl) {
     return u2f((uint32_t)__builtin_amdgcn_update_dpp(0, (int)f2u(a), decltype(ctrl)::value, 0xF, 0xF, true));
   };
   v += dpp(v, std::integral_constant<int, 0xB1>{});  // quad 1 0 3 2
   v += dpp(v, std::integral_constant<int, 0x4E>{});  // quad 2 3 0 1
-  v += dpp(v, std::integral_constant<int, 0x141>{}); // mirrored half row
-  v += dpp(v, std::integral_constant<int, 0x140>{}); // mirrored row
+  v += dpp(v, std::integral_constant<int, 0x141>{}); // eight lanes mirrored
+  if constexpr (T == 8) return v;
+  v += dpp(v, std::integral_constant<int, 0x140>{}); // sixteen lanes mirrored
+  if constexpr (T == 16) return v;
   auto lane = [&](int l) { return u2f((uint32_t)__builtin_amdgcn_readlane((int)f2u(v), l)); };
   return (lane(0) + lane(16)) + (lane(32) + lane(48));
 }
 
-// Sums of N values over the row group; slots: N * T / 64 floats of the group.
+// Sums of N values over each row group; slots: N * T / 64 floats a group.
 template <int T, int N> __device__ __forceinline__ void group_sum(float (&v)[N], float *slots) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = wave_sum(v[i]);
+  for (int i = 0; i < N; ++i) v[i] = lane_sum<T>(v[i]);
   if constexpr (T > 64) {
     constexpr int W = T / 64;
+    slots += threadIdx.x / T * (N * W);
     const int wave = (threadIdx.x % T) / 64;
     if (threadIdx.x % 64 == 0)
 #pragma unroll
@@ -52,210 +60,280 @@ template <int T, int N> __device__ __forceinline__ void group_sum(float (&v)[N],
   }
 }
 
-// valid elements of the chunk at column c
-template <int64_t D> __device__ __forceinline__ int ln_count(int64_t c) {
-  return (int)(D - c <= 0 ? 0 : D - c < 8 ? D - c : 8);
-}
-template <int EL, bool FULL> __device__ __forceinline__ Oct<EL> ln_load(const void *base, int64_t e, int n) {
-  const char *p = (const char *)base + e * el_bytes<EL>;
-  if (FULL || n == 8) return oct_load<EL>(p);
-  return oct_load_part<EL>(p, n);
+// Weight and bias of a thread's columns: V values of type PEL as they lie.
+template <int PEL, int V> struct LnParam {
+  uint32_t w[V * el_bytes<PEL> / 4];
+  __device__ __forceinline__ float get(int i) const { return word_get<PEL>(w, i); }
+  __device__ __forceinline__ void load(const void *base, int64_t c, int n) {
+    const char *p = (const char *)base + c * el_bytes<PEL>;
+#pragma unroll
+    for (int i = 0; i < V * el_bytes<PEL> / 4; ++i) w[i] = 0;
+    if (n == V) {
+#pragma unroll
+      for (int i = 0; i < V * el_bytes<PEL> / 16; ++i) {
+        const u32x4 v = reinterpret_cast<const u32x4_any *>(p)[i];
+        w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        if (i >= n) break;
+        if constexpr (PEL == EL_F32) w[i] = reinterpret_cast<const uint32_t *>(p)[i];
+        else w[i / 2] |= (uint32_t)reinterpret_cast<const uint16_t *>(p)[i] << (16 * (i % 2));
+      }
+    }
+  }
+};
+
+// valid elements of the access at column c
+template <int64_t D, int V, bool FULL> __device__ __forceinline__ int ln_count(int64_t c, bool ok) {
+  if (!ok) return 0;
+  return FULL ? V : (int)(D - c <= 0 ? 0 : D - c < V ? D - c : V);
 }
 
 // AFF: 0 neither weight nor bias, 1 gamma, 2 gamma and beta (of type PEL).
-// CK: format of the checkpoint, -1 for none.  RPB row groups a workgroup.
-// mean and rstd may be null.
+// CK: format of the checkpoint, -1 for none.  mean and rstd may be null.
 template <int EL, int PEL, int AFF, int CK, int T, int NCH, int RPB, int64_t D>
 __device__ __forceinline__ void ln_forward(const void *__restrict__ x, const void *__restrict__ gamma, const void *__restrict__ beta,
                                            void *__restrict__ y, float *__restrict__ mean, float *__restrict__ rstd,
                                            void *__restrict__ codes, void *__restrict__ scales, int64_t R, float eps) {
-  static_assert((int64_t)T * NCH * 8 >= D && (T == 64 || RPB == 1));
-  constexpr bool FULL = (int64_t)T * NCH * 8 == D;
+  constexpr int V = mx_vals<EL>, W = T > 64 ? T / 64 : 1;
+  static_assert((int64_t)T * NCH * V >= D);
+  constexpr bool FULL = (int64_t)T * NCH * V == D;
   constexpr int64_t NB = (D + 31) / 32;
-  __shared__ float slots[2][T / 64];
+  __shared__ float slots[2][RPB * W];
   const int lt = threadIdx.x % T, group = threadIdx.x / T;
-  Oct<PEL> gm[NCH], bt[NCH];
+  auto col = [&](int j) { return ((int64_t)j * T + lt) * V; };
+  LnParam<PEL, V> gm[NCH], bt[NCH];
 #pragma unroll
   for (int j = 0; j < NCH; ++j) {
-    const int64_t c = ((int64_t)j * T + lt) * 8;
-    if constexpr (AFF >= 1) gm[j] = ln_load<PEL, FULL>(gamma, c, ln_count<D>(c));
-    if constexpr (AFF >= 2) bt[j] = ln_load<PEL, FULL>(beta, c, ln_count<D>(c));
+    const int n = ln_count<D, V, FULL>(col(j), true);
+    if constexpr (AFF >= 1) gm[j].load(gamma, col(j), n);
+    if constexpr (AFF >= 2) bt[j].load(beta, col(j), n);
   }
-  for (int64_t row = (int64_t)blockIdx.x * RPB + group; row < R; row += (int64_t)gridDim.x * RPB) {
-    Oct<EL> v[NCH];
-    float s[1] = {0}, q[1] = {0};
+  auto load = [&](int64_t row, Pack<EL> (&v)[NCH]) {
 #pragma unroll
     for (int j = 0; j < NCH; ++j) {
-      const int64_t c = ((int64_t)j * T + lt) * 8;
-      v[j] = ln_load<EL, FULL>(x, row * D + c, ln_count<D>(c));
+      const int n = ln_count<D, V, FULL>(col(j), row < R);
+      const char *p = (const char *)x + (row * D + col(j)) * el_bytes<EL>;
+      v[j] = n == V ? pack_load<EL>(p) : pack_load_part<EL>(p, FULL ? 0 : n);
     }
+  };
+  const int64_t step = (int64_t)gridDim.x * RPB;
+  Pack<EL> v[NCH], next[NCH];
+  load((int64_t)blockIdx.x * RPB + group, v);
+  for (int64_t row0 = (int64_t)blockIdx.x * RPB; row0 < R; row0 += step) {
+    const int64_t row = row0 + group;
+    if (row0 + step < R) load(row + step, next);
+    float s[1] = {0}, q[1] = {0};
 #pragma unroll
     for (int j = 0; j < NCH; ++j)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s[0] += oct_get<EL>(v[j], i);
+      for (int i = 0; i < V; ++i) s[0] += pack_get<EL>(v[j], i);
     group_sum<T>(s, slots[0]);
     const float mu = s[0] / (float)D;
 #pragma unroll
     for (int j = 0; j < NCH; ++j) {
-      const int n = FULL ? 8 : ln_count<D>(((int64_t)j * T + lt) * 8);
+      const int n = ln_count<D, V, FULL>(col(j), true);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float d = oct_get<EL>(v[j], i) - mu;
+      for (int i = 0; i < V; ++i) {
+        const float d = pack_get<EL>(v[j], i) - mu;
         if (FULL || i < n) q[0] = __builtin_fmaf(d, d, q[0]);
       }
     }
     group_sum<T>(q, slots[1]);
     const float r = 1.0f / __builtin_sqrtf(q[0] / (float)D + eps);
-    if (lt == 0) {
+    if (lt == 0 && row < R) {
       if (mean) mean[row] = mu;
       if (rstd) rstd[row] = r;
     }
 #pragma unroll
     for (int j = 0; j < NCH; ++j) {
-      const int64_t c = ((int64_t)j * T + lt) * 8;
-      const int n = FULL ? 8 : ln_count<D>(c);
-      Oct<EL> o{};
+      const int n = ln_count<D, V, FULL>(col(j), row < R);
+      Pack<EL> o{};
 #pragma unroll
-      for (int i = 0; i < 8; i += 2) {
+      for (int i = 0; i < V; i += 2) {
         float a[2];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          a[k] = (oct_get<EL>(v[j], i + k) - mu) * r;
-          if constexpr (AFF == 1) a[k] *= oct_get<PEL>(gm[j], i + k);
-          if constexpr (AFF == 2) a[k] = __builtin_fmaf(a[k], oct_get<PEL>(gm[j], i + k), oct_get<PEL>(bt[j], i + k));
+          a[k] = (pack_get<EL>(v[j], i + k) - mu) * r;
+          if constexpr (AFF == 1) a[k] *= gm[j].get(i + k);
+          if constexpr (AFF == 2) a[k] = __builtin_fmaf(a[k], gm[j].get(i + k), bt[j].get(i + k));
         }
-        oct_set2<EL>(o, i, a[0], a[1]);
+        pack_set2<EL>(o, i, a[0], a[1]);
       }
-      char *dst = (char *)y + (row * D + c) * el_bytes<EL>;
-      if (FULL || n == 8) oct_store<EL>(dst, o);
-      else oct_store_part<EL>(dst, o, n);
+      char *dst = (char *)y + (row * D + col(j)) * el_bytes<EL>;
+      if (n == V) pack_store<EL>(dst, o);
+      else if (!FULL) pack_store_part<EL>(dst, o, n);
       if constexpr (CK >= 0) {
         // (zeros behind the row's end do not change a block's maximum)
-        const uint32_t byte = mx_scale_byte<CK>(quad_max(oct_amax<EL>(v[j])));
+        const uint32_t byte = mx_scale_byte<CK>(block_max<EL>(pack_amax<EL>(v[j])));
         const u32x2 w = mx_encode<EL, CK>(v[j], mx_inverse(byte), byte != 255);
-        uint8_t *cd = (uint8_t *)codes + row * D + c;
-        if (FULL || n == 8) codes_store<CK>(cd, w);
-        else codes_store_part<CK>(cd, w, n);
-        if ((lt & 3) == 0 && (FULL || n > 0)) ((uint8_t *)scales)[row * NB + c / 32] = (uint8_t)byte;
+        uint8_t *cd = (uint8_t *)codes + row * D + col(j);
+        if (n == V) codes_store<EL, CK>(cd, w);
+        else if (!FULL) codes_store_part<EL, CK>(cd, w, n);
+        if (lt % mx_lanes<EL> == 0 && n > 0) ((uint8_t *)scales)[row * NB + col(j) / 32] = (uint8_t)byte;
       }
     }
+#pragma unroll
+    for (int j = 0; j < NCH; ++j) v[j] = next[j];
   }
 }
 
 // Row groups walk the rows with a stride and keep their columns' part of
-// dgamma and dbeta in registers; each leaves one row of part [2][D] behind
-// (ln_grad_columns adds them in order).
+// dgamma and dbeta in registers; the groups of a workgroup add theirs in LDS
+// and leave one row of part [AFF][D] behind (ln_grad_columns adds those).
 template <int EL, int PEL, int AFF, int CK, int T, int NCH, int RPB, int64_t D>
 __device__ __forceinline__ void ln_grad_rows(const void *__restrict__ dy, const void *__restrict__ x, const void *__restrict__ scales,
                                              const void *__restrict__ gamma, const float *__restrict__ mean,
                                              const float *__restrict__ rstd, void *__restrict__ dx, float *__restrict__ part, int64_t R) {
-  static_assert((int64_t)T * NCH * 8 >= D && (T == 64 || RPB == 1));
-  constexpr bool FULL = (int64_t)T * NCH * 8 == D;
+  constexpr int V = mx_vals<EL>, W = T > 64 ? T / 64 : 1;
+  static_assert((int64_t)T * NCH * V >= D);
+  constexpr bool FULL = (int64_t)T * NCH * V == D;
   constexpr int64_t NB = (D + 31) / 32;
-  __shared__ float slots[2][2 * (T / 64)];
+  constexpr int CAP = T * NCH * V; // columns of a row group
+  // (a workgroup of 1024 threads has no registers for the next row of the widest f32 rows)
+  constexpr bool AHEAD = T * RPB < 1024 || NCH <= 2;
+  __shared__ float slots[2][RPB * 2 * W];
+  __shared__ __attribute__((aligned(16))) float sums[AFF >= 1 && RPB > 1 ? RPB * CAP : 4];
   const int lt = threadIdx.x % T, group = threadIdx.x / T;
-  Oct<PEL> gm[NCH];
-  float dg[NCH][8], db[NCH][8];
+  auto col = [&](int j) { return ((int64_t)j * T + lt) * V; };
+  LnParam<PEL, V> gm[NCH];
+  float dg[NCH][V], db[NCH][V];
 #pragma unroll
   for (int j = 0; j < NCH; ++j) {
-    const int64_t c = ((int64_t)j * T + lt) * 8;
-    if constexpr (AFF >= 1) gm[j] = ln_load<PEL, FULL>(gamma, c, ln_count<D>(c));
+    if constexpr (AFF >= 1) gm[j].load(gamma, col(j), ln_count<D, V, FULL>(col(j), true));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) dg[j][i] = db[j][i] = 0;
+    for (int i = 0; i < V; ++i) dg[j][i] = db[j][i] = 0;
   }
-  const int64_t first = (int64_t)blockIdx.x * RPB + group, stride = (int64_t)gridDim.x * RPB;
-  int parity = 0;
-  for (int64_t row = first; row < R; row += stride) {
-    Oct<EL> vd[NCH];
-    float xv[NCH][8];
-    const float mu = mean[row], r = rstd[row];
+  struct Row {
+    Pack<EL> d[NCH], x[NCH];
+    u32x2 code[NCH];
+    uint32_t byte[NCH];
+    float mu, r;
+  };
+  auto load = [&](int64_t row, Row &v) {
+    v.mu = v.r = 0;
+    if (row < R) v.mu = mean[row], v.r = rstd[row];
 #pragma unroll
     for (int j = 0; j < NCH; ++j) {
-      const int64_t c = ((int64_t)j * T + lt) * 8;
-      const int n = ln_count<D>(c);
-      vd[j] = ln_load<EL, FULL>(dy, row * D + c, n);
+      const int n = ln_count<D, V, FULL>(col(j), row < R);
+      const int64_t e = row * D + col(j);
+      const char *p = (const char *)dy + e * el_bytes<EL>;
+      v.d[j] = n == V ? pack_load<EL>(p) : pack_load_part<EL>(p, FULL ? 0 : n);
       if constexpr (CK >= 0) {
-        const uint8_t *p = (const uint8_t *)x + row * D + c;
-        const u32x2 w = FULL || n == 8 ? codes_load<CK>(p) : codes_load_part<CK>(p, n);
-        const uint32_t byte = FULL || n > 0 ? ((const uint8_t *)scales)[row * NB + c / 32] : 0;
-        mx_decode<CK>(w, mx_scale(byte), xv[j]);
+        const uint8_t *q = (const uint8_t *)x + e;
+        v.code[j] = n == V ? codes_load<EL, CK>(q) : codes_load_part<EL, CK>(q, FULL ? 0 : n);
+        v.byte[j] = n > 0 ? ((const uint8_t *)scales)[row * NB + col(j) / 32] : 0;
       } else {
-        const Oct<EL> o = ln_load<EL, FULL>(x, row * D + c, n);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) xv[j][i] = oct_get<EL>(o, i);
+        const char *q = (const char *)x + e * el_bytes<EL>;
+        v.x[j] = n == V ? pack_load<EL>(q) : pack_load_part<EL>(q, FULL ? 0 : n);
       }
     }
-    float s[2] = {0, 0};
+  };
+  const int64_t step = (int64_t)gridDim.x * RPB;
+  Row cur, next;
+  int parity = 0;
+  load((int64_t)blockIdx.x * RPB + group, cur);
+  for (int64_t row0 = (int64_t)blockIdx.x * RPB; row0 < R; row0 += step) {
+    const int64_t row = row0 + group;
+    if (AHEAD && row0 + step < R) load(row + step, next);
+    float xh[NCH][V], s[2] = {0, 0};
 #pragma unroll
-    for (int j = 0; j < NCH; ++j)
+    for (int j = 0; j < NCH; ++j) {
+      if constexpr (CK >= 0) mx_decode<EL, CK>(cur.code[j], mx_scale(cur.byte[j]), xh[j]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float d = oct_get<EL>(vd[j], i), xh = (xv[j][i] - mu) * r;
-        const float g = AFF >= 1 ? d * oct_get<PEL>(gm[j], i) : d;
-        // (behind the row's end dy and gamma are zeros)
+      for (int i = 0; i < V; ++i) {
+        const float d = pack_get<EL>(cur.d[j], i);
+        xh[j][i] = ((CK >= 0 ? xh[j][i] : pack_get<EL>(cur.x[j], i)) - cur.mu) * cur.r;
+        const float g = AFF >= 1 ? d * gm[j].get(i) : d;
+        // (behind the row's end, and in rows past the last, dy is zero)
         s[0] += g;
-        s[1] = __builtin_fmaf(g, xh, s[1]);
-        xv[j][i] = xh;
-        dg[j][i] = __builtin_fmaf(d, xh, dg[j][i]);
+        s[1] = __builtin_fmaf(g, xh[j][i], s[1]);
+        dg[j][i] = __builtin_fmaf(d, xh[j][i], dg[j][i]);
         db[j][i] += d;
       }
+    }
     group_sum<T>(s, slots[parity]);
     parity ^= 1;
     const float m0 = s[0] / (float)D, m1 = s[1] / (float)D;
 #pragma unroll
     for (int j = 0; j < NCH; ++j) {
-      const int64_t c = ((int64_t)j * T + lt) * 8;
-      const int n = FULL ? 8 : ln_count<D>(c);
-      Oct<EL> o{};
+      const int n = ln_count<D, V, FULL>(col(j), row < R);
+      Pack<EL> o{};
 #pragma unroll
-      for (int i = 0; i < 8; i += 2) {
+      for (int i = 0; i < V; i += 2) {
         float a[2];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const float d = oct_get<EL>(vd[j], i + k);
-          const float g = AFF >= 1 ? d * oct_get<PEL>(gm[j], i + k) : d;
-          a[k] = r * ((g - m0) - xv[j][i + k] * m1);
+          const float d = pack_get<EL>(cur.d[j], i + k);
+          const float g = AFF >= 1 ? d * gm[j].get(i + k) : d;
+          a[k] = cur.r * ((g - m0) - xh[j][i + k] * m1);
         }
-        oct_set2<EL>(o, i, a[0], a[1]);
+        pack_set2<EL>(o, i, a[0], a[1]);
       }
-      char *dst = (char *)dx + (row * D + c) * el_bytes<EL>;
-      if (FULL || n == 8) oct_store<EL>(dst, o);
-      else oct_store_part<EL>(dst, o, n);
+      char *dst = (char *)dx + (row * D + col(j)) * el_bytes<EL>;
+      if (n == V) pack_store<EL>(dst, o);
+      else if (!FULL) pack_store_part<EL>(dst, o, n);
     }
+    if constexpr (AHEAD) cur = next;
+    else if (row0 + step < R) load(row + step, cur);
   }
   if constexpr (AFF >= 1) {
-    if (first >= R) return; // (only the first min(groups, R) rows of `part` are read)
-    float *p = part + first * (AFF * D);
+    if ((int64_t)blockIdx.x * RPB >= R) return; // (its row of `part` is not read)
+    float *p = part + (int64_t)blockIdx.x * (AFF * D);
 #pragma unroll
-    for (int j = 0; j < NCH; ++j) {
-      const int64_t c = ((int64_t)j * T + lt) * 8;
-      const int n = FULL ? 8 : ln_count<D>(c);
+    for (int a = 0; a < AFF; ++a) {
+      float(&mine)[NCH][V] = a == 0 ? dg : db;
+      if constexpr (RPB == 1) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (i >= n) break;
-        p[c + i] = dg[j][i];
-        if constexpr (AFF >= 2) p[D + c + i] = db[j][i];
+        for (int j = 0; j < NCH; ++j) {
+          const int n = ln_count<D, V, FULL>(col(j), true);
+#pragma unroll
+          for (int i = 0; i < V; ++i)
+            if (FULL || i < n) p[a * D + col(j) + i] = mine[j][i];
+        }
+      } else {
+        if (a > 0) __syncthreads();
+#pragma unroll
+        for (int j = 0; j < NCH; ++j)
+#pragma unroll
+          for (int i = 0; i < V; i += 4)
+            *reinterpret_cast<v4f_ln *>(&sums[group * CAP + col(j) + i]) = v4f_ln{mine[j][i], mine[j][i + 1], mine[j][i + 2], mine[j][i + 3]};
+        __syncthreads();
+        for (int c = threadIdx.x; c < (int)D; c += T * RPB) {
+          float t = sums[c];
+#pragma unroll
+          for (int k = 1; k < RPB; ++k) t += sums[k * CAP + c];
+          p[a * D + c] = t;
+        }
       }
     }
   }
 }
 
-// dgamma and dbeta: column c of part [P][AFF D] summed over its rows, 64
-// columns a workgroup, the rows dealt to SL slices of threads.
-template <int PEL, int AFF, int SL, int64_t D>
+// dgamma and dbeta: column c of part [P][AFF D], P at most LNC_ROWS, summed
+// over its rows: 32 columns a workgroup, the rows dealt to 32 slices of
+// threads, whose loads are all in flight at once.
+constexpr int LNC_COLS = 32, LNC_SLICES = 32, LNC_ROWS = 256;
+template <int PEL, int AFF, int64_t D>
 __device__ __forceinline__ void ln_grad_columns(const float *__restrict__ part, int64_t P, void *__restrict__ dgamma, void *__restrict__ dbeta) {
-  __shared__ float s[SL][64];
-  const int lane = threadIdx.x % 64, sl = threadIdx.x / 64;
-  const int64_t c = (int64_t)blockIdx.x * 64 + lane;
-  float a = 0;
-  if (c < AFF * D)
-#pragma unroll 8
-    for (int64_t p = sl; p < P; p += SL) a += part[p * (AFF * D) + c];
+  __shared__ float s[LNC_SLICES][LNC_COLS + 1];
+  const int lane = threadIdx.x % LNC_COLS, sl = threadIdx.x / LNC_COLS;
+  const int64_t c = (int64_t)blockIdx.x * LNC_COLS + lane;
+  float v[LNC_ROWS / LNC_SLICES], a = 0;
+#pragma unroll
+  for (int i = 0; i < LNC_ROWS / LNC_SLICES; ++i) {
+    const int64_t p = sl + i * LNC_SLICES;
+    v[i] = p < P && c < AFF * D ? part[p * (AFF * D) + c] : 0.0f;
+  }
+#pragma unroll
+  for (int i = 0; i < LNC_ROWS / LNC_SLICES; ++i) a += v[i];
   s[sl][lane] = a;
   __syncthreads();
   if (sl != 0 || c >= AFF * D) return;
 #pragma unroll
-  for (int i = 1; i < SL; ++i) a += s[i][lane];
+  for (int i = 1; i < LNC_SLICES; ++i) a += s[i][lane];
   void *out = c < D ? dgamma : dbeta;
   const int64_t i = c < D ? c : c - D;
   if constexpr (PEL == EL_F32) ((float *)out)[i] = a;

@@ -25,61 +25,55 @@ enum MxFormat : int { MX_E4M3 = 0, MX_E5M2 = 1, MX_E2M1 = 4 };
 template <int EL> constexpr int el_bytes = EL == EL_F32 ? 4 : 2;
 template <int FMT> constexpr int mx_emax = FMT == MX_E4M3 ? 8 : FMT == MX_E5M2 ? 15 : 2;
 template <int FMT> constexpr float mx_top = FMT == MX_E4M3 ? 448.0f : FMT == MX_E5M2 ? 57344.0f : 6.0f;
-// bytes of eight codes
-template <int FMT> constexpr int mx_oct = FMT == MX_E2M1 ? 4 : 8;
+// values of one 16-byte access, lanes that share a block of 32, bytes of the
+// codes of one access
+template <int EL> constexpr int mx_vals = 16 / el_bytes<EL>;
+template <int EL> constexpr int mx_lanes = 32 / mx_vals<EL>;
+template <int EL, int FMT> constexpr int mx_bytes = FMT == MX_E2M1 ? mx_vals<EL> / 2 : mx_vals<EL>;
 
-// ---------------------------------------------------------------- eight values
-template <int EL> struct Oct { uint32_t w[2 * el_bytes<EL>]; };
+// ---------------------------------------------------------------- 16 bytes of values
+template <int EL> struct Pack { uint32_t w[4]; };
 
-// (16-byte accesses at any element: rows of odd lengths start anywhere)
+// (accesses at any element: rows of odd lengths start anywhere)
 typedef u32x4 u32x4_any __attribute__((aligned(1)));
 typedef u32x2 u32x2_any __attribute__((aligned(1)));
 typedef uint32_t u32_any __attribute__((aligned(1)));
+typedef uint16_t u16_any __attribute__((aligned(1)));
 
-template <int EL> __device__ __forceinline__ Oct<EL> oct_load(const void *p) {
-  Oct<EL> o;
-  const u32x4_any *q = reinterpret_cast<const u32x4_any *>(p);
-#pragma unroll
-  for (int i = 0; i < el_bytes<EL> / 2; ++i) {
-    const u32x4 v = __builtin_nontemporal_load(q + i);
-    o.w[4 * i] = v.x, o.w[4 * i + 1] = v.y, o.w[4 * i + 2] = v.z, o.w[4 * i + 3] = v.w;
-  }
-  return o;
+template <int EL> __device__ __forceinline__ Pack<EL> pack_load(const void *p) {
+  const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any *>(p));
+  return Pack<EL>{{v.x, v.y, v.z, v.w}};
 }
-// the first n of eight values, zeros behind them
-template <int EL> __device__ __forceinline__ Oct<EL> oct_load_part(const void *p, int n) {
-  Oct<EL> o{};
+// the first n values, zeros behind them
+template <int EL> __device__ __forceinline__ Pack<EL> pack_load_part(const void *p, int n) {
+  Pack<EL> o{};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < mx_vals<EL>; ++i) {
     if (i >= n) break;
     if constexpr (EL == EL_F32) o.w[i] = reinterpret_cast<const uint32_t *>(p)[i];
     else o.w[i / 2] |= (uint32_t)reinterpret_cast<const uint16_t *>(p)[i] << (16 * (i % 2));
   }
   return o;
 }
-template <int EL> __device__ __forceinline__ void oct_store(void *p, const Oct<EL> &o) {
-  u32x4_any *q = reinterpret_cast<u32x4_any *>(p);
-#pragma unroll
-  for (int i = 0; i < el_bytes<EL> / 2; ++i) {
-    const u32x4 v = {o.w[4 * i], o.w[4 * i + 1], o.w[4 * i + 2], o.w[4 * i + 3]};
-    __builtin_nontemporal_store(v, q + i);
-  }
+template <int EL> __device__ __forceinline__ void pack_store(void *p, const Pack<EL> &o) {
+  __builtin_nontemporal_store(u32x4{o.w[0], o.w[1], o.w[2], o.w[3]}, reinterpret_cast<u32x4_any *>(p));
 }
-template <int EL> __device__ __forceinline__ void oct_store_part(void *p, const Oct<EL> &o, int n) {
+template <int EL> __device__ __forceinline__ void pack_store_part(void *p, const Pack<EL> &o, int n) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < mx_vals<EL>; ++i) {
     if (i >= n) break;
     if constexpr (EL == EL_F32) reinterpret_cast<uint32_t *>(p)[i] = o.w[i];
     else reinterpret_cast<uint16_t *>(p)[i] = (uint16_t)(o.w[i / 2] >> (16 * (i % 2)));
   }
 }
-template <int EL> __device__ __forceinline__ float oct_get(const Oct<EL> &o, int i) {
-  if constexpr (EL == EL_F32) return u2f(o.w[i]);
-  else if constexpr (EL == EL_BF16) return u2f(i % 2 ? o.w[i / 2] & 0xFFFF0000u : o.w[i / 2] << 16);
-  else return f16_to_f32((uint16_t)(o.w[i / 2] >> (16 * (i % 2))));
+template <int EL> __device__ __forceinline__ float word_get(const uint32_t *w, int i) {
+  if constexpr (EL == EL_F32) return u2f(w[i]);
+  else if constexpr (EL == EL_BF16) return u2f(i % 2 ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
+  else return f16_to_f32((uint16_t)(w[i / 2] >> (16 * (i % 2))));
 }
+template <int EL> __device__ __forceinline__ float pack_get(const Pack<EL> &o, int i) { return word_get<EL>(o.w, i); }
 // two neighbouring values rounded to nearest even
-template <int EL> __device__ __forceinline__ void oct_set2(Oct<EL> &o, int i, float a, float b) {
+template <int EL> __device__ __forceinline__ void pack_set2(Pack<EL> &o, int i, float a, float b) {
   if constexpr (EL == EL_F32) o.w[i] = f2u(a), o.w[i + 1] = f2u(b);
   else if constexpr (EL == EL_BF16) o.w[i / 2] = (uint32_t)f32_to_bf16_rne(a) | (uint32_t)f32_to_bf16_rne(b) << 16;
   else {
@@ -101,12 +95,12 @@ template <int EL> __device__ __forceinline__ uint32_t mag_f32(uint32_t half) {
   if constexpr (EL == EL_BF16) return half << 16;
   else return f2u(f16_to_f32((uint16_t)half));
 }
-// f32 bits of the largest of eight magnitudes
-template <int EL> __device__ __forceinline__ uint32_t oct_amax(const Oct<EL> &o) {
+// f32 bits of the largest magnitude of a pack
+template <int EL> __device__ __forceinline__ uint32_t pack_amax(const Pack<EL> &o) {
   if constexpr (EL == EL_F32) {
     uint32_t m = o.w[0] & 0x7FFFFFFFu;
 #pragma unroll
-    for (int i = 1; i < 8; ++i) m = max_u32(m, o.w[i] & 0x7FFFFFFFu);
+    for (int i = 1; i < 4; ++i) m = max_u32(m, o.w[i] & 0x7FFFFFFFu);
     return m;
   } else {
     uint32_t m = o.w[0] & 0x7FFF7FFFu;
@@ -115,10 +109,13 @@ template <int EL> __device__ __forceinline__ uint32_t oct_amax(const Oct<EL> &o)
     return mag_f32<EL>(max_u32(m & 0xFFFFu, m >> 16));
   }
 }
-// over the four lanes of a quad (they share a block)
-__device__ __forceinline__ uint32_t quad_max(uint32_t m) {
-  m = max_u32(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xF, 0xF, true));        // lanes 1 0 3 2
-  return max_u32(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xF, 0xF, true));     // lanes 2 3 0 1
+// over the lanes that share a block
+template <int EL> __device__ __forceinline__ uint32_t block_max(uint32_t m) {
+  m = max_u32(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xF, 0xF, true)); // lanes 1 0 3 2
+  m = max_u32(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xF, 0xF, true)); // lanes 2 3 0 1
+  if constexpr (mx_lanes<EL> == 8)
+    m = max_u32(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x141, 0xF, 0xF, true)); // eight lanes mirrored
+  return m;
 }
 
 // ---------------------------------------------------------------- codes
@@ -147,20 +144,24 @@ template <int FMT> __device__ __forceinline__ uint32_t mx_pair8(float a, float b
 template <int B> __device__ __forceinline__ uint32_t mx_pair4(float a, float b, uint32_t w) {
   return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, mx_clamp<MX_E2M1>(a), mx_clamp<MX_E2M1>(b), 1.0f, B);
 }
-// eight codes: one word of e2m1, two of the 8-bit formats
-template <int EL, int FMT> __device__ __forceinline__ u32x2 mx_encode(const Oct<EL> &o, float inv, bool finite) {
+// the codes of a pack, in as many low bytes as they take
+template <int EL, int FMT> __device__ __forceinline__ u32x2 mx_encode(const Pack<EL> &o, float inv, bool finite) {
   u32x2 c = {0, 0};
-  auto v = [&](int i) { return oct_get<EL>(o, i) * inv; };
+  auto v = [&](int i) { return pack_get<EL>(o, i) * inv; };
   if constexpr (FMT == MX_E2M1) {
     c.x = mx_pair4<0>(v(0), v(1), c.x);
     c.x = mx_pair4<1>(v(2), v(3), c.x);
-    c.x = mx_pair4<2>(v(4), v(5), c.x);
-    c.x = mx_pair4<3>(v(6), v(7), c.x);
+    if constexpr (mx_vals<EL> == 8) {
+      c.x = mx_pair4<2>(v(4), v(5), c.x);
+      c.x = mx_pair4<3>(v(6), v(7), c.x);
+    }
   } else {
     c.x = mx_pair8<FMT>(v(0), v(1), c.x, false);
     c.x = mx_pair8<FMT>(v(2), v(3), c.x, true);
-    c.y = mx_pair8<FMT>(v(4), v(5), c.y, false);
-    c.y = mx_pair8<FMT>(v(6), v(7), c.y, true);
+    if constexpr (mx_vals<EL> == 8) {
+      c.y = mx_pair8<FMT>(v(4), v(5), c.y, false);
+      c.y = mx_pair8<FMT>(v(6), v(7), c.y, true);
+    }
   }
   return finite ? c : u32x2{0, 0};
 }
@@ -175,35 +176,39 @@ template <int FMT> __device__ __forceinline__ f32x2 mx_decode2(uint32_t w, int i
            : i == 2 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 2)
                     : __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 3);
 }
-template <int FMT> __device__ __forceinline__ void mx_decode(u32x2 c, float scale, float (&f)[8]) {
+template <int EL, int FMT> __device__ __forceinline__ void mx_decode(u32x2 c, float scale, float (&f)[mx_vals<EL>]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < mx_vals<EL> / 2; ++i) {
     const f32x2 v = FMT == MX_E2M1 ? mx_decode2<FMT>(c.x, i) : mx_decode2<FMT>(i < 2 ? c.x : c.y, i % 2);
     f[2 * i] = v.x * scale, f[2 * i + 1] = v.y * scale;
   }
 }
-template <int FMT> __device__ __forceinline__ void codes_store(void *p, u32x2 c) {
-  if constexpr (FMT == MX_E2M1) __builtin_nontemporal_store(c.x, reinterpret_cast<u32_any *>(p));
-  else __builtin_nontemporal_store(c, reinterpret_cast<u32x2_any *>(p));
+template <int EL, int FMT> __device__ __forceinline__ void codes_store(void *p, u32x2 c) {
+  constexpr int B = mx_bytes<EL, FMT>;
+  if constexpr (B == 8) __builtin_nontemporal_store(c, reinterpret_cast<u32x2_any *>(p));
+  else if constexpr (B == 4) __builtin_nontemporal_store(c.x, reinterpret_cast<u32_any *>(p));
+  else __builtin_nontemporal_store((uint16_t)c.x, reinterpret_cast<u16_any *>(p));
 }
-// the codes of the first n of eight values (n even for e2m1)
-template <int FMT> __device__ __forceinline__ void codes_store_part(uint8_t *p, u32x2 c, int n) {
+// the codes of the first n values (n even for e2m1)
+template <int EL, int FMT> __device__ __forceinline__ void codes_store_part(uint8_t *p, u32x2 c, int n) {
   const int bytes = FMT == MX_E2M1 ? n / 2 : n;
 #pragma unroll
-  for (int i = 0; i < mx_oct<FMT>; ++i) {
+  for (int i = 0; i < mx_bytes<EL, FMT>; ++i) {
     if (i >= bytes) break;
     p[i] = (uint8_t)((i < 4 ? c.x : c.y) >> (8 * (i % 4)));
   }
 }
-template <int FMT> __device__ __forceinline__ u32x2 codes_load(const void *p) {
-  if constexpr (FMT == MX_E2M1) return u32x2{__builtin_nontemporal_load(reinterpret_cast<const u32_any *>(p)), 0};
-  else return __builtin_nontemporal_load(reinterpret_cast<const u32x2_any *>(p));
+template <int EL, int FMT> __device__ __forceinline__ u32x2 codes_load(const void *p) {
+  constexpr int B = mx_bytes<EL, FMT>;
+  if constexpr (B == 8) return __builtin_nontemporal_load(reinterpret_cast<const u32x2_any *>(p));
+  else if constexpr (B == 4) return u32x2{__builtin_nontemporal_load(reinterpret_cast<const u32_any *>(p)), 0};
+  else return u32x2{__builtin_nontemporal_load(reinterpret_cast<const u16_any *>(p)), 0};
 }
-template <int FMT> __device__ __forceinline__ u32x2 codes_load_part(const uint8_t *p, int n) {
+template <int EL, int FMT> __device__ __forceinline__ u32x2 codes_load_part(const uint8_t *p, int n) {
   const int bytes = FMT == MX_E2M1 ? (n + 1) / 2 : n;
   u32x2 c = {0, 0};
 #pragma unroll
-  for (int i = 0; i < mx_oct<FMT>; ++i) {
+  for (int i = 0; i < mx_bytes<EL, FMT>; ++i) {
     if (i >= bytes) break;
     if (i < 4) c.x |= (uint32_t)p[i] << (8 * i);
     else c.y |= (uint32_t)p[i] << (8 * (i - 4));
@@ -211,47 +216,49 @@ template <int FMT> __device__ __forceinline__ u32x2 codes_load_part(const uint8_
   return c;
 }
 
-// The scale bytes of the blocks of this row of 16 lanes (lanes 4 j hold block
-// j of `blk` + j): one four-byte store where all four blocks exist.
-__device__ __forceinline__ void scales_store(uint8_t *__restrict__ scales, int64_t blk, int64_t nblk, uint32_t byte) {
+// One scale byte a block: lane l holds block `blk`, which counts up by one
+// every mx_lanes lanes.  Of 16-bit values the four blocks of 16 lanes leave
+// as one word where all four exist.
+template <int EL> __device__ __forceinline__ void scales_store(uint8_t *__restrict__ scales, int64_t blk, int64_t nblk, uint32_t byte) {
   const int lane = threadIdx.x & 15;
-  if ((blk | 3) < nblk) { // (blk counts up by one every four lanes, from a multiple of 4)
+  if (mx_lanes<EL> == 4 && (blk | 3) < nblk) { // (a row of lanes starts at a multiple of 4)
     uint32_t w = byte;
     w |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)byte, 0x104, 0xF, 0xF, true) << 8;  // lane + 4
     w |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)byte, 0x108, 0xF, 0xF, true) << 16; // lane + 8
     w |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)byte, 0x10C, 0xF, 0xF, true) << 24; // lane + 12
     if (lane == 0) *reinterpret_cast<u32_any *>(scales + blk) = w;
-  } else if ((lane & 3) == 0) {
+  } else if ((lane & (mx_lanes<EL> - 1)) == 0) {
     scales[blk] = (uint8_t)byte;
   }
 }
 
 // ---------------------------------------------------------------- blocks along a row
-// x [R, K] -> codes [R, K] (e2m1: [R, K/2]), scales [R, ceil(K/32)].  Four
-// lanes share a block, eight elements (one 16-byte access of a 16-bit type)
-// each; a workgroup's accesses are consecutive.
+// x [R, K] -> codes [R, K] (e2m1: [R, K/2]), scales [R, ceil(K/32)].  A lane
+// takes one 16-byte access of values, four (f32: eight) neighbouring lanes a
+// block; a workgroup's accesses are consecutive.
 template <int EL, int FMT, int64_t K>
 __device__ __forceinline__ void mx_quantize_rows(const void *__restrict__ x, void *__restrict__ codes, void *__restrict__ scales,
                                                  int64_t R) {
+  constexpr int V = mx_vals<EL>, L = mx_lanes<EL>;
   constexpr int64_t NB = (K + 31) / 32;
-  const int64_t nblk = R * NB, n = nblk * 4;
+  const int64_t nblk = R * NB, n = nblk * L;
   for (int64_t it = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; it < n; it += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t blk = it >> 2;
-    int64_t e = it * 8; // first element, flat
-    int cnt = 8;
+    const int64_t blk = it / L;
+    int64_t e = it * V; // first element, flat
+    int cnt = V;
     if constexpr (K % 32 != 0) {
-      const int64_t r = blk / NB, c = (blk - r * NB) * 32 + (it & 3) * 8;
+      const int64_t r = blk / NB, c = (blk - r * NB) * 32 + (it & (L - 1)) * V;
       e = r * K + c;
-      cnt = (int)(K - c < 0 ? 0 : K - c < 8 ? K - c : 8);
+      cnt = (int)(K - c < 0 ? 0 : K - c < V ? K - c : V);
     }
     const char *src = (const char *)x + e * el_bytes<EL>;
-    const Oct<EL> o = cnt == 8 ? oct_load<EL>(src) : oct_load_part<EL>(src, cnt);
-    const uint32_t byte = mx_scale_byte<FMT>(quad_max(oct_amax<EL>(o)));
+    const Pack<EL> o = cnt == V ? pack_load<EL>(src) : pack_load_part<EL>(src, cnt);
+    const uint32_t byte = mx_scale_byte<FMT>(block_max<EL>(pack_amax<EL>(o)));
     const u32x2 c = mx_encode<EL, FMT>(o, mx_inverse(byte), byte != 255);
     uint8_t *dst = (uint8_t *)codes + (FMT == MX_E2M1 ? e / 2 : e);
-    if (cnt == 8) codes_store<FMT>(dst, c);
-    else codes_store_part<FMT>(dst, c, cnt);
-    scales_store((uint8_t *)scales, blk, nblk, byte);
+    if (cnt == V) codes_store<EL, FMT>(dst, c);
+    else codes_store_part<EL, FMT>(dst, c, cnt);
+    scales_store<EL>((uint8_t *)scales, blk, nblk, byte);
   }
 }
 
@@ -260,27 +267,28 @@ __device__ __forceinline__ void mx_quantize_rows(const void *__restrict__ x, voi
 template <int EL, int FMT, int64_t K>
 __device__ __forceinline__ void mx_dequantize_rows(const void *__restrict__ codes, const void *__restrict__ scales, void *__restrict__ out,
                                                    int64_t R) {
+  constexpr int V = mx_vals<EL>, L = mx_lanes<EL>;
   constexpr int64_t NB = (K + 31) / 32;
-  const int64_t n = R * NB * 4;
+  const int64_t n = R * NB * L;
   for (int64_t it = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; it < n; it += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t blk = it >> 2;
-    int64_t e = it * 8;
-    int cnt = 8;
+    const int64_t blk = it / L;
+    int64_t e = it * V;
+    int cnt = V;
     if constexpr (K % 32 != 0) {
-      const int64_t r = blk / NB, c = (blk - r * NB) * 32 + (it & 3) * 8;
+      const int64_t r = blk / NB, c = (blk - r * NB) * 32 + (it & (L - 1)) * V;
       e = r * K + c;
-      cnt = (int)(K - c < 0 ? 0 : K - c < 8 ? K - c : 8);
+      cnt = (int)(K - c < 0 ? 0 : K - c < V ? K - c : V);
     }
     const uint8_t *src = (const uint8_t *)codes + (FMT == MX_E2M1 ? e / 2 : e);
-    const u32x2 c = cnt == 8 ? codes_load<FMT>(src) : codes_load_part<FMT>(src, cnt);
-    float f[8];
-    mx_decode<FMT>(c, mx_scale(((const uint8_t *)scales)[blk]), f);
-    Oct<EL> o;
+    const u32x2 c = cnt == V ? codes_load<EL, FMT>(src) : codes_load_part<EL, FMT>(src, cnt);
+    float f[V];
+    mx_decode<EL, FMT>(c, mx_scale(((const uint8_t *)scales)[blk]), f);
+    Pack<EL> o;
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) oct_set2<EL>(o, i, f[i], f[i + 1]);
+    for (int i = 0; i < V; i += 2) pack_set2<EL>(o, i, f[i], f[i + 1]);
     char *dst = (char *)out + e * el_bytes<EL>;
-    if (cnt == 8) oct_store<EL>(dst, o);
-    else oct_store_part<EL>(dst, o, cnt);
+    if (cnt == V) pack_store<EL>(dst, o);
+    else pack_store_part<EL>(dst, o, cnt);
   }
 }
 
@@ -312,11 +320,7 @@ template <int EL> __device__ __forceinline__ Quad4<EL> quad_load(const char *p, 
   }
   return q;
 }
-template <int EL> __device__ __forceinline__ float quad_get(const Quad4<EL> &q, int i) {
-  if constexpr (EL == EL_F32) return u2f(q.w[i]);
-  else if constexpr (EL == EL_BF16) return u2f(i % 2 ? q.w[i / 2] & 0xFFFF0000u : q.w[i / 2] << 16);
-  else return f16_to_f32((uint16_t)(q.w[i / 2] >> (16 * (i % 2))));
-}
+template <int EL> __device__ __forceinline__ float quad_get(const Quad4<EL> &q, int i) { return word_get<EL>(q.w, i); }
 __device__ __forceinline__ void bytes_store(uint8_t *p, uint32_t w, int n) {
   if (n == 4) {
     __builtin_nontemporal_store(w, reinterpret_cast<u32_any *>(p));
@@ -444,11 +448,11 @@ __device__ __forceinline__ void mx_dequantize_cols(const void *__restrict__ code
     if (k >= rows) return;
     a *= s[0], b *= s[1], c *= s[2], d *= s[3];
     char *p = dst + (int64_t)k * N * el_bytes<EL>;
-    Oct<EL> o{};
-    oct_set2<EL>(o, 0, a, b);
-    oct_set2<EL>(o, 2, c, d);
+    Pack<EL> o{};
+    pack_set2<EL>(o, 0, a, b);
+    pack_set2<EL>(o, 2, c, d);
     if (cols < 4) {
-      oct_store_part<EL>(p, o, cols);
+      pack_store_part<EL>(p, o, cols);
     } else if constexpr (EL == EL_F32) {
       __builtin_nontemporal_store(u32x4{o.w[0], o.w[1], o.w[2], o.w[3]}, reinterpret_cast<u32x4_any *>(p));
     } else {
