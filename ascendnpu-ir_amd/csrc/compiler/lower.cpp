@@ -2560,19 +2560,46 @@ ContractionTile pickTile(int64_t M, int64_t N, int64_t Kb, bool bT, int mk) {
   return *best;
 }
 
-// linear_mx of few rows: rows up to `top` take 16 mt x 16 nt tiles whose nw
-// waves split K
+// The tile of linear_mx straight from the codes (hf_mmwx.h): 8 md rows x 16 nt
+// columns, nw waves that split K.  The numbers are fitted to the times of these
+// tiles at 1 to 768 rows, N = 512 .. 11008, K = 4096, both code widths (us; within
+// 7 % on average): of a CU's workgroups (the busiest XCD's over its 32 CUs),
+// every round moves a workgroup's rows and codes through the L1 and multiplies
+// them, and rounds past what the LDS holds at once start anew.  The picks take
+// 1.3 % more than the best tile on average; the worst of the measured sizes is
+// M = 1, N = 11008 with 8-bit codes, 12.4 us (8x16) against 10.0 (8x32).
+// N = K = 4096, 8-bit codes: M = 1 5.4 us (8x16), M = 48 7.5 (24x32) against 9.8
+// (48x32), M = 128 11.0, M = 512 28 (64x64), where the weight as bf16 in the
+// workspace (8 us) and the bf16 contraction (37) take 45; M = 768 40 against 54,
+// M = 1024 63 against 58.
 struct WxTile {
-  int64_t top;
-  int mt, nt, nw;
-  int64_t blocksPerRow(int64_t N) const { return (N + 16 * nt - 1) / (16 * nt); }
+  int md, nt, nw;
+  int64_t rowTiles(int64_t M) const { return (M + 8 * md - 1) / (8 * md); }
+  int64_t blocksPerRow(int64_t N) const { return ((N + 16 * nt - 1) / (16 * nt) + 7) / 8 * 8; }
+  int64_t ldsBytes(int64_t K, int cpb) const {
+    return std::max<int64_t>(nw * (cpb * md + nt) * 1024, nw * ((md + 1) / 2) * nt * 1024) + (K / 32 + 8) * (16 * nt + 4);
+  }
+  double time(int64_t M, int64_t N, int64_t K, int cpb) const {
+    const double bytes = 16.0 * md * K + 16.0 * nt * K / cpb, perCU = (double)(rowTiles(M) * blocksPerRow(N) / 8) / 32;
+    const double rounds = std::ceil(perCU), held = std::min<double>((double)(160 * 1024 / ldsBytes(K, cpb)), 32 / nw);
+    const double batches = std::ceil(rounds / held), steps = (double)((md + 1) / 2 * nt * K / 32) / 1000;
+    const double c4[6] = {4.55, 0.69, 0.26, 1.9, 1.95, 0.007}, c8[6] = {2.89, 0.44, 0.17, 0.71, 3.45, 0.71};
+    const double *c = nw == 4 ? c4 : c8;
+    return c[0] + (c[1] * rounds + c[2] * perCU) * bytes / 1e5 + c[3] * (batches - 1) + c[4] * steps * rounds + c[5] * (double)(N * K / cpb) / 1e7;
+  }
+  bool operator==(const WxTile &o) const { return md == o.md && nt == o.nt && nw == o.nw; }
 };
-const WxTile kWxTiles[] = {{16, 1, 1, 8}, {32, 2, 1, 8}, {64, 4, 1, 8}};
-constexpr int64_t kWxRows = 64;
-const WxTile &wxTile(int64_t M) {
-  for (const WxTile &t : kWxTiles)
-    if (M <= t.top) return t;
-  throw CompileError("internal: linear_mx tile");
+constexpr int64_t kWxRows = 768; // more rows: the bf16 contraction
+// nullptr: no tile's scales fit the LDS (K past about 200000)
+const WxTile *wxTile(int64_t M, int64_t N, int64_t K, int cpb) {
+  static const WxTile tiles[] = {{1, 1, 8}, {1, 2, 8}, {2, 1, 8}, {2, 2, 8}, {2, 4, 8}, {3, 2, 8}, {4, 1, 8},
+                                 {4, 2, 8}, {4, 3, 8}, {6, 2, 8}, {6, 4, 4}, {8, 4, 4}, {12, 4, 4}};
+  const WxTile *best = nullptr;
+  for (const WxTile &t : tiles) {
+    if (t.ldsBytes(K, cpb) > 160 * 1024) continue;
+    if (!best || t.time(M, N, K, cpb) < best->time(M, N, K, cpb)) best = &t;
+  }
+  return best;
 }
 
 KernelPlan lowerMatmul(Analysis &A, const std::string &kname, const LowerOptions &opt) {
@@ -2662,7 +2689,8 @@ KernelPlan lowerMatmul(Analysis &A, const std::string &kname, const LowerOptions
     wfmt = mxFormatOf(mm, "rhsFormat");
     if (wfmt < 0) unsupported(mm, "linear_mx without rhsFormat");
     if (ae != Elem::BF16) unsupported(mm, "linear_mx rows of another type than bf16");
-    if (M < 0 || N < 1 || K < 32 || K % 32 != 0) unsupported(mm, "linear_mx K must be a multiple of 32 (N at least 1)");
+    if (M < 1 || N < 1) unsupported(mm, "linear_mx of no rows or no outputs");
+    if (K < 32 || K % 32 != 0) unsupported(mm, "linear_mx K must be a multiple of 32");
     checkCodes(mm, b, wfmt, {N, K}, 1);
     checkScales(mm, sb, {N, K / 32});
     if (mm->results[0]->type.elem != Elem::F32) unsupported(mm, "linear_mx accumulates in f32");
@@ -2826,9 +2854,11 @@ KernelPlan lowerMatmul(Analysis &A, const std::string &kname, const LowerOptions
   p.kernelName = kname;
   p.kind = "SINGLE_CUBE";
   std::ostringstream k;
-  // linear_mx: up to kWxRows rows straight from the codes (hf_mmwx.h), more
-  // through the weight as bf16 in the workspace and the bf16 contraction
-  const bool wxPre = wx && (A.rowsDyn || M > kWxRows);
+  // linear_mx: up to kWxRows rows straight from the codes, more through the
+  // weight as bf16 in the workspace and the bf16 contraction
+  const int cpb = wfmt == 4 ? 2 : 1;
+  const WxTile *few = wx ? wxTile(1, N, K, cpb) : nullptr;
+  const bool wxPre = wx && (A.rowsDyn || M > kWxRows || !few);
   std::string params = kernelParamList(A, p.kargs, preA || preB || mxExact || wxPre);
   // epilogue functor receives all kernel pointer arguments
   k << "namespace {\nstruct " << kname << "_args {";
@@ -2885,27 +2915,35 @@ KernelPlan lowerMatmul(Analysis &A, const std::string &kname, const LowerOptions
   };
   // linear_mx of few rows
   auto wxCall = [&](const WxTile &t) {
-    k << "  hf::linear_wx<" << wfmt << ", " << kname << "_epi, " << t.mt << ", " << t.nt << ", " << t.nw << ", " << K << "ll>((const uint16_t*)p"
+    k << "  hf::linear_wx<" << wfmt << ", " << kname << "_epi, " << t.md << ", " << t.nt << ", " << t.nw << ", " << K << "ll>((const uint16_t*)p"
       << a->argIdx << ", (const uint8_t*)p" << b->argIdx << ", (const uint8_t*)p" << sb->argIdx << ", (" << mtype(oe) << "*)"
       << resultPtr(A, 0) << ", " << Mx << ", " << N << "ll, P);\n}\n";
   };
-  if (wx && A.rowsDyn)
-    for (const WxTile &t : kWxTiles) {
-      const std::string nm = altName(kname, "wx" + std::to_string(t.top));
-      kernelHead(nm, 64 * t.nw);
-      wxCall(t);
-      p.alts.push_back({nm, t.top, 16 * t.mt, t.blocksPerRow(N), (unsigned)(64 * t.nw)});
+  if (few && A.rowsDyn) {
+    std::vector<const WxTile *> emitted;
+    for (int64_t m = 8; m <= kWxRows; m += m < 64 ? 8 : m < 256 ? 32 : 128) {
+      const WxTile *t = wxTile(m, N, K, cpb);
+      const std::string nm = altName(kname, "wx" + std::to_string(8 * t->md) + "x" + std::to_string(16 * t->nt));
+      if (std::find(emitted.begin(), emitted.end(), t) == emitted.end()) {
+        emitted.push_back(t);
+        kernelHead(nm, 64 * t->nw);
+        wxCall(*t);
+      }
+      if (!p.alts.empty() && p.alts.back().name == nm) p.alts.back().maxRows = m;
+      else p.alts.push_back({nm, m, 8 * t->md, t->blocksPerRow(N), (unsigned)(64 * t->nw)});
     }
+  }
   if (wx) {
     p.algoOps = 2.0 * (double)M * (double)N * (double)K;
     if (!wxPre) {
-      const WxTile &t = wxTile(M);
+      const WxTile &t = *wxTile(std::max<int64_t>(M, 1), N, K, cpb);
       kernelHead(kname, 64 * t.nw);
       wxCall(t);
       p.source = k.str();
-      p.grid[0] = (unsigned)std::max<int64_t>(1, (M + 16 * t.mt - 1) / (16 * t.mt) * t.blocksPerRow(N));
+      p.grid[0] = (unsigned)(std::max<int64_t>(1, t.rowTiles(M)) * t.blocksPerRow(N));
       p.block[0] = (unsigned)(64 * t.nw);
-      p.variant = std::string("bf16 rows x ") + mxFormatName(wfmt) + " weight, K split over " + std::to_string(t.nw) + " waves";
+      p.variant = std::string("bf16 rows x ") + mxFormatName(wfmt) + " weight, LDS DMA, " + std::to_string(8 * t.md) + "x" + std::to_string(16 * t.nt) +
+                  " tiles, K split over " + std::to_string(t.nw) + " waves";
       return p;
     }
     KernelPlan::PreKernel pk;
@@ -2932,7 +2970,7 @@ KernelPlan lowerMatmul(Analysis &A, const std::string &kname, const LowerOptions
     if (seq.back() == tile) seq.pop_back();
     for (size_t i = 0; i < seq.size(); ++i) {
       const ContractionTile &t = seq[i];
-      if (wx && top[i] <= kWxRows) continue;
+      if (few && top[i] <= kWxRows) continue;
       const bool main = ring && t == tile;
       const std::string nm = main ? kname : altName(kname, std::to_string(t.tm) + "x" + std::to_string(t.tn) + (t.kg > 1 ? "k" + std::to_string(t.kg) : ""));
       if (!main && std::find(emitted.begin(), emitted.end(), t) == emitted.end()) {
