@@ -41,6 +41,25 @@ def hfc():
     return _hfc
 
 
+_hfcall = None
+
+
+def hfcall():
+    """The C part of plain group calls (csrc/runtime/pycall.c)."""
+    global _hfcall
+    if _hfcall is None:
+        from importlib.machinery import ExtensionFileLoader
+        from importlib.util import module_from_spec, spec_from_file_location
+        path = os.path.join(LIB_DIR, "_hfcall.so")
+        if not os.path.exists(path):
+            raise NativeLibraryMissing(f"{path} is not built; run `make -C {PKG_ROOT}` (or __graft_entry__.build())")
+        spec = spec_from_file_location("_hfcall", path, loader=ExtensionFileLoader("_hfcall", path))
+        mod = module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        _hfcall = mod
+    return _hfcall
+
+
 class LaunchCfg(ctypes.Structure):
     _fields_ = [("grid", ctypes.c_uint * 3), ("block", ctypes.c_uint * 3), ("lds_bytes", ctypes.c_uint)]
 

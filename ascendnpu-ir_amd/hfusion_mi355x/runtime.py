@@ -173,6 +173,7 @@ class Group:
     """One loaded HFusion group kernel (hfr_group_t)."""
 
     _plan = None               # _make_plan's answer, from the first plain call
+    _call = None               # the same as one C function, False where there is none
     _row_shapes = (-1, None)   # the last launch-time row count and the argument shapes it makes
 
     def __init__(self, artifact, func=None):
@@ -212,7 +213,12 @@ class Group:
         noalloc=True goes through hfr_group_launch_noalloc (the library's
         static scratch instead of a workspace)."""
         if results is None and stream is None and workspace is None and not noalloc:
-            ret = self._launch_plain(args)
+            call = self._call
+            if call is None:
+                call = self._call = self._make_call()
+            ret = call(*args) if call else self._launch_plain(args)
+            if type(ret) is int:
+                native.check(ret)
             if ret is not None:
                 return ret
         return self._bind(args, results, stream, workspace, noalloc)()
@@ -236,6 +242,20 @@ class Group:
         return (torch, specs, first, rows_at, tied, ctypes.c_uint64 * len(specs), (ctypes.c_void_p * max(1, len(res)))(),
                 lib.hfr_group_launch_rows if dyn else lib.hfr_group_launch, len(specs), len(res),
                 raw or (lambda i: torch.cuda.current_stream(i).cuda_stream))
+
+    def _make_call(self):
+        """The plain call as one C function (native.hfcall), where every
+        argument is a tensor and every result is written into one."""
+        plan = self._plan
+        if plan is None:
+            plan = self._plan = self._make_plan()
+        if not plan:
+            return False
+        torch, specs, _, rows_at, tied, _, _, launch, _, _, raw_stream = plan
+        if any(dt is None or len(sh) > 8 for dt, sh in specs) or len(specs) > 24 or not tied or min(tied) < 0:
+            return False
+        return native.hfcall().plan(ctypes.cast(launch, ctypes.c_void_p).value, self._h.value, rows_at is not None,
+                                    torch.Tensor, raw_stream, specs, tied)
 
     def _launch_plain(self, args):
         """The launch of a call on the current stream with no options: a call
