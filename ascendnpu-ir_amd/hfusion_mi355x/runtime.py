@@ -252,9 +252,10 @@ class Group:
         if not plan:
             return False
         torch, specs, _, rows_at, tied, _, _, launch, _, _, raw_stream = plan
-        if any(dt is None or len(sh) > 8 for dt, sh in specs) or len(specs) > 24 or not tied or min(tied) < 0:
+        h = getattr(self, "_h", None)
+        if any(dt is None or len(sh) > 8 for dt, sh in specs) or len(specs) > 24 or not tied or min(tied) < 0 or not h:
             return False
-        return native.hfcall().plan(ctypes.cast(launch, ctypes.c_void_p).value, self._h.value, rows_at is not None,
+        return native.hfcall().plan(ctypes.cast(launch, ctypes.c_void_p).value, h.value, rows_at is not None,
                                     torch.Tensor, raw_stream, specs, tied)
 
     def _launch_plain(self, args):
