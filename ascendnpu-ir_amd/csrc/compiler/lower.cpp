@@ -3232,7 +3232,7 @@ static LnShape lnForwardShape(int64_t D, int64_t V) {
   return {T, (acc + T - 1) / T, std::max<int64_t>(1, 256 / T)};
 }
 // The gradient: workgroups of 512 threads, one a CU, so that few rows of
-// partial sums are left.  us, [8192, 4096] from an 8-bit checkpoint: 31.8 with
+// partial sums are left.  us, [8192, 4096] from an 8-bit checkpoint: 32.2 with
 // two row groups of 256 threads and two accesses, 39.3 of 512 and one (1024
 // threads a workgroup), 68.7 with four row groups of 256; 35.5 with 512
 // workgroups (16.8 MB of partial sums instead of 8.4).  [2048, 16384]: 39.8

@@ -60,28 +60,19 @@ template <int T, int N> __device__ __forceinline__ void group_sum(float (&v)[N],
   }
 }
 
-// Weight and bias of a thread's columns: V values of type PEL as they lie.
-template <int PEL, int V> struct LnParam {
-  uint32_t w[V * el_bytes<PEL> / 4];
-  __device__ __forceinline__ float get(int i) const { return word_get<PEL>(w, i); }
-  __device__ __forceinline__ void load(const void *base, int64_t c, int n) {
-    const char *p = (const char *)base + c * el_bytes<PEL>;
+// Weight and bias of a thread's columns: V values of type PEL as they lie,
+// zeros behind the row's end (put there by put_right).
+template <int PEL, int V, int64_t D> struct LnParam {
+  static constexpr int PV = mx_vals<PEL>, N = V / PV > 0 ? V / PV : 1;
+  Pack<PEL> p[N];
+  __device__ __forceinline__ float get(int i) const { return pack_get<PEL>(p[i / PV], i % PV); }
+  __device__ __forceinline__ void load(const void *base, int64_t c) {
 #pragma unroll
-    for (int i = 0; i < V * el_bytes<PEL> / 4; ++i) w[i] = 0;
-    if (n == V) {
+    for (int k = 0; k < N; ++k) p[k] = pack_load_row<PEL, D, false>(base, 0, c + k * PV);
+  }
+  __device__ __forceinline__ void put_right(int64_t c) {
 #pragma unroll
-      for (int i = 0; i < V * el_bytes<PEL> / 16; ++i) {
-        const u32x4 v = reinterpret_cast<const u32x4_any *>(p)[i];
-        w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        if (i >= n) break;
-        if constexpr (PEL == EL_F32) w[i] = reinterpret_cast<const uint32_t *>(p)[i];
-        else w[i / 2] |= (uint32_t)reinterpret_cast<const uint16_t *>(p)[i] << (16 * (i % 2));
-      }
-    }
+    for (int k = 0; k < N; ++k) pack_at<PEL, D>(p[k], c + k * PV);
   }
 };
 
@@ -104,28 +95,31 @@ __device__ __forceinline__ void ln_forward(const void *__restrict__ x, const voi
   __shared__ float slots[2][RPB * W];
   const int lt = threadIdx.x % T, group = threadIdx.x / T;
   auto col = [&](int j) { return ((int64_t)j * T + lt) * V; };
-  LnParam<PEL, V> gm[NCH], bt[NCH];
-#pragma unroll
-  for (int j = 0; j < NCH; ++j) {
-    const int n = ln_count<D, V, FULL>(col(j), true);
-    if constexpr (AFF >= 1) gm[j].load(gamma, col(j), n);
-    if constexpr (AFF >= 2) bt[j].load(beta, col(j), n);
-  }
+  if ((int64_t)blockIdx.x * RPB >= R) return;
+  // (a row past the last is the last one again, of which nothing is written)
   auto load = [&](int64_t row, Pack<EL> (&v)[NCH]) {
 #pragma unroll
-    for (int j = 0; j < NCH; ++j) {
-      const int n = ln_count<D, V, FULL>(col(j), row < R);
-      const char *p = (const char *)x + (row * D + col(j)) * el_bytes<EL>;
-      v[j] = n == V ? pack_load<EL>(p) : pack_load_part<EL>(p, FULL ? 0 : n);
-    }
+    for (int j = 0; j < NCH; ++j) v[j] = pack_load_row<EL, D>(x, row < R ? row : R - 1, col(j));
   };
   const int64_t step = (int64_t)gridDim.x * RPB;
-  Pack<EL> v[NCH], next[NCH];
-  load((int64_t)blockIdx.x * RPB + group, v);
-  for (int64_t row0 = (int64_t)blockIdx.x * RPB; row0 < R; row0 += step) {
-    const int64_t row = row0 + group;
-    if (row0 + step < R) load(row + step, next);
+  Pack<EL> va[NCH], vb[NCH];
+  LnParam<PEL, V, D> gm[NCH], bt[NCH];
+#pragma unroll
+  for (int j = 0; j < NCH; ++j) {
+    if constexpr (AFF >= 1) gm[j].load(gamma, col(j));
+    if constexpr (AFF >= 2) bt[j].load(beta, col(j));
+  }
+  load((int64_t)blockIdx.x * RPB + group, va);
+#pragma unroll
+  for (int j = 0; j < NCH; ++j) {
+    if constexpr (AFF >= 1 && !FULL) gm[j].put_right(col(j));
+    if constexpr (AFF >= 2 && !FULL) bt[j].put_right(col(j));
+  }
+  auto work = [&](int64_t row, Pack<EL> (&v)[NCH]) {
     float s[1] = {0}, q[1] = {0};
+    if constexpr (!FULL)
+#pragma unroll
+      for (int j = 0; j < NCH; ++j) pack_at<EL, D>(v[j], col(j));
 #pragma unroll
     for (int j = 0; j < NCH; ++j)
 #pragma unroll
@@ -175,9 +169,19 @@ __device__ __forceinline__ void ln_forward(const void *__restrict__ x, const voi
         if (lt % mx_lanes<EL> == 0 && n > 0) ((uint8_t *)scales)[row * NB + col(j) / 32] = (uint8_t)byte;
       }
     }
+  };
+  // (the last rows apart: a load that only some turns make would have the wait
+  // for the row at hand wait for the next one too, and one that reads no new
+  // row had all workgroups read the last row: [777, 5003] f32 11.9 us for 8.0)
+  int64_t row0 = (int64_t)blockIdx.x * RPB;
+  for (; row0 + step < R; row0 += step) {
+    load(row0 + step + group, vb);
+    __builtin_amdgcn_sched_barrier(0);
+    work(row0 + group, va);
 #pragma unroll
-    for (int j = 0; j < NCH; ++j) v[j] = next[j];
+    for (int j = 0; j < NCH; ++j) va[j] = vb[j];
   }
+  work(row0 + group, va);
 }
 
 // Row groups walk the rows with a stride and keep their columns' part of
@@ -198,11 +202,11 @@ __device__ __forceinline__ void ln_grad_rows(const void *__restrict__ dy, const 
   __shared__ __attribute__((aligned(16))) float sums[AFF >= 1 && RPB > 1 ? RPB * CAP : 4];
   const int lt = threadIdx.x % T, group = threadIdx.x / T;
   auto col = [&](int j) { return ((int64_t)j * T + lt) * V; };
-  LnParam<PEL, V> gm[NCH];
+  if ((int64_t)blockIdx.x * RPB >= R) return; // (its row of `part` is not read)
+  LnParam<PEL, V, D> gm[NCH];
   float dg[NCH][V], db[NCH][V];
 #pragma unroll
   for (int j = 0; j < NCH; ++j) {
-    if constexpr (AFF >= 1) gm[j].load(gamma, col(j), ln_count<D, V, FULL>(col(j), true));
 #pragma unroll
     for (int i = 0; i < V; ++i) dg[j][i] = db[j][i] = 0;
   }
@@ -212,32 +216,50 @@ __device__ __forceinline__ void ln_grad_rows(const void *__restrict__ dy, const 
     uint32_t byte[NCH];
     float mu, r;
   };
+  // (a row past the last is the last one again: its dy counts as zeros)
   auto load = [&](int64_t row, Row &v) {
-    v.mu = v.r = 0;
-    if (row < R) v.mu = mean[row], v.r = rstd[row];
+    row = row < R ? row : R - 1;
+    v.mu = mean[row], v.r = rstd[row];
 #pragma unroll
     for (int j = 0; j < NCH; ++j) {
-      const int n = ln_count<D, V, FULL>(col(j), row < R);
-      const int64_t e = row * D + col(j);
-      const char *p = (const char *)dy + e * el_bytes<EL>;
-      v.d[j] = n == V ? pack_load<EL>(p) : pack_load_part<EL>(p, FULL ? 0 : n);
+      v.d[j] = pack_load_row<EL, D>(dy, row, col(j));
       if constexpr (CK >= 0) {
-        const uint8_t *q = (const uint8_t *)x + e;
-        v.code[j] = n == V ? codes_load<EL, CK>(q) : codes_load_part<EL, CK>(q, FULL ? 0 : n);
-        v.byte[j] = n > 0 ? ((const uint8_t *)scales)[row * NB + col(j) / 32] : 0;
+        const int64_t b = col(j) / 32;
+        v.code[j] = codes_load_row<EL, CK, D>(x, row, col(j));
+        v.byte[j] = ((const uint8_t *)scales)[row * NB + (FULL || b < NB ? b : NB - 1)];
       } else {
-        const char *q = (const char *)x + e * el_bytes<EL>;
-        v.x[j] = n == V ? pack_load<EL>(q) : pack_load_part<EL>(q, FULL ? 0 : n);
+        v.x[j] = pack_load_row<EL, D>(x, row, col(j));
       }
     }
   };
+  auto put_right = [&](bool ok, Row &v) {
+#pragma unroll
+    for (int j = 0; j < NCH; ++j) {
+      if constexpr (!FULL) {
+        pack_at<EL, D>(v.d[j], col(j));
+        if constexpr (CK >= 0) v.code[j] = codes_at<EL, CK, D>(v.code[j], col(j));
+        else pack_at<EL, D>(v.x[j], col(j));
+      }
+      if (RPB > 1 && !ok) {
+        v.d[j] = Pack<EL>{};
+        if constexpr (CK >= 0) v.code[j] = u32x2{0, 0}, v.byte[j] = 0;
+        else v.x[j] = Pack<EL>{};
+      }
+    }
+    if (RPB > 1 && !ok) v.mu = v.r = 0;
+  };
   const int64_t step = (int64_t)gridDim.x * RPB;
-  Row cur, next;
+  Row ra, rb;
   int parity = 0;
-  load((int64_t)blockIdx.x * RPB + group, cur);
-  for (int64_t row0 = (int64_t)blockIdx.x * RPB; row0 < R; row0 += step) {
-    const int64_t row = row0 + group;
-    if (AHEAD && row0 + step < R) load(row + step, next);
+#pragma unroll
+  for (int j = 0; j < NCH; ++j)
+    if constexpr (AFF >= 1) gm[j].load(gamma, col(j));
+  load((int64_t)blockIdx.x * RPB + group, ra);
+#pragma unroll
+  for (int j = 0; j < NCH; ++j)
+    if constexpr (AFF >= 1 && !FULL) gm[j].put_right(col(j));
+  auto work = [&](int64_t row, Row &cur) {
+    put_right(row < R, cur);
     float xh[NCH][V], s[2] = {0, 0};
 #pragma unroll
     for (int j = 0; j < NCH; ++j) {
@@ -276,11 +298,19 @@ __device__ __forceinline__ void ln_grad_rows(const void *__restrict__ dy, const 
       if (n == V) pack_store<EL>(dst, o);
       else if (!FULL) pack_store_part<EL>(dst, o, n);
     }
-    if constexpr (AHEAD) cur = next;
-    else if (row0 + step < R) load(row + step, cur);
+  };
+  int64_t row0 = (int64_t)blockIdx.x * RPB;
+  for (; row0 + step < R; row0 += step) {
+    if constexpr (AHEAD) {
+      load(row0 + step + group, rb);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    work(row0 + group, ra);
+    if constexpr (AHEAD) ra = rb;
+    else load(row0 + step + group, ra);
   }
+  work(row0 + group, ra);
   if constexpr (AFF >= 1) {
-    if ((int64_t)blockIdx.x * RPB >= R) return; // (its row of `part` is not read)
     float *p = part + (int64_t)blockIdx.x * (AFF * D);
 #pragma unroll
     for (int a = 0; a < AFF; ++a) {

@@ -40,20 +40,47 @@ typedef u32x2 u32x2_any __attribute__((aligned(1)));
 typedef uint32_t u32_any __attribute__((aligned(1)));
 typedef uint16_t u16_any __attribute__((aligned(1)));
 
-template <int EL> __device__ __forceinline__ Pack<EL> pack_load(const void *p) {
-  const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any *>(p));
+template <int EL, bool ONCE = true> __device__ __forceinline__ Pack<EL> pack_load(const void *p) {
+  const u32x4_any *q = reinterpret_cast<const u32x4_any *>(p);
+  const u32x4 v = ONCE ? __builtin_nontemporal_load(q) : *q;
   return Pack<EL>{{v.x, v.y, v.z, v.w}};
 }
-// the first n values, zeros behind them
-template <int EL> __device__ __forceinline__ Pack<EL> pack_load_part(const void *p, int n) {
-  Pack<EL> o{};
+// The end of a row of D values: a lane whose access would pass it reads the
+// row's last 16 bytes instead (`behind` values before its own first one) and
+// moves its values to the front, zeros behind them, when it needs them: a load
+// per value, each waiting for the one before, made a short odd row slow (the
+// gradient of [45, 4441] 13.9 us, 7.7 so).  Rows of less than
+// 16 bytes are read value by value.
+template <int EL, int64_t D, bool ONCE = true>
+__device__ __forceinline__ Pack<EL> pack_load_row(const void *base, int64_t row, int64_t c) {
+  constexpr int V = mx_vals<EL>;
+  if constexpr (D >= V) {
+    return pack_load<EL, ONCE>((const char *)base + (row * D + (c < D - V ? c : D - V)) * el_bytes<EL>);
+  } else {
+    Pack<EL> o{};
+    const char *p = (const char *)base + row * D * el_bytes<EL>;
 #pragma unroll
-  for (int i = 0; i < mx_vals<EL>; ++i) {
-    if (i >= n) break;
-    if constexpr (EL == EL_F32) o.w[i] = reinterpret_cast<const uint32_t *>(p)[i];
-    else o.w[i / 2] |= (uint32_t)reinterpret_cast<const uint16_t *>(p)[i] << (16 * (i % 2));
+    for (int i = 0; i < (int)D; ++i) {
+      if constexpr (EL == EL_F32) o.w[i] = reinterpret_cast<const uint32_t *>(p)[i];
+      else o.w[i / 2] |= (uint32_t)reinterpret_cast<const uint16_t *>(p)[i] << (16 * (i % 2));
+    }
+    return o;
   }
-  return o;
+}
+// what pack_load_row read, put right: the values at column c, a multiple of
+// the pack's (so the one lane that holds the row's end has a fixed distance)
+template <int EL, int64_t D> __device__ __forceinline__ void pack_at(Pack<EL> &o, int64_t c) {
+  constexpr int V = mx_vals<EL>, END = (int)(D % V), DOWN = END ? (V - END) * el_bytes<EL> : 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (D >= V && END != 0) {
+      const int k = i + DOWN / 4; // (words further up are read before they are written)
+      const uint32_t lo = k < 4 ? o.w[k] : 0, hi = k < 3 ? o.w[k + 1] : 0;
+      const uint32_t end = DOWN % 4 ? lo >> 16 | hi << 16 : lo;
+      o.w[i] = c > D - V ? end : o.w[i];
+    }
+    o.w[i] = c >= D ? 0 : o.w[i];
+  }
 }
 template <int EL> __device__ __forceinline__ void pack_store(void *p, const Pack<EL> &o) {
   __builtin_nontemporal_store(u32x4{o.w[0], o.w[1], o.w[2], o.w[3]}, reinterpret_cast<u32x4_any *>(p));
@@ -204,16 +231,28 @@ template <int EL, int FMT> __device__ __forceinline__ u32x2 codes_load(const voi
   else if constexpr (B == 4) return u32x2{__builtin_nontemporal_load(reinterpret_cast<const u32_any *>(p)), 0};
   else return u32x2{__builtin_nontemporal_load(reinterpret_cast<const u16_any *>(p)), 0};
 }
-template <int EL, int FMT> __device__ __forceinline__ u32x2 codes_load_part(const uint8_t *p, int n) {
-  const int bytes = FMT == MX_E2M1 ? (n + 1) / 2 : n;
-  u32x2 c = {0, 0};
+// as pack_load_row and pack_at, of a row of codes (D even for e2m1)
+template <int EL, int FMT, int64_t D> __device__ __forceinline__ u32x2 codes_load_row(const void *base, int64_t row, int64_t c) {
+  constexpr int V = mx_vals<EL>, P = FMT == MX_E2M1 ? 2 : 1;
+  if constexpr (D >= V) {
+    return codes_load<EL, FMT>((const uint8_t *)base + (row * D + (c < D - V ? c : D - V)) / P);
+  } else {
+    const uint8_t *p = (const uint8_t *)base + row * D / P;
+    u32x2 o = {0, 0};
 #pragma unroll
-  for (int i = 0; i < mx_bytes<EL, FMT>; ++i) {
-    if (i >= bytes) break;
-    if (i < 4) c.x |= (uint32_t)p[i] << (8 * i);
-    else c.y |= (uint32_t)p[i] << (8 * (i - 4));
+    for (int i = 0; i < (int)D / P; ++i) {
+      if (i < 4) o.x |= (uint32_t)p[i] << (8 * i);
+      else o.y |= (uint32_t)p[i] << (8 * (i - 4));
+    }
+    return o;
   }
-  return c;
+}
+template <int EL, int FMT, int64_t D> __device__ __forceinline__ u32x2 codes_at(u32x2 o, int64_t c) {
+  constexpr int V = mx_vals<EL>, P = FMT == MX_E2M1 ? 2 : 1, END = (int)(D % V), DOWN = END ? 8 * ((V - END) / P) : 0;
+  uint64_t w = ((uint64_t)o.y << 32) | o.x;
+  if constexpr (D >= V && END != 0) w = c > D - V ? w >> DOWN : w;
+  w = c >= D ? 0 : w;
+  return u32x2{(uint32_t)w, (uint32_t)(w >> 32)};
 }
 
 // One scale byte a block: lane l holds block `blk`, which counts up by one
@@ -238,21 +277,25 @@ template <int EL> __device__ __forceinline__ void scales_store(uint8_t *__restri
 // block; a workgroup's accesses are consecutive, U of them a thread in flight.
 // Bound by HBM: [8192, 4096] bf16 to 8 bits moves 101.7 MB in 17.6 us (5.8 TB/s;
 // a large copy runs at 5.4).
-// Access `it` of the rows: its first element (flat), its block and how many of
-// its values exist.
+// Access `it` of the rows: row and column of its first value, its block, and
+// how many of its values exist.  Accesses past the last are the last one
+// again, of which nothing is written.
 template <int EL, int64_t K> struct RowAccess {
-  int64_t blk, e;
+  int64_t row, c, blk;
   int cnt;
   __device__ __forceinline__ RowAccess(int64_t it, int64_t n) {
     constexpr int V = mx_vals<EL>, L = mx_lanes<EL>;
     constexpr int64_t NB = (K + 31) / 32;
+    const int64_t at = it < n ? it : n - 1;
     blk = it / L;
-    e = it * V;
-    cnt = it < n ? V : 0;
-    if constexpr (K % 32 != 0) {
-      const int64_t r = blk / NB, c = (blk - r * NB) * 32 + (it & (L - 1)) * V;
-      e = r * K + c;
-      if (it < n) cnt = (int)(K - c < 0 ? 0 : K - c < V ? K - c : V);
+    if constexpr (K % 32 == 0) { // whole accesses only: rows follow each other
+      row = 0;
+      c = at * V;
+      cnt = it < n ? V : 0;
+    } else {
+      row = at / (NB * L);
+      c = (at - row * (NB * L)) * V;
+      cnt = it >= n || c >= K ? 0 : K - c < V ? (int)(K - c) : V;
     }
   }
 };
@@ -262,20 +305,21 @@ __device__ __forceinline__ void mx_quantize_rows(const void *__restrict__ x, voi
                                                  int64_t R) {
   constexpr int V = mx_vals<EL>;
   const int64_t nblk = R * ((K + 31) / 32), n = nblk * mx_lanes<EL>;
-  for (int64_t it0 = (int64_t)blockIdx.x * (blockDim.x * U) + threadIdx.x; it0 - threadIdx.x < n; it0 += (int64_t)gridDim.x * (blockDim.x * U)) {
+  for (int64_t it0 = (int64_t)blockIdx.x * (blockDim.x * U); it0 < n; it0 += (int64_t)gridDim.x * (blockDim.x * U)) {
     Pack<EL> o[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const RowAccess<EL, K> a(it0 + u * (int64_t)blockDim.x, n);
-      const char *src = (const char *)x + a.e * el_bytes<EL>;
-      o[u] = a.cnt == V ? pack_load<EL>(src) : pack_load_part<EL>(src, a.cnt);
+      const RowAccess<EL, K> a(it0 + u * (int64_t)blockDim.x + threadIdx.x, n);
+      if constexpr (K % 32 == 0) o[u] = pack_load<EL>((const char *)x + a.c * el_bytes<EL>);
+      else o[u] = pack_load_row<EL, K>(x, a.row, a.c);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const RowAccess<EL, K> a(it0 + u * (int64_t)blockDim.x, n);
+      const RowAccess<EL, K> a(it0 + u * (int64_t)blockDim.x + threadIdx.x, n);
+      if constexpr (K % 32 != 0) pack_at<EL, K>(o[u], a.c);
       const uint32_t byte = mx_scale_byte<FMT>(block_max<EL>(pack_amax<EL>(o[u])));
       const u32x2 c = mx_encode<EL, FMT>(o[u], mx_inverse(byte), byte != 255);
-      uint8_t *dst = (uint8_t *)codes + (FMT == MX_E2M1 ? a.e / 2 : a.e);
+      uint8_t *dst = (uint8_t *)codes + (a.row * K + a.c) / (FMT == MX_E2M1 ? 2 : 1);
       if (a.cnt == V) codes_store<EL, FMT>(dst, c);
       else codes_store_part<EL, FMT>(dst, c, a.cnt);
       if (a.blk < nblk) scales_store<EL>((uint8_t *)scales, a.blk, nblk, byte);
@@ -290,25 +334,26 @@ __device__ __forceinline__ void mx_dequantize_rows(const void *__restrict__ code
                                                    int64_t R) {
   constexpr int V = mx_vals<EL>;
   const int64_t nblk = R * ((K + 31) / 32), n = nblk * mx_lanes<EL>;
-  for (int64_t it0 = (int64_t)blockIdx.x * (blockDim.x * U) + threadIdx.x; it0 - threadIdx.x < n; it0 += (int64_t)gridDim.x * (blockDim.x * U)) {
+  for (int64_t it0 = (int64_t)blockIdx.x * (blockDim.x * U); it0 < n; it0 += (int64_t)gridDim.x * (blockDim.x * U)) {
     u32x2 c[U];
     uint32_t byte[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const RowAccess<EL, K> a(it0 + u * (int64_t)blockDim.x, n);
-      const uint8_t *src = (const uint8_t *)codes + (FMT == MX_E2M1 ? a.e / 2 : a.e);
-      c[u] = a.cnt == V ? codes_load<EL, FMT>(src) : codes_load_part<EL, FMT>(src, a.cnt);
-      byte[u] = a.cnt > 0 ? ((const uint8_t *)scales)[a.blk] : 0;
+      const RowAccess<EL, K> a(it0 + u * (int64_t)blockDim.x + threadIdx.x, n);
+      if constexpr (K % 32 == 0) c[u] = codes_load<EL, FMT>((const uint8_t *)codes + a.c / (FMT == MX_E2M1 ? 2 : 1));
+      else c[u] = codes_load_row<EL, FMT, K>(codes, a.row, a.c);
+      byte[u] = ((const uint8_t *)scales)[a.blk < nblk ? a.blk : nblk - 1];
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const RowAccess<EL, K> a(it0 + u * (int64_t)blockDim.x, n);
+      const RowAccess<EL, K> a(it0 + u * (int64_t)blockDim.x + threadIdx.x, n);
       float f[V];
+      if constexpr (K % 32 != 0) c[u] = codes_at<EL, FMT, K>(c[u], a.c);
       mx_decode<EL, FMT>(c[u], mx_scale(byte[u]), f);
       Pack<EL> o;
 #pragma unroll
       for (int i = 0; i < V; i += 2) pack_set2<EL>(o, i, f[i], f[i + 1]);
-      char *dst = (char *)out + a.e * el_bytes<EL>;
+      char *dst = (char *)out + (a.row * K + a.c) * el_bytes<EL>;
       if (a.cnt == V) pack_store<EL>(dst, o);
       else pack_store_part<EL>(dst, o, a.cnt);
     }
@@ -323,9 +368,9 @@ __device__ __forceinline__ void mx_dequantize_rows(const void *__restrict__ code
 constexpr int MXC_COLS = 256, MXC_BLOCKS = 8;
 
 template <int EL> struct Quad4 { uint32_t w[el_bytes<EL>]; }; // four values of a k-row
-template <int EL> __device__ __forceinline__ Quad4<EL> quad_load(const char *p, int n) {
+template <int EL, bool FOUR> __device__ __forceinline__ Quad4<EL> quad_load(const char *p, int n) {
   Quad4<EL> q{};
-  if (n == 4) {
+  if constexpr (FOUR) {
     if constexpr (EL == EL_F32) {
       const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any *>(p));
       q.w[0] = v.x, q.w[1] = v.y, q.w[2] = v.z, q.w[3] = v.w;
@@ -333,41 +378,63 @@ template <int EL> __device__ __forceinline__ Quad4<EL> quad_load(const char *p, 
       const u32x2 v = __builtin_nontemporal_load(reinterpret_cast<const u32x2_any *>(p));
       q.w[0] = v.x, q.w[1] = v.y;
     }
-    return q;
-  }
+  } else {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (i >= n) break;
-    if constexpr (EL == EL_F32) q.w[i] = reinterpret_cast<const uint32_t *>(p)[i];
-    else q.w[i / 2] |= (uint32_t)reinterpret_cast<const uint16_t *>(p)[i] << (16 * (i % 2));
+    for (int i = 0; i < 3; ++i) {
+      if constexpr (EL == EL_F32) q.w[i] = reinterpret_cast<const uint32_t *>(p)[i < n ? i : 0];
+      else q.w[i / 2] |= (uint32_t)reinterpret_cast<const uint16_t *>(p)[i < n ? i : 0] << (16 * (i % 2));
+    }
   }
   return q;
 }
 template <int EL> __device__ __forceinline__ float quad_get(const Quad4<EL> &q, int i) { return word_get<EL>(q.w, i); }
-__device__ __forceinline__ void bytes_store(uint8_t *p, uint32_t w, int n) {
-  if (n == 4) {
+template <bool FOUR> __device__ __forceinline__ void bytes_store(uint8_t *p, uint32_t w, int n) {
+  if constexpr (FOUR) {
     __builtin_nontemporal_store(w, reinterpret_cast<u32_any *>(p));
-    return;
-  }
+  } else {
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (i < n) p[i] = (uint8_t)(w >> (8 * i));
+    for (int i = 0; i < 3; ++i)
+      if (i < n) p[i] = (uint8_t)(w >> (8 * i));
+  }
 }
+
+// The tile of a workgroup and the four columns of a lane: the last lanes of a
+// row of N columns take its last four again (they write the same bytes); a
+// matrix of less than four columns has them one by one.
+template <int64_t K, int64_t N> struct ColTile {
+  static constexpr bool FOUR = N >= 4;
+  static constexpr int64_t NB = (K + 31) / 32, CT = (N + MXC_COLS - 1) / MXC_COLS;
+  int64_t n0, n, kb0, kb, k0;
+  int rows;
+  __device__ __forceinline__ ColTile() {
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
+    n0 = (int64_t)(blockIdx.x % CT) * MXC_COLS;
+    n = n0 + 4 * lane;
+    if (n > N - 4) n = FOUR ? N - 4 : 0;
+    kb0 = (int64_t)(blockIdx.x / CT) * MXC_BLOCKS;
+    kb = kb0 + wave;
+    k0 = kb * 32;
+    rows = (int)(K - k0 < 32 ? K - k0 : 32);
+  }
+};
 
 template <int EL, int FMT, int64_t K, int64_t N>
 __device__ __forceinline__ void mx_quantize_cols(const void *__restrict__ x, void *__restrict__ codes, void *__restrict__ scales) {
-  constexpr int64_t NB = (K + 31) / 32, CT = (N + MXC_COLS - 1) / MXC_COLS;
+  using Tile = ColTile<K, N>;
+  constexpr int64_t NB = Tile::NB;
+  constexpr bool FOUR = Tile::FOUR;
   __shared__ uint8_t sc[MXC_COLS][MXC_BLOCKS];
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  const int64_t n0 = (int64_t)(blockIdx.x % CT) * MXC_COLS, n = n0 + 4 * lane;
-  const int64_t kb0 = (int64_t)(blockIdx.x / CT) * MXC_BLOCKS, kb = kb0 + wave, k0 = kb * 32;
-  const int cols = (int)(N - n <= 0 ? 0 : N - n < 4 ? N - n : 4);
-  if (kb < NB && cols > 0) {
-    const int rows = (int)(K - k0 < 32 ? K - k0 : 32);
+  const Tile t;
+  if (t.kb < NB) {
     Quad4<EL> q[32];
-    const char *src = (const char *)x + (k0 * N + n) * el_bytes<EL>;
+    const char *src = (const char *)x + (t.k0 * N + t.n) * el_bytes<EL>;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) q[i] = i < rows ? quad_load<EL>(src + (int64_t)i * N * el_bytes<EL>, cols) : Quad4<EL>{};
+    for (int i = 0; i < 32; ++i) q[i] = quad_load<EL, FOUR>(src + (int64_t)(i < t.rows ? i : 0) * N * el_bytes<EL>, (int)N);
+    if (K % 32 != 0 && t.rows < 32) {
+#pragma unroll
+      for (int i = 1; i < 32; ++i)
+        if (i >= t.rows) q[i] = Quad4<EL>{};
+    }
     uint32_t m[4];
     if constexpr (EL == EL_F32) {
 #pragma unroll
@@ -390,10 +457,11 @@ __device__ __forceinline__ void mx_quantize_cols(const void *__restrict__ x, voi
       const uint32_t byte = mx_scale_byte<FMT>(m[j]);
       inv[j] = mx_inverse(byte);
       keep |= byte == 255 ? 0u : 0xFFu << (8 * j);
-      sc[4 * lane + j][wave] = (uint8_t)byte;
+      const int64_t c = t.n - t.n0 + j; // (before the tile: another's column)
+      if (c >= 0) sc[c][t.kb - t.kb0] = (uint8_t)byte;
     }
     if constexpr (FMT == MX_E2M1) {
-      uint8_t *dst = (uint8_t *)codes + (k0 / 2) * N + n;
+      uint8_t *dst = (uint8_t *)codes + (t.k0 / 2) * N + t.n;
 #pragma unroll
       for (int i = 0; i < 32; i += 2) {
         uint32_t w = 0;
@@ -402,80 +470,89 @@ __device__ __forceinline__ void mx_quantize_cols(const void *__restrict__ x, voi
         w = mx_pair4<1>(v(0, 1), v(1, 1), w);
         w = mx_pair4<2>(v(0, 2), v(1, 2), w);
         w = mx_pair4<3>(v(0, 3), v(1, 3), w);
-        if (i < rows) bytes_store(dst + (int64_t)(i / 2) * N, w & keep, cols);
+        if (i < t.rows) bytes_store<FOUR>(dst + (int64_t)(i / 2) * N, w & keep, (int)N);
       }
     } else {
-      uint8_t *dst = (uint8_t *)codes + k0 * N + n;
+      uint8_t *dst = (uint8_t *)codes + t.k0 * N + t.n;
 #pragma unroll
       for (int i = 0; i < 32; ++i) {
         auto v = [&](int j) { return quad_get<EL>(q[i], j) * inv[j]; };
         uint32_t w = mx_pair8<FMT>(v(0), v(1), 0, false);
         w = mx_pair8<FMT>(v(2), v(3), w, true);
-        if (i < rows) bytes_store(dst + (int64_t)i * N, w & keep, cols);
+        if (i < t.rows) bytes_store<FOUR>(dst + (int64_t)i * N, w & keep, (int)N);
       }
     }
   }
   __syncthreads();
-  const int64_t col = n0 + threadIdx.x;
+  const int64_t col = t.n0 + threadIdx.x;
   if (threadIdx.x < MXC_COLS && col < N) {
-    uint8_t *dst = (uint8_t *)scales + col * NB + kb0;
+    uint8_t *dst = (uint8_t *)scales + col * NB + t.kb0;
     const u32x2 v = *reinterpret_cast<const u32x2 *>(sc[threadIdx.x]);
-    if (kb0 + MXC_BLOCKS <= NB) {
+    if (t.kb0 + MXC_BLOCKS <= NB) {
       *reinterpret_cast<u32x2_any *>(dst) = v;
     } else {
-      for (int i = 0; i < (int)(NB - kb0); ++i) dst[i] = (uint8_t)((i < 4 ? v.x : v.y) >> (8 * (i % 4)));
+      for (int i = 0; i < (int)(NB - t.kb0); ++i) dst[i] = (uint8_t)((i < 4 ? v.x : v.y) >> (8 * (i % 4)));
     }
   }
 }
 
 template <int EL, int FMT, int64_t K, int64_t N>
 __device__ __forceinline__ void mx_dequantize_cols(const void *__restrict__ codes, const void *__restrict__ scales, void *__restrict__ out) {
-  constexpr int64_t NB = (K + 31) / 32, CT = (N + MXC_COLS - 1) / MXC_COLS;
+  using Tile = ColTile<K, N>;
+  constexpr int64_t NB = Tile::NB;
+  constexpr bool FOUR = Tile::FOUR;
   __shared__ uint8_t sc[MXC_COLS][MXC_BLOCKS];
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  const int64_t n0 = (int64_t)(blockIdx.x % CT) * MXC_COLS, n = n0 + 4 * lane;
-  const int64_t kb0 = (int64_t)(blockIdx.x / CT) * MXC_BLOCKS, kb = kb0 + wave, k0 = kb * 32;
-  const int64_t col = n0 + threadIdx.x;
+  const Tile t;
+  const int64_t col = t.n0 + threadIdx.x;
   if (threadIdx.x < MXC_COLS && col < N) {
-    const uint8_t *src = (const uint8_t *)scales + col * NB + kb0;
+    const uint8_t *p = (const uint8_t *)scales + col * NB + t.kb0;
     u32x2 v = {0, 0};
-    if (kb0 + MXC_BLOCKS <= NB) v = *reinterpret_cast<const u32x2_any *>(src);
-    else
-      for (int i = 0; i < (int)(NB - kb0); ++i) {
-        if (i < 4) v.x |= (uint32_t)src[i] << (8 * i);
-        else v.y |= (uint32_t)src[i] << (8 * (i - 4));
+    if (t.kb0 + MXC_BLOCKS <= NB) {
+      v = *reinterpret_cast<const u32x2_any *>(p);
+    } else {
+#pragma unroll
+      for (int i = 0; i < MXC_BLOCKS; ++i) {
+        const uint32_t b = p[t.kb0 + i < NB ? i : 0];
+        if (i < 4) v.x |= b << (8 * i);
+        else v.y |= b << (8 * (i - 4));
       }
+    }
     *reinterpret_cast<u32x2 *>(sc[threadIdx.x]) = v;
   }
-  __syncthreads();
-  const int cols = (int)(N - n <= 0 ? 0 : N - n < 4 ? N - n : 4);
-  if (kb >= NB || cols == 0) return;
-  const int rows = (int)(K - k0 < 32 ? K - k0 : 32);
-  float s[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) s[j] = mx_scale(sc[4 * lane + j][wave]);
   constexpr int P = FMT == MX_E2M1 ? 2 : 1; // k-rows a byte
-  const uint8_t *src = (const uint8_t *)codes + (k0 / P) * N + n;
-  char *dst = (char *)out + (k0 * N + n) * el_bytes<EL>;
+  const uint8_t *src = (const uint8_t *)codes + (t.k0 / P) * N + t.n;
+  char *dst = (char *)out + (t.k0 * N + t.n) * el_bytes<EL>;
   uint32_t w[32 / P];
 #pragma unroll
   for (int i = 0; i < 32 / P; ++i) {
-    w[i] = 0;
-    if (i * P >= rows) continue;
-    const uint8_t *p = src + (int64_t)i * N;
-    if (cols == 4) w[i] = __builtin_nontemporal_load(reinterpret_cast<const u32_any *>(p));
-    else
-      for (int j = 0; j < cols; ++j) w[i] |= (uint32_t)p[j] << (8 * j);
+    const uint8_t *p = src + (t.kb < NB && i * P < t.rows ? (int64_t)i * N : t.kb < NB ? 0 : -(t.k0 / P) * N);
+    if constexpr (FOUR) {
+      w[i] = __builtin_nontemporal_load(reinterpret_cast<const u32_any *>(p));
+    } else {
+      w[i] = 0;
+#pragma unroll
+      for (int j = 0; j < 3; ++j) w[i] |= (uint32_t)p[j < N ? j : 0] << (8 * j);
+    }
+  }
+  __syncthreads();
+  if (t.kb >= NB) return;
+  // (the row's last four columns may begin before the tile: their scales are
+  // another tile's)
+  float s[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int64_t c = t.n - t.n0 + j;
+    s[j] = mx_scale(c >= 0 && c < MXC_COLS ? sc[c][t.kb - t.kb0] : ((const uint8_t *)scales)[(t.n + (FOUR || j < N ? j : 0)) * NB + t.kb]);
   }
   auto put = [&](int k, float a, float b, float c, float d) {
-    if (k >= rows) return;
+    if (k >= t.rows) return;
     a *= s[0], b *= s[1], c *= s[2], d *= s[3];
     char *p = dst + (int64_t)k * N * el_bytes<EL>;
     Pack<EL> o{};
     pack_set2<EL>(o, 0, a, b);
     pack_set2<EL>(o, 2, c, d);
-    if (cols < 4) {
-      pack_store_part<EL>(p, o, cols);
+    if constexpr (!FOUR) {
+      pack_store_part<EL>(p, o, (int)N);
     } else if constexpr (EL == EL_F32) {
       __builtin_nontemporal_store(u32x4{o.w[0], o.w[1], o.w[2], o.w[3]}, reinterpret_cast<u32x4_any *>(p));
     } else {
