@@ -2573,9 +2573,9 @@ ContractionTile pickTile(int64_t M, int64_t N, int64_t Kb, bool bT, int mk) {
 // 1.3 % more than the best tile on average; the worst of the measured sizes is
 // M = 1, N = 11008 with 8-bit codes, 12.4 us (8x16) against 10.0 (8x32).
 // N = K = 4096, 8-bit codes: M = 1 5.4 us (8x16), M = 48 7.5 (24x32) against 9.8
-// (48x32), M = 128 11.0, M = 512 28 (64x64), where the weight as bf16 in the
-// workspace (8 us) and the bf16 contraction (37) take 45; M = 768 40 against 54,
-// M = 1024 63 against 58.
+// (48x32), M = 128 11.0, M = 512 29 (64x64), where the weight as bf16 in the
+// workspace and the bf16 contraction take 48; M = 768 41 against 49, M = 1024
+// 52 against 51.
 struct WxTile {
   int md, nt, nw;
   int64_t rowTiles(int64_t M) const { return (M + 8 * md - 1) / (8 * md); }
@@ -2593,7 +2593,7 @@ struct WxTile {
   }
   bool operator==(const WxTile &o) const { return md == o.md && nt == o.nt && nw == o.nw; }
 };
-constexpr int64_t kWxRows = 768; // more rows: the bf16 contraction
+constexpr int64_t kWxRows = 4096; // more are not looked at
 // nullptr: no tile's scales fit the LDS (K past about 200000)
 const WxTile *wxTile(int64_t M, int64_t N, int64_t K, int cpb) {
   static const WxTile tiles[] = {{1, 1, 8}, {1, 2, 8}, {2, 1, 8}, {2, 2, 8}, {2, 4, 8}, {3, 2, 8}, {4, 1, 8},
@@ -2604,6 +2604,21 @@ const WxTile *wxTile(int64_t M, int64_t N, int64_t K, int cpb) {
     if (!best || t.time(M, N, K, cpb) < best->time(M, N, K, cpb)) best = &t;
   }
   return best;
+}
+// The tile for rows straight from the codes, nullptr where the weight as bf16
+// in the workspace and the bf16 contraction are estimated to take less.  (Past
+// the rows that the tiles' times are fitted to, more and more is added to
+// them.)  Over 112 sizes of 384 to 3328 rows, N = 512 .. 11008, K = 448 .. 4096,
+// both code widths, both sides measured: 1.1 % more than the better side on
+// average and 23 % at most; 6.5 % and 67 % with a limit of 768 rows.  us, codes
+// against bf16: [1536, 4096] x [1024, 4096] 21.9 and 34.8, [1024, 512] x [4096,
+// 512] 14.0 and 12.7, [1536, 448] x [1374, 448] 9.7 and 14.4.
+const WxTile *wxFew(int64_t M, int64_t N, int64_t K, int cpb) {
+  if (M > kWxRows) return nullptr;
+  const WxTile *t = wxTile(std::max<int64_t>(M, 1), N, K, cpb);
+  const double weight = 3.5 + (double)(N * K) * (2 + 1.0 / cpb) / 5.2e6;
+  if (t && M > 256 && t->time(M, N, K, cpb) * (1 + M / 1e4) > weight + pickTile(M, N, 2 * K, true, 1).time(M, N, 2 * K)) return nullptr;
+  return t;
 }
 
 KernelPlan lowerMatmul(Analysis &A, const std::string &kname, const LowerOptions &opt) {
@@ -2858,11 +2873,8 @@ KernelPlan lowerMatmul(Analysis &A, const std::string &kname, const LowerOptions
   p.kernelName = kname;
   p.kind = "SINGLE_CUBE";
   std::ostringstream k;
-  // linear_mx: up to kWxRows rows straight from the codes, more through the
-  // weight as bf16 in the workspace and the bf16 contraction
-  const int cpb = wfmt == 4 ? 2 : 1;
-  const WxTile *few = wx ? wxTile(1, N, K, cpb) : nullptr;
-  const bool wxPre = wx && (A.rowsDyn || M > kWxRows || !few);
+  const int cpb = wfmt == 4 ? 2 : 1; // linear_mx: codes a byte
+  const bool wxPre = wx && (A.rowsDyn || !wxFew(M, N, K, cpb));
   std::string params = kernelParamList(A, p.kargs, preA || preB || mxExact || wxPre);
   // epilogue functor receives all kernel pointer arguments
   k << "namespace {\nstruct " << kname << "_args {";
@@ -2923,24 +2935,10 @@ KernelPlan lowerMatmul(Analysis &A, const std::string &kname, const LowerOptions
       << a->argIdx << ", (const uint8_t*)p" << b->argIdx << ", (const uint8_t*)p" << sb->argIdx << ", (" << mtype(oe) << "*)"
       << resultPtr(A, 0) << ", " << Mx << ", " << N << "ll, P);\n}\n";
   };
-  if (few && A.rowsDyn) {
-    std::vector<const WxTile *> emitted;
-    for (int64_t m = 8; m <= kWxRows; m += m < 64 ? 8 : m < 256 ? 32 : 128) {
-      const WxTile *t = wxTile(m, N, K, cpb);
-      const std::string nm = altName(kname, "wx" + std::to_string(8 * t->md) + "x" + std::to_string(16 * t->nt));
-      if (std::find(emitted.begin(), emitted.end(), t) == emitted.end()) {
-        emitted.push_back(t);
-        kernelHead(nm, 64 * t->nw);
-        wxCall(*t);
-      }
-      if (!p.alts.empty() && p.alts.back().name == nm) p.alts.back().maxRows = m;
-      else p.alts.push_back({nm, m, 8 * t->md, t->blocksPerRow(N), (unsigned)(64 * t->nw)});
-    }
-  }
   if (wx) {
     p.algoOps = 2.0 * (double)M * (double)N * (double)K;
     if (!wxPre) {
-      const WxTile &t = *wxTile(std::max<int64_t>(M, 1), N, K, cpb);
+      const WxTile &t = *wxFew(M, N, K, cpb);
       kernelHead(kname, 64 * t.nw);
       wxCall(t);
       p.source = k.str();
@@ -2963,27 +2961,34 @@ KernelPlan lowerMatmul(Analysis &A, const std::string &kname, const LowerOptions
   // a runtime row count: the tile that each count would be given, up to the
   // last that differs from the main kernel's
   if (A.rowsDyn && tiles) {
-    std::vector<ContractionTile> seq, emitted;
-    std::vector<int64_t> top;
-    for (int64_t m = 16; m <= 16384; m += m < 64 ? 16 : 64) {
-      const ContractionTile t = pickTile(m, N, K * esz, bT, mk);
-      if (!seq.empty() && seq.back() == t) { top.back() = m; continue; }
-      seq.push_back(t);
-      top.push_back(m);
+    struct Choice { const WxTile *few; ContractionTile t; int64_t top; };
+    std::vector<Choice> seq;
+    std::vector<std::string> emitted;
+    auto same = [](const Choice &c, const WxTile *few, const ContractionTile &t) { return c.few == few && (few || c.t == t); };
+    // (linear_mx of few rows has smaller tiles)
+    auto step = [&](int64_t m) { return wx && m < 64 ? 8 : m < 64 ? 16 : wx && m < 256 ? 32 : 64; };
+    for (int64_t m = step(0); m <= 16384; m += step(m)) {
+      const Choice c = {wx ? wxFew(m, N, K, cpb) : nullptr, pickTile(m, N, K * esz, bT, mk), m};
+      if (!seq.empty() && same(seq.back(), c.few, c.t)) seq.back().top = m;
+      else seq.push_back(c);
     }
-    if (seq.back() == tile) seq.pop_back();
-    for (size_t i = 0; i < seq.size(); ++i) {
-      const ContractionTile &t = seq[i];
-      if (few && top[i] <= kWxRows) continue;
-      const bool main = ring && t == tile;
-      const std::string nm = main ? kname : altName(kname, std::to_string(t.tm) + "x" + std::to_string(t.tn) + (t.kg > 1 ? "k" + std::to_string(t.kg) : ""));
-      if (!main && std::find(emitted.begin(), emitted.end(), t) == emitted.end()) {
-        emitted.push_back(t);
-        kernelHead(nm, t.threads());
-        if (t.kind == 'r') ringCall();
+    if (same(seq.back(), nullptr, tile)) seq.pop_back();
+    for (const Choice &c : seq) {
+      const ContractionTile &t = c.t;
+      const bool main = !c.few && ring && t == tile;
+      const std::string nm = main    ? kname
+                             : c.few ? altName(kname, "wx" + std::to_string(8 * c.few->md) + "x" + std::to_string(16 * c.few->nt))
+                                     : altName(kname, std::to_string(t.tm) + "x" + std::to_string(t.tn) + (t.kg > 1 ? "k" + std::to_string(t.kg) : ""));
+      const unsigned threads = c.few ? 64 * c.few->nw : t.threads();
+      if (!main && std::find(emitted.begin(), emitted.end(), nm) == emitted.end()) {
+        emitted.push_back(nm);
+        kernelHead(nm, threads);
+        if (c.few) wxCall(*c.few);
+        else if (t.kind == 'r') ringCall();
         else tileCall(t);
       }
-      p.alts.push_back({nm, top[i], t.tm, t.blocksPerRow(N), (unsigned)t.threads(), wx});
+      if (c.few) p.alts.push_back({nm, c.top, 8 * c.few->md, c.few->blocksPerRow(N), threads});
+      else p.alts.push_back({nm, c.top, t.tm, t.blocksPerRow(N), threads, wx});
     }
   }
   kernelHead(kname, threads);
