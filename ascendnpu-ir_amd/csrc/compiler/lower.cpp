@@ -2936,6 +2936,7 @@ KernelPlan lowerMatmul(Analysis &A, const std::string &kname, const LowerOptions
       << resultPtr(A, 0) << ", " << Mx << ", " << N << "ll, P);\n}\n";
   };
   if (wx) {
+    p.align16 = {a->argIdx, b->argIdx};
     p.algoOps = 2.0 * (double)M * (double)N * (double)K;
     if (!wxPre) {
       const WxTile &t = *wxFew(M, N, K, cpb);
@@ -3271,6 +3272,7 @@ static KernelPlan lowerLayerNorm(Analysis &A, const std::string &kname, const Op
   int64_t R, per;
   const std::string rows = leadRows(A, op, sh, R, per);
   const int64_t D = sh.back();
+  if (!A.rowsDyn && R == 0) unsupported(op, "an empty tensor");
   if (D > 16384) unsupported(op, "rows of more than 16384 elements (one workgroup keeps a row)");
   const std::vector<int64_t> lead(sh.begin(), sh.end() - 1);
   std::vector<int64_t> ssh = sh;
@@ -4944,6 +4946,7 @@ std::string emitManifest(const KernelPlan &p, const std::string &hsacoName) {
     << "algo_ops " << (uint64_t)p.algoOps << "\n";
   if (p.rowsDyn) s << "rows_dyn " << p.rowsA << " " << p.rowsB << " " << p.rowsC << " " << p.rowsCap << "\n";
   if (p.rowsZero) s << "rows_zero 1\n";
+  for (const int i : p.align16) s << "align " << i << " 16\n";
   auto shp = [](const std::vector<int64_t> &v) {
     std::string r = std::to_string(v.size());
     for (auto d : v) r += " " + std::to_string(d);

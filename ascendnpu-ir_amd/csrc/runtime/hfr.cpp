@@ -66,6 +66,18 @@ struct RowAlt {
   bool pre = false; // after the group's pre kernels
 };
 
+// Workspaces that a handle owns for launches without a caller's: one a
+// stream, so that launches on two streams may overlap.  A zeroed one keeps
+// what its kernels left there from launch to launch and stays the only one.
+struct OwnWorkspace {
+  void *first = nullptr; // allocated and zeroed when the handle is loaded
+  int device = -1;
+  std::mutex mu;
+  bool taken = false;
+  void *firstStream = nullptr;
+  std::vector<std::pair<void *, void *>> more; // stream, workspace
+};
+
 struct hfr_group {
   std::string func, kernel, hsaco;
   std::vector<PreLaunch> pre;
@@ -87,8 +99,8 @@ struct hfr_group {
   std::vector<Buf> paramBufs, resultBufs;
   std::vector<int> resultTied;
   std::vector<Karg> kargs;
-  void *ownWs = nullptr;
-  int ownWsDevice = -1;
+  std::vector<std::pair<int, int>> align; // parameter, bytes it has to start on
+  std::shared_ptr<OwnWorkspace> own = std::make_shared<OwnWorkspace>();
   // dense staging copies of strided memref views (hfr_group_launch_memref)
   void *stage = nullptr;
   size_t stageBytes = 0;
@@ -114,8 +126,8 @@ struct hfr_program {
   std::vector<uint64_t> tempOffset;
   uint64_t wsBytes = 0;
   std::vector<ProgramStep> steps;
-  void *ownWs = nullptr;
-  int ownWsDevice = -1;
+  uint64_t stepWs = 0; // where the steps' own workspace lies in the program's
+  OwnWorkspace own;
 };
 
 namespace {
@@ -169,6 +181,12 @@ int parseBlock(const std::vector<std::string> &lines, hfr_group &g) {
       g.rowsDyn = true;
       if (g.rowsA < 0 || g.rowsB <= 0 || g.rowsC <= 0 || g.rowsCap < 0)
         return fail(HFR_ERR_MANIFEST, "bad rows_dyn line: " + ln);
+    }
+    else if (key == "align") {
+      int i = -1, bytes = 0;
+      is >> i >> bytes;
+      if (i < 0 || bytes <= 0) return fail(HFR_ERR_MANIFEST, "bad align line: " + ln);
+      g.align.push_back({i, bytes});
     }
     else if (key == "rows_zero") {
       int z = 0;
@@ -291,7 +309,61 @@ int launchRaw(hipFunction_t fn, const hfr_launch_cfg &cfg, const uint64_t *args,
   return HFR_OK;
 }
 
-// Checks a group launch's arguments (counts, null pointers).
+hipError_t ownWorkspaceInit(OwnWorkspace &o, uint64_t bytes) {
+  (void)hipGetDevice(&o.device);
+  hipError_t e = hipMalloc(&o.first, bytes);
+  if (e != hipSuccess) o.first = nullptr;
+  else if ((e = hipMemset(o.first, 0, bytes)) != hipSuccess) {
+    (void)hipFree(o.first);
+    o.first = nullptr;
+  }
+  return e;
+}
+hipError_t ownWorkspaceFree(OwnWorkspace &o) {
+  if (!o.first) return hipSuccess;
+  int cur = 0;
+  (void)hipGetDevice(&cur);
+  (void)hipSetDevice(o.device);
+  hipError_t e = hipFree(o.first);
+  for (auto &m : o.more) {
+    const hipError_t e2 = hipFree(m.second);
+    if (e == hipSuccess) e = e2;
+  }
+  o.first = nullptr;
+  o.more.clear();
+  (void)hipSetDevice(cur);
+  return e;
+}
+// the workspace of a launch on `stream`, allocated at the stream's first one
+int ownWorkspaceOf(OwnWorkspace &o, uint64_t bytes, bool zeroed, void *stream, const char *what, void **ws) {
+  int dev = 0;
+  (void)hipGetDevice(&dev);
+  if (dev != o.device) return fail(HFR_ERR_INVALID, std::string(what) + " workspace belongs to another device");
+  std::lock_guard<std::mutex> lk(o.mu);
+  if (!o.taken) {
+    o.taken = true;
+    o.firstStream = stream;
+  }
+  *ws = o.first;
+  if (zeroed || stream == o.firstStream) return HFR_OK;
+  for (auto &m : o.more)
+    if (m.first == stream) {
+      *ws = m.second;
+      return HFR_OK;
+    }
+  // (a stream under capture somewhere does not mind an allocation of this kind)
+  hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+  (void)hipThreadExchangeStreamCaptureMode(&mode);
+  void *p = nullptr;
+  const hipError_t e = hipMalloc(&p, bytes);
+  (void)hipThreadExchangeStreamCaptureMode(&mode);
+  if (e != hipSuccess) return hipFail(e, "workspace allocation");
+  o.more.push_back({stream, p});
+  *ws = p;
+  return HFR_OK;
+}
+
+// Checks a group launch's arguments (counts, null pointers, alignment).
 int checkGroupArgs(const hfr_group *g, const uint64_t *params, size_t nparams, void *const *results, size_t nresults,
                    int64_t rows = -1) {
   if (!g) return fail(HFR_ERR_INVALID, "null group");
@@ -308,6 +380,10 @@ int checkGroupArgs(const hfr_group *g, const uint64_t *params, size_t nparams, v
   for (size_t i = 0; i < nparams; ++i)
     if (g->paramRoles[i] != "scalar" && params[i] == 0 && !empty(g->paramBufs, i))
       return fail(HFR_ERR_INVALID, "null device pointer for argument " + std::to_string(i));
+  for (const auto &a : g->align)
+    if ((size_t)a.first < nparams && params[a.first] % (uint64_t)a.second)
+      return fail(HFR_ERR_INVALID, "argument " + std::to_string(a.first) + " of @" + g->func + " does not start on " +
+                                       std::to_string(a.second) + " bytes");
   for (size_t i = 0; i < nresults; ++i)
     if (g->resultTied[i] < 0 && (!results || (!results[i] && !empty(g->resultBufs, i))))
       return fail(HFR_ERR_INVALID, "null device pointer for result " + std::to_string(i));
@@ -448,16 +524,11 @@ int hfr_group_load(const char *manifest_path, const char *func, hfr_group_t *out
   // the group's own workspace lives on the device current at load time, so
   // that launches stay asynchronous
   if (g->wsBytes) {
-    int dev = 0;
-    (void)hipGetDevice(&dev);
-    e = hipMalloc(&g->ownWs, g->wsBytes);
-    if (e == hipSuccess) e = hipMemset(g->ownWs, 0, g->wsBytes);
+    e = ownWorkspaceInit(*g->own, g->wsBytes);
     if (e != hipSuccess) {
-      if (g->ownWs) (void)hipFree(g->ownWs);
       hfr_module_unload(g->mod);
       return hipFail(e, "workspace allocation");
     }
-    g->ownWsDevice = dev;
   }
   *out = g.release();
   return HFR_OK;
@@ -466,14 +537,7 @@ int hfr_group_load(const char *manifest_path, const char *func, hfr_group_t *out
 int hfr_group_unload(hfr_group_t g) {
   if (!g) return fail(HFR_ERR_INVALID, "null group");
   int rc = HFR_OK;
-  if (g->ownWs) {
-    int cur = 0;
-    (void)hipGetDevice(&cur);
-    if (g->ownWsDevice >= 0) (void)hipSetDevice(g->ownWsDevice);
-    hipError_t e = hipFree(g->ownWs);
-    (void)hipSetDevice(cur);
-    if (e != hipSuccess) rc = hipFail(e, "hipFree(workspace)");
-  }
+  if (hipError_t e = ownWorkspaceFree(*g->own); e != hipSuccess) rc = hipFail(e, "hipFree(workspace)");
   if (g->stage) {
     int cur = 0;
     (void)hipGetDevice(&cur);
@@ -518,11 +582,10 @@ int hfr_group_launch_rows(hfr_group_t g, const uint64_t *params, size_t nparams,
   if (rc) return rc;
   if (g->rowsDyn && rows == 0 && !g->rowsZero) return HFR_OK; // nothing to do
   void *ws = workspace;
+  if (g->wsBytes && (uintptr_t)ws % 16) return fail(HFR_ERR_INVALID, "a workspace of group @" + g->func + " has to start on 16 bytes");
   if (g->wsBytes && !ws) {
-    int dev = 0;
-    (void)hipGetDevice(&dev);
-    if (dev != g->ownWsDevice) return fail(HFR_ERR_INVALID, "group workspace belongs to another device");
-    ws = g->ownWs;
+    rc = ownWorkspaceOf(*g->own, g->wsBytes, g->wsZero, stream, "group", &ws);
+    if (rc) return rc;
   }
   return launchGroup(g, params, results, ws, stream, rows);
 }
@@ -547,13 +610,7 @@ bool sameBinding(const Binding &a, const Binding &b) { return a.kind == b.kind &
 void freeProgram(hfr_program *p) {
   for (auto &st : p->steps)
     if (st.group) hfr_group_unload(st.group);
-  if (p->ownWs) {
-    int cur = 0;
-    (void)hipGetDevice(&cur);
-    if (p->ownWsDevice >= 0) (void)hipSetDevice(p->ownWsDevice);
-    (void)hipFree(p->ownWs);
-    (void)hipSetDevice(cur);
-  }
+  (void)ownWorkspaceFree(p->own);
   delete p;
 }
 
@@ -644,16 +701,22 @@ int hfr_program_load(const char *manifest_path, const char *name, hfr_program_t 
       }
     }
   }
+  // behind the temporaries the largest workspace of a step (the steps run one
+  // after another; zeroed ones stay their groups')
+  uint64_t most = 0;
+  for (const auto &st : p->steps)
+    if (!st.group->wsZero) {
+      most = std::max(most, st.group->wsBytes);
+      (void)ownWorkspaceFree(*st.group->own);
+    }
+  p->stepWs = (p->wsBytes + 255) / 256 * 256;
+  if (most) p->wsBytes = p->stepWs + most;
   if (p->wsBytes) {
-    int dev = 0;
-    (void)hipGetDevice(&dev);
-    hipError_t e = hipMalloc(&p->ownWs, p->wsBytes);
+    hipError_t e = ownWorkspaceInit(p->own, p->wsBytes);
     if (e != hipSuccess) {
-      p->ownWs = nullptr;
       freeProgram(p);
       return hipFail(e, "hipMalloc(program workspace)");
     }
-    p->ownWsDevice = dev;
   }
   *out = p;
   return HFR_OK;
@@ -690,13 +753,10 @@ int hfr_program_launch(hfr_program_t p, const uint64_t *params, size_t nparams, 
   for (size_t i = 0; i < nresults; ++i)
     if (p->resultParam[i] < 0 && (!results || !results[i]))
       return fail(HFR_ERR_INVALID, "null device pointer for result " + std::to_string(i));
-  char *ws = (char *)workspace;
-  if (p->wsBytes && !ws) {
-    int dev = 0;
-    (void)hipGetDevice(&dev);
-    if (dev != p->ownWsDevice) return fail(HFR_ERR_INVALID, "program workspace belongs to another device");
-    ws = (char *)p->ownWs;
-  }
+  void *wsp = workspace;
+  if (p->wsBytes && !wsp)
+    if (const int rc = ownWorkspaceOf(p->own, p->wsBytes, false, stream, "program", &wsp)) return rc;
+  char *const ws = (char *)wsp;
   auto resolve = [&](const Binding &b) -> uint64_t {
     switch (b.kind) {
     case Binding::Param: return params[b.index];
@@ -713,7 +773,8 @@ int hfr_program_launch(hfr_program_t p, const uint64_t *params, size_t nparams, 
     res.clear();
     for (auto &b : st.args) args.push_back(resolve(b));
     for (auto &b : st.results) res.push_back((void *)(uintptr_t)resolve(b));
-    int rc = hfr_group_launch(st.group, args.data(), args.size(), res.data(), res.size(), nullptr, stream);
+    const bool shares = st.group->wsBytes && !st.group->wsZero;
+    int rc = hfr_group_launch(st.group, args.data(), args.size(), res.data(), res.size(), shares ? ws + p->stepWs : nullptr, stream);
     if (rc) return rc;
   }
   return HFR_OK;

@@ -32,7 +32,7 @@ typedef struct {
 typedef struct {
   PyObject_HEAD
   vectorcallfunc call;
-  PyObject *tensor_type, *raw_stream;
+  PyObject *tensor_type, *raw_stream, *capturing; /* capturing: None, or asked before a call that takes the group's workspace */
   void *fn, *handle;
   int n, nres, dyn;
   Spec spec[MAX_ARGS];
@@ -75,6 +75,13 @@ static int take(const Spec *sp, PyObject *a, int64_t *rows, uint64_t *ptr) {
 static PyObject *call_call(PyObject *self, PyObject *const *args, size_t nargsf, PyObject *kwnames) {
   Call *c = (Call *)self;
   if (PyVectorcall_NARGS(nargsf) != c->n || (kwnames && PyTuple_GET_SIZE(kwnames))) Py_RETURN_NONE;
+  if (c->capturing != Py_None) {
+    PyObject *v = PyObject_CallNoArgs(c->capturing);
+    if (!v) return NULL;
+    const int yes = v == Py_True;
+    Py_DECREF(v);
+    if (yes) Py_RETURN_NONE; /* (the graph's own workspace: the Python path's work) */
+  }
   uint64_t slots[MAX_ARGS];
   void *results[MAX_ARGS] = {0}; /* every result is written into an argument */
   int64_t rows = -1;
@@ -116,6 +123,7 @@ static void call_dealloc(PyObject *self) {
   for (int i = 0; i < c->n; ++i) Py_XDECREF(c->spec[i].dtype);
   Py_XDECREF(c->tensor_type);
   Py_XDECREF(c->raw_stream);
+  Py_XDECREF(c->capturing);
   Py_TYPE(self)->tp_free(self);
 }
 
@@ -131,13 +139,14 @@ static PyTypeObject CallType = {
 };
 
 /* plan(launch address, handle, launch takes rows, torch.Tensor, stream getter,
- *      ((dtype, shape), ...) per argument, tied argument per result) */
+ *      ((dtype, shape), ...) per argument, tied argument per result, capture query) */
 static PyObject *plan(PyObject *self, PyObject *args) {
   (void)self;
   unsigned long long fn, handle;
   int dyn;
-  PyObject *tensor_type, *raw_stream, *specs, *tied;
-  if (!PyArg_ParseTuple(args, "KKpOOO!O!", &fn, &handle, &dyn, &tensor_type, &raw_stream, &PyTuple_Type, &specs, &PyTuple_Type, &tied))
+  PyObject *tensor_type, *raw_stream, *specs, *tied, *capturing = Py_None;
+  if (!PyArg_ParseTuple(args, "KKpOOO!O!|O", &fn, &handle, &dyn, &tensor_type, &raw_stream, &PyTuple_Type, &specs, &PyTuple_Type, &tied,
+                        &capturing))
     return NULL;
   const Py_ssize_t n = PyTuple_GET_SIZE(specs), nres = PyTuple_GET_SIZE(tied);
   if (n < 1 || n > MAX_ARGS || nres < 1 || nres > MAX_ARGS || !fn || !handle) {
@@ -148,7 +157,7 @@ static PyObject *plan(PyObject *self, PyObject *args) {
   if (!c) return NULL;
   c->call = call_call;
   c->n = 0;
-  c->tensor_type = c->raw_stream = NULL;
+  c->tensor_type = c->raw_stream = c->capturing = NULL;
   c->fn = (void *)(uintptr_t)fn;
   c->handle = (void *)(uintptr_t)handle;
   c->dyn = dyn;
@@ -179,8 +188,10 @@ static PyObject *plan(PyObject *self, PyObject *args) {
   }
   Py_INCREF(tensor_type);
   Py_INCREF(raw_stream);
+  Py_INCREF(capturing);
   c->tensor_type = tensor_type;
   c->raw_stream = raw_stream;
+  c->capturing = capturing;
   return (PyObject *)c;
 fail:
   Py_DECREF(c);

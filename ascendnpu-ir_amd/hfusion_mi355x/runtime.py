@@ -174,6 +174,7 @@ class Group:
 
     _plan = None               # _make_plan's answer, from the first plain call
     _call = None               # the same as one C function, False where there is none
+    _scratch = False           # the group has a workspace that no launch reads another's values from
     _row_shapes = (-1, None)   # the last launch-time row count and the argument shapes it makes
 
     def __init__(self, artifact, func=None):
@@ -193,6 +194,7 @@ class Group:
         info = native.GroupInfo()
         native.check(native.hfr().hfr_group_info_get(self._h, ctypes.byref(info)))
         self.info = info
+        self._scratch = info.workspace_bytes > 0 and not self.meta.get("workspace_zero", False)
 
     @property
     def algo_bytes(self):
@@ -211,12 +213,16 @@ class Group:
     def __call__(self, *args, results=None, stream=None, workspace=None, noalloc=False):
         """Launches the group on `stream` (torch's current stream by default).
         noalloc=True goes through hfr_group_launch_noalloc (the library's
-        static scratch instead of a workspace)."""
+        static scratch instead of a workspace).  Without `workspace` the group
+        has one of its own per stream, and under graph capture on the current
+        stream one in the graph's memory, so that launches on several streams
+        and replays of several graphs may overlap (a zeroed workspace, as
+        argmax has, stays the group's only one)."""
         if results is None and stream is None and workspace is None and not noalloc:
             call = self._call
             if call is None:
                 call = self._call = self._make_call()
-            ret = call(*args) if call else self._launch_plain(args)
+            ret = call(*args) if call else None if self._scratch and _capturing() else self._launch_plain(args)
             if type(ret) is int:
                 native.check(ret)
             if ret is not None:
@@ -256,7 +262,7 @@ class Group:
         if any(dt is None or len(sh) > 8 for dt, sh in specs) or len(specs) > 24 or not tied or min(tied) < 0 or not h:
             return False
         return native.hfcall().plan(ctypes.cast(launch, ctypes.c_void_p).value, h.value, rows_at is not None,
-                                    torch.Tensor, raw_stream, specs, tied)
+                                    torch.Tensor, raw_stream, specs, tied, _capture_query() if self._scratch else None)
 
     def _launch_plain(self, args):
         """The launch of a call on the current stream with no options: a call
@@ -370,30 +376,50 @@ class Group:
                     raise ValueError(f"result {j} of @{self.func}: expected {r['elem']}{list(want(r['shape']))}")
                 outs.append(t)
                 rptrs[j] = t.data_ptr()
+        fresh = self._scratch and stream is None and not noalloc and _capturing()
         if stream is None:
             stream = torch.cuda.current_stream(device).cuda_stream
         ret = outs[0] if len(outs) == 1 else tuple(outs)
         lib, h, n, nr = native.hfr(), self._h, len(params), len(res_meta)
-        if noalloc:
-            if workspace is not None:
+        if workspace is not None:
+            if noalloc:
                 raise ValueError("noalloc launches take no workspace")
+            _check_workspace(workspace, self.info.workspace_bytes, self.func)
+        elif fresh:
+            workspace = torch.empty(self.info.workspace_bytes, dtype=torch.uint8, device=device)
+        if noalloc:
 
-            def launch():
+            def launch(keep=workspace):
                 native.check(lib.hfr_group_launch_noalloc(h, slots, n, rptrs, nr, stream))
                 return ret
         elif dyn:
             ws = workspace.data_ptr() if workspace is not None else None
 
-            def launch():
+            def launch(keep=workspace):
                 native.check(lib.hfr_group_launch_rows(h, slots, n, rptrs, nr, rows, ws, stream))
                 return ret
         else:
             ws = workspace.data_ptr() if workspace is not None else None
 
-            def launch():
+            def launch(keep=workspace):
                 native.check(lib.hfr_group_launch(h, slots, n, rptrs, nr, ws, stream))
                 return ret
         return launch
+
+
+def _capture_query():
+    import torch
+    return getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
+
+
+def _capturing():
+    return _capture_query()()
+
+
+def _check_workspace(ws, nbytes, name):
+    import torch
+    if not isinstance(ws, torch.Tensor) or not ws.is_cuda or not ws.is_contiguous() or ws.numel() * ws.element_size() < nbytes:
+        raise ValueError(f"@{name} needs a workspace of {nbytes} bytes (a contiguous device tensor)")
 
 
 def _check_arg(i, a, p, name):
@@ -468,10 +494,13 @@ class Program:
                     raise ValueError(f"result {j} of @{self.name}: expected {r['elem']}{list(r['shape'])}")
                 outs.append(t)
                 rptrs[j] = t.data_ptr()
+        stream_is_current = stream is None
         if stream is None:
             stream = torch.cuda.current_stream(device).cuda_stream
-        if workspace is not None and workspace.numel() * workspace.element_size() < self.workspace_bytes:
-            raise ValueError(f"@{self.name} needs a workspace of {self.workspace_bytes} bytes")
+        if workspace is not None:
+            _check_workspace(workspace, self.workspace_bytes, self.name)
+        elif self.workspace_bytes and stream_is_current and _capturing():
+            workspace = torch.empty(self.workspace_bytes, dtype=torch.uint8, device=device)
         ws = workspace.data_ptr() if workspace is not None else None
         native.check(native.hfr().hfr_program_launch(self._h, slots, len(params), rptrs, len(res_meta), ws, stream))
         return outs[0] if len(outs) == 1 else tuple(outs)

@@ -25,6 +25,11 @@ LINEAR = [
     (17, 100, 1024, "e2m1", True, "bf16"), (33, 257, 2080, "e2m1", False, "bf16"), (64, 50, 4096, "e5m2", False, "bf16"), (48, 129, 512, "e4m3", True, "f32"),
     (65, 100, 544, "e2m1", True, "bf16"), (300, 520, 256, "e4m3", False, "bf16"), (129, 31, 160, "e5m2", True, "f32"),
 ]
+# rows enough for the weight as bf16 in the workspace
+LINEAR_MANY = [(2300, 520, 1024, "e4m3", True, "bf16"), (4500, 40, 288, "e2m1", False, "f32"), (4200, 129, 96, "e5m2", True, "bf16")]
+# more rows than the workgroups take at once
+NORM_LONG = [(2081, 2001, "bf16", "f32", None, 2), (9000, 33, "f16", "f16", "e4m3", 2), (777, 5003, "f32", "f32", None, 1),
+             (4200, 160, "f32", "f32", "e5m2", 2)]
 # the same at a launch-time row count, and the row counts they are called with
 RT_ROWS = [1, 5, 16, 17, 40, 64, 65, 130, 515]
 
@@ -64,10 +69,10 @@ def entries():
         r, n, el, fmt, ax = c
         e[quant_name(c)] = g.quantize_mx(r, n, src=el, fmt=fmt, axis=ax)
         e[quant_name(c, "dequant")] = g.dequantize_mx(r, n, dst=el, fmt=fmt, axis=ax)
-    for c in NORM:
+    for c in NORM + NORM_LONG:
         e[norm_name(c)] = g.layer_norm(**_norm_kw(c))
         e[norm_name(c, "lngrad")] = g.layer_norm_grad(**_norm_kw(c))
-    for m, n, k, fmt, bias, out in LINEAR:
+    for m, n, k, fmt, bias, out in LINEAR + LINEAR_MANY:
         e[linear_name((m, n, k, fmt, bias, out))] = g.linear_mx(m, n, k, fmt=fmt, bias=bias, out=out)
     e["ln_rank3"], e["lngrad_rank3"] = norm_rank3(), norm_grad_rank3()
     rt = lambda ir: g.with_dynamic_rows(ir, _ANY)  # noqa: E731
@@ -82,4 +87,5 @@ def entries():
     # the norm, the quantisation of its result and the block-scaled product
     e["prog_norm_matmul_mx"] = g.layer_norm_matmul_mx(100, 208, 384)
     e["prog_norm_linear_mx"] = g.layer_norm_linear_mx(20, 208, 384)
+    e["prog_norm_linear_mx_many"] = g.layer_norm_linear_mx(2300, 1040, 1024)
     return e

@@ -710,3 +710,291 @@ def test_gradient_without_allocation(gpu):
     outs = grp(*(to_dev(a, p["elem"], gpu) for a, p in zip(args, grp.meta["params"])), noalloc=True)
     torch.cuda.synchronize()
     check_grad(c, [to_host(o, q["elem"]) for o, q in zip(outs, grp.meta["results"])], xv, gm, dy, mean, rstd)
+
+
+# ---------------------------------------------------------------- workspaces, alignment, empty rows
+def test_refused_empty_rows():
+    for ir in (g.layer_norm(0, 64), g.layer_norm_grad(0, 64)):
+        with pytest.raises(RuntimeError, match="empty tensor"):
+            hf.compile(ir)
+
+
+@pytest.mark.gpu
+def test_refused_operands_off_their_alignment(gpu):
+    """Rows and codes of the weight product start on 16 bytes, or the launch
+    is refused and writes nothing; scales may start anywhere."""
+    import torch
+    note("alignment")
+    m, n, k, fmt, bias, out = c = (17, 100, 1024, "e2m1", True, "bf16")
+    grp = hf.compile(cat.get(nc.linear_name(c)), require_cached=True).load()
+    as_, a, w, s, b, wv = linear_inputs(m, n, k, fmt)
+    good = [to_dev(v, p["elem"], gpu) for v, p in zip([as_, w, s, b], grp.meta["params"])]
+
+    def moved(t, by):  # a contiguous view `by` elements into a buffer
+        big = torch.zeros(t.numel() + by, dtype=t.dtype, device=gpu)
+        big[by:] = t.reshape(-1)
+        return big[by:].view(t.shape)
+    for i, by in ((0, 1), (0, 4), (1, 1), (1, 8)):
+        o = torch.full((m, n), 9.0, dtype=torch.bfloat16, device=gpu)
+        with pytest.raises(RuntimeError, match="does not start on 16 bytes"):
+            grp(*(moved(t, by) if j == i else t for j, t in enumerate(good)), o)
+        assert (o == 9.0).all()
+    o = moved(torch.full((m, n), 9.0, dtype=torch.bfloat16, device=gpu), 1)
+    grp(moved(good[0], 8), moved(good[1], 16), moved(good[2], 3), moved(good[3], 1), o)
+    check_linear(to_host(o, "bf16"), "bf16", a, wv, b, k)
+
+
+@pytest.mark.gpu
+def test_refused_workspaces(gpu):
+    import torch
+    note("workspaces refused")
+    c = (6, 33, "f32", "f32", "e5m2", 2)
+    grp = hf.compile(cat.get(nc.norm_name(c, "lngrad")), require_cached=True).load()
+    xs, x, gs, gm, _, _, ds, dy = norm_inputs(c)
+    args, xv, mean, rstd = grad_args(c, xs, x, gs, ds)
+    args = [to_dev(a, p["elem"], gpu) for a, p in zip(args, grp.meta["params"])]
+    need = grp.info.workspace_bytes
+    for ws in (torch.zeros(need - 1, dtype=torch.uint8, device=gpu), torch.zeros(need, dtype=torch.uint8),
+               torch.zeros(2 * need, dtype=torch.uint8, device=gpu)[::2]):
+        with pytest.raises(ValueError, match="needs a workspace"):
+            grp(*args, workspace=ws)
+    with pytest.raises(RuntimeError, match="start on 16 bytes"):
+        grp(*args, workspace=torch.zeros(need + 4, dtype=torch.uint8, device=gpu)[4:])
+    outs = grp(*args, workspace=torch.zeros(need, dtype=torch.uint8, device=gpu))
+    check_grad(c, [to_host(o, q["elem"]) for o, q in zip(outs, grp.meta["results"])], xv, gm, dy, mean, rstd)
+
+
+@pytest.mark.gpu
+def test_plain_calls_on_two_streams_and_graphs_that_overlap(gpu):
+    """One group, plain calls in flight on two streams, and two captured
+    graphs replayed on two streams at once: each has a workspace of its own."""
+    import torch
+    note("overlapping plain calls")
+    grp = hf.compile(cat.get("lngrad_rt"), options=cat.options("lngrad_rt"), require_cached=True).load()
+    lin = hf.compile(cat.get("linmx_e4m3_rt"), options=cat.options("linmx_e4m3_rt"), require_cached=True).load()
+    c = (2100, 1000, "bf16", "f32", "e4m3", 2)
+    cases = []
+    for seed in (3, 4):
+        xs, x, gs, gm, _, _, ds, dy = norm_inputs(c, seed=seed)
+        args, _, _, _ = grad_args(c, xs, x, gs, ds)
+        as_, _, w, s, _, _ = linear_inputs(2100, 1040, 1024, "e4m3", seed=seed)
+        cases.append(([to_dev(a, p["elem"], gpu) for a, p in zip(args, grp.meta["params"])],
+                      [to_dev(a, p["elem"], gpu) for a, p in zip([as_, w, s], lin.meta["params"])]
+                      + [torch.zeros((2100, 1040), dtype=torch.bfloat16, device=gpu)]))
+
+    def run(case):
+        grp(*case[0])
+        lin(*case[1])
+
+    def results(case):
+        return [t.clone() for t in case[0][-3:] + case[1][-1:]]
+
+    def wipe():
+        for case in cases:
+            for t in case[0][-3:] + case[1][-1:]:
+                t.zero_()
+        torch.cuda.synchronize()
+    want = []
+    for case in cases:  # one after another
+        run(case)
+        torch.cuda.synchronize()
+        want.append(results(case))
+    streams = [torch.cuda.Stream() for _ in cases]
+
+    def check():
+        torch.cuda.synchronize()
+        for case, w in zip(cases, want):
+            for p, q in zip(results(case), w):
+                assert torch.equal(p.view(torch.uint8), q.view(torch.uint8))
+    wipe()
+    for _ in range(8):
+        for case, s in zip(cases, streams):
+            with torch.cuda.stream(s):
+                run(case)
+    check()
+    graphs = []
+    for case in cases:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            run(case)
+    for _ in range(3):
+        wipe()
+        for _ in range(4):
+            for gr, s in zip(graphs, streams):
+                with torch.cuda.stream(s):
+                    gr.replay()
+        check()
+
+
+@pytest.mark.gpu
+def test_programs_of_two_graphs(gpu):
+    """A program whose product takes the weight through a workspace, captured
+    twice and replayed on two streams at once."""
+    import torch
+    note("programs of two graphs")
+    m, n, k = 2300, 1040, 1024
+    prog = hf.compile(cat.get("prog_norm_linear_mx_many"), require_cached=True).load()
+    assert prog.workspace_bytes >= 2 * n * k  # (the weight as bf16)
+    cases, want = [], []
+    for seed in (1, 2):
+        rng = np.random.default_rng(seed)
+        (xs, x), (gs, gm), (ts, bt) = (stored(a, "bf16") for a in (activations(rng, m, k), rng.uniform(0.5, 1.5, k), rng.normal(0, 0.1, k)))
+        _, _, w, s, _, wv = linear_inputs(8, n, k, "e2m1", seed=seed)
+        cases.append([to_dev(v, p["elem"], gpu) for v, p in zip([xs, gs, ts, w, s], prog.meta["params"])])
+        want.append(prog(*cases[-1]))
+        torch.cuda.synchronize()
+        # the norm's result is within half a step of bf16 (2^-8) and its f32 sums'
+        # error (below 2^-14 of a value of order 4), the product rounds once more
+        y, _, _ = bs.layer_norm(x, gm, bt, 1e-5)
+        t = (2.0 ** -8 * np.abs(y) + 2.0 ** -12) @ np.abs(wv).T
+        t = t * (1 + 2.0 ** -8) + (2.0 ** -8 + 100 * E24) * (np.abs(y) @ np.abs(wv).T)
+        assert (np.abs(value(to_host(want[-1], "bf16"), "bf16") - y @ wv.T) <= t).all()
+    graphs, held = [], []
+    for args in cases:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            held.append(prog(*args))
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(3):
+        for h in held:
+            h.zero_()
+        torch.cuda.synchronize()
+        for _ in range(4):
+            for gr, s in zip(graphs, streams):
+                with torch.cuda.stream(s):
+                    gr.replay()
+        torch.cuda.synchronize()
+        for h, w in zip(held, want):
+            assert torch.equal(h.view(torch.uint8), w.view(torch.uint8))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("c", nc.LINEAR_MANY, ids=nc.linear_name)
+def test_linear_through_the_workspace(gpu, c):
+    """More rows: the weight as bf16 in the workspace; scale bytes 0 and 255
+    and the largest that bf16 holds go through it too."""
+    m, n, k, fmt, bias, out = c
+    note(nc.linear_name(c))
+    grp = hf.compile(cat.get(nc.linear_name(c)), require_cached=True).load()
+    assert grp.info.workspace_bytes >= 2 * n * k
+    as_, a, w, s, b, wv = linear_inputs(m, n, k, fmt)
+    got, = run_gpu(nc.linear_name(c), [as_, w, s] + [b] * bias + [np.zeros((m, n), interp.NP[out])], gpu)
+    check_linear(got, out, a, wv, b if bias else 0 * b, k)
+    sb = s.view(np.uint8).copy()
+    sb[0, 0], sb[3, -1], sb[5, 0] = 0, 255, 0
+    wv = bs.dequantize(w, sb, fmt, 1)
+    got, = run_gpu(nc.linear_name(c), [as_, w, sb.view(np.int8)] + [b] * bias + [np.zeros((m, n), interp.NP[out])], gpu)
+    nan = np.isnan(wv).any(axis=1)
+    assert nan.sum() == 1 and np.isnan(value(got, out)[:, nan]).all()
+    check_linear(got[:, ~nan], out, a, wv[~nan], (b if bias else 0 * b)[~nan], k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name,n,k,fmt,bias", [("linmx_e2m1_rt", 130, 544, "e2m1", True), ("linmx_e4m3_rt", 1040, 1024, "e4m3", False)])
+def test_linear_of_many_rows_at_launch_time(gpu, name, n, k, fmt, bias):
+    """Past every kernel that reads the codes themselves."""
+    import torch
+    art = hf.compile(cat.get(name), options=cat.options(name), require_cached=True)
+    grp = art.load()
+    with open(art.manifest) as f:
+        few = max(int(ln.split()[2]) for ln in f if ln.startswith("alt ") and not ln.split()[-1] == "pre")
+    for m in (few, few + 1, 4500):
+        note(f"{name} {m}")
+        as_, a, w, s, b, wv = linear_inputs(m, n, k, fmt)
+        out = torch.full((m + 3, n), 9.0, dtype=torch.bfloat16, device=gpu)
+        got = grp(*(to_dev(v, p["elem"], gpu) for v, p in zip([as_, w, s] + [b] * bias, grp.meta["params"])), out[:m])
+        check_linear(to_host(got, "bf16"), "bf16", a, wv, b if bias else 0 * b, k)
+        assert (out[m:] == 9.0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("c", nc.NORM_LONG, ids=nc.norm_name)
+def test_layer_norm_of_many_rows(gpu, c):
+    """Workgroups that walk several rows, the last of them partly or not there."""
+    note(nc.norm_name(c))
+    xs, x, gs, gm, ts, bt, ds, dy = norm_inputs(c)
+    check_norm(c, run_gpu(nc.norm_name(c), norm_args(c, xs, gs, ts), gpu), x, gm, bt)
+    args, x, mean, rstd = grad_args(c, xs, x, gs, ds)
+    # (fewer row groups than 512: more additions one after another)
+    check_grad(c, run_gpu(nc.norm_name(c, "lngrad"), args, gpu), x, gm, dy, mean, rstd, groups=256)
+
+
+@pytest.mark.gpu
+def test_gradient_of_rows_that_are_no_numbers(gpu):
+    """NaN or infinity in dy or x: NaN in that row of dx alone, and in the
+    weight's gradients where the row's values are none."""
+    note("gradient of rows that are no numbers")
+    c = (700, 2001, "bf16", "f32", None, 2)
+    xs, x, gs, gm, _, _, ds, dy = norm_inputs(c)
+    clean, xv, mean, rstd = grad_args(c, xs, x, gs, ds)
+    want = run_gpu(nc.norm_name(c, "lngrad"), clean, gpu)
+    dy[5, 77], dy[9, 2000] = np.nan, np.inf
+    ds, dy = stored(dy, "bf16")
+    got = run_gpu(nc.norm_name(c, "lngrad"), [ds] + clean[1:], gpu)
+    bad = np.zeros(700, bool)
+    bad[[5, 9]] = True
+    dx = value(got[0], "bf16")
+    assert np.isnan(dx[5]).all() and not np.isfinite(dx[9]).any()
+    assert np.array_equal(got[0][~bad].view(np.uint8), want[0][~bad].view(np.uint8))
+    cols = np.zeros(2001, bool)
+    cols[[77, 2000]] = True
+    assert np.isnan(got[2][77]) and np.isinf(got[2][2000]) and not np.isfinite(got[1][cols]).any()
+    for a, b in zip(got[1:], want[1:]):
+        assert np.array_equal(a[~cols], b[~cols])
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits(gpu):
+    """More than 2^31 elements (4.3 GB of bf16): the last rows come out as the
+    same rows alone do."""
+    import torch
+    note("offsets past 32 bits")
+    load = lambda n: hf.compile(cat.get(n), options=cat.options(n), require_cached=True).load()  # noqa: E731
+    tail = 64
+    e = lambda s, d: torch.zeros(s, dtype=d, device=gpu)  # noqa: E731
+
+    def both(grp, cols, rows, make):
+        """The group over `rows` rows, whose last `tail` are random, and over those."""
+        x = e((rows, cols), torch.bfloat16)
+        x[-tail:] = torch.randn(tail, cols, device=gpu)
+        big, small = make(rows), make(tail)
+        grp(x, *big)
+        grp(x[-tail:].clone(), *small)
+        return x, big, small
+    rows, cols = 2 ** 31 // 4096 + 200, 4096
+    x, big, small = both(load("quantmx_e2m1_rt"), cols, rows, lambda r: [e((r, cols // 2), torch.int8), e((r, cols // 32), torch.int8)])
+    for p, q in zip(big, small):
+        assert torch.equal(p[-tail:], q) and not p[:-tail:4099].any()
+    back = e((tail, cols), torch.bfloat16)
+    load("dequantmx_e2m1_rt")(*big, x)
+    load("dequantmx_e2m1_rt")(*small, back)
+    assert torch.equal(x[-tail:], back) and not x[:-tail:4099].any()
+    del x, big, small, back
+    rows, cols = 2 ** 31 // 1000 + 200, 1000
+    gm, bt = e((cols,), torch.bfloat16) + 1.5, e((cols,), torch.bfloat16) + 0.25
+    fwd, bwd = load("ln_rt"), load("lngrad_rt")
+    outs = lambda r: [e((r, cols), torch.bfloat16), e((r,), torch.float32), e((r,), torch.float32),  # noqa: E731
+                      e((r, cols), torch.uint8).view(torch.float8_e4m3fn), e((r, 32), torch.int8)]
+    x, big, small = both(fwd, cols, rows, lambda r: [gm, bt] + outs(r))
+    for p, q in zip(big[2:], small[2:]):
+        assert torch.equal(p[-tail:].view(torch.uint8), q.view(torch.uint8))
+    assert (big[2][:-tail:4099] == 0.25).all()
+    del big[2]
+    # the gradient: x takes dy's place; rows of zeros add nothing to the weight's
+    grads = lambda r: [e((r, cols), torch.bfloat16), e((cols,), torch.float32), e((cols,), torch.float32)]  # noqa: E731
+    gb, gs = grads(rows), grads(tail)
+    bwd(x, big[4], big[5], gm.float(), big[2], big[3], *gb)
+    bwd(x[-tail:].clone(), small[5], small[6], gm.float(), small[3], small[4], *gs)
+    assert torch.equal(gb[0][-tail:], gs[0]) and not gb[0][:-tail:4099].any()
+    for p, q in zip(gb[1:], gs[1:]):  # (the same terms in another order)
+        assert torch.allclose(p, q, rtol=0, atol=float(tail * 64 * E24 * 64))
+    del x, big, small, gb, gs
+    n, k = 130, 544
+    as_, a, w, s, b, wv = linear_inputs(tail, n, k, "e2m1")
+    lin = load("linmx_e2m1_rt")
+    rows = 2 ** 31 // k + 200
+    x, out = e((rows, k), torch.bfloat16), e((rows, n), torch.bfloat16)
+    x[-tail:] = to_dev(as_, "bf16", gpu)
+    lin(x, *(to_dev(v, p["elem"], gpu) for v, p in zip([w, s, b], lin.meta["params"][1:])), out)
+    check_linear(to_host(out[-tail:], "bf16"), "bf16", a, wv, b, k)
+    assert torch.equal(out[0], out[rows // 2]) and torch.equal(out[0], torch.from_numpy(b).to(gpu).bfloat16())

@@ -100,6 +100,29 @@ def test_refused_plans():
             plan(*bad)
 
 
+def test_under_capture():
+    """A group with a workspace leaves a captured call to the Python path."""
+    seen, state = [], [False]
+
+    def launch(*a):
+        seen.append(a[0])
+        return 0
+    fn = LAUNCH(launch)
+    call_keep.append(fn)
+    call = native.hfcall().plan(ctypes.cast(fn, ctypes.c_void_p).value, 0x55, False, Fake, lambda dev: 0, ((F32, (4,)),), (0,),
+                                lambda: state[0])
+    a = Fake(F32, (4,), 0x10)
+    assert call(a) is a and len(seen) == 1
+    state[0] = True
+    assert call(a) is None and len(seen) == 1
+
+    def broken():
+        raise OSError("capture")
+    call = native.hfcall().plan(ctypes.cast(fn, ctypes.c_void_p).value, 0x55, False, Fake, lambda dev: 0, ((F32, (4,)),), (0,), broken)
+    with pytest.raises(OSError, match="capture"):
+        call(a)
+
+
 @pytest.mark.gpu
 def test_same_as_a_launcher(gpu):
     import torch
