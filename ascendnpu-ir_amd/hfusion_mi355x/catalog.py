@@ -3,8 +3,9 @@
 `__graft_entry__.build()` compiles each entry, so that `smoke()` and
 `bench.py` on a GPU machine load prebuilt code objects: the headline
 workloads of `groups.CONFIGS` at their full sizes, the bf16 and [K, N]-layout
-contractions, the block-scaled fp8 contraction, the transpose+cast group, and the reduced RMSNorm+quant group
-the smoke check runs.  The parity cases the tests compile (ragged sizes,
+contractions, the block-scaled fp8 contraction, the transpose+cast group, the layer norm,
+block-scaled codes and weight product of a 4096-wide layer, and the reduced
+RMSNorm+quant group the smoke check runs.  The parity cases the tests compile (ragged sizes,
 every op family of the generic lowering, dynamic dims) live beside the tests.
 """
 from . import groups as g

@@ -12,12 +12,15 @@
  *
  * Ownership: the caller allocates and frees every tensor buffer.  The runtime
  * owns module/group handles and one zero-initialised workspace per group
- * handle that needs one, allocated by hfr_group_load on the current device
- * (launches never allocate).
+ * handle that needs one, allocated by hfr_group_load on the current device.
+ * The first stream that the handle is launched on has it; every other stream
+ * gets one of its own at its first launch of the handle (the only launch that
+ * allocates), except where launches rely on what earlier ones left in a zeroed
+ * workspace: that one stays the handle's only one.
  * Threading: launches are asynchronous on the given stream; the caller
  * synchronises.  A handle must not be used from two threads at once, and two
- * in-flight launches of one group handle that both use its internal workspace
- * must be on the same stream.
+ * in-flight launches that use one workspace must be on the same stream (graphs
+ * captured on one stream share that stream's).
  * Errors: every call returns 0 or a negative HFR_ERR_* code; hfr_last_error()
  * gives the message for the calling thread.
  */
@@ -74,13 +77,15 @@ int hfr_group_info_get(hfr_group_t g, hfr_group_info *info);
 /* params: one slot per group argument (device pointer, or the raw bits of a
  * scalar argument); results: one pointer per group result (ignored — may be
  * NULL — for results written into an argument); workspace: NULL to use the
- * group's own, or a caller buffer of workspace_bytes (zeroed before its first
- * use when the group requires it). */
+ * group's own, or a caller buffer of workspace_bytes that starts on 16 bytes
+ * (zeroed before its first use when the group requires it).  An argument that
+ * the manifest gives an `align` line is refused off those bytes. */
 int hfr_group_launch(hfr_group_t g, const uint64_t *params, size_t nparams, void *const *results, size_t nresults,
                      void *workspace, void *stream);
 /* A group compiled with runtime row counts (compiler option dyn=runtime; its
  * manifest holds `rows_dyn`, and -1 for the row dim of each shape): the same
- * launch over `rows` rows (0: no launch).  One compiled kernel serves every
+ * launch over `rows` rows (0: no launch, unless the manifest holds `rows_zero
+ * 1`: there are results to write, and tensors of no rows may be null).  One compiled kernel serves every
  * row count, where the reference schedules a dynamic-shape kernel once and
  * reads the sizes at run time from its memref descriptors
  * (bishengir/lib/Dialect/HFusion/Transforms/AutoSchedule/AnyPBRSchedule.cpp).
@@ -101,7 +106,7 @@ typedef struct hfr_program_info {
   int nparams;
   int nresults;
   int nsteps;
-  uint64_t workspace_bytes; /* intermediate tensors, 256-byte aligned */
+  uint64_t workspace_bytes; /* intermediate tensors and the steps' workspace, 256-byte aligned */
 } hfr_program_info;
 
 /* name may be NULL when the manifest holds one program. */
@@ -110,9 +115,10 @@ int hfr_program_unload(hfr_program_t p);
 int hfr_program_info_get(hfr_program_t p, hfr_program_info *info);
 /* params: one slot per argument of the original function; results: one
  * pointer per result (ignored for results written into an argument);
- * workspace: NULL to use the program's own (allocated at load), or a
- * caller buffer of workspace_bytes.  Steps are enqueued on `stream`; each
- * group uses its own internal workspace. */
+ * workspace: NULL to use the program's own (allocated at load,
+ * and one for every other stream at its first launch there), or a caller
+ * buffer of workspace_bytes.  Steps are enqueued on `stream`; their groups'
+ * workspaces are part of it (a zeroed one stays the group's own). */
 int hfr_program_launch(hfr_program_t p, const uint64_t *params, size_t nparams, void *const *results, size_t nresults,
                        void *workspace, void *stream);
 

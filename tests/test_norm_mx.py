@@ -998,3 +998,27 @@ def test_offsets_past_32_bits(gpu):
     lin(x, *(to_dev(v, p["elem"], gpu) for v, p in zip([w, s, b], lin.meta["params"][1:])), out)
     check_linear(to_host(out[-tail:], "bf16"), "bf16", a, wv, b, k)
     assert torch.equal(out[0], out[rows // 2]) and torch.equal(out[0], torch.from_numpy(b).to(gpu).bfloat16())
+
+
+@pytest.mark.gpu
+def test_captured_on_a_stream_without_a_workspace_yet(gpu):
+    """A launch with an explicit stream, first met there under capture."""
+    import torch
+    note("captured on a new stream")
+    grp = hf.compile(cat.get("lngrad_rt"), options=cat.options("lngrad_rt"), require_cached=True).load()
+    c = (300, 1000, "bf16", "f32", "e4m3", 2)
+    xs, x, gs, gm, _, _, ds, dy = norm_inputs(c)
+    args, xv, mean, rstd = grad_args(c, xs, x, gs, ds)
+    args = [to_dev(a, p["elem"], gpu) for a, p in zip(args, grp.meta["params"])]
+    grp(*args)  # (the first stream's)
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        grp(*args, stream=side.cuda_stream)
+    for _ in range(3):
+        for t in args[-3:]:
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        check_grad(c, [to_host(o, q["elem"]) for o, q in zip(args[-3:], grp.meta["results"])], xv, gm, dy, mean, rstd)
+        grp(*args)
