@@ -3250,6 +3250,24 @@ static LnShape lnGradShape(int64_t D, int64_t V) {
   return {T, (acc + T - 1) / T, std::max<int64_t>(1, 512 / T)};
 }
 
+// The gradient of few rows in one launch (hf_ln.h, ln_grad_once): it reads dy
+// and x a second time, by columns, where the two launches write and read
+// partial sums.  Columns a workgroup: as many of 8 .. 32 as still make 96
+// workgroups (a CU pulls about 20 GB/s past its L2: [777, 2001] f32 12.1 us with
+// 32, 10.0 with 16).
+static int64_t lnGradSlab(int64_t D) {
+  int64_t c = 32;
+  while (c > 8 && (D + c - 1) / c < 96) c /= 2;
+  return c;
+}
+// Rows up to which one launch takes less, us of a call, one launch and two:
+// bf16 [256, 4096] 6.5 and 8.6, [777, 4096] 12.1 and 13.3, [1024, 4096] 13.9 and
+// 13.4, [777, 16384] 29.7 and 31.5, [1024, 16384] 36.5 and 33.8; f32 [64, 1024] 5.3
+// and 9.0, [777, 8192] 21.7 and 24.5, [1024, 8192] 28.3 and 26.2; short rows: bf16
+// [1536, 1024] 8.0 and 11.1, f32 [1536, 1024] 14.1 and 11.2, [2048, 256] 6.9 and 11.4,
+// [4096, 256] 15.6 and 11.1.
+static int64_t lnGradOnceRows(int64_t D) { return std::max<int64_t>(896, std::min<int64_t>(2048, 1200000 / D)); }
+
 static KernelPlan lowerLayerNorm(Analysis &A, const std::string &kname, const Op *op, const std::vector<std::string> &outPtr) {
   const bool grad = op->name == "hfusion.layer_norm_grad";
   const int ck = mxFormatOf(op, "format");
@@ -3298,9 +3316,9 @@ static KernelPlan lowerLayerNorm(Analysis &A, const std::string &kname, const Op
   const int64_t V = y->type.elem == Elem::F32 ? 4 : 8;
   const LnShape s = grad ? lnGradShape(D, V) : lnForwardShape(D, V);
   const int64_t threads = s.T * s.RPB;
-  auto targs = [&](const std::string &pel) {
+  auto targs = [&](const std::string &pel, const char *more = "") {
     return "<" + el + ", " + pel + ", " + std::to_string(aff) + ", " + std::to_string(ck) + ", " + std::to_string(s.T) + ", " +
-           std::to_string(s.NCH) + ", " + std::to_string(s.RPB) + ", " + std::to_string(D) + "ll>(";
+           std::to_string(s.NCH) + ", " + std::to_string(s.RPB) + ", " + std::to_string(D) + "ll" + more + ">(";
   };
   p.block[0] = (unsigned)threads;
   p.variant = std::to_string(s.T) + " threads a row" + (ck >= 0 ? std::string(", 8-bit checkpoint ") + mxFormatName(ck) : "");
@@ -3341,17 +3359,33 @@ static KernelPlan lowerLayerNorm(Analysis &A, const std::string &kname, const Op
   p.kind = "LAYER_NORM_GRAD";
   // workgroups that walk the rows, each leaving one row of partial sums
   const int64_t cap = 256;
-  const std::string call = "  hf::ln_grad_rows" + targs(param ? mxElem(op, param) : el);
+  const std::string pel = param ? mxElem(op, param) : el, call = "  hf::ln_grad_rows" + targs(pel, aff > 0 ? ", true" : ", false");
   // the row kernel's arguments by name: dy x scales gamma mean rstd dx ws
   auto body = [&](const std::vector<std::string> &a) {
     return call + a[0] + ", " + a[1] + ", " + a[2] + ", " + a[3] + ", (const float *)" + a[4] + ", (const float *)" + a[5] + ", " + a[6] +
-           ", (float *)" + a[7] + ", " + rows + ");\n}\n";
+           ", (float *)" + a[7] + ", " + rows + ", blockIdx.x, gridDim.x);\n}\n";
   };
   const std::string scl = ck >= 0 ? in(2) : "nullptr", gam = aff > 0 ? in(at - 1) : "nullptr";
   if (aff == 0) {
     k << "extern \"C\" __global__ __launch_bounds__(" << threads << ") void " << kname << "(" << kernelParamList(A, p.kargs, false) << ") {\n"
       << body({in(0), in(1), scl, gam, in(at), in(at + 1), outPtr[0], "nullptr"});
     rowGrid(A, p, R, per, 1, s.RPB, cap);
+    p.source = k.str();
+    return p;
+  }
+  // few rows: one launch
+  const int64_t once = lnGradOnceRows(D), slab = lnGradSlab(D), columns = ((D + slab - 1) / slab + 7) / 8 * 8;
+  auto onceBlocks = [&](int64_t rows) { return columns + std::min(256 * std::max<int64_t>(1, 1024 / threads), (rows + s.RPB - 1) / s.RPB); };
+  auto onceKernel = [&](const std::string &name, const std::string &params) {
+    k << "extern \"C\" __global__ __launch_bounds__(" << threads << ") void " << name << "(" << params << ") {\n"
+      << "  hf::ln_grad_once" << targs(pel, (", " + std::to_string(slab)).c_str()) << in(0) << ", " << in(1) << ", " << scl << ", " << gam << ", (const float *)" << in(at)
+      << ", (const float *)" << in(at + 1) << ", " << outPtr[0] << ", " << outPtr[1] << ", " << (aff > 1 ? outPtr[2] : "nullptr") << ", "
+      << rows << ");\n}\n";
+  };
+  if (!A.rowsDyn && R <= once) {
+    onceKernel(kname, kernelParamList(A, p.kargs, false));
+    p.grid[0] = (unsigned)onceBlocks(R);
+    p.variant += ", one launch";
     p.source = k.str();
     return p;
   }
@@ -3369,6 +3403,13 @@ static KernelPlan lowerLayerNorm(Analysis &A, const std::string &kname, const Op
     << pk.grid << ", " << outPtr[1] << ", " << (aff > 1 ? outPtr[2] : "nullptr") << ");\n}\n";
   p.grid[0] = (unsigned)(((int64_t)aff * D + 31) / 32);
   p.block[0] = 1024;
+  if (A.rowsDyn && once > 0) {
+    const std::string nm = altName(kname, "once");
+    std::vector<std::string> kargs;
+    onceKernel(nm, kernelParamList(A, kargs, true));
+    for (const int64_t top : {std::min(32 * s.RPB, once), once})
+      if (p.alts.empty() || p.alts.back().maxRows < top) p.alts.push_back({nm, top, top, onceBlocks(top), (unsigned)threads});
+  }
   p.rowsDyn = A.rowsDyn;
   p.rowsZero = A.rowsDyn; // no rows: the weight's gradients are zeros
   p.workspaceBytes = (uint64_t)pk.grid * aff * D * 4;

@@ -431,7 +431,7 @@ int launchGroup(const hfr_group *g, const uint64_t *params, void *const *results
         if (rc) return rc;
       }
       hfr_launch_cfg cfg{};
-      cfg.grid[0] = (unsigned)((rows + alt.rowsB - 1) / alt.rowsB * alt.rowsC);
+      cfg.grid[0] = (unsigned)((std::max<int64_t>(rows, 1) + alt.rowsB - 1) / alt.rowsB * alt.rowsC); // (no rows only with rows_zero)
       cfg.grid[1] = cfg.grid[2] = cfg.block[1] = cfg.block[2] = 1;
       cfg.block[0] = alt.block;
       return launch(alt.fn, cfg, g->kargs);
