@@ -27,6 +27,8 @@ LINEAR = [
 ]
 # rows enough for the weight as bf16 in the workspace
 LINEAR_MANY = [(2300, 520, 1024, "e4m3", True, "bf16"), (4500, 40, 288, "e2m1", False, "f32"), (4200, 129, 96, "e5m2", True, "bf16")]
+# k to the end of what a workgroup's scales leave of LDS, and past it
+LINEAR_LONG = [(3, 20, 131072, "e2m1", False, "f32"), (9, 33, 98304, "e4m3", False, "f32"), (2, 16, 262144, "e5m2", False, "f32")]
 # more rows than the workgroups take at once
 NORM_LONG = [(2081, 2001, "bf16", "f32", None, 2), (9000, 33, "f16", "f16", "e4m3", 2), (777, 5003, "f32", "f32", None, 1),
              (4200, 160, "f32", "f32", "e5m2", 2)]
@@ -72,8 +74,9 @@ def entries():
     for c in NORM + NORM_LONG:
         e[norm_name(c)] = g.layer_norm(**_norm_kw(c))
         e[norm_name(c, "lngrad")] = g.layer_norm_grad(**_norm_kw(c))
-    for m, n, k, fmt, bias, out in LINEAR + LINEAR_MANY:
+    for m, n, k, fmt, bias, out in LINEAR + LINEAR_MANY + LINEAR_LONG:
         e[linear_name((m, n, k, fmt, bias, out))] = g.linear_mx(m, n, k, fmt=fmt, bias=bias, out=out)
+    e["linmx_filled"] = g.linear_mx(5, 48, 64, out="f32").replace("0.000000e+00", "1.500000e+00")
     e["ln_rank3"], e["lngrad_rank3"] = norm_rank3(), norm_grad_rank3()
     rt = lambda ir: g.with_dynamic_rows(ir, _ANY)  # noqa: E731
     e["quantmx_e4m3_rt"] = rt(g.quantize_mx(_ANY, 100))

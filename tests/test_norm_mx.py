@@ -1025,3 +1025,24 @@ def test_captured_on_a_stream_without_a_workspace_yet(gpu):
         torch.cuda.synchronize()
         check_grad(c, [to_host(o, q["elem"]) for o, q in zip(args[-3:], grp.meta["results"])], xv, gm, dy, mean, rstd, groups=256)
         grp(*args)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("c", nc.LINEAR_LONG, ids=nc.linear_name)
+def test_linear_of_long_k(gpu, c):
+    m, n, k, fmt, bias, out = c
+    note(nc.linear_name(c))
+    grp = hf.compile(cat.get(nc.linear_name(c)), require_cached=True).load()
+    assert (grp.info.workspace_bytes > 0) == (k > 200000)
+    as_, a, w, s, b, wv = linear_inputs(m, n, k, fmt)
+    got, = run_gpu(nc.linear_name(c), [as_, w, s, np.zeros((m, n), np.float32)], gpu)
+    check_linear(got, out, a, wv, 0 * b, k)
+
+
+@pytest.mark.gpu
+def test_linear_onto_a_constant(gpu):
+    """The accumulator's fill is added, as matmul_mx does."""
+    note("linear onto a constant")
+    as_, a, w, s, b, wv = linear_inputs(5, 48, 64, "e2m1")
+    got, = run_gpu("linmx_filled", [as_, w, s, np.zeros((5, 48), np.float32)], gpu)
+    check_linear(got, "f32", a, wv, 0 * b + 1.5, 64)
