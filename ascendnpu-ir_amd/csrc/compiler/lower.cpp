@@ -3224,25 +3224,26 @@ static KernelPlan lowerMxCodes(Analysis &A, const std::string &kname, const Op *
 // Layer norm and its gradient.  Threads of a row group, chunks of eight
 // elements a thread and row groups a workgroup by the row's length.
 struct LnShape { int64_t T, NCH, RPB; };
-// D elements of a row, V to a 16-byte access.  us, bf16 with an 8-bit
-// checkpoint: [8192, 4096] 31.9 with 256 threads of two accesses a row, 33.4
-// with 512 of one, 30.8 with 128 of four, which cost [16, 4096] 4.0 instead of
-// 3.5; [2048, 16384] 30.7 with 512 threads of four, 34.6 with 1024 of two
-// (f32 rows are twice the bytes).  A row of at most 16 accesses has 8 or 16
+// D elements of a row, V to a 16-byte access.  us of a call, bf16 with an 8-bit
+// checkpoint: [8192, 4096] 32.4 with 256 threads of two accesses a row, 34.0
+// with 512 of one, 31.7 with 128 of four, which costs few rows more ([16, 4096]
+// 6.2 for 6.0); [2048, 16384] 33.9 with 1024 threads of two, 34.6 with 512 of
+// four (f32 rows are twice the bytes).  A row of at most 16 accesses has 8 or 16
 // lanes of a wave.
 static LnShape lnForwardShape(int64_t D, int64_t V) {
   const int64_t acc = (D + V - 1) / V;
   if (acc <= 16) return {acc <= 8 ? 8 : 16, 1, acc <= 8 ? 32 : 16};
-  const int64_t most = V == 4 || acc > 1024 ? 4 : 2;
+  const int64_t most = V == 4 ? 4 : 2;
   const int64_t T = (acc + 64 * most - 1) / (64 * most) * 64;
   return {T, (acc + T - 1) / T, std::max<int64_t>(1, 256 / T)};
 }
 // The gradient: workgroups of 512 threads, one a CU, so that few rows of
-// partial sums are left.  us, [8192, 4096] from an 8-bit checkpoint: 32.2 with
-// two row groups of 256 threads and two accesses, 39.3 of 512 and one (1024
-// threads a workgroup), 68.7 with four row groups of 256; 35.5 with 512
-// workgroups (16.8 MB of partial sums instead of 8.4).  [2048, 16384]: 39.8
-// with 1024 threads of two accesses, 47.7 with 512 of four.
+// partial sums are left.  us of a call from an 8-bit checkpoint, [8192, 4096]:
+// 35.8 with two row groups of 256 threads and two accesses, 35.3 of 512 and one
+// (1024 threads a workgroup), 46.6 with four groups of 256, 38.2 with 512
+// workgroups (16.8 MB of partial sums instead of 8.4).  [8192, 8192]: 64.0 with 512
+// threads of two, 71.2 with 1024 of one; [2048, 16384]: 49.5 with 1024 of two, 54.4
+// with 512 of four.
 static LnShape lnGradShape(int64_t D, int64_t V) {
   const int64_t acc = (D + V - 1) / V;
   if (acc <= 16) return {acc <= 8 ? 8 : 16, 1, acc <= 8 ? 32 : 16};
