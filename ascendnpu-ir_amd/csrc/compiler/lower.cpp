@@ -2937,6 +2937,7 @@ KernelPlan lowerMatmul(Analysis &A, const std::string &kname, const LowerOptions
   };
   if (wx) {
     p.align16 = {a->argIdx, b->argIdx};
+    p.apart = {a->argIdx, b->argIdx, sb->argIdx}; // (what the epilogue reads, it reads where it writes)
     p.algoOps = 2.0 * (double)M * (double)N * (double)K;
     if (!wxPre) {
       const WxTile &t = *wxFew(M, N, K, cpb);
@@ -3191,6 +3192,7 @@ static KernelPlan lowerMxCodes(Analysis &A, const std::string &kname, const Op *
   checkScales(op, scales, ssh);
   const std::string el = mxElem(op, x);
   KernelPlan p;
+  for (size_t i = 0; i < A.params.size(); ++i) p.apart.push_back((int)i);
   p.kernelName = kname;
   p.kind = de ? "DEQUANTIZE_MX" : "QUANTIZE_MX";
   p.variant = std::string(mxFormatName(fmt)) + (cols ? ", blocks down the columns" : ", blocks along the rows");
@@ -3312,6 +3314,7 @@ static KernelPlan lowerLayerNorm(Analysis &A, const std::string &kname, const Op
   };
   auto in = [&](size_t i) { return "p" + std::to_string(op->ins[i]->argIdx); };
   KernelPlan p;
+  for (size_t i = 0; i < A.params.size(); ++i) p.apart.push_back((int)i);
   p.kernelName = kname;
   std::ostringstream k;
   const int64_t V = y->type.elem == Elem::F32 ? 4 : 8;
@@ -4988,6 +4991,11 @@ std::string emitManifest(const KernelPlan &p, const std::string &hsacoName) {
     << "algo_ops " << (uint64_t)p.algoOps << "\n";
   if (p.rowsDyn) s << "rows_dyn " << p.rowsA << " " << p.rowsB << " " << p.rowsC << " " << p.rowsCap << "\n";
   if (p.rowsZero) s << "rows_zero 1\n";
+  if (!p.apart.empty()) {
+    s << "apart";
+    for (const int i : p.apart) s << " " << i;
+    s << "\n";
+  }
   for (const int i : p.align16) s << "align " << i << " 16\n";
   auto shp = [](const std::vector<int64_t> &v) {
     std::string r = std::to_string(v.size());

@@ -65,6 +65,7 @@ struct KernelPlan {
   bool rowsDyn = false;
   int64_t rowsA = 0, rowsB = 1, rowsC = 1, rowsCap = 0;
   bool rowsZero = false; // a launch of no rows has results to write
+  std::vector<int> apart; // arguments that no destination may overlap (refused at launch)
   std::vector<int> align16; // arguments that have to start on 16 bytes (refused at launch)
 };
 

@@ -99,6 +99,7 @@ struct hfr_group {
   std::vector<Buf> paramBufs, resultBufs;
   std::vector<int> resultTied;
   std::vector<Karg> kargs;
+  std::vector<int> apart;                 // parameters that no written one may overlap
   std::vector<std::pair<int, int>> align; // parameter, bytes it has to start on
   std::shared_ptr<OwnWorkspace> own = std::make_shared<OwnWorkspace>();
   // dense staging copies of strided memref views (hfr_group_launch_memref)
@@ -181,6 +182,10 @@ int parseBlock(const std::vector<std::string> &lines, hfr_group &g) {
       g.rowsDyn = true;
       if (g.rowsA < 0 || g.rowsB <= 0 || g.rowsC <= 0 || g.rowsCap < 0)
         return fail(HFR_ERR_MANIFEST, "bad rows_dyn line: " + ln);
+    }
+    else if (key == "apart") {
+      for (int i; is >> i;) g.apart.push_back(i);
+      is.clear();
     }
     else if (key == "align") {
       int i = -1, bytes = 0;
@@ -380,6 +385,19 @@ int checkGroupArgs(const hfr_group *g, const uint64_t *params, size_t nparams, v
   for (size_t i = 0; i < nparams; ++i)
     if (g->paramRoles[i] != "scalar" && params[i] == 0 && !empty(g->paramBufs, i))
       return fail(HFR_ERR_INVALID, "null device pointer for argument " + std::to_string(i));
+  if (!g->apart.empty()) {
+    auto end = [&](size_t i) {
+      uint64_t n = elemSize(g->paramBufs[i].elem);
+      for (const int64_t d : g->paramBufs[i].shape) n *= (uint64_t)(d < 0 ? rows : d);
+      return params[i] + n;
+    };
+    for (size_t o = 0; o < nparams && o < g->paramBufs.size(); ++o) {
+      if (g->paramRoles[o] == "in" || g->paramRoles[o] == "scalar") continue;
+      for (const int j : g->apart)
+        if ((size_t)j != o && (size_t)j < g->paramBufs.size() && params[o] < end(j) && params[j] < end(o))
+          return fail(HFR_ERR_INVALID, "argument " + std::to_string(o) + " of @" + g->func + " is written and overlaps argument " + std::to_string(j));
+    }
+  }
   for (const auto &a : g->align)
     if ((size_t)a.first < nparams && params[a.first] % (uint64_t)a.second)
       return fail(HFR_ERR_INVALID, "argument " + std::to_string(a.first) + " of @" + g->func + " does not start on " +

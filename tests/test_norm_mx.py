@@ -1046,3 +1046,37 @@ def test_linear_onto_a_constant(gpu):
     as_, a, w, s, b, wv = linear_inputs(5, 48, 64, "e2m1")
     got, = run_gpu("linmx_filled", [as_, w, s, np.zeros((5, 48), np.float32)], gpu)
     check_linear(got, "f32", a, wv, 0 * b + 1.5, 64)
+
+
+@pytest.mark.gpu
+def test_refused_overlapping_operands(gpu):
+    """A destination over an operand, or over another destination, is refused
+    and nothing is written; buffers side by side are not."""
+    import torch
+    note("overlaps")
+    grp = hf.compile(cat.get("lngrad_wide_rt"), options=cat.options("lngrad_wide_rt"), require_cached=True).load()
+    c = (20, 4096, "bf16", "bf16", None, 2)
+    xs, x, gs, gm, _, _, ds, dy = norm_inputs(c)
+    args, xv, mean, rstd = grad_args(c, xs, x, gs, ds)
+    args = [to_dev(a, p["elem"], gpu) for a, p in zip(args, grp.meta["params"])]
+    before = [t.clone() for t in args]
+    for out, other in ((5, 0), (5, 1), (6, 2), (6, 7)):
+        bad = list(args)
+        bad[out] = bad[other]
+        with pytest.raises(RuntimeError, match="is written and overlaps"):
+            grp(*bad)
+    both = torch.empty(2 * 20 * 4096 - 1, dtype=torch.bfloat16, device=gpu)
+    both[:20 * 4096] = args[0].reshape(-1)
+    with pytest.raises(RuntimeError, match="is written and overlaps"):
+        grp(both[:20 * 4096].view(20, 4096), *args[1:5], both[20 * 4096 - 1:].view(20, 4096), *args[6:])
+    for t, b in zip(args, before):
+        assert torch.equal(t, b)
+    both = torch.empty((40, 4096), dtype=torch.bfloat16, device=gpu)
+    both[:20] = args[0]
+    outs = grp(both[:20], *args[1:5], both[20:], *args[6:])
+    check_grad(c, [to_host(o, q["elem"]) for o, q in zip(outs, grp.meta["results"])], xv, gm, dy, mean, rstd)
+    lin = hf.compile(cat.get("linmx_e2m1_rt"), options=cat.options("linmx_e2m1_rt"), require_cached=True).load()
+    a = torch.zeros((130, 544), dtype=torch.bfloat16, device=gpu)
+    w, s, b = (torch.zeros(p["shape"], dtype=hf.runtime.torch_dtype(p["elem"]), device=gpu) for p in lin.meta["params"][1:4])
+    with pytest.raises(RuntimeError, match="is written and overlaps"):
+        lin(a, w, s, b, a.reshape(-1)[:130 * 130].view(130, 130))
