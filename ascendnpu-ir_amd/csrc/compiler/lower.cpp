@@ -3239,6 +3239,16 @@ static LnShape lnForwardShape(int64_t D, int64_t V) {
   const int64_t T = (acc + 64 * most - 1) / (64 * most) * 64;
   return {T, (acc + T - 1) / T, std::max<int64_t>(1, 256 / T)};
 }
+// Workgroups of the forward pass, which walk the rows: as many a CU as hold 6 MB
+// of rows (as much again is on its way).  More take turns at HBM that the last
+// rows wait for, fewer leave it idle.  us of a call with 512, 768, 1024 and 2048
+// workgroups: [8192, 4096] bf16 with an 8-bit checkpoint 35.4, 31.5, 32.4, 32.0;
+// [777, 5003] f32 8.4, 9.0, 9.3, -; [777, 8192] bf16 6.8, 8.2, 8.2, 8.2; [3000, 2001]
+// bf16 7.8, 7.0, 6.9, 7.9; [20000, 320] bf16 11.7, 9.9, 9.6, 8.0.
+static int64_t lnForwardBlocks(const LnShape &s, int64_t rowBytes) {
+  const int64_t cu = 256 * s.RPB * rowBytes;
+  return 256 * std::min<int64_t>(8, ((6 << 20) + cu - 1) / cu);
+}
 // The gradient: workgroups of 512 threads, one a CU, so that few rows of
 // partial sums are left.  us of a call from an 8-bit checkpoint, [8192, 4096]:
 // 35.8 with two row groups of 256 threads and two accesses, 35.3 of 512 and one
@@ -3343,7 +3353,7 @@ static KernelPlan lowerLayerNorm(Analysis &A, const std::string &kname, const Op
       << "  hf::ln_forward" << targs(param ? mxElem(op, param) : el) << in(0) << ", " << (aff > 0 ? in(1) : "nullptr") << ", "
       << (aff > 1 ? in(2) : "nullptr") << ", " << outPtr[0] << ", (float *)" << outPtr[1] << ", (float *)" << outPtr[2] << ", "
       << (ck >= 0 ? outPtr[3] + ", " + outPtr[4] : "nullptr, nullptr") << ", " << rows << ", " << floatLit(eps) << ");\n}\n";
-    rowGrid(A, p, R, per, 1, s.RPB, 256 * std::max<int64_t>(1, 1024 / threads));
+    rowGrid(A, p, R, per, 1, s.RPB, lnForwardBlocks(s, D * (16 / V)));
     p.source = k.str();
     return p;
   }
