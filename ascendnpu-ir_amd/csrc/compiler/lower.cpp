@@ -2454,6 +2454,15 @@ std::string altName(const std::string &kname, const std::string &what) { return 
 
 constexpr int MK_BF16_CODE = 1; // hf::MK_BF16
 
+int mxFormatOf(const Op *op, const char *attr);
+void checkCodes(const Op *op, const Value *v, int fmt, std::vector<int64_t> shape, size_t axis);
+void checkScales(const Op *op, const Value *v, const std::vector<int64_t> &shape);
+const char *mxFormatName(int fmt);
+// 16-byte accesses of values that a thread has in flight (hf_mx.h).  us:
+// quantising [8192, 4096] bf16 to 8 bits 17.6 with two, 17.9 with four, 21.8 with
+// one; reading e2m1 [4096, 4096] back to bf16 8.2 with four, 10.3 with one.
+constexpr int kMxAhead = 2, kMxReadAhead = 4;
+
 // The tile of a contraction.  A tile's time is what its CU takes to pull
 // (tm + tn) K bytes through its LDS and multiply them, and 256 CUs work at
 // once: large tiles move fewer bytes, small ones fill the chip.  The numbers
@@ -2475,14 +2484,6 @@ constexpr int MK_BF16_CODE = 1; // hf::MK_BF16
 // (256x128) against 46.1 (128x128 and 256x256); M = 5000 103 (256x256) against
 // 125 (128x128).  bf16, M = 5000, N = 1024, K = 4096: 60 (256x128) against 65
 // (256x256) and 93 (128x64).
-int mxFormatOf(const Op *op, const char *attr);
-void checkCodes(const Op *op, const Value *v, int fmt, std::vector<int64_t> shape, size_t axis);
-void checkScales(const Op *op, const Value *v, const std::vector<int64_t> &shape);
-const char *mxFormatName(int fmt);
-// 16-byte accesses of values that a thread has in flight (hf_mx.h).  us:
-// quantising [8192, 4096] bf16 to 8 bits 17.6 with two, 17.9 with four, 21.8 with
-// one; reading e2m1 [4096, 4096] back to bf16 8.2 with four, 10.3 with one.
-constexpr int kMxAhead = 2, kMxReadAhead = 4;
 
 struct TileTime {
   double fixed, queued, one, second, more, part1, part, tall;
