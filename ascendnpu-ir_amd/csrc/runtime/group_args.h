@@ -1,0 +1,146 @@
+// A group's arguments as its manifest describes them, and the checks that a
+// launch's pass before anything runs.  No HIP in here: what a launch accepts
+// does not depend on the device.
+#pragma once
+#include <algorithm>
+#include <cstddef>
+#include <cstdint>
+#include <sstream>
+#include <string>
+#include <utility>
+#include <vector>
+
+// element size of a manifest element type name (i1 is one byte)
+inline int elemSize(const std::string &e) {
+  if (e == "f64" || e == "i64" || e == "index") return 8;
+  if (e == "f32" || e == "i32") return 4;
+  if (e == "f16" || e == "bf16" || e == "i16") return 2;
+  return 1;
+}
+
+struct Buf {
+  std::string elem;
+  std::vector<int64_t> shape;
+};
+
+struct GroupArgs {
+  std::string func;
+  bool rowsDyn = false; // the row count comes with the launch (-1 in the shapes)
+  // a launch of no rows has results to write (manifest `rows_zero 1`); its
+  // tensors of no rows may be null
+  bool rowsZero = false;
+  std::vector<std::string> paramRoles;
+  std::vector<Buf> paramBufs, resultBufs;
+  std::vector<int> resultTied;
+  std::vector<int> apart;                 // parameters that no written one may overlap
+  std::vector<std::pair<int, int>> align; // parameter, bytes it has to start on
+
+  // Takes a manifest line of these; false: the key is another's.  A malformed
+  // line leaves the stream failed.
+  bool line(const std::string &key, std::istringstream &is) {
+    if (key == "apart") {
+      for (int i; is >> i;) apart.push_back(i);
+      is.clear();
+    } else if (key == "align") {
+      int i = -1, bytes = 0;
+      is >> i >> bytes;
+      if (i < 0 || bytes <= 0) is.setstate(std::ios::failbit);
+      align.push_back({i, bytes});
+    } else if (key == "rows_zero") {
+      int z = 0;
+      is >> z;
+      rowsZero = z != 0;
+    } else if (key == "param" || key == "result") {
+      int i, tied = -1, rank = 0;
+      std::string role;
+      Buf b;
+      is >> i;
+      if (key == "param") is >> role;
+      else is >> tied;
+      is >> b.elem >> rank;
+      for (int d = 0; d < rank && is; ++d) { int64_t x; is >> x; b.shape.push_back(x); }
+      if (key == "param") { paramRoles.push_back(role); paramBufs.push_back(b); }
+      else { resultTied.push_back(tied); resultBufs.push_back(b); }
+    } else {
+      return false;
+    }
+    return true;
+  }
+
+  // After the manifest's last line: what the overlap check needs of it, so
+  // that a launch only adds and compares (names compared and shapes multiplied
+  // at every launch made a call of few rows 0.4 us longer).  False: more
+  // arguments than a launch passes.
+  bool prepare() {
+    spans.clear();
+    pairs.clear();
+    if (apart.empty()) return true;
+    auto at = [&](int i) {
+      for (size_t s = 0; s < spans.size(); ++s)
+        if (spans[s].index == i) return s;
+      Span sp;
+      sp.index = i;
+      uint64_t n = (uint64_t)elemSize(paramBufs[i].elem);
+      for (const int64_t d : paramBufs[i].shape) {
+        if (d < 0) sp.rows = true;
+        else n *= (uint64_t)d;
+      }
+      sp.bytes = n;
+      spans.push_back(sp);
+      return spans.size() - 1;
+    };
+    for (size_t o = 0; o < paramRoles.size(); ++o) {
+      if (paramRoles[o] == "in" || paramRoles[o] == "scalar") continue;
+      for (const int j : apart)
+        if ((size_t)j != o && j >= 0 && (size_t)j < paramBufs.size() && paramRoles[j] != "scalar") {
+          const size_t a = at((int)o), b = at(j);
+          if (std::find(pairs.begin(), pairs.end(), std::make_pair(b, a)) == pairs.end()) pairs.push_back({a, b});
+        }
+    }
+    return spans.size() <= MAX_SPANS;
+  }
+
+  // Why a launch's arguments are refused, empty where they are not.
+  std::string check(const uint64_t *params, size_t nparams, void *const *results, size_t nresults, int64_t rows) const {
+    if (nparams != paramRoles.size())
+      return "group @" + func + " takes " + std::to_string(paramRoles.size()) + " arguments, got " + std::to_string(nparams);
+    if (nresults != resultTied.size())
+      return "group @" + func + " has " + std::to_string(resultTied.size()) + " results, got " + std::to_string(nresults);
+    if (nparams && !params) return "null params array";
+    auto empty = [&](const std::vector<Buf> &bufs, size_t i) {
+      return rowsZero && rows == 0 && i < bufs.size() && std::count(bufs[i].shape.begin(), bufs[i].shape.end(), int64_t(-1)) != 0;
+    };
+    for (size_t i = 0; i < nparams; ++i)
+      if (params[i] == 0 && paramRoles[i] != "scalar" && !empty(paramBufs, i))
+        return "null device pointer for argument " + std::to_string(i);
+    if (!pairs.empty()) {
+      uint64_t lo[MAX_SPANS], hi[MAX_SPANS];
+      for (size_t s = 0; s < spans.size(); ++s) {
+        const uint64_t n = spans[s].bytes * (spans[s].rows ? (uint64_t)rows : 1), at = params[spans[s].index];
+        lo[s] = n ? at : UINT64_MAX; // (nothing overlaps an empty one)
+        hi[s] = n ? at + n : 0;
+      }
+      for (const auto &p : pairs)
+        if (lo[p.first] < hi[p.second] && lo[p.second] < hi[p.first])
+          return "argument " + std::to_string(spans[p.first].index) + " of @" + func + " is written and overlaps argument " +
+                 std::to_string(spans[p.second].index);
+    }
+    for (const auto &a : align)
+      if ((size_t)a.first < nparams && params[a.first] % (uint64_t)a.second)
+        return "argument " + std::to_string(a.first) + " of @" + func + " does not start on " + std::to_string(a.second) + " bytes";
+    for (size_t i = 0; i < nresults; ++i)
+      if (resultTied[i] < 0 && (!results || (!results[i] && !empty(resultBufs, i))))
+        return "null device pointer for result " + std::to_string(i);
+    return {};
+  }
+
+private:
+  static constexpr size_t MAX_SPANS = 64;
+  struct Span {
+    int index = 0;
+    bool rows = false;  // `bytes` are a row's
+    uint64_t bytes = 0;
+  };
+  std::vector<Span> spans;
+  std::vector<std::pair<size_t, size_t>> pairs; // a written span, one that it may not overlap
+};

@@ -4,6 +4,7 @@
 // of the CANN rtDevBinaryRegister / rtFunctionRegister / rtKernelLaunch calls
 // of bishengir/test/Integration/HIVM/VecAdd/main.cpp.
 #include "../../../include/hfr.h"
+#include "group_args.h"
 
 #include <hip/hip_runtime.h>
 
@@ -27,19 +28,6 @@ struct hfr_module {
 struct hfr_kernel {
   hipFunction_t fn = nullptr;
   hfr_module *owner = nullptr;
-};
-
-// element size of a manifest element type name (i1 is one byte)
-int elemSize(const std::string &e) {
-  if (e == "f64" || e == "i64" || e == "index") return 8;
-  if (e == "f32" || e == "i32") return 4;
-  if (e == "f16" || e == "bf16" || e == "i16") return 2;
-  return 1;
-}
-
-struct Buf {
-  std::string elem;
-  std::vector<int64_t> shape;
 };
 
 struct Karg {
@@ -78,8 +66,8 @@ struct OwnWorkspace {
   std::vector<std::pair<void *, void *>> more; // stream, workspace
 };
 
-struct hfr_group {
-  std::string func, kernel, hsaco;
+struct hfr_group : GroupArgs {
+  std::string kernel, hsaco;
   std::vector<PreLaunch> pre;
   std::vector<RowAlt> alts; // ascending maxRows
   hfr_module *mod = nullptr;
@@ -90,17 +78,8 @@ struct hfr_group {
   uint64_t algoBytes = 0, algoOps = 0;
   // runtime row count (manifest `rows_dyn a b c cap`): grid.x =
   // min(ceil(R * a / b) * c, cap) (cap 0: none), or the static grid when a is 0
-  bool rowsDyn = false;
   int64_t rowsA = 0, rowsB = 1, rowsC = 1, rowsCap = 0;
-  // a launch of no rows has results to write (manifest `rows_zero 1`); its
-  // tensors of no rows may be null
-  bool rowsZero = false;
-  std::vector<std::string> paramRoles;
-  std::vector<Buf> paramBufs, resultBufs;
-  std::vector<int> resultTied;
   std::vector<Karg> kargs;
-  std::vector<int> apart;                 // parameters that no written one may overlap
-  std::vector<std::pair<int, int>> align; // parameter, bytes it has to start on
   std::shared_ptr<OwnWorkspace> own = std::make_shared<OwnWorkspace>();
   // dense staging copies of strided memref views (hfr_group_launch_memref)
   void *stage = nullptr;
@@ -168,7 +147,8 @@ int parseBlock(const std::vector<std::string> &lines, hfr_group &g) {
     std::istringstream is(ln);
     std::string key;
     is >> key;
-    if (key == "func") is >> g.func;
+    if (g.line(key, is)) {}
+    else if (key == "func") is >> g.func;
     else if (key == "kernel") is >> g.kernel;
     else if (key == "hsaco") is >> g.hsaco;
     else if (key == "grid") is >> g.cfg.grid[0] >> g.cfg.grid[1] >> g.cfg.grid[2];
@@ -182,33 +162,6 @@ int parseBlock(const std::vector<std::string> &lines, hfr_group &g) {
       g.rowsDyn = true;
       if (g.rowsA < 0 || g.rowsB <= 0 || g.rowsC <= 0 || g.rowsCap < 0)
         return fail(HFR_ERR_MANIFEST, "bad rows_dyn line: " + ln);
-    }
-    else if (key == "apart") {
-      for (int i; is >> i;) g.apart.push_back(i);
-      is.clear();
-    }
-    else if (key == "align") {
-      int i = -1, bytes = 0;
-      is >> i >> bytes;
-      if (i < 0 || bytes <= 0) return fail(HFR_ERR_MANIFEST, "bad align line: " + ln);
-      g.align.push_back({i, bytes});
-    }
-    else if (key == "rows_zero") {
-      int z = 0;
-      is >> z;
-      g.rowsZero = z != 0;
-    }
-    else if (key == "param" || key == "result") {
-      int i, tied = -1, rank = 0;
-      std::string role;
-      Buf b;
-      is >> i;
-      if (key == "param") is >> role;
-      else is >> tied;
-      is >> b.elem >> rank;
-      for (int d = 0; d < rank && is; ++d) { int64_t x; is >> x; b.shape.push_back(x); }
-      if (key == "param") { g.paramRoles.push_back(role); g.paramBufs.push_back(b); }
-      else { g.resultTied.push_back(tied); g.resultBufs.push_back(b); }
     }
     else if (key == "karg") {
       std::string k;
@@ -250,6 +203,7 @@ int parseBlock(const std::vector<std::string> &lines, hfr_group &g) {
     }
     if (is.fail()) return fail(HFR_ERR_MANIFEST, "malformed manifest line: " + ln);
   }
+  if (!g.prepare()) return fail(HFR_ERR_MANIFEST, "more arguments than a launch passes");
   if (!g.alts.empty() && !g.rowsDyn) return fail(HFR_ERR_MANIFEST, "alt kernels without rows_dyn");
   if (g.kernel.empty() || g.hsaco.empty()) return fail(HFR_ERR_MANIFEST, "manifest block without kernel/hsaco");
   if (!g.cfg.block[0] || !g.cfg.grid[0]) return fail(HFR_ERR_MANIFEST, "manifest block without launch shape");
@@ -368,44 +322,11 @@ int ownWorkspaceOf(OwnWorkspace &o, uint64_t bytes, bool zeroed, void *stream, c
   return HFR_OK;
 }
 
-// Checks a group launch's arguments (counts, null pointers, alignment).
 int checkGroupArgs(const hfr_group *g, const uint64_t *params, size_t nparams, void *const *results, size_t nresults,
                    int64_t rows = -1) {
   if (!g) return fail(HFR_ERR_INVALID, "null group");
-  if (nparams != g->paramRoles.size())
-    return fail(HFR_ERR_INVALID, "group @" + g->func + " takes " + std::to_string(g->paramRoles.size()) +
-                                     " arguments, got " + std::to_string(nparams));
-  if (nresults != g->resultTied.size())
-    return fail(HFR_ERR_INVALID, "group @" + g->func + " has " + std::to_string(g->resultTied.size()) +
-                                     " results, got " + std::to_string(nresults));
-  if (nparams && !params) return fail(HFR_ERR_INVALID, "null params array");
-  auto empty = [&](const std::vector<Buf> &bufs, size_t i) {
-    return g->rowsZero && rows == 0 && i < bufs.size() && std::count(bufs[i].shape.begin(), bufs[i].shape.end(), int64_t(-1)) != 0;
-  };
-  for (size_t i = 0; i < nparams; ++i)
-    if (g->paramRoles[i] != "scalar" && params[i] == 0 && !empty(g->paramBufs, i))
-      return fail(HFR_ERR_INVALID, "null device pointer for argument " + std::to_string(i));
-  if (!g->apart.empty()) {
-    auto end = [&](size_t i) {
-      uint64_t n = elemSize(g->paramBufs[i].elem);
-      for (const int64_t d : g->paramBufs[i].shape) n *= (uint64_t)(d < 0 ? rows : d);
-      return params[i] + n;
-    };
-    for (size_t o = 0; o < nparams && o < g->paramBufs.size(); ++o) {
-      if (g->paramRoles[o] == "in" || g->paramRoles[o] == "scalar") continue;
-      for (const int j : g->apart)
-        if ((size_t)j != o && (size_t)j < g->paramBufs.size() && params[o] < end(j) && params[j] < end(o))
-          return fail(HFR_ERR_INVALID, "argument " + std::to_string(o) + " of @" + g->func + " is written and overlaps argument " + std::to_string(j));
-    }
-  }
-  for (const auto &a : g->align)
-    if ((size_t)a.first < nparams && params[a.first] % (uint64_t)a.second)
-      return fail(HFR_ERR_INVALID, "argument " + std::to_string(a.first) + " of @" + g->func + " does not start on " +
-                                       std::to_string(a.second) + " bytes");
-  for (size_t i = 0; i < nresults; ++i)
-    if (g->resultTied[i] < 0 && (!results || (!results[i] && !empty(g->resultBufs, i))))
-      return fail(HFR_ERR_INVALID, "null device pointer for result " + std::to_string(i));
-  return HFR_OK;
+  const std::string why = g->check(params, nparams, results, nresults, rows);
+  return why.empty() ? (int)HFR_OK : fail(HFR_ERR_INVALID, why);
 }
 
 // Assembles the kernel arguments (params, own result buffers, workspace) and

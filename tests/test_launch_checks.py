@@ -1,0 +1,49 @@
+"""What a launch accepts, without a GPU: the runtime's argument checks over
+the manifests that the compiler writes."""
+import pytest
+
+import group_catalog as cat
+from launch_checks import Checked
+
+
+@pytest.fixture(scope="module")
+def folder(tmp_path_factory):
+    return tmp_path_factory.mktemp("checks")
+
+
+def checked(name, folder, rows=-1):
+    return Checked(cat.get(name), folder, options=cat.options(name), rows=rows)
+
+
+@pytest.mark.parametrize("which", ["norm", "gradient", "codes", "product"])
+def test_a_check_costs_little(folder, which):
+    """A kernel of a few microseconds waits for its call: the checks of six to
+    eight arguments took 1.0 us where their shapes were multiplied and their
+    types compared at every launch."""
+    name, rows = {"norm": ("ln_rt", 16), "gradient": ("lngrad_wide_rt", 64), "codes": ("quantmx_e2m1_rt", 16),
+                  "product": ("linmx_e2m1_rt", 1)}[which]
+    c = checked(name, folder, rows)
+    assert c.why() == ""
+    assert 0 < c.ns() < 250
+
+
+def test_overlap_of_arguments(folder):
+    """A written argument over another is refused, one beside it is not, at
+    whatever row count the launch has."""
+    for rows in (1, 20, 3000):
+        c = checked("lngrad_wide_rt", folder, rows)  # dy x gamma mean rstd dx dgamma dbeta
+        assert c.why() == ""
+        for out in (5, 6, 7):
+            for other in range(8):
+                if other == out:
+                    continue
+                a = c.at[other]
+                assert "is written and overlaps" in c.why({out: a})
+                assert "is written and overlaps" in c.why({out: a + c.param_bytes(other) - 1})
+                assert "is written and overlaps" in c.why({out: a - c.param_bytes(out) + 1})
+                assert c.why({out: a + c.param_bytes(other)}) == "" and c.why({out: a - c.param_bytes(out)}) == ""
+        # operands may share what they read
+        assert c.why({1: c.at[0], 3: c.at[4]}) == ""
+    # without rows there is nothing to overlap
+    c = checked("lngrad_wide_rt", folder, 0)
+    assert c.why({5: c.at[2] + 64}) == "" and "overlaps" in c.why({6: c.at[2]})
