@@ -32,7 +32,7 @@ struct GroupArgs {
   std::vector<std::string> paramRoles;
   std::vector<Buf> paramBufs, resultBufs;
   std::vector<int> resultTied;
-  std::vector<int> apart;                 // parameters that no written one may overlap
+  std::vector<int> apart;                 // parameters that no destination may overlap
   std::vector<std::pair<int, int>> align; // parameter, bytes it has to start on
 
   // Takes a manifest line of these; false: the key is another's.  A malformed
@@ -75,28 +75,34 @@ struct GroupArgs {
     spans.clear();
     pairs.clear();
     if (apart.empty()) return true;
-    auto at = [&](int i) {
+    auto at = [&](bool result, size_t i) {
       for (size_t s = 0; s < spans.size(); ++s)
-        if (spans[s].index == i) return s;
+        if (spans[s].index == i && spans[s].result == result) return s;
+      const Buf &b = result ? resultBufs[i] : paramBufs[i];
       Span sp;
+      sp.result = result;
       sp.index = i;
-      uint64_t n = (uint64_t)elemSize(paramBufs[i].elem);
-      for (const int64_t d : paramBufs[i].shape) {
+      sp.bytes = (uint64_t)elemSize(b.elem);
+      for (const int64_t d : b.shape) {
         if (d < 0) sp.rows = true;
-        else n *= (uint64_t)d;
+        else sp.bytes *= (uint64_t)d;
       }
-      sp.bytes = n;
       spans.push_back(sp);
       return spans.size() - 1;
     };
-    for (size_t o = 0; o < paramRoles.size(); ++o) {
-      if (paramRoles[o] == "in" || paramRoles[o] == "scalar") continue;
-      for (const int j : apart)
-        if ((size_t)j != o && j >= 0 && (size_t)j < paramBufs.size() && paramRoles[j] != "scalar") {
-          const size_t a = at((int)o), b = at(j);
-          if (std::find(pairs.begin(), pairs.end(), std::make_pair(b, a)) == pairs.end()) pairs.push_back({a, b});
-        }
-    }
+    std::vector<size_t> written, kept;
+    for (size_t i = 0; i < paramRoles.size(); ++i)
+      if (paramRoles[i] != "in" && paramRoles[i] != "scalar") written.push_back(at(false, i));
+    for (size_t i = 0; i < resultTied.size(); ++i)
+      if (resultTied[i] < 0) written.push_back(at(true, i));
+    for (const int j : apart)
+      if (j >= 0 && (size_t)j < paramBufs.size() && paramRoles[j] != "scalar") kept.push_back(at(false, (size_t)j));
+    kept.insert(kept.end(), written.begin(), written.end()); // (destinations may not overlap each other either)
+    for (const size_t a : written)
+      for (const size_t b : kept)
+        if (a != b && std::find(pairs.begin(), pairs.end(), std::make_pair(b, a)) == pairs.end() &&
+            std::find(pairs.begin(), pairs.end(), std::make_pair(a, b)) == pairs.end())
+          pairs.push_back({a, b});
     return spans.size() <= MAX_SPANS;
   }
 
@@ -113,33 +119,36 @@ struct GroupArgs {
     for (size_t i = 0; i < nparams; ++i)
       if (params[i] == 0 && paramRoles[i] != "scalar" && !empty(paramBufs, i))
         return "null device pointer for argument " + std::to_string(i);
+    for (size_t i = 0; i < nresults; ++i)
+      if (resultTied[i] < 0 && (!results || (!results[i] && !empty(resultBufs, i))))
+        return "null device pointer for result " + std::to_string(i);
     if (!pairs.empty()) {
       uint64_t lo[MAX_SPANS], hi[MAX_SPANS];
       for (size_t s = 0; s < spans.size(); ++s) {
-        const uint64_t n = spans[s].bytes * (spans[s].rows ? (uint64_t)rows : 1), at = params[spans[s].index];
+        const Span &sp = spans[s];
+        const uint64_t n = sp.bytes * (sp.rows ? (uint64_t)rows : 1);
+        const uint64_t at = sp.result ? (uint64_t)(uintptr_t)results[sp.index] : params[sp.index];
         lo[s] = n ? at : UINT64_MAX; // (nothing overlaps an empty one)
         hi[s] = n ? at + n : 0;
       }
       for (const auto &p : pairs)
         if (lo[p.first] < hi[p.second] && lo[p.second] < hi[p.first])
-          return "argument " + std::to_string(spans[p.first].index) + " of @" + func + " is written and overlaps argument " +
-                 std::to_string(spans[p.second].index);
+          return spans[p.first].name() + " of @" + func + " is written and overlaps " + spans[p.second].name();
     }
     for (const auto &a : align)
       if ((size_t)a.first < nparams && params[a.first] % (uint64_t)a.second)
         return "argument " + std::to_string(a.first) + " of @" + func + " does not start on " + std::to_string(a.second) + " bytes";
-    for (size_t i = 0; i < nresults; ++i)
-      if (resultTied[i] < 0 && (!results || (!results[i] && !empty(resultBufs, i))))
-        return "null device pointer for result " + std::to_string(i);
     return {};
   }
 
 private:
   static constexpr size_t MAX_SPANS = 64;
   struct Span {
-    int index = 0;
-    bool rows = false;  // `bytes` are a row's
+    bool result = false; // of a buffer of its own, not one written into an argument
+    size_t index = 0;
+    bool rows = false; // `bytes` are a row's
     uint64_t bytes = 0;
+    std::string name() const { return (result ? "result " : "argument ") + std::to_string(index); }
   };
   std::vector<Span> spans;
   std::vector<std::pair<size_t, size_t>> pairs; // a written span, one that it may not overlap

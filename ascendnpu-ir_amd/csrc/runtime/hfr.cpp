@@ -985,10 +985,10 @@ extern "C" uint64_t hfr_scratch_bytes(void) { return HFR_SCRATCH_BYTES; }
 
 extern "C" int hfr_group_launch_noalloc(hfr_group_t g, const uint64_t *params, size_t nparams, void *const *results,
                                         size_t nresults, void *stream) {
+  if (g && g->rowsDyn)
+    return fail(HFR_ERR_INVALID, "group @" + g->func + " takes its row count at launch (hfr_group_launch_rows)");
   int rc = checkGroupArgs(g, params, nparams, results, nresults);
   if (rc) return rc;
-  if (g->rowsDyn)
-    return fail(HFR_ERR_INVALID, "group @" + g->func + " takes its row count at launch (hfr_group_launch_rows)");
   if (g->wsBytes > HFR_SCRATCH_BYTES)
     return fail(HFR_ERR_INVALID, "group @" + g->func + " needs " + std::to_string(g->wsBytes) +
                                      " workspace bytes; the static scratch holds " + std::to_string(HFR_SCRATCH_BYTES));

@@ -79,8 +79,9 @@ int hfr_group_info_get(hfr_group_t g, hfr_group_info *info);
  * NULL — for results written into an argument); workspace: NULL to use the
  * group's own, or a caller buffer of workspace_bytes that starts on 16 bytes
  * (zeroed before its first use when the group requires it).  An argument that
- * the manifest gives an `align` line is refused off those bytes, a written one
- * that overlaps an argument of its `apart` line too. */
+ * the manifest gives an `align` line is refused off those bytes; where it has
+ * an `apart` line, so is a destination (an argument that is written, or a
+ * result's buffer) over an argument of that line or over another destination. */
 int hfr_group_launch(hfr_group_t g, const uint64_t *params, size_t nparams, void *const *results, size_t nresults,
                      void *workspace, void *stream);
 /* A group compiled with runtime row counts (compiler option dyn=runtime; its

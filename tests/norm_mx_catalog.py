@@ -77,6 +77,8 @@ def entries():
     for m, n, k, fmt, bias, out in LINEAR + LINEAR_MANY + LINEAR_LONG:
         e[linear_name((m, n, k, fmt, bias, out))] = g.linear_mx(m, n, k, fmt=fmt, bias=bias, out=out)
     e["linmx_filled"] = g.linear_mx(5, 48, 64, out="f32").replace("0.000000e+00", "1.500000e+00")
+    e["ln_untied"], e["lngrad_untied"] = untied(g.layer_norm(9, 96, ckpt="e4m3")), untied(g.layer_norm_grad(64, 256))
+    e["quantmx_untied"] = untied(g.quantize_mx(70, 64, fmt="e5m2"))
     e["ln_rank3"], e["lngrad_rank3"] = norm_rank3(), norm_grad_rank3()
     rt = lambda ir: g.with_dynamic_rows(ir, _ANY)  # noqa: E731
     e["quantmx_e4m3_rt"] = rt(g.quantize_mx(_ANY, 100))
@@ -92,3 +94,18 @@ def entries():
     e["prog_norm_linear_mx"] = g.layer_norm_linear_mx(20, 208, 384)
     e["prog_norm_linear_mx_many"] = g.layer_norm_linear_mx(2300, 1040, 1024)
     return e
+
+
+def untied(ir):
+    """The group with buffers of its own for its results: their destinations
+    are tensor.empty, not arguments."""
+    head, body = ir.split(") -> (", 1) if ") -> (" in ir else ir.split(") -> ", 1)
+    outs = body[body.index("outs(") + 5:]
+    outs = outs[:outs.index(")")]
+    names, types = (v.split(", ") for v in outs.split(" : "))
+    for n, t in zip(names, types):
+        assert f", {n}: {t}" in head
+        head = head.replace(f", {n}: {t}", "")
+    empties = "".join(f"    {n} = tensor.empty() : {t}\n" for n, t in zip(names, types))
+    at = body.index("{\n") + 2
+    return head + (") -> (" if ") -> (" in ir else ") -> ") + body[:at] + empties + body[at:]

@@ -3,6 +3,8 @@ the manifests that the compiler writes."""
 import pytest
 
 import group_catalog as cat
+import norm_mx_catalog as nc
+from hfusion_mi355x import groups as g
 from launch_checks import Checked
 
 
@@ -47,3 +49,32 @@ def test_overlap_of_arguments(folder):
     # without rows there is nothing to overlap
     c = checked("lngrad_wide_rt", folder, 0)
     assert c.why({5: c.at[2] + 64}) == "" and "overlaps" in c.why({6: c.at[2]})
+
+
+@pytest.mark.parametrize("name", ["ln_untied", "lngrad_untied", "quantmx_untied"])
+def test_overlap_of_results(folder, name):
+    """Results in buffers of their own are destinations too: none over an
+    operand, none over another.  (The gradient of few rows reads dy by columns
+    while other workgroups write dx.)"""
+    c = checked(name, folder)
+    n, m = len(c.at), len(c.res)
+    assert m > 1 and all(r["tied"] < 0 for r in c.meta["results"]) and c.why() == ""
+    for j in range(m):
+        for i in range(n):
+            assert f"result {j} of" in c.why(res={j: c.at[i]}) and f"overlaps argument {i}" in c.why(res={j: c.at[i]})
+            assert "overlaps" in c.why(res={j: c.at[i] + c.param_bytes(i) - 1}) and "overlaps" in c.why(res={j: c.at[i] - c.result_bytes(j) + 1})
+            assert c.why(res={j: c.at[i] + c.param_bytes(i)}) == "" and c.why(res={j: c.at[i] - c.result_bytes(j)}) == ""
+        for i in range(m):
+            if i != j:
+                assert "is written and overlaps result" in c.why(res={j: c.res[i]})
+                assert c.why(res={j: c.res[i] + c.result_bytes(i)}) == ""
+    assert "null device pointer for result 1" in c.why(res={1: 0})
+
+
+def test_overlap_of_a_result_and_a_written_argument(folder):
+    """Some destinations arguments, some not."""
+    ir = nc.untied(g.quantize_mx(64, 96)).replace("%x: tensor<64x96xbf16>)", "%x: tensor<64x96xbf16>, %s: tensor<64x3xui8>)") \
+        .replace("    %s = tensor.empty() : tensor<64x3xui8>\n", "")
+    c = Checked(ir, folder)
+    assert [r["tied"] for r in c.meta["results"]] == [-1, 1] and c.why() == ""
+    assert "overlaps" in c.why(res={0: c.at[0]}) and "overlaps" in c.why(res={0: c.at[1]}) and "overlaps" in c.why(at={1: c.at[0] + 5})
