@@ -2938,7 +2938,16 @@ KernelPlan lowerMatmul(Analysis &A, const std::string &kname, const LowerOptions
   };
   if (wx) {
     p.align16 = {a->argIdx, b->argIdx};
-    p.apart = {a->argIdx, b->argIdx, sb->argIdx}; // (what the epilogue reads, it reads where it writes)
+    // of what the epilogue reads, it reads only [m, n] where it writes; a bias
+    // is read by every row tile, after another may have written its output
+    p.apart = {a->argIdx, b->argIdx, sb->argIdx};
+    for (const auto &v : name) {
+      if (v.first->argIdx < 0 || !v.first->type.tensor) continue;
+      const bool here = A.map.at(v.first).size() == 2 && elemBytes(v.first->type.elem) == elemBytes(oe);
+      (here ? p.inplace : p.apart).push_back(v.first->argIdx);
+    }
+    std::sort(p.apart.begin(), p.apart.end());
+    std::sort(p.inplace.begin(), p.inplace.end());
     p.algoOps = 2.0 * (double)M * (double)N * (double)K;
     if (!wxPre) {
       const WxTile &t = *wxFew(M, N, K, cpb);
@@ -5002,11 +5011,14 @@ std::string emitManifest(const KernelPlan &p, const std::string &hsacoName) {
     << "algo_ops " << (uint64_t)p.algoOps << "\n";
   if (p.rowsDyn) s << "rows_dyn " << p.rowsA << " " << p.rowsB << " " << p.rowsC << " " << p.rowsCap << "\n";
   if (p.rowsZero) s << "rows_zero 1\n";
-  if (!p.apart.empty()) {
-    s << "apart";
-    for (const int i : p.apart) s << " " << i;
+  auto indices = [&](const char *key, const std::vector<int> &v) {
+    if (v.empty()) return;
+    s << key;
+    for (const int i : v) s << " " << i;
     s << "\n";
-  }
+  };
+  indices("apart", p.apart);
+  indices("inplace", p.inplace);
   for (const int i : p.align16) s << "align " << i << " 16\n";
   auto shp = [](const std::vector<int64_t> &v) {
     std::string r = std::to_string(v.size());

@@ -66,6 +66,7 @@ struct KernelPlan {
   int64_t rowsA = 0, rowsB = 1, rowsC = 1, rowsCap = 0;
   bool rowsZero = false; // a launch of no rows has results to write
   std::vector<int> apart; // arguments that no destination may overlap (refused at launch)
+  std::vector<int> inplace; // arguments that a destination may be, but not overlap otherwise
   std::vector<int> align16; // arguments that have to start on 16 bytes (refused at launch)
 };
 

@@ -33,13 +33,14 @@ struct GroupArgs {
   std::vector<Buf> paramBufs, resultBufs;
   std::vector<int> resultTied;
   std::vector<int> apart;                 // parameters that no destination may overlap
+  std::vector<int> inplace;               // ones that it may be, but overlap in no other way
   std::vector<std::pair<int, int>> align; // parameter, bytes it has to start on
 
   // Takes a manifest line of these; false: the key is another's.  A malformed
   // line leaves the stream failed.
   bool line(const std::string &key, std::istringstream &is) {
-    if (key == "apart") {
-      for (int i; is >> i;) apart.push_back(i);
+    if (key == "apart" || key == "inplace") {
+      for (int i; is >> i;) (key == "apart" ? apart : inplace).push_back(i);
       is.clear();
     } else if (key == "align") {
       int i = -1, bytes = 0;
@@ -74,7 +75,7 @@ struct GroupArgs {
   bool prepare() {
     spans.clear();
     pairs.clear();
-    if (apart.empty()) return true;
+    if (apart.empty() && inplace.empty()) return true;
     auto at = [&](bool result, size_t i) {
       for (size_t s = 0; s < spans.size(); ++s)
         if (spans[s].index == i && spans[s].result == result) return s;
@@ -95,14 +96,19 @@ struct GroupArgs {
       if (paramRoles[i] != "in" && paramRoles[i] != "scalar") written.push_back(at(false, i));
     for (size_t i = 0; i < resultTied.size(); ++i)
       if (resultTied[i] < 0) written.push_back(at(true, i));
-    for (const int j : apart)
-      if (j >= 0 && (size_t)j < paramBufs.size() && paramRoles[j] != "scalar") kept.push_back(at(false, (size_t)j));
-    kept.insert(kept.end(), written.begin(), written.end()); // (destinations may not overlap each other either)
-    for (const size_t a : written)
-      for (const size_t b : kept)
-        if (a != b && std::find(pairs.begin(), pairs.end(), std::make_pair(b, a)) == pairs.end() &&
-            std::find(pairs.begin(), pairs.end(), std::make_pair(a, b)) == pairs.end())
-          pairs.push_back({a, b});
+    auto tensor = [&](int j) { return j >= 0 && (size_t)j < paramBufs.size() && paramRoles[j] != "scalar"; };
+    auto add = [&](size_t a, size_t b, bool same) {
+      for (const Pair &p : pairs)
+        if ((p.a == a && p.b == b) || (p.a == b && p.b == a)) return;
+      if (a != b) pairs.push_back({a, b, same});
+    };
+    for (const size_t a : written) {
+      for (const int j : apart)
+        if (tensor(j)) add(a, at(false, (size_t)j), false);
+      for (const size_t b : written) add(a, b, false);
+      for (const int j : inplace)
+        if (tensor(j)) add(a, at(false, (size_t)j), true);
+    }
     return spans.size() <= MAX_SPANS;
   }
 
@@ -132,8 +138,8 @@ struct GroupArgs {
         hi[s] = n ? at + n : 0;
       }
       for (const auto &p : pairs)
-        if (lo[p.first] < hi[p.second] && lo[p.second] < hi[p.first])
-          return spans[p.first].name() + " of @" + func + " is written and overlaps " + spans[p.second].name();
+        if (lo[p.a] < hi[p.b] && lo[p.b] < hi[p.a] && !(p.same && lo[p.a] == lo[p.b] && hi[p.a] == hi[p.b]))
+          return spans[p.a].name() + " of @" + func + " is written and overlaps " + spans[p.b].name();
     }
     for (const auto &a : align)
       if ((size_t)a.first < nparams && params[a.first] % (uint64_t)a.second)
@@ -151,5 +157,9 @@ private:
     std::string name() const { return (result ? "result " : "argument ") + std::to_string(index); }
   };
   std::vector<Span> spans;
-  std::vector<std::pair<size_t, size_t>> pairs; // a written span, one that it may not overlap
+  struct Pair {
+    size_t a, b; // a written span, one that it may not overlap
+    bool same;   // unless the two are one buffer
+  };
+  std::vector<Pair> pairs;
 };

@@ -81,7 +81,8 @@ int hfr_group_info_get(hfr_group_t g, hfr_group_info *info);
  * (zeroed before its first use when the group requires it).  An argument that
  * the manifest gives an `align` line is refused off those bytes; where it has
  * an `apart` line, so is a destination (an argument that is written, or a
- * result's buffer) over an argument of that line or over another destination. */
+ * result's buffer) over an argument of that line or over another destination.
+ * It may be an argument of an `inplace` line, but not overlap it otherwise. */
 int hfr_group_launch(hfr_group_t g, const uint64_t *params, size_t nparams, void *const *results, size_t nresults,
                      void *workspace, void *stream);
 /* A group compiled with runtime row counts (compiler option dyn=runtime; its

@@ -79,6 +79,8 @@ def entries():
     e["linmx_filled"] = g.linear_mx(5, 48, 64, out="f32").replace("0.000000e+00", "1.500000e+00")
     e["ln_untied"], e["lngrad_untied"] = untied(g.layer_norm(9, 96, ckpt="e4m3")), untied(g.layer_norm_grad(64, 256))
     e["quantmx_untied"] = untied(g.quantize_mx(70, 64, fmt="e5m2"))
+    e["linmx_residual"], e["linmx_residual_bf16"] = linear_epilogue(70, 48, 96), linear_epilogue(70, 48, 96, out="bf16")
+    e["linmx_residual_many"] = linear_epilogue(2300, 520, 1024)
     e["ln_rank3"], e["lngrad_rank3"] = norm_rank3(), norm_grad_rank3()
     rt = lambda ir: g.with_dynamic_rows(ir, _ANY)  # noqa: E731
     e["quantmx_e4m3_rt"] = rt(g.quantize_mx(_ANY, 100))
@@ -109,3 +111,15 @@ def untied(ir):
     empties = "".join(f"    {n} = tensor.empty() : {t}\n" for n, t in zip(names, types))
     at = body.index("{\n") + 2
     return head + (") -> (" if ") -> (" in ir else ") -> ") + body[:at] + empties + body[at:]
+
+
+def linear_epilogue(m, n, k, out="f32"):
+    """linear_mx with a residual [m, n] and a factor per row: (a w + residual) * factor."""
+    C, O = f"tensor<{m}x{n}xf32>", f"tensor<{m}x{n}x{out}>"
+    ir = g.linear_mx(m, n, k, bias=True, out=out)
+    ir = ir.replace(f"%bias: tensor<{n}xf32>", f"%res: {C}, %factor: tensor<{m}xf32>")
+    ir = ir.replace(f"%bb = linalg.broadcast ins(%bias : tensor<{n}xf32>) outs(%e1 : {C}) dimensions = [0]",
+                    f"%bb = linalg.broadcast ins(%factor : tensor<{m}xf32>) outs(%e1 : {C}) dimensions = [1]\n"
+                    f"    %e5 = tensor.empty() : {C}\n"
+                    f"    %cr = linalg.elemwise_binary {{fun = #linalg.binary_fn<add>}} ins(%c, %res : {C}, {C}) outs(%e5 : {C}) -> {C}")
+    return ir.replace("binary_fn<add>}} ins(%c, %bb".replace("}}", "}"), "binary_fn<mul>} ins(%cr, %bb")

@@ -78,3 +78,25 @@ def test_overlap_of_a_result_and_a_written_argument(folder):
     c = Checked(ir, folder)
     assert [r["tied"] for r in c.meta["results"]] == [-1, 1] and c.why() == ""
     assert "overlaps" in c.why(res={0: c.at[0]}) and "overlaps" in c.why(res={0: c.at[1]}) and "overlaps" in c.why(at={1: c.at[0] + 5})
+
+
+def test_overlap_of_an_epilogue(folder):
+    """A bias is read by every row tile, a factor of a row by every column
+    tile: no result over them.  A residual is read where the result is
+    written: the two may be one buffer, of elements of one size."""
+    for name, rows in (("linmx_e2m1_rt", 65), (nc.linear_name(nc.LINEAR[3]), -1)):
+        c = checked(name, folder, rows)  # a w scales bias out
+        assert c.why() == ""
+        for i in range(4):
+            assert f"overlaps argument {i}" in c.why({4: c.at[i]}) and f"overlaps argument {i}" in c.why({4: c.at[i] - 16})
+            assert c.why({4: c.at[i] + c.param_bytes(i)}) == ""
+    c = checked("linmx_residual", folder)  # a w scales residual factor out
+    assert "overlaps argument 4" in c.why({5: c.at[4]}) and "overlaps argument 4" in c.why({5: c.at[4] - 4})
+    assert c.why({5: c.at[3]}) == ""
+    assert "overlaps argument 3" in c.why({5: c.at[3] + 4}) and "overlaps argument 3" in c.why({5: c.at[3] - 48 * 4})
+    c = checked("linmx_residual_bf16", folder)
+    assert "overlaps argument 3" in c.why({5: c.at[3]}) and c.why() == ""
+    untied = Checked(cat.get("linmx_residual").replace(", %out: tensor<70x48xf32>) ->", ") ->").replace("outs(%out :", "outs(%e5 :"), folder)
+    assert [r["tied"] for r in untied.meta["results"]] == [-1]
+    assert untied.why() == "" and untied.why(res={0: untied.at[3]}) == "" and "result 0 of" in untied.why(res={0: untied.at[4]})
+    assert "overlaps argument 1" in untied.why(res={0: untied.at[1]})

@@ -10,7 +10,7 @@ import group_catalog as cat
 import norm_mx_catalog as nc
 from helpers import to_dev, to_host
 from oracle import blockscaled as bs
-from test_norm_mx import check_grad, check_norm, grad_args, norm_inputs, note, stored
+from test_norm_mx import E24, check_grad, check_norm, grad_args, linear_inputs, norm_inputs, note, stored
 
 
 def load(name):
@@ -59,3 +59,34 @@ def test_results_in_buffers_of_their_own(gpu):
     q, s = host(grp(to_dev(xs, "bf16", gpu)), grp)
     wq, ws = bs.quantize(x, "e5m2", 1)
     assert np.array_equal(q, wq) and np.array_equal(s.view(np.uint8), ws)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name,m,n,k", [("linmx_residual", 70, 48, 96), ("linmx_residual_many", 2300, 520, 1024)])
+def test_product_onto_its_residual(gpu, name, m, n, k):
+    """(a w + residual) * factor over the residual itself; over the factor, or
+    next to its own place in the residual, it is refused."""
+    import torch
+    note(name)
+    as_, a, w, s, _, wv = linear_inputs(m, n, k, "e2m1")
+    rng = np.random.default_rng(m)
+    res, factor = rng.normal(size=(m, n)).astype(np.float32), rng.uniform(0.5, 2, m).astype(np.float32)
+    grp = load(name)
+    args = device_args(grp, [as_, w, s, res, factor], gpu)
+    out = torch.zeros((m, n), device=gpu)
+    grp(*args, out)
+    # test_norm_mx's bound of the sums, one more addition, one product: a step each
+    mag = np.abs(a) @ np.abs(wv).T + np.abs(res)
+    tol = ((2 * (40 + k / 32) + 4) * E24 * mag) * factor[:, None]
+    assert (np.abs(out.cpu().numpy() - (a @ wv.T + res) * factor[:, None]) <= tol).all()
+    flat = torch.zeros(m * n + 8, device=gpu)
+    flat[:m * n] = args[3].view(-1)
+    here = flat[:m * n].view(m, n)
+    for bad in (flat[4:m * n + 4].view(m, n), flat[8:].view(m, n)):
+        with pytest.raises(RuntimeError, match="is written and overlaps argument 3"):
+            grp(*args[:3], here, args[4], bad)
+    wide = torch.ones(m * n + m, device=gpu)
+    with pytest.raises(RuntimeError, match="is written and overlaps argument 4"):
+        grp(*args[:4], wide[m * n - 4:m * n - 4 + m], wide[:m * n].view(m, n))
+    grp(*args[:3], here, args[4], here)
+    assert torch.equal(here, out) and not flat[m * n:].any()
