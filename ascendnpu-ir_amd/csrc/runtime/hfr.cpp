@@ -379,6 +379,27 @@ int launchGroup(const hfr_group *g, const uint64_t *params, void *const *results
   return launch(g->fn, rowsCfg(g->cfg), g->kargs);
 }
 
+// Everything that a launch is refused for.
+int checkLaunch(const hfr_group *g, const uint64_t *params, size_t nparams, void *const *results, size_t nresults, int64_t rows,
+                const void *workspace) {
+  if (g && !g->rowsDyn && rows != -1)
+    return fail(HFR_ERR_INVALID, "group @" + g->func + " has a static row count");
+  if (g && g->rowsDyn && rows < 0) return fail(HFR_ERR_INVALID, "negative row count for group @" + g->func);
+  if (const int rc = checkGroupArgs(g, params, nparams, results, nresults, rows)) return rc;
+  if (g->wsBytes && (uintptr_t)workspace % 16)
+    return fail(HFR_ERR_INVALID, "a workspace of group @" + g->func + " has to start on 16 bytes");
+  return HFR_OK;
+}
+
+// The launch of checked arguments.
+int runChecked(hfr_group *g, const uint64_t *params, void *const *results, int64_t rows, void *workspace, void *stream) {
+  if (g->rowsDyn && rows == 0 && !g->rowsZero) return HFR_OK; // nothing to do
+  void *ws = workspace;
+  if (g->wsBytes && !ws)
+    if (const int rc = ownWorkspaceOf(*g->own, g->wsBytes, g->wsZero, stream, "group", &ws)) return rc;
+  return launchGroup(g, params, results, ws, stream, rows);
+}
+
 } // namespace
 
 extern "C" {
@@ -514,19 +535,8 @@ int hfr_group_launch(hfr_group_t g, const uint64_t *params, size_t nparams, void
 
 int hfr_group_launch_rows(hfr_group_t g, const uint64_t *params, size_t nparams, void *const *results, size_t nresults,
                           int64_t rows, void *workspace, void *stream) {
-  if (g && !g->rowsDyn && rows != -1)
-    return fail(HFR_ERR_INVALID, "group @" + g->func + " has a static row count");
-  if (g && g->rowsDyn && rows < 0) return fail(HFR_ERR_INVALID, "negative row count for group @" + g->func);
-  int rc = checkGroupArgs(g, params, nparams, results, nresults, rows);
-  if (rc) return rc;
-  if (g->rowsDyn && rows == 0 && !g->rowsZero) return HFR_OK; // nothing to do
-  void *ws = workspace;
-  if (g->wsBytes && (uintptr_t)ws % 16) return fail(HFR_ERR_INVALID, "a workspace of group @" + g->func + " has to start on 16 bytes");
-  if (g->wsBytes && !ws) {
-    rc = ownWorkspaceOf(*g->own, g->wsBytes, g->wsZero, stream, "group", &ws);
-    if (rc) return rc;
-  }
-  return launchGroup(g, params, results, ws, stream, rows);
+  if (const int rc = checkLaunch(g, params, nparams, results, nresults, rows, workspace)) return rc;
+  return runChecked(g, params, results, rows, workspace, stream);
 }
 
 } // extern "C"
@@ -707,15 +717,19 @@ int hfr_program_launch(hfr_program_t p, const uint64_t *params, size_t nparams, 
   };
   std::vector<uint64_t> args;
   std::vector<void *> res;
-  for (auto &st : p->steps) {
-    args.clear();
-    res.clear();
-    for (auto &b : st.args) args.push_back(resolve(b));
-    for (auto &b : st.results) res.push_back((void *)(uintptr_t)resolve(b));
-    const bool shares = st.group->wsBytes && !st.group->wsZero;
-    int rc = hfr_group_launch(st.group, args.data(), args.size(), res.data(), res.size(), shares ? ws + p->stepWs : nullptr, stream);
-    if (rc) return rc;
-  }
+  // every step is checked before the first is launched: a refused program has
+  // written nothing
+  for (const bool run : {false, true})
+    for (auto &st : p->steps) {
+      args.clear();
+      res.clear();
+      for (auto &b : st.args) args.push_back(resolve(b));
+      for (auto &b : st.results) res.push_back((void *)(uintptr_t)resolve(b));
+      void *const own = st.group->wsBytes && !st.group->wsZero ? ws + p->stepWs : nullptr;
+      const int rc = run ? runChecked(st.group, args.data(), res.data(), -1, own, stream)
+                         : checkLaunch(st.group, args.data(), args.size(), res.data(), res.size(), -1, own);
+      if (rc) return rc;
+    }
   return HFR_OK;
 }
 

@@ -90,3 +90,32 @@ def test_product_onto_its_residual(gpu, name, m, n, k):
         grp(*args[:4], wide[m * n - 4:m * n - 4 + m], wide[:m * n].view(m, n))
     grp(*args[:3], here, args[4], here)
     assert torch.equal(here, out) and not flat[m * n:].any()
+
+
+@pytest.mark.gpu
+def test_refused_programs_write_nothing(gpu):
+    """A program whose last step is refused: its first ones have not run."""
+    import torch
+    note("refused programs")
+    rng = np.random.default_rng(12)
+    for name, m, n, k in (("prog_norm_linear_mx", 20, 208, 384), ("prog_norm_linear_mx_many", 2300, 1040, 1024)):
+        (xs, x), (gs, gm), (ts, bt) = (stored(a, "bf16") for a in (rng.normal(size=(m, k)), rng.uniform(0.5, 1.5, k), rng.normal(0, 0.1, k)))
+        _, _, w, s, _, wv = linear_inputs(8, n, k, "e2m1")
+        prog = load(name)
+        args = [to_dev(v, p["elem"], gpu) for v, p in zip([xs, gs, ts, w, s], prog.meta["params"])]
+        room = torch.zeros(prog.workspace_bytes + 16, dtype=torch.uint8, device=gpu)
+        # the result over the scales
+        both = torch.zeros(2 * m * n + s.size, dtype=torch.uint8, device=gpu)
+        over = both[2 * m * n - 8:2 * m * n - 8 + s.size].view(torch.int8).view(s.shape)
+        over.copy_(args[4])
+        keep = both.clone()
+        with pytest.raises(RuntimeError, match="is written and overlaps"):
+            prog(*args[:4], over, results=[both[:2 * m * n].view(torch.bfloat16).view(m, n)], workspace=room)
+        if name.endswith("many"):
+            with pytest.raises(RuntimeError, match="start on 16 bytes"):
+                prog(*args, workspace=room[8:])
+        torch.cuda.synchronize()
+        assert not room.any() and torch.equal(both, keep)
+        want = prog(*args)
+        got = prog(*args, results=[torch.zeros((m, n), dtype=torch.bfloat16, device=gpu)], workspace=room)
+        assert torch.equal(got, want) and room.any()
