@@ -26,9 +26,7 @@ struct Buf {
 struct GroupArgs {
   std::string func;
   bool rowsDyn = false; // the row count comes with the launch (-1 in the shapes)
-  // a launch of no rows has results to write (manifest `rows_zero 1`); its
-  // tensors of no rows may be null
-  bool rowsZero = false;
+  bool rowsZero = false; // a launch of no rows has results to write (manifest `rows_zero 1`)
   std::vector<std::string> paramRoles;
   std::vector<Buf> paramBufs, resultBufs;
   std::vector<int> resultTied;
@@ -119,8 +117,9 @@ struct GroupArgs {
     if (nresults != resultTied.size())
       return "group @" + func + " has " + std::to_string(resultTied.size()) + " results, got " + std::to_string(nresults);
     if (nparams && !params) return "null params array";
+    // (a tensor of no rows has no address)
     auto empty = [&](const std::vector<Buf> &bufs, size_t i) {
-      return rowsZero && rows == 0 && i < bufs.size() && std::count(bufs[i].shape.begin(), bufs[i].shape.end(), int64_t(-1)) != 0;
+      return rows == 0 && i < bufs.size() && std::count(bufs[i].shape.begin(), bufs[i].shape.end(), int64_t(-1)) != 0;
     };
     for (size_t i = 0; i < nparams; ++i)
       if (params[i] == 0 && paramRoles[i] != "scalar" && !empty(paramBufs, i))

@@ -784,9 +784,10 @@ int readDesc(const Buf &b, const void *desc, const char *what, size_t idx, View 
     expect *= sizes[k];
     v.numel *= sizes[k];
   }
-  if (!aligned) return fail(HFR_ERR_INVALID, std::string("null aligned pointer for ") + what + " " + std::to_string(idx));
+  if (v.numel == 0) v.dense = true; // (nothing to stage, and no address)
+  else if (!aligned) return fail(HFR_ERR_INVALID, std::string("null aligned pointer for ") + what + " " + std::to_string(idx));
   if (offset < 0) return fail(HFR_ERR_INVALID, std::string("negative offset for ") + what + " " + std::to_string(idx));
-  v.base = aligned + offset * elemSize(b.elem);
+  v.base = aligned ? aligned + offset * elemSize(b.elem) : nullptr;
   return HFR_OK;
 }
 

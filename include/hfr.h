@@ -88,7 +88,8 @@ int hfr_group_launch(hfr_group_t g, const uint64_t *params, size_t nparams, void
 /* A group compiled with runtime row counts (compiler option dyn=runtime; its
  * manifest holds `rows_dyn`, and -1 for the row dim of each shape): the same
  * launch over `rows` rows (0: no launch, unless the manifest holds `rows_zero
- * 1`: there are results to write, and tensors of no rows may be null).  One compiled kernel serves every
+ * 1`: there are results to write; tensors of no rows may be null, also as the
+ * aligned pointer of a memref descriptor).  One compiled kernel serves every
  * row count, where the reference schedules a dynamic-shape kernel once and
  * reads the sizes at run time from its memref descriptors
  * (bishengir/lib/Dialect/HFusion/Transforms/AutoSchedule/AnyPBRSchedule.cpp).

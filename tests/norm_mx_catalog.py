@@ -89,6 +89,7 @@ def entries():
     e["ln_rt"] = rt(g.layer_norm(_ANY, 1000, ckpt="e4m3"))
     e["lngrad_rt"] = rt(g.layer_norm_grad(_ANY, 1000, ckpt="e4m3", params="f32"))
     e["lngrad_wide_rt"] = rt(g.layer_norm_grad(_ANY, 4096))
+    e["lngrad_plain_rt"] = rt(g.layer_norm_grad(_ANY, 96, affine=0))
     e["linmx_e2m1_rt"] = rt(g.linear_mx(_ANY, 130, 544, bias=True))
     e["linmx_e4m3_rt"] = rt(g.linear_mx(_ANY, 1040, 1024, fmt="e4m3"))
     # the norm, the quantisation of its result and the block-scaled product

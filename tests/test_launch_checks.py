@@ -100,3 +100,18 @@ def test_overlap_of_an_epilogue(folder):
     assert [r["tied"] for r in untied.meta["results"]] == [-1]
     assert untied.why() == "" and untied.why(res={0: untied.at[3]}) == "" and "result 0 of" in untied.why(res={0: untied.at[4]})
     assert "overlaps argument 1" in untied.why(res={0: untied.at[1]})
+
+
+@pytest.mark.parametrize("name", ["ln_rt", "lngrad_rt", "lngrad_plain_rt", "quantmx_e4m3_rt", "dequantmx_e2m1_rt", "linmx_e2m1_rt", "linmx_e4m3_rt"])
+def test_tensors_of_no_rows_have_no_address(folder, name):
+    """An empty batch: null where a tensor has no rows, and nowhere else."""
+    c = checked(name, folder, 0)
+    rows = [i for i, p in enumerate(c.meta["params"]) if -1 in p["shape"]]
+    null = {i: 0 for i in rows}
+    assert rows and c.why(null) == ""
+    for i in range(len(c.at)):
+        if i not in rows:
+            assert c.why({**null, i: 0}) == f"null device pointer for argument {i}"
+    c = checked(name, folder, 1)
+    for i in rows:
+        assert c.why({i: 0}) == f"null device pointer for argument {i}"

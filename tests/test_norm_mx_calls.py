@@ -119,3 +119,41 @@ def test_refused_programs_write_nothing(gpu):
         want = prog(*args)
         got = prog(*args, results=[torch.zeros((m, n), dtype=torch.bfloat16, device=gpu)], workspace=room)
         assert torch.equal(got, want) and room.any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["ln_rt", "lngrad_rt", "lngrad_plain_rt", "quantmx_e4m3_rt", "quantmx_e2m1_rt", "dequantmx_e2m1_rt",
+                                  "linmx_e2m1_rt", "linmx_e4m3_rt"])
+def test_empty_batch(gpu, name):
+    """No rows: the call returns its destinations and what has no row dim is as
+    it was, but for the weight's gradients, which are zeros.  Plain calls,
+    packed ones, slices of a batch, memref descriptors."""
+    import ctypes
+    import torch
+    from hfusion_mi355x import native
+    note("empty batch " + name)
+    grp = load(name)
+    assert grp.meta["params"] and all(r["tied"] >= 0 for r in grp.meta["results"])
+
+    def make(rows):
+        return [torch.full([rows if d == -1 else d for d in p["shape"]], 3, dtype=torch.float32, device=gpu)
+                .to(hf.runtime.torch_dtype(p["elem"])) for p in grp.meta["params"]]
+    args, batch = make(0), make(5)
+    assert any(t.data_ptr() == 0 for t in args)
+    cut = [t[:0] if -1 in p["shape"] else t for t, p in zip(batch, grp.meta["params"])]
+    descs = [native.memref_descriptor(t.data_ptr(), list(t.shape)) for t in args]
+    ptrs = (ctypes.c_void_p * len(descs))(*[ctypes.addressof(d) for d in descs])
+    grads = [i for i, p in enumerate(grp.meta["params"]) if name == "lngrad_rt" and p["role"] != "in" and -1 not in p["shape"]]
+    for tensors, call in ((args, lambda: grp(*args)), (args, lambda: grp.launcher(*args)()), (cut, lambda: grp(*cut)),
+                          (args, lambda: native.check(native.hfr().hfr_group_launch_memref(grp._h, ptrs, len(descs), torch.cuda.current_stream().cuda_stream)))):
+        for i in grads:
+            tensors[i].fill_(7)
+        before = [t.clone() for t in tensors]
+        ret = call()
+        torch.cuda.synchronize()
+        if ret is not None:
+            outs = ret if isinstance(ret, tuple) else (ret,)
+            assert all(o is tensors[r["tied"]] for o, r in zip(outs, grp.meta["results"]))
+        for i, (t, b) in enumerate(zip(tensors, before)):
+            assert not t.any() if i in grads else torch.equal(t.view(torch.uint8), b.view(torch.uint8))
+    assert all((t.float() == 3).all() for i, t in enumerate(batch) if i not in grads)
