@@ -27,6 +27,8 @@ struct GroupArgs {
   std::string func;
   bool rowsDyn = false; // the row count comes with the launch (-1 in the shapes)
   bool rowsZero = false; // a launch of no rows has results to write (manifest `rows_zero 1`)
+  uint64_t wsBytes = 0;
+  bool wsZero = false; // zero when first used, and what a launch leaves there the next one reads
   std::vector<std::string> paramRoles;
   std::vector<Buf> paramBufs, resultBufs;
   std::vector<int> resultTied;
@@ -45,6 +47,10 @@ struct GroupArgs {
       is >> i >> bytes;
       if (i < 0 || bytes <= 0) is.setstate(std::ios::failbit);
       align.push_back({i, bytes});
+    } else if (key == "workspace") {
+      int z = 0;
+      is >> wsBytes >> z;
+      wsZero = z != 0;
     } else if (key == "rows_zero") {
       int z = 0;
       is >> z;
@@ -144,6 +150,14 @@ struct GroupArgs {
       if ((size_t)a.first < nparams && params[a.first] % (uint64_t)a.second)
         return "argument " + std::to_string(a.first) + " of @" + func + " does not start on " + std::to_string(a.second) + " bytes";
     return {};
+  }
+
+  // Why a caller's workspace is refused: zeroed ones hold 64-bit words, of the
+  // others 16 bytes a lane are read and written.
+  std::string checkWorkspace(const void *ws) const {
+    const uintptr_t on = wsZero ? 8 : 16;
+    if (!wsBytes || (uintptr_t)ws % on == 0) return {};
+    return "a workspace of group @" + func + " has to start on " + std::to_string(on) + " bytes";
   }
 
 private:

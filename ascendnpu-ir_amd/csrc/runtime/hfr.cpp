@@ -73,8 +73,6 @@ struct hfr_group : GroupArgs {
   hfr_module *mod = nullptr;
   hipFunction_t fn = nullptr;
   hfr_launch_cfg cfg{};
-  uint64_t wsBytes = 0;
-  bool wsZero = false;
   uint64_t algoBytes = 0, algoOps = 0;
   // runtime row count (manifest `rows_dyn a b c cap`): grid.x =
   // min(ceil(R * a / b) * c, cap) (cap 0: none), or the static grid when a is 0
@@ -154,7 +152,6 @@ int parseBlock(const std::vector<std::string> &lines, hfr_group &g) {
     else if (key == "grid") is >> g.cfg.grid[0] >> g.cfg.grid[1] >> g.cfg.grid[2];
     else if (key == "block") is >> g.cfg.block[0] >> g.cfg.block[1] >> g.cfg.block[2];
     else if (key == "lds") is >> g.cfg.lds_bytes;
-    else if (key == "workspace") { int z = 0; is >> g.wsBytes >> z; g.wsZero = z != 0; }
     else if (key == "algo_bytes") is >> g.algoBytes;
     else if (key == "algo_ops") is >> g.algoOps;
     else if (key == "rows_dyn") {
@@ -386,9 +383,8 @@ int checkLaunch(const hfr_group *g, const uint64_t *params, size_t nparams, void
     return fail(HFR_ERR_INVALID, "group @" + g->func + " has a static row count");
   if (g && g->rowsDyn && rows < 0) return fail(HFR_ERR_INVALID, "negative row count for group @" + g->func);
   if (const int rc = checkGroupArgs(g, params, nparams, results, nresults, rows)) return rc;
-  if (g->wsBytes && (uintptr_t)workspace % 16)
-    return fail(HFR_ERR_INVALID, "a workspace of group @" + g->func + " has to start on 16 bytes");
-  return HFR_OK;
+  const std::string why = g->checkWorkspace(workspace);
+  return why.empty() ? (int)HFR_OK : fail(HFR_ERR_INVALID, why);
 }
 
 // The launch of checked arguments.

@@ -78,7 +78,7 @@ int hfr_group_info_get(hfr_group_t g, hfr_group_info *info);
  * scalar argument); results: one pointer per group result (ignored — may be
  * NULL — for results written into an argument); workspace: NULL to use the
  * group's own, or a caller buffer of workspace_bytes that starts on 16 bytes
- * (zeroed before its first use when the group requires it).  An argument that
+ * (on 8 and zeroed before its first use when the group requires a zeroed one).  An argument that
  * the manifest gives an `align` line is refused off those bytes; where it has
  * an `apart` line, so is a destination (an argument that is written, or a
  * result's buffer) over an argument of that line or over another destination.

@@ -33,6 +33,10 @@ const char *args_check(const GroupArgs *g, const uint64_t *p, size_t n, void *co
   why = g->check(p, n, r, nr, rows);
   return why.c_str();
 }
+const char *args_workspace(const GroupArgs *g, uint64_t at) {
+  why = g->checkWorkspace((const void *)(uintptr_t)at);
+  return why.c_str();
+}
 // ns of a check that passes, the best of 200 runs of 1000
 double args_time(const GroupArgs *g, const uint64_t *p, size_t n, void *const *r, size_t nr, int64_t rows) {
   double best = 1e30;
@@ -65,6 +69,7 @@ def lib(folder):
         _lib.args_load.argtypes, _lib.args_load.restype = [ctypes.c_char_p], p
         _lib.args_free.argtypes = [p]
         _lib.args_check.argtypes, _lib.args_check.restype = call, ctypes.c_char_p
+        _lib.args_workspace.argtypes, _lib.args_workspace.restype = [p, ctypes.c_uint64], ctypes.c_char_p
         _lib.args_time.argtypes, _lib.args_time.restype = call, ctypes.c_double
     return _lib
 
@@ -115,6 +120,9 @@ class Checked:
     def why(self, at=None, res=None):
         """What a launch says with these addresses in place of its own."""
         return self.lib.args_check(*self._packed(at, res)).decode()
+
+    def why_workspace(self, at):
+        return self.lib.args_workspace(self.h, at).decode()
 
     def ns(self):
         return self.lib.args_time(*self._packed(None, None))

@@ -115,3 +115,12 @@ def test_tensors_of_no_rows_have_no_address(folder, name):
     c = checked(name, folder, 1)
     for i in rows:
         assert c.why({i: 0}) == f"null device pointer for argument {i}"
+
+
+def test_where_a_workspace_starts(folder):
+    """argmax keeps 64-bit words there, and took any buffer of them; a weight
+    as bf16 is read 16 bytes a lane; a group without one takes what comes."""
+    for name, rows, on in (("argmax_16", -1, 8), ("lngrad_rt", 9, 16), ("linmx_e2m1_rt", 9, 16), ("ln_rt", 9, 1)):
+        c = checked(name, folder, rows)
+        for at in range(0x1000, 0x1020):
+            assert c.why_workspace(at) == ("" if at % on == 0 else f"a workspace of group @{c.meta['func']} has to start on {on} bytes")

@@ -157,3 +157,21 @@ def test_empty_batch(gpu, name):
         for i, (t, b) in enumerate(zip(tensors, before)):
             assert not t.any() if i in grads else torch.equal(t.view(torch.uint8), b.view(torch.uint8))
     assert all((t.float() == 3).all() for i, t in enumerate(batch) if i not in grads)
+
+
+@pytest.mark.gpu
+def test_argmax_with_a_workspace_off_16_bytes(gpu):
+    """Any buffer of 64-bit words is a workspace of argmax, as it was."""
+    import torch
+    note("argmax workspace")
+    grp = load("argmax_16")
+    p = grp.meta["params"]
+    x = torch.randn(p[0]["shape"], device=gpu)
+    rest = [torch.zeros(q["shape"], dtype=hf.runtime.torch_dtype(q["elem"]), device=gpu) for q in p[1:]]
+    want = [t.clone() for t in grp(x, *rest)]
+    room = torch.zeros(grp.info.workspace_bytes + 8, dtype=torch.uint8, device=gpu)
+    for _ in range(2):
+        got = grp(x, *rest, workspace=room[8:])
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with pytest.raises(RuntimeError, match="start on 8 bytes"):
+        grp(x, *rest, workspace=room[4:-4])
