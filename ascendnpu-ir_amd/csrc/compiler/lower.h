@@ -48,8 +48,8 @@ struct KernelPlan {
   std::vector<PreKernel> pre;
   // other kernels of the group for small runtime row counts, by ascending
   // maxRows: a launch of R <= maxRows rows runs the first that fits, without
-  // the pre kernels (unless `pre`), on ceil(R / rowsB) * rowsC blocks, instead
-  // of the main one
+  // the pre kernels and the workspace (unless `pre`), on ceil(R / rowsB) * rowsC
+  // blocks, instead of the main one
   struct RowAlt {
     std::string name;
     int64_t maxRows = 0, rowsB = 1, rowsC = 1;

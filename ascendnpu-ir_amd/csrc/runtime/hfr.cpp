@@ -44,8 +44,9 @@ struct PreLaunch {
   std::vector<Karg> kargs;
 };
 
-// A kernel that takes the main kernel's place (without the pre kernels) for
-// launches of at most maxRows runtime rows: ceil(R / rowsB) * rowsC blocks.
+// A kernel that takes the main kernel's place for launches of at most maxRows
+// runtime rows: ceil(R / rowsB) * rowsC blocks, without the pre kernels (unless
+// `pre`) and then without the workspace.
 struct RowAlt {
   std::string kernel;
   hipFunction_t fn = nullptr;
@@ -58,7 +59,10 @@ struct RowAlt {
 // stream, so that launches on two streams may overlap.  A zeroed one keeps
 // what its kernels left there from launch to launch and stays the only one.
 struct OwnWorkspace {
-  void *first = nullptr; // allocated and zeroed when the handle is loaded
+  // allocated and zeroed when the handle is loaded, or, where the row count
+  // decides whether a launch uses one, at the first launch that does (a weight
+  // product that only ever has a few rows holds no bf16 copy of its weight)
+  void *first = nullptr;
   int device = -1;
   std::mutex mu;
   bool taken = false;
@@ -291,17 +295,18 @@ hipError_t ownWorkspaceFree(OwnWorkspace &o) {
   return e;
 }
 // the workspace of a launch on `stream`, allocated at the stream's first one
+// that uses it
 int ownWorkspaceOf(OwnWorkspace &o, uint64_t bytes, bool zeroed, void *stream, const char *what, void **ws) {
   int dev = 0;
   (void)hipGetDevice(&dev);
   if (dev != o.device) return fail(HFR_ERR_INVALID, std::string(what) + " workspace belongs to another device");
   std::lock_guard<std::mutex> lk(o.mu);
-  if (!o.taken) {
+  if (o.first && !o.taken) {
     o.taken = true;
     o.firstStream = stream;
   }
   *ws = o.first;
-  if (zeroed || stream == o.firstStream) return HFR_OK;
+  if (o.first && (zeroed || stream == o.firstStream)) return HFR_OK;
   for (auto &m : o.more)
     if (m.first == stream) {
       *ws = m.second;
@@ -314,7 +319,12 @@ int ownWorkspaceOf(OwnWorkspace &o, uint64_t bytes, bool zeroed, void *stream, c
   const hipError_t e = hipMalloc(&p, bytes);
   (void)hipThreadExchangeStreamCaptureMode(&mode);
   if (e != hipSuccess) return hipFail(e, "workspace allocation");
-  o.more.push_back({stream, p});
+  if (o.first) o.more.push_back({stream, p});
+  else {
+    o.first = p;
+    o.taken = true;
+    o.firstStream = stream;
+  }
   *ws = p;
   return HFR_OK;
 }
@@ -324,6 +334,19 @@ int checkGroupArgs(const hfr_group *g, const uint64_t *params, size_t nparams, v
   if (!g) return fail(HFR_ERR_INVALID, "null group");
   const std::string why = g->check(params, nparams, results, nresults, rows);
   return why.empty() ? (int)HFR_OK : fail(HFR_ERR_INVALID, why);
+}
+
+// The kernel that a launch of `rows` rows runs in the main one's place.
+const RowAlt *altFor(const hfr_group *g, int64_t rows) {
+  for (const RowAlt &alt : g->alts)
+    if (rows <= alt.maxRows) return &alt;
+  return nullptr;
+}
+// Bytes of workspace that a launch of `rows` rows (-1: a static count) uses.
+uint64_t workspaceOf(const hfr_group *g, int64_t rows) {
+  if (g->rowsDyn && rows == 0 && !g->rowsZero) return 0;
+  const RowAlt *alt = altFor(g, rows);
+  return alt && !alt->pre ? 0 : g->wsBytes;
 }
 
 // Assembles the kernel arguments (params, own result buffers, workspace) and
@@ -360,18 +383,15 @@ int launchGroup(const hfr_group *g, const uint64_t *params, void *const *results
     }
     return (int)HFR_OK;
   };
-  for (auto &alt : g->alts)
-    if (rows <= alt.maxRows) {
-      if (alt.pre) {
-        const int rc = runPre();
-        if (rc) return rc;
-      }
-      hfr_launch_cfg cfg{};
-      cfg.grid[0] = (unsigned)((std::max<int64_t>(rows, 1) + alt.rowsB - 1) / alt.rowsB * alt.rowsC); // (no rows only with rows_zero)
-      cfg.grid[1] = cfg.grid[2] = cfg.block[1] = cfg.block[2] = 1;
-      cfg.block[0] = alt.block;
-      return launch(alt.fn, cfg, g->kargs);
-    }
+  if (const RowAlt *alt = altFor(g, rows)) {
+    if (alt->pre)
+      if (const int rc = runPre()) return rc;
+    hfr_launch_cfg cfg{};
+    cfg.grid[0] = (unsigned)((std::max<int64_t>(rows, 1) + alt->rowsB - 1) / alt->rowsB * alt->rowsC); // (no rows only with rows_zero)
+    cfg.grid[1] = cfg.grid[2] = cfg.block[1] = cfg.block[2] = 1;
+    cfg.block[0] = alt->block;
+    return launch(alt->fn, cfg, g->kargs);
+  }
   if (const int rc = runPre()) return rc;
   return launch(g->fn, rowsCfg(g->cfg), g->kargs);
 }
@@ -391,7 +411,7 @@ int checkLaunch(const hfr_group *g, const uint64_t *params, size_t nparams, void
 int runChecked(hfr_group *g, const uint64_t *params, void *const *results, int64_t rows, void *workspace, void *stream) {
   if (g->rowsDyn && rows == 0 && !g->rowsZero) return HFR_OK; // nothing to do
   void *ws = workspace;
-  if (g->wsBytes && !ws)
+  if (!ws && workspaceOf(g, rows))
     if (const int rc = ownWorkspaceOf(*g->own, g->wsBytes, g->wsZero, stream, "group", &ws)) return rc;
   return launchGroup(g, params, results, ws, stream, rows);
 }
@@ -479,7 +499,11 @@ int hfr_group_load(const char *manifest_path, const char *func, hfr_group_t *out
   }
   // the group's own workspace lives on the device current at load time, so
   // that launches stay asynchronous
-  if (g->wsBytes) {
+  bool always = true; // every launch uses the workspace
+  for (const RowAlt &alt : g->alts) always = always && alt.pre;
+  if (g->wsBytes && !always && !g->wsZero) {
+    (void)hipGetDevice(&g->own->device);
+  } else if (g->wsBytes) {
     e = ownWorkspaceInit(*g->own, g->wsBytes);
     if (e != hipSuccess) {
       hfr_module_unload(g->mod);
@@ -521,6 +545,8 @@ int hfr_group_info_get(hfr_group_t g, hfr_group_info *info) {
   info->cfg = g->cfg;
   return HFR_OK;
 }
+
+uint64_t hfr_group_workspace_rows(hfr_group_t g, int64_t rows) { return g ? workspaceOf(g, rows) : 0; }
 
 int hfr_group_launch(hfr_group_t g, const uint64_t *params, size_t nparams, void *const *results, size_t nresults,
                      void *workspace, void *stream) {

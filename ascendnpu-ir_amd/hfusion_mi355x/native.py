@@ -101,6 +101,8 @@ def hfr():
         lib.hfr_group_launch_noalloc.argtypes = [vp, ctypes.POINTER(ctypes.c_uint64), ctypes.c_size_t,
                                                  ctypes.POINTER(vp), ctypes.c_size_t, vp]
         lib.hfr_scratch_bytes.restype = ctypes.c_uint64
+        lib.hfr_group_workspace_rows.argtypes = [vp, ctypes.c_int64]
+        lib.hfr_group_workspace_rows.restype = ctypes.c_uint64
         for fn in ("hfr_module_load", "hfr_module_unload", "hfr_kernel_get", "hfr_launch", "hfr_group_load",
                    "hfr_group_unload", "hfr_group_info_get", "hfr_group_launch", "hfr_program_load",
                    "hfr_program_unload", "hfr_program_info_get", "hfr_program_launch", "hfr_group_launch_memref",

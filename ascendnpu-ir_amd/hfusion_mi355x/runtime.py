@@ -376,7 +376,8 @@ class Group:
                     raise ValueError(f"result {j} of @{self.func}: expected {r['elem']}{list(want(r['shape']))}")
                 outs.append(t)
                 rptrs[j] = t.data_ptr()
-        fresh = self._scratch and stream is None and not noalloc and _capturing()
+        need = native.hfr().hfr_group_workspace_rows(self._h, rows if dyn else -1) if self.info.workspace_bytes else 0
+        fresh = self._scratch and need and stream is None and not noalloc and _capturing()
         if stream is None:
             stream = torch.cuda.current_stream(device).cuda_stream
         ret = outs[0] if len(outs) == 1 else tuple(outs)
@@ -384,9 +385,9 @@ class Group:
         if workspace is not None:
             if noalloc:
                 raise ValueError("noalloc launches take no workspace")
-            _check_workspace(workspace, self.info.workspace_bytes, self.func)
+            _check_workspace(workspace, need, self.func)
         elif fresh:
-            workspace = torch.empty(self.info.workspace_bytes, dtype=torch.uint8, device=device)
+            workspace = torch.empty(need, dtype=torch.uint8, device=device)
         if noalloc:
 
             def launch(keep=workspace):

@@ -11,12 +11,15 @@
  * buffers for results that are not written into an argument.
  *
  * Ownership: the caller allocates and frees every tensor buffer.  The runtime
- * owns module/group handles and one zero-initialised workspace per group
- * handle that needs one, allocated by hfr_group_load on the current device.
- * The first stream that the handle is launched on has it; every other stream
- * gets one of its own at its first launch of the handle (the only launch that
- * allocates), except where launches rely on what earlier ones left in a zeroed
- * workspace: that one stays the handle's only one.
+ * owns module/group handles and one workspace per group handle that needs
+ * one, allocated and zeroed by hfr_group_load on the current device.  The first
+ * stream that the handle is launched on has it; every other stream gets one of
+ * its own at its first launch of the handle, except where launches rely on what
+ * earlier ones left in a zeroed workspace: that one stays the handle's only
+ * one.  Where the launch's row count decides whether it uses a workspace
+ * (hfr_group_workspace_rows), the first one is allocated at the first launch
+ * that does too.  No other launch allocates.  All of them are freed with the
+ * handle, not with their streams.
  * Threading: launches are asynchronous on the given stream; the caller
  * synchronises.  A handle must not be used from two threads at once, and two
  * in-flight launches that use one workspace must be on the same stream (graphs
@@ -97,6 +100,11 @@ int hfr_group_launch(hfr_group_t g, const uint64_t *params, size_t nparams, void
  * unless rows is -1. */
 int hfr_group_launch_rows(hfr_group_t g, const uint64_t *params, size_t nparams, void *const *results,
                           size_t nresults, int64_t rows, void *workspace, void *stream);
+
+/* Bytes of the workspace that a launch over `rows` rows uses (-1 for a group
+ * with a static row count): at most hfr_group_info.workspace_bytes, 0 where the
+ * kernels for so few rows need none. */
+uint64_t hfr_group_workspace_rows(hfr_group_t g, int64_t rows);
 
 /* ---- launch programs (an un-fused function split into fused groups)
  * Replaces the host function the reference's HFusion auto-fusion leaves

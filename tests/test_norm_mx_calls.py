@@ -175,3 +175,73 @@ def test_argmax_with_a_workspace_off_16_bytes(gpu):
         assert all(torch.equal(a, b) for a, b in zip(got, want))
     with pytest.raises(RuntimeError, match="start on 8 bytes"):
         grp(x, *rest, workspace=room[4:-4])
+
+
+@pytest.mark.gpu
+def test_workspace_of_the_launches_that_use_one(gpu):
+    """A weight product at launch-time rows holds the weight as bf16 only once
+    a launch of many rows needs it there; nor does a stream or a captured
+    graph of few rows."""
+    import torch
+    note("workspace when used")
+    art = hf.compile(hf.catalog.get("linear_mx_rt"), options="dyn=runtime", require_cached=True)
+    n = k = 4096
+    torch.cuda.synchronize()
+    w = torch.randint(-128, 128, (n, k // 2), dtype=torch.int8, device=gpu)
+    s = torch.randint(115, 125, (n, k // 32), dtype=torch.int8, device=gpu)
+    bias = torch.randn(n, device=gpu)
+
+    def tensors(rows):
+        return torch.randn(rows, k, device=gpu).bfloat16(), torch.zeros((rows, n), dtype=torch.bfloat16, device=gpu)
+    few, many = tensors(3), tensors(4096)
+    whole = 2 * n * k
+
+    def free():  # (what torch caches goes back at a capture, so before every look)
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        return torch.cuda.mem_get_info()[0]
+    rows_of = hf.native.hfr().hfr_group_workspace_rows
+    torch.cuda.synchronize()
+    start = free()
+    grp = art.load()
+    assert grp.info.workspace_bytes == whole and [rows_of(grp._h, r) for r in (0, 1, 3, 4096, 10 ** 6)] == [0, 0, 0, whole, whole]
+    loaded = free()
+    assert start - loaded < whole // 2  # (its code)
+    side = torch.cuda.Stream()
+    grp(few[0], w, s, bias, few[1])
+    want = few[1].clone()
+    with torch.cuda.stream(side):
+        grp(few[0], w, s, bias, few[1])
+    grp(few[0], w, s, bias, few[1], workspace=torch.zeros(16, dtype=torch.uint8, device=gpu))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.reset_peak_memory_stats()
+    held = torch.cuda.memory_allocated()
+    with torch.cuda.graph(graph):
+        grp(few[0], w, s, bias, few[1])
+    assert torch.cuda.max_memory_allocated() - held < whole // 2
+    few[1].zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(few[1], want) and loaded - free() < whole // 2
+    with pytest.raises(ValueError, match=f"needs a workspace of {whole} bytes"):
+        grp(many[0], w, s, bias, many[1], workspace=torch.zeros(16, dtype=torch.uint8, device=gpu))
+    grp(many[0], w, s, bias, many[1])
+    first = many[1].clone()
+    one = free()
+    assert loaded - one >= whole
+    with torch.cuda.stream(side):
+        many[1].zero_()
+        grp(many[0], w, s, bias, many[1])
+    torch.cuda.synchronize()
+    assert torch.equal(many[1], first) and one - free() >= whole
+    given = torch.zeros(whole, dtype=torch.uint8, device=gpu)
+    grp(many[0], w, s, bias, many[1].zero_(), workspace=given)
+    assert torch.equal(many[1], first) and given.any()
+    del grp, graph
+    # a gradient of few rows is one launch without one, of none too
+    grp = load("lngrad_rt")
+    assert [rows_of(grp._h, r) > 0 for r in (0, 1, 1200, 1201)] == [False, False, False, True]
+    grp = load("argmax_16")
+    assert rows_of(grp._h, -1) == grp.info.workspace_bytes > 0
+    assert rows_of(load("ln_rt")._h, 5) == 0
