@@ -377,7 +377,6 @@ class Group:
                 outs.append(t)
                 rptrs[j] = t.data_ptr()
         need = native.hfr().hfr_group_workspace_rows(self._h, rows if dyn else -1) if self.info.workspace_bytes else 0
-        fresh = self._scratch and need and stream is None and not noalloc and _capturing()
         if stream is None:
             stream = torch.cuda.current_stream(device).cuda_stream
         ret = outs[0] if len(outs) == 1 else tuple(outs)
@@ -386,25 +385,19 @@ class Group:
             if noalloc:
                 raise ValueError("noalloc launches take no workspace")
             _check_workspace(workspace, need, self.func)
-        elif fresh:
-            workspace = torch.empty(need, dtype=torch.uint8, device=device)
         if noalloc:
 
-            def launch(keep=workspace):
+            def launch():
                 native.check(lib.hfr_group_launch_noalloc(h, slots, n, rptrs, nr, stream))
                 return ret
-        elif dyn:
-            ws = workspace.data_ptr() if workspace is not None else None
+            return launch
+        entry, at = (lib.hfr_group_launch_rows, (rows,)) if dyn else (lib.hfr_group_launch, ())
+        own = workspace is None and self._scratch and need
 
-            def launch(keep=workspace):
-                native.check(lib.hfr_group_launch_rows(h, slots, n, rptrs, nr, rows, ws, stream))
-                return ret
-        else:
-            ws = workspace.data_ptr() if workspace is not None else None
-
-            def launch(keep=workspace):
-                native.check(lib.hfr_group_launch(h, slots, n, rptrs, nr, ws, stream))
-                return ret
+        def launch():
+            ws = _graph_workspace(need, device, stream) if own else workspace
+            native.check(entry(h, slots, n, rptrs, nr, *at, ws.data_ptr() if ws is not None else None, stream))
+            return ret
         return launch
 
 
@@ -415,6 +408,18 @@ def _capture_query():
 
 def _capturing():
     return _capture_query()()
+
+
+def _graph_workspace(nbytes, device, stream):
+    """Workspace of a launch on `stream` if that is the current stream and
+    under capture: one in the graph's memory.  (A launch's own: a packed one
+    may be captured into several graphs.)"""
+    if not _capturing():
+        return None
+    import torch
+    if torch.cuda.current_stream(device).cuda_stream != stream:
+        return None
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
 def _check_workspace(ws, nbytes, name):
@@ -495,13 +500,12 @@ class Program:
                     raise ValueError(f"result {j} of @{self.name}: expected {r['elem']}{list(r['shape'])}")
                 outs.append(t)
                 rptrs[j] = t.data_ptr()
-        stream_is_current = stream is None
         if stream is None:
             stream = torch.cuda.current_stream(device).cuda_stream
         if workspace is not None:
             _check_workspace(workspace, self.workspace_bytes, self.name)
-        elif self.workspace_bytes and stream_is_current and _capturing():
-            workspace = torch.empty(self.workspace_bytes, dtype=torch.uint8, device=device)
+        elif self.workspace_bytes:
+            workspace = _graph_workspace(self.workspace_bytes, device, stream)
         ws = workspace.data_ptr() if workspace is not None else None
         native.check(native.hfr().hfr_program_launch(self._h, slots, len(params), rptrs, len(res_meta), ws, stream))
         return outs[0] if len(outs) == 1 else tuple(outs)

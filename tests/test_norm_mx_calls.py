@@ -245,3 +245,66 @@ def test_workspace_of_the_launches_that_use_one(gpu):
     grp = load("argmax_16")
     assert rows_of(grp._h, -1) == grp.info.workspace_bytes > 0
     assert rows_of(load("ln_rt")._h, 5) == 0
+
+
+class Spy:
+    """The runtime library, with the workspaces that launches are given."""
+
+    def __init__(self, lib):
+        self.lib, self.seen = lib, []
+
+    def __getattr__(self, name):
+        fn = getattr(self.lib, name)
+        at = {"hfr_group_launch_rows": 6, "hfr_group_launch": 5, "hfr_program_launch": 5}.get(name)
+        if at is None:
+            return fn
+
+        def call(*args):
+            self.seen.append(args[at])
+            return fn(*args)
+        return call
+
+
+@pytest.mark.gpu
+def test_every_capture_has_a_workspace_of_its_own(gpu, monkeypatch):
+    """Under capture on the stream that a launch goes to, its workspace lies in
+    the graph's memory: with the stream named, through a packed launch, through
+    one that was packed before the capture, or in one and used behind it."""
+    import torch
+    from hfusion_mi355x import native
+    note("workspaces under capture")
+    spy = Spy(native.hfr())
+    monkeypatch.setattr(native, "hfr", lambda: spy)
+    c = (2100, 1000, "bf16", "f32", "e4m3", 2)
+    xs, x, gs, gm, _, _, ds, dy = norm_inputs(c)
+    arrays, xv, mean, rstd = grad_args(c, xs, x, gs, ds)
+    grp, prog = load("lngrad_rt"), load("prog_norm_linear_mx")
+    args = device_args(grp, arrays, gpu)
+    m, n, k = 20, 208, 384
+    pargs = [torch.zeros(p["shape"], dtype=hf.runtime.torch_dtype(p["elem"]), device=gpu) for p in prog.meta["params"]]
+    out = torch.zeros((m, n), dtype=torch.bfloat16, device=gpu)
+    side = torch.cuda.Stream()
+    packed = grp.launcher(*args, stream=side.cuda_stream)
+    torch.cuda.synchronize()
+    graphs, inside = [], []
+    for make in (lambda: grp(*args, stream=side.cuda_stream), packed, packed,
+                 lambda: inside.append(grp.launcher(*args)) or inside[0](),
+                 lambda: prog(*pargs, results=[out], stream=side.cuda_stream)):
+        graphs.append(torch.cuda.CUDAGraph())
+        spy.seen.clear()
+        with torch.cuda.graph(graphs[-1], stream=side):
+            make()
+        assert len(spy.seen) == 1 and spy.seen[0] is not None
+        graphs[-1].first = spy.seen[0]
+    assert len({g.first for g in graphs}) == len(graphs)
+    # outside a capture: the stream's
+    spy.seen.clear()
+    packed(), inside[0](), grp(*args, stream=side.cuda_stream), prog(*pargs, results=[out])
+    assert spy.seen == [None] * 4
+    torch.cuda.synchronize()
+    for graph in graphs[:4]:
+        for t in args[-3:]:
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        check_grad(c, host(args[-3:], grp), xv, gm, dy, mean, rstd, groups=256)
