@@ -251,7 +251,8 @@ class Group:
 
     def _make_call(self):
         """The plain call as one C function (native.hfcall), where every
-        argument is a tensor and every result is written into one."""
+        argument is a tensor and every result is written into one.  False: the
+        Python path makes it (2 to 3 us later)."""
         plan = self._plan
         if plan is None:
             plan = self._plan = self._make_plan()
@@ -261,7 +262,11 @@ class Group:
         h = getattr(self, "_h", None)
         if any(dt is None or len(sh) > 8 for dt, sh in specs) or len(specs) > 24 or not tied or min(tied) < 0 or not h:
             return False
-        return native.hfcall().plan(ctypes.cast(launch, ctypes.c_void_p).value, h.value, rows_at is not None,
+        try:
+            hfcall = native.hfcall()
+        except (native.NativeLibraryMissing, ImportError):  # (built without Python's headers, or for another Python)
+            return False
+        return hfcall.plan(ctypes.cast(launch, ctypes.c_void_p).value, h.value, rows_at is not None,
                                     torch.Tensor, raw_stream, specs, tied, _capture_query() if self._scratch else None)
 
     def _launch_plain(self, args):
