@@ -32,6 +32,11 @@ LINEAR_LONG = [(3, 20, 131072, "e2m1", False, "f32"), (9, 33, 98304, "e4m3", Fal
 # more rows than the workgroups take at once
 NORM_LONG = [(2081, 2001, "bf16", "f32", None, 2), (9000, 33, "f16", "f16", "e4m3", 2), (777, 5003, "f32", "f32", None, 1),
              (4200, 160, "f32", "f32", "e5m2", 2)]
+# rows too wide for two row groups a workgroup, and more of them than one launch
+# of the gradient takes: every thread stores its partial sums itself; f32 rows
+# past 8192 are not loaded ahead
+NORM_WIDE = [(1000, 5003, "f32", "f32", None, 2), (1100, 8200, "bf16", "f32", "e4m3", 2), (900, 16383, "f32", "f32", None, 1),
+             (1030, 4104, "f16", "f16", "e5m2", 1)]
 # the same at a launch-time row count, and the row counts they are called with
 RT_ROWS = [1, 5, 16, 17, 40, 64, 65, 130, 515]
 
@@ -89,6 +94,10 @@ def entries():
     e["ln_rt"] = rt(g.layer_norm(_ANY, 1000, ckpt="e4m3"))
     e["lngrad_rt"] = rt(g.layer_norm_grad(_ANY, 1000, ckpt="e4m3", params="f32"))
     e["lngrad_wide_rt"] = rt(g.layer_norm_grad(_ANY, 4096))
+    for c in NORM_WIDE:
+        e[norm_name(c)] = g.layer_norm(**_norm_kw(c))
+        e[norm_name(c, "lngrad")] = g.layer_norm_grad(**_norm_kw(c))
+    e["lngrad_long_rt"] = rt(g.layer_norm_grad(_ANY, 5000, params="f32"))
     e["lngrad_plain_rt"] = rt(g.layer_norm_grad(_ANY, 96, affine=0))
     e["linmx_e2m1_rt"] = rt(g.linear_mx(_ANY, 130, 544, bias=True))
     e["linmx_e4m3_rt"] = rt(g.linear_mx(_ANY, 1040, 1024, fmt="e4m3"))

@@ -10,7 +10,7 @@ import group_catalog as cat
 import norm_mx_catalog as nc
 from helpers import to_dev, to_host
 from oracle import blockscaled as bs
-from test_norm_mx import E24, check_grad, check_norm, grad_args, linear_inputs, norm_inputs, note, stored
+from test_norm_mx import E24, check_grad, check_norm, grad_args, linear_inputs, norm_args, norm_inputs, note, stored
 
 
 def load(name):
@@ -308,3 +308,41 @@ def test_every_capture_has_a_workspace_of_its_own(gpu, monkeypatch):
         graph.replay()
         torch.cuda.synchronize()
         check_grad(c, host(args[-3:], grp), xv, gm, dy, mean, rstd, groups=256)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("c", nc.NORM_WIDE, ids=lambda c: nc.norm_name(c, "lngrad"))
+def test_gradient_of_many_wide_rows(gpu, c):
+    """Two launches, a row a workgroup: each thread leaves its columns' partial
+    sums, the row's ragged end among them."""
+    note(nc.norm_name(c, "lngrad"))
+    grp = load(nc.norm_name(c, "lngrad"))
+    assert grp.info.workspace_bytes == 256 * c[5] * c[1] * 4 and len(grp.meta["pre"]) == 1
+    xs, x, gs, gm, _, _, ds, dy = norm_inputs(c)
+    arrays, xv, mean, rstd = grad_args(c, xs, x, gs, ds)
+    check_grad(c, host(grp(*device_args(grp, arrays, gpu)), grp), xv, gm, dy, mean, rstd, groups=256)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("c", nc.NORM_WIDE, ids=nc.norm_name)
+def test_norm_of_many_wide_rows(gpu, c):
+    """Workgroups of one row each that walk several."""
+    note(nc.norm_name(c))
+    grp = load(nc.norm_name(c))
+    assert grp.meta["grid"][0] < c[0]
+    xs, x, gs, gm, ts, bt, _, _ = norm_inputs(c)
+    check_norm(c, host(grp(*device_args(grp, norm_args(c, xs, gs, ts), gpu)), grp), x, gm, bt)
+
+
+@pytest.mark.gpu
+def test_gradient_of_wide_rows_at_launch_time(gpu):
+    """Both sides of the row count up to which one launch makes it."""
+    note("lngrad_long_rt")
+    grp = load("lngrad_long_rt")
+    for rows in (1, 255, 896, 897, 1300):
+        note(f"rows {rows}")
+        assert (hf.native.hfr().hfr_group_workspace_rows(grp._h, rows) > 0) == (rows > 896)
+        c = (rows, 5000, "bf16", "f32", None, 2)
+        xs, x, gs, gm, _, _, ds, dy = norm_inputs(c)
+        arrays, xv, mean, rstd = grad_args(c, xs, x, gs, ds)
+        check_grad(c, host(grp(*device_args(grp, arrays, gpu)), grp), xv, gm, dy, mean, rstd, groups=256)
