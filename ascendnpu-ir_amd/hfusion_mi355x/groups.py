@@ -547,8 +547,10 @@ def linear_mx(m, n, k, fmt="e2m1", bias=False, out="bf16"):
     sum_k a[m, k] w[n, k] 2^E[n, k/32] (+ f32 bias[n]), f32 sums, one rounding
     to `out`.  w is [n, k] fp8 or [n, k/2] bytes of two e2m1 codes (the layout
     quantize_mx gives a weight [n, k] along its rows); k is a multiple of 32.
-    The weight's values are multiplied as bf16: one past its range (2^128,
-    scale bytes above 246) is infinite."""
+    The weight's values are multiplied as bf16, exactly but at the ends of its
+    range: 2^128 and more (possible at scale bytes above 239 for e5m2, 246 for
+    e4m3, 252 for e2m1) is infinite, and what is no multiple of 2^-133 (at
+    scale bytes below 10 for e5m2, 3 for e4m3) is rounded to one."""
     A, O, C = _t([m, k], "bf16"), _t([m, n], out), _t([m, n], "f32")
     W, S = _mx_types(n, k, fmt, 1)
     B = _t([n], "f32")

@@ -10,7 +10,7 @@ import group_catalog as cat
 import norm_mx_catalog as nc
 from helpers import to_dev, to_host
 from oracle import blockscaled as bs
-from test_norm_mx import E24, check_grad, check_norm, grad_args, linear_inputs, norm_args, norm_inputs, note, stored
+from test_norm_mx import E24, check_grad, check_linear, check_norm, grad_args, linear_inputs, norm_args, norm_inputs, note, stored, value
 
 
 def load(name):
@@ -346,3 +346,66 @@ def test_gradient_of_wide_rows_at_launch_time(gpu):
         xs, x, gs, gm, _, _, ds, dy = norm_inputs(c)
         arrays, xv, mean, rstd = grad_args(c, xs, x, gs, ds)
         check_grad(c, host(grp(*device_args(grp, arrays, gpu)), grp), xv, gm, dy, mean, rstd, groups=256)
+
+
+# the largest scale byte at which every finite code of the format is finite as bf16
+LAST_FINITE = {"e5m2": 239, "e4m3": 246, "e2m1": 252}
+ENDS = [(3, 33, 96, "e5m2", False, "f32"), (48, 129, 512, "e4m3", True, "f32"), (17, 100, 1024, "e2m1", True, "bf16"),
+        (2300, 520, 1024, "e4m3", True, "bf16"), (4200, 129, 96, "e5m2", True, "bf16"), (4500, 40, 288, "e2m1", False, "f32")]
+
+
+def bf16_of(w):
+    """f64 values rounded to bf16, its subnormals (steps of 2^-133) among them."""
+    step = np.ldexp(1.0, np.maximum(np.frexp(w)[1] - 8, -133))
+    v = np.rint(w / step) * step
+    return np.where(np.abs(v) >= 2.0 ** 128, np.copysign(np.inf, v), v)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("c", ENDS, ids=nc.linear_name)
+def test_product_of_the_smallest_weights(gpu, c):
+    """Small codes under the smallest scale bytes lie below bf16's smallest
+    subnormal or between two of them: they count as what they round to."""
+    m, n, k, fmt, bias, out = c
+    note("smallest weights " + nc.linear_name(c))
+    rng = np.random.default_rng(m + k)
+    # (8-bit codes up to 1, both signs)
+    codes = rng.integers(0, 16, (n, k)) if fmt == "e2m1" else rng.integers(0, 0x3C if fmt == "e5m2" else 0x38, (n, k)) + 128 * rng.integers(0, 2, (n, k))
+    codes = codes.astype(np.uint8)
+    w = bs.pack(codes, 1).view(np.int8) if fmt == "e2m1" else codes
+    s = rng.integers(0, 4, (n, k // 32)).astype(np.uint8)
+    exact = bs.dequantize(w, s, fmt, 1)
+    wv = bf16_of(exact)
+    assert (wv == exact).all() if fmt == "e2m1" else ((wv != exact).mean() > 0.1 and ((wv == 0) & (exact != 0)).any())
+    as_, a = stored(np.ldexp(rng.normal(size=(m, k)), 110), "bf16")
+    grp = load(nc.linear_name(c))
+    args = [as_, w, s.view(np.int8)] + [np.zeros(n, np.float32)] * bias + [np.zeros((m, n), np.float32 if out == "f32" else np.uint16)]
+    check_linear(host([grp(*device_args(grp, args, gpu))], grp)[0], out, a, wv, np.zeros(n), k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("c", ENDS, ids=nc.linear_name)
+def test_product_of_the_largest_weights(gpu, c):
+    """Up to the format's last scale byte the largest code is a finite weight,
+    past it an infinite one."""
+    m, n, k, fmt, bias, out = c
+    note("largest weights " + nc.linear_name(c))
+    top = {"e5m2": 0x7B, "e4m3": 0x7E, "e2m1": 7}[fmt]
+    rng = np.random.default_rng(m + k)
+    codes = np.zeros((n, k), np.uint8)
+    codes[:, ::32] = top + (8 if fmt == "e2m1" else 128) * rng.integers(0, 2, (n, k // 32))
+    w = bs.pack(codes, 1).view(np.int8) if fmt == "e2m1" else codes
+    as_, a = stored(np.ldexp(rng.uniform(1, 2, (m, k)), -40), "bf16")
+    grp = load(nc.linear_name(c))
+    for byte in (LAST_FINITE[fmt], LAST_FINITE[fmt] + 1):
+        s = np.full((n, k // 32), 127, np.uint8)
+        s[:: 2, -1] = byte
+        exact = bs.dequantize(w, s, fmt, 1)
+        wv = bf16_of(exact)
+        assert np.isfinite(wv).all() == (byte == LAST_FINITE[fmt]) and np.isfinite(exact).all()
+        args = [as_, w, s.view(np.int8)] + [np.zeros(n, np.float32)] * bias + [np.zeros((m, n), np.float32 if out == "f32" else np.uint16)]
+        got = host([grp(*device_args(grp, args, gpu))], grp)[0]
+        far = np.isinf(wv).any(axis=1)
+        check_linear(got[:, ~far], out, a, wv[~far], np.zeros((~far).sum()), k)
+        want = np.broadcast_to(np.sign(exact[far, -32]) * np.inf, (m, far.sum()))
+        assert np.array_equal(value(got[:, far], out), want)
