@@ -37,6 +37,8 @@ NORM_LONG = [(2081, 2001, "bf16", "f32", None, 2), (9000, 33, "f16", "f16", "e4m
 # past 8192 are not loaded ahead
 NORM_WIDE = [(1000, 5003, "f32", "f32", None, 2), (1100, 8200, "bf16", "f32", "e4m3", 2), (900, 16383, "f32", "f32", None, 1),
              (1030, 4104, "f16", "f16", "e5m2", 1)]
+# a training step of norm and linear layer: rows, columns of the norm, outputs
+STEP = (96, 512, 192)
 # the same at a launch-time row count, and the row counts they are called with
 RT_ROWS = [1, 5, 16, 17, 40, 64, 65, 130, 515]
 
@@ -97,6 +99,10 @@ def entries():
     for c in NORM_WIDE:
         e[norm_name(c)] = g.layer_norm(**_norm_kw(c))
         e[norm_name(c, "lngrad")] = g.layer_norm_grad(**_norm_kw(c))
+    m, k, n = STEP
+    e["step_norm"], e["step_norm_grad"] = g.layer_norm(m, k, ckpt="e4m3"), g.layer_norm_grad(m, k, ckpt="e4m3")
+    e["step_codes"], e["step_values"] = g.quantize_mx(n, k, fmt="e2m1"), g.dequantize_mx(n, k, fmt="e2m1")
+    e["step_linear"], e["step_linear_grad"] = g.linear_mx(m, n, k, bias=True), g.bf16_mmad(m, k, n, b_layout="kn")
     e["lngrad_long_rt"] = rt(g.layer_norm_grad(_ANY, 5000, params="f32"))
     e["lngrad_plain_rt"] = rt(g.layer_norm_grad(_ANY, 96, affine=0))
     e["linmx_e2m1_rt"] = rt(g.linear_mx(_ANY, 130, 544, bias=True))

@@ -409,3 +409,48 @@ def test_product_of_the_largest_weights(gpu, c):
         check_linear(got[:, ~far], out, a, wv[~far], np.zeros((~far).sum()), k)
         want = np.broadcast_to(np.sign(exact[far, -32]) * np.inf, (m, far.sum()))
         assert np.array_equal(value(got[:, far], out), want)
+
+
+@pytest.mark.gpu
+def test_training_step_with_its_weight(gpu):
+    """Norm with an 8-bit checkpoint, the weight to 4 bits, the product; back
+    through the weight's values (a bf16 contraction) into the norm's gradient.
+    On the device throughout; each stage is held to its own tolerance on what
+    the stage before left."""
+    import torch
+    note("training step with its weight")
+    m, k, n = nc.STEP
+    c = (m, k, "bf16", "bf16", "e4m3", 2)
+    xs, x, gs, gm, ts, bt, _, _ = norm_inputs(c)
+    rng = np.random.default_rng(31)
+    (ws, w), (dcs, dc) = stored(rng.normal(size=(n, k)) / np.sqrt(k), "bf16"), stored(rng.normal(0, 0.1, (m, n)), "bf16")
+    bias = rng.normal(0, 0.1, n).astype(np.float32)
+    bf = lambda a: to_dev(a, "bf16", gpu)  # noqa: E731
+    new = lambda name: [torch.empty(p["shape"], dtype=hf.runtime.torch_dtype(p["elem"]), device=gpu)  # noqa: E731
+                        for p in groups[name].meta["params"] if p["role"] != "in"]
+    groups = {s: load("step_" + s) for s in ("norm", "codes", "linear", "values", "linear_grad", "norm_grad")}
+    gamma, beta, dout = bf(gs), bf(ts), bf(dcs)
+    y, mean, rstd, kept, kept_s = groups["norm"](bf(xs), gamma, beta, *new("norm"))
+    codes, scales = groups["codes"](bf(ws), *new("codes"))
+    out = groups["linear"](y, codes, scales, torch.from_numpy(bias).to(gpu), *new("linear"))
+    wd = groups["values"](codes, scales, *new("values"))
+    dy = groups["linear_grad"](dout, wd, *new("linear_grad"))
+    grads = groups["norm_grad"](dy, kept, kept_s, gamma, mean, rstd, *new("norm_grad"))
+    torch.cuda.synchronize()
+    fwd = host((y, mean, rstd, kept, kept_s), groups["norm"])
+    check_norm(c, fwd, x, gm, bt)
+    wq, wsc = bs.quantize(w, "e2m1", 1)
+    assert np.array_equal(scales.cpu().numpy().view(np.uint8), wsc)
+    assert np.array_equal(codes.cpu().numpy().view(np.uint8), bs.pack(wq, 1))
+    wv = bs.dequantize(bs.pack(wq, 1), wsc, "e2m1", 1)
+    assert np.array_equal(value(to_host(wd, "bf16"), "bf16"), wv)  # (exact in bf16)
+    yv, dyv = value(fwd[0], "bf16"), value(to_host(dy, "bf16"), "bf16")
+    check_linear(to_host(out, "bf16"), "bf16", yv, wv, bias, k)
+    check_linear(to_host(dy, "bf16"), "bf16", dc, wv.T, np.zeros(k), n)
+    xv = bs.dequantize(fwd[3], fwd[4], "e4m3", 1)
+    check_grad(c, host(grads, groups["norm_grad"]), xv, gm, dyv, fwd[1].astype(np.float64), fwd[2].astype(np.float64))
+    # in 64 bits, the same step's loss sum(out dc) moves along dy as the product says
+    step = rng.normal(size=(m, k)) * 2.0 ** -10
+    moved = (((yv + step) @ wv.T) * dc).sum() - ((yv - step) @ wv.T * dc).sum()
+    bound = (2.0 ** -8 * np.abs(dyv) + (2 * (40 + n / 32) + 2) * E24 * (np.abs(dc) @ np.abs(wv))) * np.abs(step)
+    assert abs(moved / 2 - (dyv * step).sum()) <= bound.sum()
