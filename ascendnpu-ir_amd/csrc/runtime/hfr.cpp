@@ -294,13 +294,14 @@ hipError_t ownWorkspaceFree(OwnWorkspace &o) {
   (void)hipSetDevice(cur);
   return e;
 }
-// the workspace of a launch on `stream`, allocated at the stream's first one
-// that uses it
+// The workspace of a launch on `stream`, allocated at the stream's first one
+// that uses it.  The caller holds o.mu until it has enqueued what uses it: a
+// launch of another thread on the same stream comes behind, not between a pre
+// kernel and the kernel that reads what it left.
 int ownWorkspaceOf(OwnWorkspace &o, uint64_t bytes, bool zeroed, void *stream, const char *what, void **ws) {
   int dev = 0;
   (void)hipGetDevice(&dev);
   if (dev != o.device) return fail(HFR_ERR_INVALID, std::string(what) + " workspace belongs to another device");
-  std::lock_guard<std::mutex> lk(o.mu);
   if (o.first && !o.taken) {
     o.taken = true;
     o.firstStream = stream;
@@ -411,8 +412,11 @@ int checkLaunch(const hfr_group *g, const uint64_t *params, size_t nparams, void
 int runChecked(hfr_group *g, const uint64_t *params, void *const *results, int64_t rows, void *workspace, void *stream) {
   if (g->rowsDyn && rows == 0 && !g->rowsZero) return HFR_OK; // nothing to do
   void *ws = workspace;
-  if (!ws && workspaceOf(g, rows))
+  std::unique_lock<std::mutex> lock(g->own->mu, std::defer_lock);
+  if (!ws && workspaceOf(g, rows)) {
+    lock.lock();
     if (const int rc = ownWorkspaceOf(*g->own, g->wsBytes, g->wsZero, stream, "group", &ws)) return rc;
+  }
   return launchGroup(g, params, results, ws, stream, rows);
 }
 
@@ -725,8 +729,11 @@ int hfr_program_launch(hfr_program_t p, const uint64_t *params, size_t nparams, 
     if (p->resultParam[i] < 0 && (!results || !results[i]))
       return fail(HFR_ERR_INVALID, "null device pointer for result " + std::to_string(i));
   void *wsp = workspace;
-  if (p->wsBytes && !wsp)
+  std::unique_lock<std::mutex> lock(p->own.mu, std::defer_lock);
+  if (p->wsBytes && !wsp) {
+    lock.lock();
     if (const int rc = ownWorkspaceOf(p->own, p->wsBytes, false, stream, "program", &wsp)) return rc;
+  }
   char *const ws = (char *)wsp;
   auto resolve = [&](const Binding &b) -> uint64_t {
     switch (b.kind) {

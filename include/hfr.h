@@ -21,9 +21,11 @@
  * that does too.  No other launch allocates.  All of them are freed with the
  * handle, not with their streams.
  * Threading: launches are asynchronous on the given stream; the caller
- * synchronises.  A handle must not be used from two threads at once, and two
- * in-flight launches that use one workspace must be on the same stream (graphs
- * captured on one stream share that stream's).
+ * synchronises.  Two in-flight launches that use one workspace must be on the
+ * same stream (graphs captured on one stream share that stream's).  Launches of
+ * one handle may come from several threads; those with a caller's workspace on
+ * one stream, of memref views that are staged, and of a handle that is being
+ * unloaded, may not at once.
  * Errors: every call returns 0 or a negative HFR_ERR_* code; hfr_last_error()
  * gives the message for the calling thread.
  */

@@ -454,3 +454,44 @@ def test_training_step_with_its_weight(gpu):
     moved = (((yv + step) @ wv.T) * dc).sum() - ((yv - step) @ wv.T * dc).sum()
     bound = (2.0 ** -8 * np.abs(dyv) + (2 * (40 + n / 32) + 2) * E24 * (np.abs(dc) @ np.abs(wv))) * np.abs(step)
     assert abs(moved / 2 - (dyv * step).sum()) <= bound.sum()
+
+
+@pytest.mark.gpu
+def test_two_threads_on_one_stream(gpu):
+    """Calls of one group and of one program from two threads, both on the
+    default stream: a launch's kernels follow each other."""
+    import threading
+    import torch
+    note("two threads")
+    c = (1300, 1000, "bf16", "f32", "e4m3", 2)
+    grp, prog = load("lngrad_rt"), load("prog_norm_linear_mx")
+    m, n, k = 20, 208, 384
+    work = []
+    for seed in (1, 2):
+        xs, x, gs, gm, _, _, ds, dy = norm_inputs(c, seed=seed)
+        arrays, _, _, _ = grad_args(c, xs, x, gs, ds)
+        args = device_args(grp, arrays, gpu)
+        rng = np.random.default_rng(seed)
+        xs, gs, ts = (stored(a, "bf16")[0] for a in (rng.normal(size=(m, k)), rng.uniform(0.5, 1.5, k), rng.normal(0, 0.1, k)))
+        _, _, w, s, _, _ = linear_inputs(8, n, k, "e2m1", seed=seed)
+        pargs = [to_dev(v, p["elem"], gpu) for v, p in zip([xs, gs, ts, w, s], prog.meta["params"])]
+        want = [t.clone() for t in grp(*args)] + [prog(*pargs)]
+        torch.cuda.synchronize()
+        work.append((args, pargs, want))
+    start, bad = threading.Barrier(2), []
+
+    def run(args, pargs, want):
+        try:
+            start.wait()
+            for _ in range(300):
+                got = [t.clone() for t in grp(*args)] + [prog(*pargs)]
+                if not all(torch.equal(a, b) for a, b in zip(got, want)):
+                    bad.append(1)
+        except Exception as e:  # (a thread's own would be lost)
+            bad.append(e)
+    threads = [threading.Thread(target=run, args=w) for w in work]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
