@@ -377,8 +377,8 @@ class Group:
             else:
                 t = results[j] if results is not None else torch.empty(want(r["shape"]), dtype=torch_dtype(r["elem"]),
                                                                       device=device)
-                if tuple(t.shape) != want(r["shape"]) or t.dtype != torch_dtype(r["elem"]) or not t.is_cuda:
-                    raise ValueError(f"result {j} of @{self.func}: expected {r['elem']}{list(want(r['shape']))}")
+                if tuple(t.shape) != want(r["shape"]) or t.dtype != torch_dtype(r["elem"]) or not t.is_cuda or not t.is_contiguous():
+                    raise ValueError(f"result {j} of @{self.func}: expected contiguous {r['elem']}{list(want(r['shape']))}")
                 outs.append(t)
                 rptrs[j] = t.data_ptr()
         need = native.hfr().hfr_group_workspace_rows(self._h, rows if dyn else -1) if self.info.workspace_bytes else 0
@@ -501,8 +501,8 @@ class Program:
             else:
                 t = results[j] if results is not None else torch.empty(r["shape"], dtype=torch_dtype(r["elem"]),
                                                                       device=device)
-                if tuple(t.shape) != r["shape"] or t.dtype != torch_dtype(r["elem"]) or not t.is_cuda:
-                    raise ValueError(f"result {j} of @{self.name}: expected {r['elem']}{list(r['shape'])}")
+                if tuple(t.shape) != r["shape"] or t.dtype != torch_dtype(r["elem"]) or not t.is_cuda or not t.is_contiguous():
+                    raise ValueError(f"result {j} of @{self.name}: expected contiguous {r['elem']}{list(r['shape'])}")
                 outs.append(t)
                 rptrs[j] = t.data_ptr()
         if stream is None:

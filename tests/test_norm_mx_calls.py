@@ -495,3 +495,31 @@ def test_two_threads_on_one_stream(gpu):
     for t in threads:
         t.join()
     assert not bad
+
+
+class OnDevice:
+    """Stands for a device tensor where nothing is launched."""
+
+    def __init__(self, t):
+        self.t, self.is_cuda = t, True
+
+    def __getattr__(self, name):
+        return getattr(self.t, name)
+
+
+def test_refused_results_that_are_not_dense():
+    """A result's buffer is written whole from its address on: a strided or an
+    expanded view of the right shape is refused."""
+    import torch
+    grp = object.__new__(hf.runtime.Group)
+    grp.meta = {"params": [], "results": [dict(tied=-1, elem="f32", shape=(4, 8))]}
+    grp.func, grp._h = "f", None
+    grp.info = hf.native.GroupInfo()
+    prog = object.__new__(hf.runtime.Program)
+    prog.meta, prog.name, prog._h = grp.meta, "p", None
+    for t in (torch.zeros(8, 8)[::2], torch.zeros(8, 4).t(), torch.zeros(4, 1).expand(4, 8), torch.zeros(4, 16)[:, 8:]):
+        assert tuple(t.shape) == (4, 8)
+        with pytest.raises(ValueError, match="result 0 of @f: expected contiguous"):
+            grp._bind((), [OnDevice(t)], 1, None, False)
+        with pytest.raises(ValueError, match="result 0 of @p: expected contiguous"):
+            prog(results=[OnDevice(t)], stream=1)
