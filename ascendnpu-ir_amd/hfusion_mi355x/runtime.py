@@ -385,7 +385,7 @@ class Group:
         if stream is None:
             stream = torch.cuda.current_stream(device).cuda_stream
         ret = outs[0] if len(outs) == 1 else tuple(outs)
-        lib, h, n, nr = native.hfr(), self._h, len(params), len(res_meta)
+        lib, n, nr = native.hfr(), len(params), len(res_meta)  # (the handle stays self's: a packed launch keeps its group)
         if workspace is not None:
             if noalloc:
                 raise ValueError("noalloc launches take no workspace")
@@ -393,7 +393,7 @@ class Group:
         if noalloc:
 
             def launch():
-                native.check(lib.hfr_group_launch_noalloc(h, slots, n, rptrs, nr, stream))
+                native.check(lib.hfr_group_launch_noalloc(self._h, slots, n, rptrs, nr, stream))
                 return ret
             return launch
         entry, at = (lib.hfr_group_launch_rows, (rows,)) if dyn else (lib.hfr_group_launch, ())
@@ -401,7 +401,7 @@ class Group:
 
         def launch():
             ws = _graph_workspace(need, device, stream) if own else workspace
-            native.check(entry(h, slots, n, rptrs, nr, *at, ws.data_ptr() if ws is not None else None, stream))
+            native.check(entry(self._h, slots, n, rptrs, nr, *at, ws.data_ptr() if ws is not None else None, stream))
             return ret
         return launch
 

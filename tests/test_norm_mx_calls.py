@@ -523,3 +523,35 @@ def test_refused_results_that_are_not_dense():
             grp._bind((), [OnDevice(t)], 1, None, False)
         with pytest.raises(ValueError, match="result 0 of @p: expected contiguous"):
             prog(results=[OnDevice(t)], stream=1)
+
+
+@pytest.mark.parametrize("noalloc", [False, True])
+def test_a_packed_launch_keeps_its_group(noalloc):
+    """hf.load(...).launcher(...): the group goes when the launch does."""
+    import gc
+    import weakref
+    import torch
+    grp = object.__new__(hf.runtime.Group)
+    grp.meta = {"params": [], "results": [dict(tied=-1, elem="f32", shape=(4,))]}
+    grp.func, grp._h, grp.info = "f", None, hf.native.GroupInfo()
+    packed, alive = grp.launcher(results=[OnDevice(torch.zeros(4))], stream=1, noalloc=noalloc), weakref.ref(grp)
+    del grp
+    gc.collect()
+    assert alive() is not None
+    del packed
+    gc.collect()
+    assert alive() is None
+
+
+@pytest.mark.gpu
+def test_a_packed_launch_of_a_group_that_nobody_holds(gpu):
+    import gc
+    import torch
+    note("packed launch alone")
+    x = torch.randn(9, 96, device=gpu).bfloat16()
+    g, b = torch.rand(96, device=gpu).bfloat16(), torch.randn(96, device=gpu).bfloat16()
+    want = load("ln_untied")(x, g, b)
+    packed = load("ln_untied").launcher(x, g, b)
+    gc.collect()
+    got = packed()
+    assert all(torch.equal(p.view(torch.uint8), q.view(torch.uint8)) for p, q in zip(got, want))
