@@ -3084,7 +3084,8 @@ bool isSingleOpKernel(const std::string &n) {
   return n == "hfusion.cumsum" || n == "hfusion.cumprod" || n == "hfusion.cummax" || n == "hfusion.cummin" ||
          n == "hfusion.histogram" || n == "hfusion.deinterleave" || n == "hfusion.interleave" || n == "hfusion.flip" ||
          n == "hfusion.mulext" || n == "hfusion.mulextui" || n == "hfusion.arange" || n == "hfusion.gather" || n == "hfusion.sort" ||
-         n == "hfusion.quantize_mx" || n == "hfusion.dequantize_mx" || n == "hfusion.layer_norm" || n == "hfusion.layer_norm_grad";
+         n == "hfusion.quantize_mx" || n == "hfusion.dequantize_mx" || n == "hfusion.layer_norm" || n == "hfusion.layer_norm_grad" ||
+         n == "hfusion.rms_norm" || n == "hfusion.append_kv" || n == "hfusion.paged_attention";
 }
 
 static std::vector<int64_t> intList(const std::string &s) {
@@ -3441,6 +3442,220 @@ static KernelPlan lowerLayerNorm(Analysis &A, const std::string &kname, const Op
   return p;
 }
 
+// Root-mean-square norm of a residual stream into 8-bit codes (hf_rms.h):
+// x [residual] gamma -> [sum] codes scales.
+static KernelPlan lowerResidualNorm(Analysis &A, const std::string &kname, const Op *op, const std::vector<std::string> &outPtr) {
+  const bool res = op->ins.size() == 3;
+  checkOwnOperands(op, res ? 3 : 2, res ? 3 : 2);
+  const int fmt = mxFormatOf(op, "format");
+  if (fmt == 4) unsupported(op, "4-bit codes");
+  const Value *x = op->ins[0], *gamma = op->ins[res ? 2 : 1], *codes = op->results[res ? 1 : 0], *scales = op->results[res ? 2 : 1];
+  const auto &sh = x->type.shape;
+  int64_t R, per;
+  const std::string rows = leadRows(A, op, sh, R, per);
+  const int64_t D = sh.back();
+  if (!A.rowsDyn && R == 0) unsupported(op, "an empty tensor");
+  if (D > 16384) unsupported(op, "rows of more than 16384 elements (one workgroup keeps a row)");
+  const std::string el = mxElem(op, x);
+  if (res)
+    for (const Value *v : {op->ins[1], op->results[0]})
+      if (v->type.shape != sh || v->type.elem != x->type.elem) unsupported(op, "operand " + v->type.str() + " beside " + x->type.str());
+  if (gamma->type.shape != std::vector<int64_t>{D}) unsupported(op, "a weight of other than one element per column");
+  if (gamma->type.elem != Elem::F32 && gamma->type.elem != x->type.elem) unsupported(op, "a weight of another type than f32 or the rows'");
+  std::vector<int64_t> ssh = sh;
+  if (fmt < 0) {
+    ssh.pop_back();
+    if (codes->type.elem != Elem::I8 || codes->type.uns || codes->type.shape != sh) unsupported(op, "codes " + codes->type.str() + " (i8 without a format)");
+    if (scales->type.elem != Elem::F32 || scales->type.shape != ssh) unsupported(op, "scales of i8 codes must be f32, one per row");
+  } else {
+    ssh.back() = (D + 31) / 32;
+    checkCodes(op, codes, fmt, sh, sh.size() - 1);
+    checkScales(op, scales, ssh);
+  }
+  double eps = -1;
+  try { eps = std::stod(op->attr("eps", "")); } catch (const std::exception &) { unsupported(op, "a missing eps"); }
+  if (!(eps >= 0) || std::isinf(eps)) unsupported(op, "eps that is negative or no number");
+  const int64_t V = x->type.elem == Elem::F32 ? 4 : 8;
+  const LnShape s = lnForwardShape(D, V);
+  const int64_t threads = s.T * s.RPB;
+  auto in = [&](size_t i) { return "p" + std::to_string(op->ins[i]->argIdx); };
+  KernelPlan p;
+  p.kernelName = kname;
+  p.kind = "RMS_NORM";
+  p.variant = std::to_string(s.T) + " threads a row, " + (fmt < 0 ? "int8" : mxFormatName(fmt)) + " codes";
+  for (size_t i = 0; i < A.params.size(); ++i)
+    if (!res || (int)i != op->ins[1]->argIdx) p.apart.push_back((int)i);
+  std::string params = kernelParamList(A, p.kargs, false);
+  if (res) {
+    // the sum may be the residual's own buffer (and nothing else's)
+    p.inplace.push_back(op->ins[1]->argIdx);
+    for (const std::string &q : {in(1), outPtr[0]}) {
+      const std::string was = "__restrict__ " + q + ",";
+      const size_t at = params.find(was);
+      if (at != std::string::npos) params.replace(at, was.size(), q + ",");
+    }
+  }
+  char lit[40];
+  std::snprintf(lit, sizeof lit, "%.17g", eps);
+  std::ostringstream k;
+  k << "extern \"C\" __global__ __launch_bounds__(" << threads << ") void " << kname << "(" << params << ") {\n"
+    << "  hf::rms_rows<" << el << ", " << mxElem(op, gamma) << ", " << (res ? "true" : "false") << ", " << fmt << ", " << s.T << ", " << s.NCH << ", "
+    << s.RPB << ", " << D << "ll>(" << in(0) << ", " << (res ? in(1) : "nullptr") << ", " << in(res ? 2 : 1) << ", " << (res ? outPtr[0] : "nullptr")
+    << ", " << outPtr[res ? 1 : 0] << ", " << outPtr[res ? 2 : 1] << ", " << rows << ", (double)" << lit << ");\n}\n";
+  rowGrid(A, p, R, per, 1, s.RPB, lnForwardBlocks(s, D * (16 / V) * (res ? 2 : 1)));
+  p.block[0] = (unsigned)threads;
+  p.source = k.str();
+  return p;
+}
+
+// ---- the paged 8-bit cache (hf_kv.h, hf_attn.h)
+
+namespace {
+// Sizes that append_kv and paged_attention read from their operands.
+struct PagedSizes {
+  int fmt;
+  int64_t T, HQ, HK, D, block, slots, per, blocks;
+};
+// q [T, HQ, D]; k [blocks, HK, block, D], v [blocks, HK, D, block], a scale byte a
+// block and head; seq and pos [T], table [slots, blocks of a sequence]
+PagedSizes pagedSizes(const Analysis &A, const Op *op, const Value *q, const Value *const cache[4], const Value *seq, const Value *pos, const Value *table) {
+  PagedSizes z;
+  z.fmt = mxFormatOf(op, "format");
+  if (z.fmt < 0) unsupported(op, "a missing format");
+  if (z.fmt == 4) unsupported(op, "a 4-bit cache");
+  auto rank = [&](const Value *v, size_t n, const char *what) {
+    if (v->type.shape.size() != n) unsupported(op, std::string(what) + " " + v->type.str());
+    for (auto d : v->type.shape)
+      if (d < 1) unsupported(op, "an empty tensor");
+  };
+  rank(q, 3, "queries");
+  rank(cache[0], 4, "keys");
+  rank(cache[2], 4, "values");
+  rank(seq, 1, "sequence numbers");
+  rank(table, 2, "block table");
+  const auto &k = cache[0]->type.shape;
+  z.T = q->type.shape[0], z.HQ = q->type.shape[1], z.D = q->type.shape[2];
+  z.blocks = k[0], z.HK = k[1], z.block = k[2];
+  z.slots = table->type.shape[0], z.per = table->type.shape[1];
+  if (A.rowsDyn && z.T != kRuntimeRows) unsupported(op, "a runtime row count other than the batch's rows");
+  if (z.HQ % z.HK) unsupported(op, "query heads that are no multiple of the cache's heads");
+  if (z.D % 32 || z.D > 256) unsupported(op, "heads that are no multiple of 32 channels up to 256");
+  if (z.block != 16 && z.block != 32 && z.block != 64 && z.block != 128) unsupported(op, "blocks of other than 16, 32, 64 or 128 tokens");
+  if (z.per * z.block > (int64_t(1) << 30) || z.slots > (int64_t(1) << 30) || z.blocks > (int64_t(1) << 30))
+    unsupported(op, "a cache of more than 2^30 blocks, sequences or positions");
+  if (z.HQ > 1024) unsupported(op, "more than 1024 heads");
+  checkCodes(op, cache[0], z.fmt, {z.blocks, z.HK, z.block, z.D}, 3);
+  checkCodes(op, cache[2], z.fmt, {z.blocks, z.HK, z.D, z.block}, 3);
+  for (const Value *s : {cache[1], cache[3]}) {
+    if (s->type.elem != Elem::I8) unsupported(op, "scales that are not ui8 / i8 (e8m0)");
+    if (s->type.shape != std::vector<int64_t>{z.blocks, z.HK}) unsupported(op, "scales shape " + s->type.str() + " (one byte per block and head)");
+  }
+  for (const Value *v : {seq, pos})
+    if (v->type.elem != Elem::I32 || v->type.shape != std::vector<int64_t>{z.T}) unsupported(op, "sequence numbers and positions must be i32, one per row");
+  if (table->type.elem != Elem::I32) unsupported(op, "a block table that is not i32");
+  return z;
+}
+// what is not written of the destinations stays: the staged copy of a strided
+// one has to begin as the view is
+void keepsRest(Analysis &A, const Op *op) {
+  for (const Value *o : op->outs)
+    if (const int t = tiedArgOf(o); t >= 0) A.params[t].role = "inout";
+}
+// blocks = ceil(rows / rowsB) * rowsC, refused where a static count is past what a launch takes
+void tileGrid(const Analysis &A, const Op *op, KernelPlan &p, int64_t T, int64_t rowsB, int64_t rowsC) {
+  if (A.rowsDyn) {
+    p.rowsDyn = true;
+    p.rowsA = 1, p.rowsB = rowsB, p.rowsC = rowsC;
+    return;
+  }
+  const int64_t blocks = (T + rowsB - 1) / rowsB * rowsC;
+  if (blocks > (int64_t(1) << 30)) unsupported(op, "more rows than a launch takes");
+  p.grid[0] = (unsigned)blocks;
+}
+} // namespace
+
+// qkv rot seq pos table -> q k ks v vs
+static KernelPlan lowerAppendKv(Analysis &A, const std::string &kname, const Op *op, const std::vector<std::string> &outPtr) {
+  checkOwnOperands(op, 5, 5);
+  for (size_t i = 1; i < 5; ++i)
+    if (tiedArgOf(op->outs[i]) < 0) unsupported(op, "a cache that is not a group argument (its other blocks stay as they are)");
+  keepsRest(A, op);
+  const Value *cache[4] = {op->results[1], op->results[2], op->results[3], op->results[4]};
+  const Value *qkv = op->ins[0], *rot = op->ins[1], *q = op->results[0];
+  const PagedSizes z = pagedSizes(A, op, q, cache, op->ins[2], op->ins[3], op->ins[4]);
+  if (qkv->type.elem != q->type.elem || qkv->type.shape != std::vector<int64_t>{z.T, (z.HQ + 2 * z.HK) * z.D})
+    unsupported(op, "rows " + qkv->type.str() + " (the queries', keys' and values' heads, of the queries' type)");
+  if (rot->type.elem != Elem::F32 || rot->type.shape.size() != 2) unsupported(op, "rotations that are not f32, one row a position");
+  const int64_t far = std::min(rot->type.shape[0], z.per * z.block), turn = rot->type.shape[1];
+  if (far < 1 || turn < 16 || turn % 16 || turn > z.D) unsupported(op, "rotated channels that are no multiple of 16 up to the head's");
+  int pairs = -1;
+  try { pairs = std::stoi(op->attr("pairs", "0")); } catch (const std::exception &) {}
+  if (pairs != 0 && pairs != 1) unsupported(op, "pairs other than 0 or 1");
+  auto in = [&](size_t i) { return "p" + std::to_string(op->ins[i]->argIdx); };
+  KernelPlan p;
+  p.kernelName = kname;
+  p.kind = "APPEND_KV";
+  for (size_t i = 0; i < A.params.size(); ++i) p.apart.push_back((int)i);
+  const std::string params = kernelParamList(A, p.kargs, false), el = mxElem(op, q);
+  // workgroups of a tile of `rows` rows that rotate its queries
+  auto parts = [&](int64_t rows) { return std::max<int64_t>(1, (rows * z.HQ * z.D / 8 + 2047) / 2048); };
+  std::ostringstream k;
+  auto kernel = [&](const std::string &name, int64_t C, int64_t QB) {
+    k << "extern \"C\" __global__ __launch_bounds__(256) void " << name << "(" << params << ") {\n  hf::kv_append<" << el << ", " << z.fmt << ", " << z.HQ
+      << ", " << z.HK << ", " << z.D << ", " << turn << ", " << (pairs ? "true" : "false") << ", " << z.block << ", " << z.slots << "ll, " << z.per
+      << "ll, " << far << "ll, " << z.blocks << "ll, " << C << ", " << QB << ">(" << in(0) << ", (const float *)" << in(1) << ", (const int *)" << in(2)
+      << ", (const int *)" << in(3) << ", (const int *)" << in(4) << ", " << outPtr[0] << ", (uint8_t *)" << outPtr[1] << ", (uint8_t *)" << outPtr[2]
+      << ", (uint8_t *)" << outPtr[3] << ", (uint8_t *)" << outPtr[4] << ", " << (A.rowsDyn ? "hf_rows" : std::to_string(z.T) + "ll") << ");\n}\n";
+  };
+  const int64_t C = 16, QB = parts(C);
+  kernel(kname, C, QB);
+  tileGrid(A, op, p, z.T, C, 2 * z.HK + QB);
+  p.block[0] = 256;
+  // (of the cache the codes of the rows alone)
+  p.algoBytes = (double)z.T * ((2 * z.HQ + 2 * z.HK) * z.D * elemBytes(q->type.elem) + 2 * z.HK * z.D + 8);
+  p.variant = "tiles of " + std::to_string(C) + " rows, " + mxFormatName(z.fmt) + " cache";
+  p.source = k.str();
+  return p;
+}
+
+// q k ks v vs seq pos table -> out
+static KernelPlan lowerPagedAttention(Analysis &A, const std::string &kname, const Op *op, const std::vector<std::string> &outPtr) {
+  checkOwnOperands(op, 8, 1);
+  keepsRest(A, op);
+  const Value *cache[4] = {op->ins[1], op->ins[2], op->ins[3], op->ins[4]}, *q = op->ins[0], *out = op->results[0];
+  const PagedSizes z = pagedSizes(A, op, q, cache, op->ins[5], op->ins[6], op->ins[7]);
+  if (q->type.elem != Elem::BF16 && q->type.elem != Elem::F16) unsupported(op, "queries of another type than bf16 or f16");
+  if (out->type.shape != q->type.shape || out->type.elem != q->type.elem) unsupported(op, "result " + out->type.str() + " beside " + q->type.str());
+  float scale = 0;
+  try { scale = std::stof(op->attr("scale", "")); } catch (const std::exception &) { unsupported(op, "a missing scale"); }
+  if (!std::isfinite(scale)) unsupported(op, "a scale that is no number");
+  int64_t window = 0;
+  try { window = std::stoll(op->attr("window", "0")); } catch (const std::exception &) { unsupported(op, "window"); }
+  if (window < 0 || window > (int64_t(1) << 30)) unsupported(op, "a negative window, or one of more than 2^30 positions");
+  auto in = [&](size_t i) { return "p" + std::to_string(op->ins[i]->argIdx); };
+  KernelPlan p;
+  p.kernelName = kname;
+  p.kind = "PAGED_ATTENTION";
+  for (size_t i = 0; i < A.params.size(); ++i) p.apart.push_back((int)i);
+  const std::string params = kernelParamList(A, p.kargs, false), el = mxElem(op, q);
+  std::ostringstream k;
+  k << "extern \"C\" __global__ __launch_bounds__(256, 2) void " << kname << "(" << params << ") {\n"
+    << "  using S = hf::Paged<" << el << ", " << z.fmt << ", " << z.HQ << ", " << z.HK << ", " << z.D << ", " << z.block << ", " << z.slots << "ll, "
+    << z.per << "ll, " << z.blocks << "ll, " << window << ">;\n"
+    << "  const hf::PagedArgs a{(const uint16_t *)" << in(0);
+  for (size_t i = 1; i < 5; ++i) k << ", (const uint8_t *)" << in(i);
+  for (size_t i = 5; i < 8; ++i) k << ", (const int *)" << in(i);
+  k << ", (uint16_t *)" << outPtr[0] << ", " << floatLit((float)(scale * 1.4426950408889634)) << "};\n"
+    << "  hf::paged_rows<S>(a, " << (A.rowsDyn ? "hf_rows" : std::to_string(z.T) + "ll") << ");\n}\n";
+  tileGrid(A, op, p, z.T, 1, z.HK * ((z.HQ / z.HK + 15) / 16));
+  p.block[0] = 256;
+  // (what is read of the cache depends on the positions and is not counted)
+  p.algoBytes = (double)z.T * (2 * z.HQ * z.D * 2 + 8);
+  p.variant = "groups of tokens, " + std::string(mxFormatName(z.fmt)) + " cache" + (window ? ", window " + std::to_string(window) : "");
+  p.source = k.str();
+  return p;
+}
+
 static KernelPlan lowerSingleOp(Analysis &A, const std::string &kname, const Op *op) {
   Func &f = *A.f;
   for (const Op *o : f.ops)
@@ -3475,6 +3690,9 @@ static KernelPlan lowerSingleOp(Analysis &A, const std::string &kname, const Op 
   std::ostringstream k;
   if (n == "quantize_mx" || n == "dequantize_mx") return lowerMxCodes(A, kname, op, outPtr);
   if (n == "layer_norm" || n == "layer_norm_grad") return lowerLayerNorm(A, kname, op, outPtr);
+  if (n == "rms_norm") return lowerResidualNorm(A, kname, op, outPtr);
+  if (n == "append_kv") return lowerAppendKv(A, kname, op, outPtr);
+  if (n == "paged_attention") return lowerPagedAttention(A, kname, op, outPtr);
   if (n == "cumsum" || n == "cumprod" || n == "cummax" || n == "cummin") {
     // CPU meaning (cumprod: ConvertHFusionToUpstream.cpp:385-450): along the
     // cumulation dim, in index order (reverse: from the end), acc_0 = x_0 and
@@ -4843,6 +5061,7 @@ std::vector<KernelPlan> lowerModule(Module &m, const LowerOptions &opt) {
     for (const Op *op : f.ops) {
       if (op->name == "hfusion.matmul_mx" || op->name == "hfusion.linear_mx" || op->name == "hfusion.quantize_mx" ||
           op->name == "hfusion.dequantize_mx" || op->name == "hfusion.layer_norm" || op->name == "hfusion.layer_norm_grad" ||
+          op->name == "hfusion.rms_norm" || op->name == "hfusion.append_kv" || op->name == "hfusion.paged_attention" ||
           op->name == "func.return")
         continue;
       for (const Value *v : op->ins)
@@ -4959,7 +5178,7 @@ std::vector<KernelPlan> lowerModule(Module &m, const LowerOptions &opt) {
     p.funcName = f.name;
     p.params = A.params;
     p.results = A.results;
-    p.algoBytes = algoBytes(A);
+    if (p.algoBytes == 0) p.algoBytes = algoBytes(A);
     if (A.rowsDyn) {
       if (!p.rowsDyn)
         throw CompileError("runtime row counts: @" + f.name + " lowers to a " + p.kind + " kernel (" + p.variant +
@@ -4991,7 +5210,7 @@ std::string emitTranslationUnit(const std::vector<KernelPlan> &plans) {
   std::ostringstream s;
   s << "// Generated by bishengir-compile --target=mi355x (ConvertHFusionToHIP).\n"
     << "#include \"hf_ops.h\"\n#include \"hf_row.h\"\n#include \"hf_argmax.h\"\n#include \"hf_mmad.h\"\n#include \"hf_mmsk.h\"\n#include \"hf_mmtl.h\"\n#include \"hf_misc.h\"\n"
-    << "#include \"hf_rmsq.h\"\n#include \"hf_rmsn.h\"\n#include \"hf_sort.h\"\n#include \"hf_mx.h\"\n#include \"hf_mmwx.h\"\n#include \"hf_ln.h\"\n\n";
+    << "#include \"hf_rmsq.h\"\n#include \"hf_rmsn.h\"\n#include \"hf_sort.h\"\n#include \"hf_mx.h\"\n#include \"hf_mmwx.h\"\n#include \"hf_ln.h\"\n#include \"hf_rms.h\"\n#include \"hf_kv.h\"\n#include \"hf_attn.h\"\n\n";
   for (auto &p : plans) s << "// group @" << p.funcName << ": " << p.kind << " (" << p.variant << ")\n" << p.source << "\n";
   return s.str();
 }

@@ -698,3 +698,117 @@ def layer_norm_linear_mx(m=16, n=4096, k=4096, fmt="e2m1", eps=1e-5):
   }}
 }}
 """
+
+
+# ---- a decoder layer's attention in serving (ops of this backend)
+
+def _group_text(name, op, attrs, ins, outs, kind="ANY_PB"):
+    """The group of one op whose operands and destinations are its arguments:
+    `ins` and `outs` are (name, type) pairs."""
+    sig = ", ".join(f"%{n}: {t}" for n, t in ins + outs)
+    tys = ", ".join(t for _, t in outs)
+    grp = lambda v: ", ".join("%" + n for n, _ in v) + " : " + ", ".join(t for _, t in v)  # noqa: E731
+    many = len(outs) > 1
+    lhs = f"%r:{len(outs)}" if many else "%r"
+    rets = ", ".join(f"%r#{i}" for i in range(len(outs))) if many else "%r"
+    return f"""module {{
+  func.func @{name}({sig}) -> {f"({tys})" if many else tys}
+      {_ATTRS.format(kind=kind)} {{
+    {lhs} = {op} {{{attrs}}} ins({grp(ins)}) outs({grp(outs)}) -> {tys}
+    return {rets} : {tys}
+  }}
+}}
+"""
+
+
+def _rms_operands(rows, cols, elem, params, out, residual):
+    """Operands and destinations of rms_norm, and its format attribute."""
+    X = _t([rows, cols], elem)
+    if out == "i8":
+        Q, S, fmt = _t([rows, cols], "i8"), _t([rows], "f32"), ""
+    elif out in ("e4m3", "e5m2"):
+        (Q, S), fmt = _mx_types(rows, cols, out, 1), f", format = {_MX_CODE[out]} : i32"
+    else:
+        raise ValueError(f"codes {out!r} (i8, e4m3 or e5m2)")
+    ins = [("x", X)] + ([("residual", X)] if residual else []) + [("gamma", _t([cols], params or elem))]
+    return ins, ([("sum", X)] if residual else []) + [("q", Q), ("s", S)], fmt
+
+
+def rms_norm(rows, cols, elem="bf16", params=None, out="i8", residual=True, eps=1e-6):
+    """Root-mean-square norm of a residual stream into 8-bit codes
+    (hfusion.rms_norm): sum = x + residual in the rows' type (without
+    `residual`, sum is x and not a result), y = sum / sqrt(mean(sum^2) + eps) *
+    gamma.  out "i8": codes y / scale to the nearest even with scale = max|y|
+    f32(1/127) of the row in f32, the A and the per-token scales of w8a8_dequant;
+    "e4m3" / "e5m2": quantize_mx's codes and scales of y along the rows,
+    matmul_mx's A.  The squares are summed in 64 bits, so that codes do not
+    depend on an order of additions.  `params`: type of gamma (`elem`, or f32).
+    sum may be the residual's own buffer."""
+    ins, outs, fmt = _rms_operands(rows, cols, elem, params, out, residual)
+    return _group_text("rms_norm", "hfusion.rms_norm", f"eps = {eps:.17e} : f64{fmt}", ins, outs)
+
+
+def _paged_types(rows, heads, kv_heads, dim, slots, room, blocks, block, elem, fmt):
+    """Types of the paged cache's tensors by name."""
+    if fmt not in ("e4m3", "e5m2"):
+        raise ValueError(f"cache format {fmt!r} (e4m3 or e5m2)")
+    if kv_heads < 1 or heads % kv_heads:
+        raise ValueError("query heads are a multiple of the cache's heads")
+    if dim % 32 or not 32 <= dim <= 256 or block not in (16, 32, 64, 128):
+        raise ValueError("heads of a multiple of 32 channels up to 256, blocks of 16, 32, 64 or 128 tokens")
+    S, I = _t([blocks, kv_heads], "ui8"), _t([rows], "i32")
+    return dict(q=_t([rows, heads, dim], elem), k=_t([blocks, kv_heads, block, dim], _MX_TYPE[fmt]), ks=S,
+                v=_t([blocks, kv_heads, dim, block], _MX_TYPE[fmt]), vs=S, seq=I, pos=I, table=_t([slots, -(-room // block)], "i32"))
+
+
+def append_kv(rows, heads, kv_heads, dim, slots, room, blocks, block=64, rot=None, elem="bf16", fmt="e4m3", pairs=False):
+    """A batch's queries, keys and values rotated to their positions, the keys
+    and values appended to a paged 8-bit cache (hfusion.append_kv).
+
+    qkv [rows, (heads + 2 kv_heads) dim] holds each token's queries, keys and
+    values; seq [rows] and pos [rows] (i32) its sequence, a row of `table`, and
+    its position there.  rot [room, rot] f32 holds a position's rot/2 cosines,
+    then its sines, for the first `rot` channels of a head (all, by default):
+    channel i turns with i + rot/2, with `pairs` 2 i with 2 i + 1.  table [slots,
+    room / block] i32 names each sequence's blocks in order.
+
+    Results: q [rows, heads, dim], and the cache: k [blocks, kv_heads, block,
+    dim], v [blocks, kv_heads, dim, block] with one e8m0 scale byte for each
+    block and head, ks and vs [blocks, kv_heads].  The byte is the smallest
+    whose codes hold the block's tokens without saturation; a block's first
+    token sets it, later ones only raise it, and then the codes before them are
+    rounded to the new scale.  A block with an infinity or NaN has the byte 255
+    and codes 0.
+
+    A sequence's rows lie together with positions that follow each other, and
+    a block that gets tokens is one sequence's alone.  Rows whose position is
+    negative or past `room`, or whose sequence is not in the table, pad the
+    batch: nothing of them is written.  Keys and values whose block is not in
+    [0, blocks) are dropped."""
+    t = _paged_types(rows, heads, kv_heads, dim, slots, room, blocks, block, elem, fmt)
+    rot = dim if rot is None else rot
+    ins = [("qkv", _t([rows, (heads + 2 * kv_heads) * dim], elem)), ("rot", _t([room, rot], "f32"))] + [(n, t[n]) for n in ("seq", "pos", "table")]
+    outs = [(n, t[n]) for n in ("q", "k", "ks", "v", "vs")]
+    return _group_text("append_kv", "hfusion.append_kv", f"format = {_MX_CODE[fmt]} : i32, pairs = {int(pairs)} : i32", ins, outs)
+
+
+def paged_attention(rows, heads, kv_heads, dim, slots, room, blocks, block=64, elem="bf16", fmt="e4m3", scale=None, window=0):
+    """Attention of a batch's queries over the paged 8-bit cache that append_kv
+    fills (hfusion.paged_attention): row t, a token of sequence seq[t] at
+    position pos[t], sees the positions up to its own, with `window` only the
+    last `window` of them.  out [rows, heads, dim] = softmax(scale q k) v,
+    `scale` 1 / sqrt(dim) by default; query head h reads kv head h / (heads /
+    kv_heads).  Sums and softmax statistics are f32, a probability is rounded
+    to bf16 before it multiplies its value.
+
+    Positions whose block is not in [0, blocks) are not seen, a row that sees
+    none is zeros, and rows whose position is negative or past the table, or
+    whose sequence is not in it, are left as they are.  Tokens of a sequence
+    that follow each other are read together.  Codes are finite, as append_kv
+    writes them; what lies behind a sequence's last row may be anything."""
+    t = _paged_types(rows, heads, kv_heads, dim, slots, room, blocks, block, elem, fmt)
+    scale = dim ** -0.5 if scale is None else scale
+    ins = [(n, t[n]) for n in ("q", "k", "ks", "v", "vs", "seq", "pos", "table")]
+    more = f", window = {window} : i32" if window else ""
+    return _group_text("paged_attention", "hfusion.paged_attention", f"format = {_MX_CODE[fmt]} : i32, scale = {scale:.9e} : f32{more}",
+                       ins, [("out", t["q"])])

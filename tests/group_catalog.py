@@ -1351,6 +1351,8 @@ def entries():
     e["prog_exp_cumsum_scale"] = g.exp_cumsum_scale(64, 1000)
     import norm_mx_catalog
     e.update(norm_mx_catalog.entries())
+    import serving_catalog
+    e.update(serving_catalog.entries())
     return e
 
 
