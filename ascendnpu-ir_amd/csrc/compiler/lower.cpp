@@ -3574,6 +3574,17 @@ void tileGrid(const Analysis &A, const Op *op, KernelPlan &p, int64_t T, int64_t
 }
 } // namespace
 
+// Rows whose blocks a workgroup of append_kv owns: a decoding step's rows are
+// all in blocks of their own, which one workgroup takes one after another; a
+// prompt's rows share theirs, and workgroups that own none are for nothing.  us
+// of a call, tiles of 1, 4, 16 and 64 rows (32 heads over 8, 128 channels, blocks
+// of 64): 64 sequences of one token 5.5, 10.3, 32.0, 121; 256 of them 12.4, 14.2,
+// 35.5, 119; 1024 39.5, 36.6, 46.0, 141; 4000 183, 155, 161, 330; a prompt of 256
+// tokens 6.1, 5.4, 5.5, 5.3; 1024 11.9, 7.3, 5.6, 5.7; 8192 87, 37, 34, 34 (5.4 TB/s).
+// Query heads a thread 1, 4 and 8, that prompt: 35.4, 34.2, 34.1.
+constexpr int64_t kAppendOne = 256, kAppendFour = 1024;
+static int64_t appendTile(int64_t T) { return T <= kAppendOne ? 1 : T <= kAppendFour ? 4 : 16; }
+
 // qkv rot seq pos table -> q k ks v vs
 static KernelPlan lowerAppendKv(Analysis &A, const std::string &kname, const Op *op, const std::vector<std::string> &outPtr) {
   checkOwnOperands(op, 5, 5);
@@ -3597,19 +3608,25 @@ static KernelPlan lowerAppendKv(Analysis &A, const std::string &kname, const Op 
   p.kind = "APPEND_KV";
   for (size_t i = 0; i < A.params.size(); ++i) p.apart.push_back((int)i);
   const std::string params = kernelParamList(A, p.kargs, false), el = mxElem(op, q);
-  // workgroups of a tile of `rows` rows that rotate its queries
-  auto parts = [&](int64_t rows) { return std::max<int64_t>(1, (rows * z.HQ * z.D / 8 + 2047) / 2048); };
   std::ostringstream k;
-  auto kernel = [&](const std::string &name, int64_t C, int64_t QB) {
+  // tiles of C rows, HB query heads a thread; returns the workgroups of a tile
+  auto kernel = [&](const std::string &name, int64_t C, int64_t HB) {
+    const int64_t QB = std::max<int64_t>(1, (C * ((z.HQ + HB - 1) / HB) * (z.D / 16) + 255) / 256);
     k << "extern \"C\" __global__ __launch_bounds__(256) void " << name << "(" << params << ") {\n  hf::kv_append<" << el << ", " << z.fmt << ", " << z.HQ
       << ", " << z.HK << ", " << z.D << ", " << turn << ", " << (pairs ? "true" : "false") << ", " << z.block << ", " << z.slots << "ll, " << z.per
-      << "ll, " << far << "ll, " << z.blocks << "ll, " << C << ", " << QB << ">(" << in(0) << ", (const float *)" << in(1) << ", (const int *)" << in(2)
+      << "ll, " << far << "ll, " << z.blocks << "ll, " << C << ", " << QB << ", " << HB << ">(" << in(0) << ", (const float *)" << in(1) << ", (const int *)" << in(2)
       << ", (const int *)" << in(3) << ", (const int *)" << in(4) << ", " << outPtr[0] << ", (uint8_t *)" << outPtr[1] << ", (uint8_t *)" << outPtr[2]
       << ", (uint8_t *)" << outPtr[3] << ", (uint8_t *)" << outPtr[4] << ", " << (A.rowsDyn ? "hf_rows" : std::to_string(z.T) + "ll") << ");\n}\n";
+    return 2 * z.HK + QB;
   };
-  const int64_t C = 16, QB = parts(C);
-  kernel(kname, C, QB);
-  tileGrid(A, op, p, z.T, C, 2 * z.HK + QB);
+  const int64_t C = appendTile(z.T);
+  tileGrid(A, op, p, z.T, C, kernel(kname, C, 4));
+  if (A.rowsDyn)
+    for (const int64_t top : {kAppendOne, kAppendFour}) {
+      const int64_t tile = appendTile(top);
+      const std::string nm = altName(kname, "r" + std::to_string(top));
+      p.alts.push_back({nm, top, tile, kernel(nm, tile, 4), 256});
+    }
   p.block[0] = 256;
   // (of the cache the codes of the rows alone)
   p.algoBytes = (double)z.T * ((2 * z.HQ + 2 * z.HK) * z.D * elemBytes(q->type.elem) + 2 * z.HK * z.D + 8);

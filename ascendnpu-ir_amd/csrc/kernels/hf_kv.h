@@ -41,36 +41,35 @@ template <int EL> __device__ __forceinline__ void store8(void *p, const float (&
   }
 }
 
-// Channels d .. d + 7 of a head whose first ROT are rotated by `turn` (ROT / 2
-// cosines, then sines): channel i with i + ROT / 2, or 2 i with 2 i + 1.  Two
-// products and an addition, each rounded to f32.
-template <int EL, int ROT, bool PAIRS> __device__ __forceinline__ void rotate8(const char *head, int d, const float *turn, float (&f)[8]) {
-  load8<EL>(head + d * el_bytes<EL>, f);
-  if (d >= ROT) return;
-  if constexpr (PAIRS) {
-    const f32x2 *c = reinterpret_cast<const f32x2 *>(turn + d / 2), *s = reinterpret_cast<const f32x2 *>(turn + ROT / 2 + d / 2);
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const f32x2 ck = c[k], sk = s[k];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float a = f[4 * k + 2 * i], b = f[4 * k + 2 * i + 1], cc = i ? ck.y : ck.x, ss = i ? sk.y : sk.x;
-        f[4 * k + 2 * i] = a * cc - b * ss;
-        f[4 * k + 2 * i + 1] = b * cc + a * ss;
-      }
-    }
-  } else {
-    constexpr int HALF = ROT / 2;
-    const bool lo = d < HALF;
-    const int i0 = lo ? d : d - HALF;
-    float o[8], c[8], s[8];
-    load8<EL>(head + (lo ? d + HALF : d - HALF) * el_bytes<EL>, o);
-    load8<EL_F32>(turn + i0, c);
-    load8<EL_F32>(turn + HALF + i0, s);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = lo ? f[i] * c[i] - o[i] * s[i] : f[i] * c[i] + o[i] * s[i];
+// Rotation of a head's first ROT channels by `turn` (ROT / 2 cosines, then
+// sines): channel i with i + ROT / 2, or (PAIRS) 2 i with 2 i + 1.  Two products
+// and an addition, each rounded to f32.  A head's channels as slots of 16 that
+// turn among themselves, two runs of eight each: the first at at(slot), the
+// second next(slot) behind it.
+template <int ROT, bool PAIRS> struct Turn {
+  static constexpr int HALF = ROT / 2, TURNED = ROT / 16; // slots that turn
+  float c[8], s[8];
+  __device__ static __forceinline__ int at(int slot) { return PAIRS || slot >= TURNED ? 16 * slot : 8 * slot; }
+  __device__ static __forceinline__ int next(int slot) { return PAIRS || slot >= TURNED ? 8 : HALF; }
+  __device__ __forceinline__ void load(const float *turn, int slot) {
+    if (slot >= TURNED) return;
+    load8<EL_F32>(turn + 8 * slot, c);
+    load8<EL_F32>(turn + HALF + 8 * slot, s);
   }
-}
+  __device__ __forceinline__ void apply(int slot, float (&a)[8], float (&b)[8]) const {
+    if (slot >= TURNED) return;
+    float f[16];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = a[i], f[8 + i] = b[i];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float x = PAIRS ? f[2 * i] : f[i], y = PAIRS ? f[2 * i + 1] : f[8 + i];
+      const float u = x * c[i] - y * s[i], v = y * c[i] + x * s[i];
+      if constexpr (PAIRS) (i < 4 ? a : b)[2 * i % 8] = u, (i < 4 ? a : b)[(2 * i + 1) % 8] = v;
+      else a[i] = u, b[i] = v;
+    }
+  }
+};
 
 // ---------------------------------------------------------------- scales
 // the byte of a block whose largest magnitude has these f32 bits (TOP is 1.75
@@ -110,35 +109,48 @@ template <int FMT> __device__ __forceinline__ u32x2 kv_rescale(u32x2 w, uint32_t
 // leave as q [T, HQ, D] and codes.  A tile of C rows owns the blocks whose
 // first new row is one of them (that row's neighbour above lies in another
 // block or sequence); a workgroup takes one head's keys or values of them, the
-// tile's other QB workgroups its queries.  Rows with a sequence or position
-// out of range, and blocks out of range, are left alone.
-template <int EL, int FMT, int HQ, int HK, int D, int ROT, bool PAIRS, int BLOCK, int64_t SLOTS, int64_t PER, int64_t FAR, int64_t NBLK, int C, int QB>
+// tile's other QB workgroups its queries, HB heads a thread that turn alike.
+// Rows with a sequence or position out of range, and blocks out of range, are
+// left alone.
+template <int EL, int FMT, int HQ, int HK, int D, int ROT, bool PAIRS, int BLOCK, int64_t SLOTS, int64_t PER, int64_t FAR, int64_t NBLK, int C, int QB, int HB>
 __device__ __forceinline__ void kv_append(const void *__restrict__ qkv, const float *__restrict__ rot, const int *__restrict__ seq,
                                           const int *__restrict__ pos, const int *__restrict__ table, void *__restrict__ q,
                                           uint8_t *__restrict__ kc, uint8_t *__restrict__ ks, uint8_t *__restrict__ vc,
                                           uint8_t *__restrict__ vs, int64_t T) {
-  constexpr int E = el_bytes<EL>, CH = D / 8, SUBS = 2 * HK + QB, W = (HQ + 2 * HK) * D;
+  constexpr int E = el_bytes<EL>, SUBS = 2 * HK + QB, W = (HQ + 2 * HK) * D;
   static_assert(C <= 64 && D % 32 == 0 && ROT % 16 == 0 && ROT <= D && BLOCK % 16 == 0 && BLOCK <= 128);
   const int64_t t0 = (int64_t)(blockIdx.x / SUBS) * C;
   const int sub = blockIdx.x % SUBS, tid = threadIdx.x;
   auto inside = [](int s, int p) { return s >= 0 && s < SLOTS && p >= 0 && p < FAR; };
+  using R = Turn<ROT, PAIRS>;
+  constexpr int SLOT = D / 16, PARTS = (HQ + HB - 1) / HB;
   if (sub >= 2 * HK) {
-    const int n = (int)(T - t0 < C ? T - t0 : C) * (HQ * CH);
+    const int n = (int)(T - t0 < C ? T - t0 : C) * (PARTS * SLOT);
     for (int i = (sub - 2 * HK) * 256 + tid; i < n; i += QB * 256) {
-      const int64_t t = t0 + i / (HQ * CH);
-      const int h = i / CH % HQ, d = i % CH * 8;
-      const int p = pos[t];
+      const int64_t t = t0 + i / (PARTS * SLOT);
+      const int slot = i % SLOT, h0 = i / SLOT % PARTS * HB, p = pos[t];
       if (!inside(seq[t], p)) continue;
-      float f[8];
-      rotate8<EL, ROT, PAIRS>((const char *)qkv + (t * W + h * D) * E, d, rot + (int64_t)p * ROT, f);
-      store8<EL>((char *)q + ((t * HQ + h) * D + d) * E, f);
+      R turn;
+      turn.load(rot + (int64_t)p * ROT, slot);
+      const char *src = (const char *)qkv + (t * W + h0 * D + R::at(slot)) * E;
+      char *dst = (char *)q + ((t * HQ + h0) * D + R::at(slot)) * E;
+#pragma unroll
+      for (int h = 0; h < HB; ++h) {
+        if (HQ % HB != 0 && h0 + h >= HQ) break;
+        float a[8], b[8];
+        load8<EL>(src + h * D * E, a);
+        load8<EL>(src + (h * D + R::next(slot)) * E, b);
+        turn.apply(slot, a, b);
+        store8<EL>(dst + h * D * E, a);
+        store8<EL>(dst + (h * D + R::next(slot)) * E, b);
+      }
     }
     return;
   }
   const bool values = sub >= HK;
   const int h = values ? sub - HK : sub;
   uint8_t *const codes = values ? vc : kc, *const scales = values ? vs : ks;
-  constexpr int RPP = 256 / CH, NP = (BLOCK + RPP - 1) / RPP; // tokens a pass, passes
+  constexpr int RPP = 256 / SLOT, NP = (BLOCK + RPP - 1) / RPP; // tokens a pass, passes
   constexpr int PITCH = BLOCK + 8;
   __shared__ uint32_t tops[4];
   __shared__ __attribute__((aligned(16))) uint8_t turned[D * PITCH]; // the values' codes by channel
@@ -167,18 +179,23 @@ __device__ __forceinline__ void kv_append(const void *__restrict__ qkv, const fl
     }
     const int64_t at = ((int64_t)blk * HK + h) * (BLOCK * D);
     const uint32_t old = off > 0 ? scales[(int64_t)blk * HK + h] : 0;
-    float f[NP][8];
+    float f[NP][2][8];
     uint32_t top = 0;
-    const int c = tid % CH, r0 = tid / CH;
+    const int slot = tid % SLOT, r0 = tid / SLOT, c0 = R::at(slot), c1 = c0 + R::next(slot);
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
       const int r = i * RPP + r0;
       if (r0 < RPP && r < n) {
         const char *head = (const char *)qkv + ((t + r) * W + (values ? HQ + HK + h : HQ + h) * D) * E;
-        if (values) load8<EL>(head + 8 * c * E, f[i]);
-        else rotate8<EL, ROT, PAIRS>(head, 8 * c, rot + (int64_t)(p + r) * ROT, f[i]);
+        load8<EL>(head + c0 * E, f[i][0]);
+        load8<EL>(head + c1 * E, f[i][1]);
+        if (!values) {
+          R turn;
+          turn.load(rot + (int64_t)(p + r) * ROT, slot);
+          turn.apply(slot, f[i][0], f[i][1]);
+        }
 #pragma unroll
-        for (int k = 0; k < 8; ++k) top = max_u32(top, f2u(f[i][k]) & 0x7FFFFFFFu);
+        for (int k = 0; k < 16; ++k) top = max_u32(top, f2u(f[i][k / 8][k % 8]) & 0x7FFFFFFFu);
       }
     }
 #pragma unroll
@@ -192,12 +209,16 @@ __device__ __forceinline__ void kv_append(const void *__restrict__ qkv, const fl
     for (int i = 0; i < NP; ++i) {
       const int r = i * RPP + r0;
       if (r0 < RPP && r < n) {
-        const u32x2 w = kv_encode<FMT>(f[i], now);
-        if (!values) {
-          *reinterpret_cast<u32x2_any *>(codes + at + (off + r) * D + 8 * c) = w;
-        } else {
 #pragma unroll
-          for (int k = 0; k < 8; ++k) turned[(8 * c + k) * PITCH + off + r] = (uint8_t)((k < 4 ? w.x : w.y) >> (8 * (k % 4)));
+        for (int k = 0; k < 2; ++k) {
+          const u32x2 w = kv_encode<FMT>(f[i][k], now);
+          const int c = k ? c1 : c0;
+          if (!values) {
+            *reinterpret_cast<u32x2_any *>(codes + at + (off + r) * D + c) = w;
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) turned[(c + j) * PITCH + off + r] = (uint8_t)(w[j / 4] >> (8 * (j % 4)));
+          }
         }
       }
     }
@@ -220,7 +241,7 @@ __device__ __forceinline__ void kv_append(const void *__restrict__ qkv, const fl
     }
     if ((now != old || now == 255) && off > 0) {
       if (!values) {
-        for (int i = tid; i < off * CH; i += 256) {
+        for (int i = tid; i < off * (D / 8); i += 256) {
           u32x2_any *w = reinterpret_cast<u32x2_any *>(codes + at + 8 * i);
           *w = kv_rescale<FMT>(*w, old, now);
         }
