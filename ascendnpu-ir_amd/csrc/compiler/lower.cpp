@@ -3541,8 +3541,8 @@ PagedSizes pagedSizes(const Analysis &A, const Op *op, const Value *q, const Val
   if (z.HQ % z.HK) unsupported(op, "query heads that are no multiple of the cache's heads");
   if (z.D % 32 || z.D > 256) unsupported(op, "heads that are no multiple of 32 channels up to 256");
   if (z.block != 16 && z.block != 32 && z.block != 64 && z.block != 128) unsupported(op, "blocks of other than 16, 32, 64 or 128 tokens");
-  if (z.per * z.block > (int64_t(1) << 30) || z.slots > (int64_t(1) << 30) || z.blocks > (int64_t(1) << 30))
-    unsupported(op, "a cache of more than 2^30 blocks, sequences or positions");
+  if (z.per * z.block > (int64_t(1) << 26) || z.slots > (int64_t(1) << 30) || z.blocks > (int64_t(1) << 30))
+    unsupported(op, "a cache of more than 2^30 blocks or sequences, or of more than 2^26 positions a sequence");
   if (z.HQ > 1024) unsupported(op, "more than 1024 heads");
   checkCodes(op, cache[0], z.fmt, {z.blocks, z.HK, z.block, z.D}, 3);
   checkCodes(op, cache[2], z.fmt, {z.blocks, z.HK, z.D, z.block}, 3);
@@ -3635,6 +3635,13 @@ static KernelPlan lowerAppendKv(Analysis &A, const std::string &kname, const Op 
   return p;
 }
 
+// Rows up to which the attention's tiles are dealt out (PagedSplit::MOST).
+constexpr int64_t kSplitRows = 1024;
+// ... and units, at most, that leave parts (SHARED), workgroups that add them (BLOCKS).
+constexpr int64_t kSplitShared = 768, kSplitJoin = 1024;
+// Positions of a sequence up to which its units are never in pieces.
+constexpr int64_t kWholeFar = 2048;
+
 // q k ks v vs seq pos table -> out
 static KernelPlan lowerPagedAttention(Analysis &A, const std::string &kname, const Op *op, const std::vector<std::string> &outPtr) {
   checkOwnOperands(op, 8, 1);
@@ -3654,21 +3661,54 @@ static KernelPlan lowerPagedAttention(Analysis &A, const std::string &kname, con
   p.kernelName = kname;
   p.kind = "PAGED_ATTENTION";
   for (size_t i = 0; i < A.params.size(); ++i) p.apart.push_back((int)i);
-  const std::string params = kernelParamList(A, p.kargs, false), el = mxElem(op, q);
-  std::ostringstream k;
-  k << "extern \"C\" __global__ __launch_bounds__(256, 2) void " << kname << "(" << params << ") {\n"
-    << "  using S = hf::Paged<" << el << ", " << z.fmt << ", " << z.HQ << ", " << z.HK << ", " << z.D << ", " << z.block << ", " << z.slots << "ll, "
-    << z.per << "ll, " << z.blocks << "ll, " << window << ">;\n"
-    << "  const hf::PagedArgs a{(const uint16_t *)" << in(0);
-  for (size_t i = 1; i < 5; ++i) k << ", (const uint8_t *)" << in(i);
-  for (size_t i = 5; i < 8; ++i) k << ", (const int *)" << in(i);
-  k << ", (uint16_t *)" << outPtr[0] << ", " << floatLit((float)(scale * 1.4426950408889634)) << "};\n"
-    << "  hf::paged_rows<S>(a, " << (A.rowsDyn ? "hf_rows" : std::to_string(z.T) + "ll") << ");\n}\n";
-  tileGrid(A, op, p, z.T, 1, z.HK * ((z.HQ / z.HK + 15) / 16));
+  const std::string el = mxElem(op, q);
+  const int64_t G = z.HQ / z.HK, GT = std::min<int64_t>(G, 16), N = 16 / GT, heads = z.HK * ((G + 15) / 16);
+  const std::string rows = A.rowsDyn ? "hf_rows" : std::to_string(z.T) + "ll";
+  std::ostringstream k, pre;
+  pre << "  using S = hf::Paged<" << el << ", " << z.fmt << ", " << z.HQ << ", " << z.HK << ", " << z.D << ", " << z.block << ", " << z.slots << "ll, "
+      << z.per << "ll, " << z.blocks << "ll, " << window << ">;\n"
+      << "  const hf::PagedArgs a{(const uint16_t *)" << in(0);
+  for (size_t i = 1; i < 5; ++i) pre << ", (const uint8_t *)" << in(i);
+  for (size_t i = 5; i < 8; ++i) pre << ", (const int *)" << in(i);
+  pre << ", (uint16_t *)" << outPtr[0] << ", " << floatLit((float)(scale * 1.4426950408889634)) << "};\n";
+  auto kernel = [&](const std::string &name, const std::string &params, const std::string &bounds, const std::string &call) {
+    k << "extern \"C\" __global__ __launch_bounds__(" << bounds << ") void " << name << "(" << params << ") {\n" << pre.str() << "  " << call << ";\n}\n";
+  };
+  // units in pieces of equal lengths where some may be long: the second launch
+  // and the sums before the first cost some 4 us (18 rows over up to 500
+  // positions 11.6 and 7.8 us, 64 over up to 2000 38.7 and 34.5; 48 over up to 8100 80
+  // and 114, 4 over up to 4000 14.1 and 30)
+  const bool split = z.per * z.block > kWholeFar;
+  const std::string form = "hf::PagedSplit<S, 4>::";
   p.block[0] = 256;
+  if (split && (A.rowsDyn || z.T <= kSplitRows)) {
+    KernelPlan::PreKernel pk;
+    pk.name = kname + "_parts";
+    const std::string params = kernelParamList(A, pk.kargs, true);
+    pk.grid = (unsigned)(kSplitShared + (A.rowsDyn ? 0 : z.T * heads));
+    pk.perRow = A.rowsDyn ? heads : 0;
+    kernel(pk.name, params, "256, 2", form + "rows(a, " + rows + ", (char *)ws)");
+    p.pre.push_back(pk);
+    kernel(kname, kernelParamList(A, p.kargs, true), "256", form + "join(a, (const char *)ws)");
+    p.grid[0] = kSplitJoin;
+    p.workspaceBytes = (uint64_t)(32 + kSplitShared * (32 * N + 2 * GT * N * (8 + 4 * z.D)));
+    p.variant = "units in pieces";
+    if (A.rowsDyn) {
+      p.rowsDyn = true;
+      p.alts.push_back({kname, kSplitRows, kSplitRows, kSplitJoin, 256, true});
+      const std::string nm = altName(kname, "units");
+      std::vector<std::string> kargs;
+      kernel(nm, kernelParamList(A, kargs, true), "256, 2", "hf::paged_rows<S, 4>(a, " + rows + ")");
+      p.alts.push_back({nm, int64_t(1) << 31, 1, heads, 256});
+    }
+  } else {
+    kernel(kname, kernelParamList(A, p.kargs, false), "256, 2", "hf::paged_rows<S, 4>(a, " + rows + ")");
+    tileGrid(A, op, p, z.T, 1, heads);
+    p.variant = "a workgroup a unit";
+  }
   // (what is read of the cache depends on the positions and is not counted)
   p.algoBytes = (double)z.T * (2 * z.HQ * z.D * 2 + 8);
-  p.variant = "groups of tokens, " + std::string(mxFormatName(z.fmt)) + " cache" + (window ? ", window " + std::to_string(window) : "");
+  p.variant += std::string(", ") + mxFormatName(z.fmt) + " cache" + (window ? ", window " + std::to_string(window) : "");
   p.source = k.str();
   return p;
 }
@@ -5270,6 +5310,7 @@ std::string emitManifest(const KernelPlan &p, const std::string &hsacoName) {
     s << "pre " << pk.name << " " << pk.grid << " 1 1 " << pk.block << " 1 1 " << pk.kargs.size();
     for (auto &k : pk.kargs) s << " " << k;
     s << "\n";
+    if (pk.perRow) s << "pre_rows " << pk.perRow << "\n";
   }
   for (auto &a : p.alts)
     s << "alt " << a.name << " " << a.maxRows << " " << a.rowsB << " " << a.rowsC << " " << a.block << (a.pre ? " pre" : "") << "\n";

@@ -44,6 +44,7 @@ struct KernelPlan {
     std::string name;
     unsigned grid = 1, block = 256;
     std::vector<std::string> kargs;
+    int64_t perRow = 0; // launch-time rows: blocks a row, besides `grid`
   };
   std::vector<PreKernel> pre;
   // other kernels of the group for small runtime row counts, by ascending

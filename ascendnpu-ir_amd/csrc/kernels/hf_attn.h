@@ -69,15 +69,22 @@ template <int EL_, int FMT_, int HQ_, int HK_, int D_, int BLOCK_, int64_t SLOTS
   __device__ static __forceinline__ bool inside(int s, int p) { return s >= 0 && s < SLOTS && p >= 0 && p < FAR; }
   // whether row t begins a group of tokens, and how many follow it there: rows
   // of a sequence with positions p, p + 1, ... up to a multiple of N
-  __device__ static __forceinline__ int tokens(const int *seq, const int *pos, int64_t t, int64_t T) {
-    const int s = seq[t], p = pos[t];
-    if (!inside(s, p)) return 0;
-    if (N == 1) return 1;
-    if (t > 0 && p % N != 0 && seq[t - 1] == s && pos[t - 1] == p - 1) return 0;
+  // (all of them are asked for at once)
+  __device__ static __forceinline__ int tokens(const int *seq, const int *pos, int64_t t, int64_t T, int &s, int &p) {
+    int sn[N], pn[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int64_t at = t + i < T ? t + i : T - 1;
+      sn[i] = seq[at], pn[i] = pos[at];
+    }
+    const int64_t up = t > 0 ? t - 1 : 0;
+    const int su = N > 1 ? seq[up] : 0, pu = N > 1 ? pos[up] : 0;
+    s = sn[0], p = pn[0];
+    if (!inside(s, p) || (N > 1 && t > 0 && p % N != 0 && su == s && pu == p - 1)) return 0;
     int n = 1;
 #pragma unroll
     for (int i = 1; i < N; ++i)
-      if (n == i && t + i < T && (p + i) % N != 0 && p + i < FAR && seq[t + i] == s && pos[t + i] == p + i) ++n;
+      if (n == i && t + i < T && (p + i) % N != 0 && p + i < FAR && sn[i] == s && pn[i] == p + i) ++n;
     return n;
   }
 };
@@ -114,14 +121,18 @@ template <typename S> struct PagedTile {
   u32x4 k[4][(S::KS + 1) / 2], v[S::DT];
   uint32_t ks, vs; // scale bytes of the lane group's tokens
   bool there;      // their block is in the table
-  __device__ __forceinline__ void load(const PagedArgs &a, int seq, int h, int b0) {
-    const int lane = threadIdx.x % 64, r = lane % 16, g = lane / 16;
+  // the blocks of the lane's keys and values
+  __device__ static __forceinline__ void blocks(const PagedArgs &a, int seq, int b0, int &bk, int &bv) {
+    const int lane = threadIdx.x % 64;
     const int *row = a.table + (int64_t)seq * S::PER;
     auto block = [&](int tok) {
       const int i = tok / S::BLOCK;
       return i < S::PER ? row[i] : -1;
     };
-    const int bv = block(b0 + 16 * g), bk = S::BLOCK >= 64 ? bv : block(b0 + 16 * (r / 4));
+    bv = block(b0 + 16 * (lane / 16)), bk = S::BLOCK >= 64 ? bv : block(b0 + 16 * (lane % 16 / 4));
+  }
+  __device__ __forceinline__ void load(const PagedArgs &a, int h, int b0, int bk, int bv) {
+    const int lane = threadIdx.x % 64, r = lane % 16, g = lane / 16;
     there = bv >= 0 && bv < S::NBLK;
     const int64_t pv = (int64_t)(there ? bv : 0) * S::HK + h, pk = (int64_t)(bk >= 0 && bk < S::NBLK ? bk : 0) * S::HK + h;
     ks = a.ks[pv], vs = a.vs[pv];
@@ -272,53 +283,255 @@ template <typename S> __device__ __forceinline__ void paged_step(PagedState<S> &
   }
 }
 
-// Rows of a few tokens: a workgroup has the rows of one group of tokens of a
-// kv head, its four waves take its tiles in turn and meet in LDS.
-template <typename S> __device__ __forceinline__ void paged_rows(const PagedArgs &a, int64_t T) {
-  constexpr int HEADS = S::HK * S::GTILES, PITCH = S::D + 4, CH = S::D / 8;
-  __shared__ __attribute__((aligned(16))) float so[4][16][PITCH];
-  __shared__ float sm[4][16], ss[4][16];
-  const int64_t t = blockIdx.x / HEADS;
-  const int h = blockIdx.x % HEADS / S::GTILES, gt = blockIdx.x % S::GTILES;
-  const int n = S::tokens(a.seq, a.pos, t, T);
-  if (n == 0) return;
+// ---------------------------------------------------------------- rows of a few tokens
+// A unit is the rows of one group of tokens and one kv head (of a group of more
+// than 16 query heads, 16 of them); its tiles are those that hold a visible
+// position.
+template <typename S> struct PagedUnits {
+  static constexpr int HEADS = S::HK * S::GTILES, ROWS = S::GT * S::N, CH = S::D / 8;
+  __device__ static __forceinline__ int first(int lo) { return S::WINDOW && lo >= S::WINDOW ? (lo - S::WINDOW + 1) / 64 : 0; }
+  // tiles of a group of n tokens from position lo on
+  __device__ static __forceinline__ int tiles(int lo, int n) { return (lo + n - 1) / 64 - first(lo) + 1; }
+};
+// What WV waves share when they join their states.
+template <typename S, int WV> struct PagedJoin {
+  float o[WV][16][S::D + 4], m[WV][16], sum[WV][16];
+};
+
+// Tiles t0 .. t1 - 1 of the unit of n tokens from row t on (sequence seq,
+// positions from lo on), by the workgroup's WV waves in turn, joined in LDS: the
+// rows' results to out, or as a part (not divided by the sum; the running
+// maximum and the sum in stats, two of each row) to o and stats.
+template <typename S, int WV>
+__device__ __forceinline__ void paged_part(const PagedArgs &a, PagedJoin<S, WV> &join, int64_t t, int n, int seq, int lo, int hh, int t0, int t1,
+                                           float *o, float *stats) {
+  using U = PagedUnits<S>;
+  const int h = hh / S::GTILES, gt = hh % S::GTILES;
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, r = lane % 16, g = lane / 16;
-  const int seq = a.seq[t], lo = a.pos[t], hi = lo + n - 1;
+  const int hi = lo + n - 1;
   v4i q[S::KS];
   paged_query<S>(a, t, n, h, gt, q);
   const int pos = r / S::GT < n ? lo + r / S::GT : -1;
   PagedState<S> st;
   st.clear();
-  int b = S::WINDOW && lo >= S::WINDOW ? (lo - S::WINDOW + 1) / 64 * 64 : 0;
-  for (b += 64 * wave; b <= hi; b += 256) {
+  int bk = 0, bv = 0;
+  if (t0 + wave < t1) PagedTile<S>::blocks(a, seq, 64 * (t0 + wave), bk, bv);
+  for (int i = t0 + wave; i < t1; i += WV) {
     PagedTile<S> tile;
-    tile.load(a, seq, h, b);
-    paged_step<S>(st, tile, q, a, b, pos, lo, hi);
+    tile.load(a, h, 64 * i, bk, bv);
+    // (the next tile's blocks are asked for ahead, its codes are not: their
+    // registers cost a third of the waves, and the other waves' codes are on
+    // their way instead)
+    if (i + WV < t1) PagedTile<S>::blocks(a, seq, 64 * (i + WV), bk, bv);
+    paged_step<S>(st, tile, q, a, 64 * i, pos, lo, hi);
   }
   if constexpr (S::EL != EL_BF16) st.times(mx_scale(st.ref));
   const float sum = group_add(st.sum);
-  if (g == 0) sm[wave][r] = st.m, ss[wave][r] = sum;
+  if (g == 0) join.m[wave][r] = st.m, join.sum[wave][r] = sum;
 #pragma unroll
-  for (int dt = 0; dt < S::DT; ++dt) *reinterpret_cast<v4f *>(&so[wave][r][16 * dt + 4 * g]) = st.o[dt];
+  for (int dt = 0; dt < S::DT; ++dt) *reinterpret_cast<v4f *>(&join.o[wave][r][16 * dt + 4 * g]) = st.o[dt];
   __syncthreads();
-  for (int i = threadIdx.x; i < 16 * CH; i += 256) {
-    const int row = i / CH, d = i % CH * 8, tok = row / S::GT, head = gt * 16 + row % S::GT;
+  for (int i = threadIdx.x; i < U::ROWS * U::CH; i += 64 * WV) {
+    const int row = i / U::CH, d = i % U::CH * 8, tok = row / S::GT, head = gt * 16 + row % S::GT;
     if (tok >= n || head >= S::G) continue;
-    float m = sm[0][row];
+    float m = join.m[0][row];
 #pragma unroll
-    for (int w = 1; w < 4; ++w) m = __builtin_fmaxf(m, sm[w][row]);
+    for (int w = 1; w < WV; ++w) m = __builtin_fmaxf(m, join.m[w][row]);
     float f[8] = {0, 0, 0, 0, 0, 0, 0, 0}, l = 0;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float by = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(sm[w][row] - m);
-      l += ss[w][row] * by;
+    for (int w = 0; w < WV; ++w) {
+      // (a wave that has seen nothing; its sum may be NaN)
+      const float by = join.m[w][row] == m ? 1.0f : __builtin_amdgcn_exp2f(join.m[w][row] - m);
+      l += join.sum[w][row] * by;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) f[k] += so[w][row][d + k] * by;
+      for (int k = 0; k < 8; ++k) f[k] += join.o[w][row][d + k] * by;
     }
+    if (o) {
+      *reinterpret_cast<v4f *>(o + row * S::D + d) = v4f{f[0], f[1], f[2], f[3]};
+      *reinterpret_cast<v4f *>(o + row * S::D + d + 4) = v4f{f[4], f[5], f[6], f[7]};
+      if (d == 0) stats[2 * row] = m, stats[2 * row + 1] = l;
+    } else {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] = l == 0 ? 0.0f : f[k] / l;
-    store8<S::EL>(a.out + ((t + tok) * S::HQ + h * S::G + head) * S::D + d, f);
+      for (int k = 0; k < 8; ++k) f[k] = l == 0 ? 0.0f : f[k] / l;
+      store8<S::EL>(a.out + ((t + tok) * S::HQ + h * S::G + head) * S::D + d, f);
+    }
   }
+  __syncthreads(); // (join is written again)
 }
+
+// A workgroup a unit.
+template <typename S, int WV> __device__ __forceinline__ void paged_rows(const PagedArgs &a, int64_t T) {
+  using U = PagedUnits<S>;
+  __shared__ __attribute__((aligned(16))) PagedJoin<S, WV> join;
+  const int64_t t = blockIdx.x / U::HEADS;
+  int seq, lo;
+  const int n = S::tokens(a.seq, a.pos, t, T, seq, lo);
+  if (n == 0) return;
+  const int t0 = U::first(lo);
+  paged_part<S, WV>(a, join, t, n, seq, lo, blockIdx.x % U::HEADS, t0, t0 + U::tiles(lo, n), nullptr, nullptr);
+}
+
+// Units of different lengths: one is cut into pieces of at most `run` tiles, a
+// workgroup a piece, the longest first; units of several pieces leave parts,
+// which join() adds in order.  run makes as many pieces as fill the chip with
+// the units that stay whole: PIECES less the units, LEAST to SHARED of them.  us of
+// a call, with 512, 768 (taken), 1536 at most: one row over 32768 positions 19.5,
+// 19.6, 23; over 131072 49, 53, 58; 48 rows over up to 8100 90, 80, 87 (5.1 TB/s;
+// a workgroup a unit 114, as long as the longest takes).
+// Up to MOST rows: every workgroup adds up the units' tiles itself, which takes
+// it some 2 us.
+// ws: the number of records, one a token of a unit in parts; then for each part
+// the rows' maximum and sum, and the rows.
+template <typename S, int WV> struct PagedSplit {
+  using U = PagedUnits<S>;
+  static constexpr int MOST = 1024, PIECES = 1024, LEAST = 256, SHARED = 768, THREADS = 64 * WV, PER = (MOST + THREADS - 1) / THREADS;
+  static_assert((S::FAR / 64 + 1) * MOST < (int64_t(1) << 31) && (int64_t)MOST * U::HEADS < (int64_t(1) << 30));
+  struct Record { // a token (row t, `token` of its unit) of a unit in parts
+    int t, token, hh, part, parts, pad[3];
+  };
+  // units in parts are at most SHARED, and have at most SHARED parts more than that
+  static constexpr int64_t STATS = 32 + SHARED * S::N * sizeof(Record), ROWS = STATS + 2 * SHARED * U::ROWS * 8, BYTES = ROWS + 2ll * SHARED * U::ROWS * S::D * 4;
+  __device__ static __forceinline__ float *stats(char *ws, int part) { return reinterpret_cast<float *>(ws + STATS) + part * (U::ROWS * 2); }
+  __device__ static __forceinline__ float *part(char *ws, int part) { return reinterpret_cast<float *>(ws + ROWS) + (int64_t)part * (U::ROWS * S::D); }
+
+  // sums of M values over the threads before this one, and over all
+  template <int M> __device__ static __forceinline__ void before(int (&v)[M], int (&total)[M], int (*tops)[WV]) {
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    int sum[M];
+    auto step = [](int a, auto ctrl, auto rows) { return a + __builtin_amdgcn_update_dpp(0, a, decltype(ctrl)::value, decltype(rows)::value, 0xF, false); };
+    using All = std::integral_constant<int, 0xF>;
+#pragma unroll
+    for (int j = 0; j < M; ++j) {
+      sum[j] = step(v[j], std::integral_constant<int, 0x111>{}, All{});                                // one lane up in its row of sixteen
+      sum[j] = step(sum[j], std::integral_constant<int, 0x112>{}, All{});                              // two
+      sum[j] = step(sum[j], std::integral_constant<int, 0x114>{}, All{});                              // four
+      sum[j] = step(sum[j], std::integral_constant<int, 0x118>{}, All{});                              // eight
+      sum[j] = step(sum[j], std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{}); // a row's last lane to the next row
+      sum[j] = step(sum[j], std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{}); // lane 31 to the upper half
+      if (lane == 63) tops[j][wave] = sum[j];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < M; ++j) {
+      sum[j] -= v[j], total[j] = 0;
+#pragma unroll
+      for (int w = 0; w < WV; ++w) {
+        sum[j] += w < wave ? tops[j][w] : 0;
+        total[j] += tops[j][w];
+      }
+      v[j] = sum[j];
+    }
+  }
+
+  // grid: T * HEADS + SHARED
+  __device__ static __forceinline__ void rows(const PagedArgs &a, int64_t T, char *ws) {
+    __shared__ __attribute__((aligned(16))) PagedJoin<S, WV> join;
+    __shared__ int tops[6][WV];
+    struct Found {
+      int t, n, seq, lo, tiles, in, shared, part;
+    };
+    __shared__ Found found;
+    // a thread has PER rows, one after another
+    const int tid = threadIdx.x, per = (int)((T + THREADS - 1) / THREADS);
+    int tiles[PER], n[PER], seq[PER], lo[PER], size[2] = {0, 0}, sizes[2];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int64_t t = tid * per + i;
+      n[i] = i < per && t < T ? S::tokens(a.seq, a.pos, t, T, seq[i], lo[i]) : 0;
+      tiles[i] = n[i] ? U::tiles(lo[i], n[i]) : 0;
+      size[0] += tiles[i], size[1] += n[i] > 0;
+    }
+    before(size, sizes, tops);
+    const int64_t all = (int64_t)sizes[0] * U::HEADS;
+    int want = PIECES - sizes[1] * U::HEADS;
+    want = want < LEAST ? LEAST : want > SHARED ? SHARED : want;
+    const int run = ((int)((all + want - 1) / want) + WV - 1) / WV * WV; // (every wave as many)
+    // pieces of `run` tiles, shorter ones, tokens of units in parts, and parts, of the thread's rows
+    int count[4] = {0, 0, 0, 0}, counts[4];
+    auto add = [&](int i) {
+      const int full = tiles[i] / run, rest = tiles[i] % run != 0, c = full + rest;
+      count[0] += full, count[1] += rest, count[2] += c > 1 ? n[i] : 0, count[3] += c > 1 ? c : 0;
+    };
+#pragma unroll
+    for (int i = 0; i < PER; ++i) add(i);
+    before(count, counts, tops + 2);
+    if (blockIdx.x == 0 && tid == 0) *reinterpret_cast<int *>(ws) = counts[2] * U::HEADS;
+    // the longest pieces first: those that start last are short
+    int piece = (int)blockIdx.x;
+    const bool shorter = piece >= counts[0] * U::HEADS;
+    if (shorter) piece -= counts[0] * U::HEADS;
+    if (shorter && piece >= counts[1] * U::HEADS) return;
+    // the row whose piece this is: the thread that has it says so
+    const int x = piece / U::HEADS;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int b = shorter ? count[1] : count[0], shared = count[2], part = count[3];
+      add(i);
+      if (b <= x && x < (shorter ? count[1] : count[0])) found = Found{tid * per + i, n[i], seq[i], lo[i], tiles[i], piece - b * U::HEADS, shared, part};
+    }
+    __syncthreads();
+    auto one = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+    const int w = one(found.tiles), full = w / run, cuts = full + (w % run != 0), in = one(found.in);
+    // (a head's pieces lie together)
+    const int hh = shorter ? in : in / full, k = shorter ? full : in % full, t0 = U::first(one(found.lo)), b = k * run, e = b + run < w ? b + run : w;
+    const int slot = one(found.part) * U::HEADS + hh * cuts + k;
+    if (cuts > 1 && k == 0 && tid < found.n)
+      reinterpret_cast<Record *>(ws + 32)[(found.shared + tid) * U::HEADS + hh] = Record{found.t + tid, tid, hh, slot, cuts, {0, 0, 0}};
+    paged_part<S, WV>(a, join, one(found.t), one(found.n), one(found.seq), one(found.lo), hh, t0 + b, t0 + e, cuts > 1 ? part(ws, slot) : nullptr,
+                      stats(ws, slot));
+  }
+
+  // The tokens of units in parts: a workgroup a head, its four waves a quarter
+  // of the parts each.
+  static constexpr int BLOCKS = 1024;
+  __device__ static __forceinline__ void join(const PagedArgs &a, const char *ws_) {
+    constexpr int L = S::D / 4, GROUPS = 64 / L; // lanes a part, parts at once
+    __shared__ __attribute__((aligned(16))) v4f sums[4][64];
+    __shared__ float by[4][SHARED / 4 + 1];
+    char *ws = const_cast<char *>(ws_);
+    const int count = *reinterpret_cast<const int *>(ws) * S::GT, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    for (int i = blockIdx.x; i < count; i += BLOCKS) {
+      const Record rec = reinterpret_cast<const Record *>(ws + 32)[i / S::GT];
+      const int row = rec.token * S::GT + i % S::GT, gt = rec.hh % S::GTILES, h = rec.hh / S::GTILES, head = gt * 16 + i % S::GT;
+      if (head >= S::G) continue;
+      float m = -__builtin_inff(), l = 0;
+      for (int k = lane; k < rec.parts; k += 64) m = __builtin_fmaxf(m, stats(ws, rec.part + k)[2 * row]);
+#pragma unroll
+      for (int k = 1; k < 64; k *= 2) m = __builtin_fmaxf(m, __shfl_xor(m, k));
+      for (int k = lane; k < rec.parts; k += 64) {
+        const float *st = stats(ws, rec.part + k) + 2 * row;
+        const float f = st[0] == m ? 1.0f : __builtin_amdgcn_exp2f(st[0] - m);
+        l += st[1] * f;
+        if (k % 4 == wave) by[wave][k / 4] = f;
+      }
+#pragma unroll
+      for (int k = 1; k < 64; k *= 2) l += __shfl_xor(l, k);
+      v4f o = {0, 0, 0, 0};
+      if (lane < GROUPS * L) {
+#pragma unroll 4
+        for (int k = lane / L; 4 * k + wave < rec.parts; k += GROUPS)
+          o += *reinterpret_cast<const v4f *>(part(ws, rec.part + 4 * k + wave) + row * S::D + lane % L * 4) * by[wave][k];
+      }
+      sums[wave][lane] = o;
+      __syncthreads();
+      if (wave == 0 && lane < L) {
+        o = v4f{0, 0, 0, 0};
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+#pragma unroll
+          for (int k = 0; k < GROUPS; ++k) o += sums[v][k * L + lane];
+        uint16_t e[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float v = l == 0 ? 0.0f : o[k] / l;
+          e[k] = S::EL == EL_BF16 ? f32_to_bf16_rne(v) : __builtin_bit_cast(uint16_t, (_Float16)v);
+        }
+        *reinterpret_cast<u32x2_any *>(a.out + (rec.t * (int64_t)S::HQ + h * S::G + head) * S::D + lane * 4) =
+            u32x2{(uint32_t)e[0] | (uint32_t)e[1] << 16, (uint32_t)e[2] | (uint32_t)e[3] << 16};
+      }
+      __syncthreads();
+    }
+  }
+};
 
 } // namespace hf

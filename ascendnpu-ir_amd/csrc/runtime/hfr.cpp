@@ -41,6 +41,7 @@ struct PreLaunch {
   std::string kernel;
   hipFunction_t fn = nullptr;
   hfr_launch_cfg cfg{};
+  int64_t perRow = 0; // at launch-time rows: blocks a row, besides the grid's own
   std::vector<Karg> kargs;
 };
 
@@ -186,6 +187,13 @@ int parseBlock(const std::vector<std::string> &lines, hfr_group &g) {
       }
       if (!pl.cfg.grid[0] || !pl.cfg.block[0]) return fail(HFR_ERR_MANIFEST, "pre kernel without launch shape");
       g.pre.push_back(pl);
+    }
+    else if (key == "pre_rows") {
+      // pre_rows <blocks a row>: of the pre kernel before it, besides its grid
+      int64_t n = 0;
+      is >> n;
+      if (is.fail() || n <= 0 || g.pre.empty() || !g.rowsDyn) return fail(HFR_ERR_MANIFEST, "bad pre_rows line: " + ln);
+      g.pre.back().perRow = n;
     }
     else if (key == "alt") {
       // alt <kernel> <max rows> <rows per block row> <blocks per block row> <threads> [pre]
@@ -379,7 +387,9 @@ int launchGroup(const hfr_group *g, const uint64_t *params, void *const *results
   };
   auto runPre = [&]() {
     for (auto &pl : g->pre) {
-      const int rc = launch(pl.fn, pl.cfg, pl.kargs);
+      hfr_launch_cfg cfg = pl.cfg;
+      if (pl.perRow) cfg.grid[0] += (unsigned)(rows * pl.perRow);
+      const int rc = launch(pl.fn, cfg, pl.kargs);
       if (rc) return rc;
     }
     return (int)HFR_OK;
