@@ -3639,8 +3639,13 @@ static KernelPlan lowerAppendKv(Analysis &A, const std::string &kname, const Op 
 constexpr int64_t kSplitRows = 1024;
 // ... and units, at most, that leave parts (SHARED), workgroups that add them (BLOCKS).
 constexpr int64_t kSplitShared = 768, kSplitJoin = 1024;
-// Positions of a sequence up to which its units are never in pieces.
+// Positions of a sequence up to which its groups of tokens are never in pieces.
 constexpr int64_t kWholeFar = 2048;
+// Rows that count as groups of tokens whatever the number of sequences.
+constexpr int64_t kPagedFew = 64;
+// Pieces of a prompt's units, units up to which it has some, and their shortest
+// length in tiles (PagedPrompt::PIECES, CUT).
+constexpr int64_t kPieces = 1024, kPieceUnits = 512, kPieceTiles = 16;
 
 // q k ks v vs seq pos table -> out
 static KernelPlan lowerPagedAttention(Analysis &A, const std::string &kname, const Op *op, const std::vector<std::string> &outPtr) {
@@ -3674,37 +3679,69 @@ static KernelPlan lowerPagedAttention(Analysis &A, const std::string &kname, con
   auto kernel = [&](const std::string &name, const std::string &params, const std::string &bounds, const std::string &call) {
     k << "extern \"C\" __global__ __launch_bounds__(" << bounds << ") void " << name << "(" << params << ") {\n" << pre.str() << "  " << call << ";\n}\n";
   };
-  // units in pieces of equal lengths where some may be long: the second launch
-  // and the sums before the first cost some 4 us (18 rows over up to 500
-  // positions 11.6 and 7.8 us, 64 over up to 2000 38.7 and 34.5; 48 over up to 8100 80
-  // and 114, 4 over up to 4000 14.1 and 30)
-  const bool split = z.per * z.block > kWholeFar;
-  const std::string form = "hf::PagedSplit<S, 4>::";
+  // The kernels, by the row count.  More rows than the sequences' groups of N
+  // tokens are a prompt's, unless they are few: 64 rows behind 8000 positions 44
+  // us as groups of tokens, 52 as a prompt's rows, 256 behind 30000 364 and 178.
+  const int64_t tile = 128 / GT, tokens = std::max<int64_t>(kPagedFew, std::min<int64_t>(int64_t(1) << 30, N * z.slots)), far = z.per * z.block;
+  // Groups of tokens in pieces where some may be long: the second launch and the
+  // sums before the first cost some 4 us (18 rows over up to 500 positions 11.6 and
+  // 7.6 us, 64 over up to 2000 38.7 and 34.5; 48 over up to 8100 80 and 114, 4 over up to
+  // 4000 14.1 and 30)
+  const int64_t split = far > kWholeFar ? std::min(tokens, kSplitRows) : 0;
+  // Prompt's rows in pieces while they do not fill the chip (PagedPrompt), of
+  // contexts that may be longer than the shortest piece
+  const int64_t pieces = far > kPieceTiles * 64 ? kPieceUnits / heads * tile : 0;
+  const std::string splitForm = "hf::PagedSplit<S, 4>::", promptForm = "hf::PagedPrompt<S>::", bounds = z.D > 128 ? "256" : "256, 2";
+  struct Schedule {
+    const char *name;
+    int64_t most; // rows
+    std::string pre, preBounds;
+    int64_t preGrid, prePerRow;
+    uint64_t ws;
+    std::string call, bounds;
+    int64_t rowsB, rowsC; // 0: rowsC workgroups
+  };
+  std::vector<Schedule> all;
+  if (split)
+    all.push_back({"parts", split, splitForm + "rows(a, " + rows + ", (char *)ws)", "256, 2", kSplitShared, heads,
+                   (uint64_t)(32 + kSplitShared * (32 * N + 2 * GT * N * (8 + 4 * z.D))), splitForm + "join(a, (const char *)ws)", "256", 0, kSplitJoin});
+  if (tokens > split) all.push_back({"units", tokens, "", "", 0, 0, 0, "hf::paged_rows<S, 4>(a, " + rows + ")", "256, 2", 1, heads});
+  if (pieces > tokens)
+    all.push_back({"pieces", pieces, promptForm + "rows<true>(a, " + rows + ", (char *)ws)", bounds, kPieces, 0, (uint64_t)(kPieces * 128 * (8 + 4 * z.D)),
+                   promptForm + "join(a, " + rows + ", (const char *)ws)", "256", 0, kPieceUnits * 4});
+  all.push_back({"prompt", int64_t(1) << 31, "", "", 0, 0, 0, promptForm + "rows<false>(a, " + rows + ", nullptr)", bounds, tile, heads});
+  if (!A.rowsDyn) {
+    while (all.front().most < z.T) all.erase(all.begin());
+    all.resize(1);
+  }
+  uint64_t ws = 0;
+  for (const Schedule &s : all) ws = std::max(ws, s.ws);
+  p.workspaceBytes = ws;
+  p.rowsDyn = A.rowsDyn;
   p.block[0] = 256;
-  if (split && (A.rowsDyn || z.T <= kSplitRows)) {
-    KernelPlan::PreKernel pk;
-    pk.name = kname + "_parts";
-    const std::string params = kernelParamList(A, pk.kargs, true);
-    pk.grid = (unsigned)(kSplitShared + (A.rowsDyn ? 0 : z.T * heads));
-    pk.perRow = A.rowsDyn ? heads : 0;
-    kernel(pk.name, params, "256, 2", form + "rows(a, " + rows + ", (char *)ws)");
-    p.pre.push_back(pk);
-    kernel(kname, kernelParamList(A, p.kargs, true), "256", form + "join(a, (const char *)ws)");
-    p.grid[0] = kSplitJoin;
-    p.workspaceBytes = (uint64_t)(32 + kSplitShared * (32 * N + 2 * GT * N * (8 + 4 * z.D)));
-    p.variant = "units in pieces";
-    if (A.rowsDyn) {
-      p.rowsDyn = true;
-      p.alts.push_back({kname, kSplitRows, kSplitRows, kSplitJoin, 256, true});
-      const std::string nm = altName(kname, "units");
-      std::vector<std::string> kargs;
-      kernel(nm, kernelParamList(A, kargs, true), "256, 2", "hf::paged_rows<S, 4>(a, " + rows + ")");
-      p.alts.push_back({nm, int64_t(1) << 31, 1, heads, 256});
+  for (const Schedule &s : all) {
+    int pre = -1;
+    if (s.ws) {
+      KernelPlan::PreKernel pk;
+      pk.name = kname + "_" + s.name;
+      const std::string params = kernelParamList(A, pk.kargs, true);
+      pk.grid = (unsigned)(s.preGrid + (A.rowsDyn ? 0 : z.T * s.prePerRow));
+      pk.perRow = A.rowsDyn ? s.prePerRow : 0;
+      pk.wsBytes = s.ws;
+      pk.block = 256;
+      kernel(pk.name, params, s.preBounds, s.pre);
+      pre = (int)p.pre.size();
+      p.pre.push_back(pk);
     }
-  } else {
-    kernel(kname, kernelParamList(A, p.kargs, false), "256, 2", "hf::paged_rows<S, 4>(a, " + rows + ")");
-    tileGrid(A, op, p, z.T, 1, heads);
-    p.variant = "a workgroup a unit";
+    // (the last one is the group's kernel)
+    const std::string nm = &s == &all.back() ? kname : altName(kname, s.name);
+    std::vector<std::string> kargs;
+    kernel(nm, kernelParamList(A, kargs, ws > 0), s.bounds, s.call);
+    p.kargs = kargs;
+    if (A.rowsDyn) p.alts.push_back({nm, s.most, s.rowsB ? s.rowsB : s.most, s.rowsC, 256, pre >= 0, pre});
+    else p.grid[0] = (unsigned)(s.rowsB ? (z.T + s.rowsB - 1) / s.rowsB * s.rowsC : s.rowsC);
+    if (!A.rowsDyn && s.rowsB && (z.T + s.rowsB - 1) / s.rowsB * s.rowsC > (int64_t(1) << 30)) unsupported(op, "more rows than a launch takes");
+    p.variant += (p.variant.empty() ? "" : ", ") + std::string(s.name);
   }
   // (what is read of the cache depends on the positions and is not counted)
   p.algoBytes = (double)z.T * (2 * z.HQ * z.D * 2 + 8);
@@ -5311,9 +5348,11 @@ std::string emitManifest(const KernelPlan &p, const std::string &hsacoName) {
     for (auto &k : pk.kargs) s << " " << k;
     s << "\n";
     if (pk.perRow) s << "pre_rows " << pk.perRow << "\n";
+    if (pk.wsBytes) s << "pre_workspace " << pk.wsBytes << "\n";
   }
   for (auto &a : p.alts)
-    s << "alt " << a.name << " " << a.maxRows << " " << a.rowsB << " " << a.rowsC << " " << a.block << (a.pre ? " pre" : "") << "\n";
+    s << "alt " << a.name << " " << a.maxRows << " " << a.rowsB << " " << a.rowsC << " " << a.block << (a.pre ? " pre" : "")
+      << (a.only >= 0 ? " " + std::to_string(a.only) : "") << "\n";
   s << "variant " << p.variant << "\n";
   return s.str();
 }

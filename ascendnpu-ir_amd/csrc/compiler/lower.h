@@ -44,7 +44,8 @@ struct KernelPlan {
     std::string name;
     unsigned grid = 1, block = 256;
     std::vector<std::string> kargs;
-    int64_t perRow = 0; // launch-time rows: blocks a row, besides `grid`
+    int64_t perRow = 0;   // launch-time rows: blocks a row, besides `grid`
+    uint64_t wsBytes = 0; // what a launch behind this one alone needs of the workspace (0: all)
   };
   std::vector<PreKernel> pre;
   // other kernels of the group for small runtime row counts, by ascending
@@ -56,6 +57,7 @@ struct KernelPlan {
     int64_t maxRows = 0, rowsB = 1, rowsC = 1;
     unsigned block = 256;
     bool pre = false;
+    int only = -1; // ... behind one of them (-1: all)
   };
   std::vector<RowAlt> alts;
   // runtime row count (compiler option dyn=runtime): the kernel takes the

@@ -42,20 +42,24 @@ template <int EL> __device__ __forceinline__ v4i attn_round8(const float *p) {
   v4i o;
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
-    if constexpr (EL == EL_BF16) o[w] = (int)((uint32_t)f32_to_bf16_rne(p[2 * w]) | (uint32_t)f32_to_bf16_rne(p[2 * w + 1]) << 16);
-    else
-      o[w] = (int)((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)p[2 * w]) | (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)p[2 * w + 1]) << 16);
+    using T = std::conditional_t<EL == EL_BF16, __bf16, _Float16>;
+    typedef T t2 __attribute__((ext_vector_type(2)));
+    o[w] = __builtin_bit_cast(int, __builtin_convertvector(f32x2{p[2 * w], p[2 * w + 1]}, t2));
   }
   return o;
 }
-// over the four lane groups that share a row
-__device__ __forceinline__ float group_max(float v) {
-  v = __builtin_fmaxf(v, __shfl_xor(v, 16));
-  return __builtin_fmaxf(v, __shfl_xor(v, 32));
+// the value of the lane 16 or 32 lanes away, combined with this one's
+template <int BY, typename F> __device__ __forceinline__ float with_lane(float v, F f) {
+  typedef unsigned u2 __attribute__((ext_vector_type(2)));
+  const u2 r = __builtin_bit_cast(u2, BY == 16 ? __builtin_amdgcn_permlane16_swap(f2u(v), f2u(v), false, false) : __builtin_amdgcn_permlane32_swap(f2u(v), f2u(v), false, false));
+  return f(u2f(r.x), u2f(r.y));
 }
+__device__ __forceinline__ float max2(float a, float b) { return __builtin_fmaxf(a, b); }
+// over the four lane groups that share a row
+__device__ __forceinline__ float group_max(float v) { return with_lane<32>(with_lane<16>(v, max2), max2); }
 __device__ __forceinline__ float group_add(float v) {
-  v += __shfl_xor(v, 16);
-  return v + __shfl_xor(v, 32);
+  auto add = [](float a, float b) { return a + b; };
+  return with_lane<32>(with_lane<16>(v, add), add);
 }
 
 // What a group of this op knows when it is compiled.  Sixteen matrix-core
@@ -193,12 +197,13 @@ template <typename S> __device__ __forceinline__ void paged_step(PagedState<S> &
   // tokens that some row does not see
   const int at = b0 + 16 * g;
   const bool whole = __all(t.there && b0 + 63 <= lo && (S::WINDOW == 0 || b0 > hi - S::WINDOW));
-  auto sees = [&](int tok) { return t.there && tok <= pos && (S::WINDOW == 0 || tok > pos - S::WINDOW); };
+  const int to = pos - at, from = to - S::WINDOW; // (compares with constants)
+  auto sees = [&](int i) { return t.there && i <= to && (S::WINDOW == 0 || i > from); };
   if (!whole) {
 #pragma unroll
     for (int u = 0; u < 4; ++u)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[u][i] = sees(at + 4 * u + i) ? s[u][i] : -__builtin_inff();
+      for (int i = 0; i < 4; ++i) s[u][i] = sees(4 * u + i) ? s[u][i] : -__builtin_inff();
     // (behind the last position the cache may hold anything, NaN too)
     const int n = t.there ? hi + 1 - at : 0;
 #pragma unroll
@@ -232,7 +237,7 @@ template <typename S> __device__ __forceinline__ void paged_step(PagedState<S> &
     for (int i = 0; i < 16; ++i) p[i] *= by;
     if (!whole)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) p[i] = sees(at + i) ? p[i] : 0.0f;
+      for (int i = 0; i < 16; ++i) p[i] = sees(i) ? p[i] : 0.0f;
   };
   if constexpr (S::EL == EL_BF16) {
     if (!__all(was == 1.0f)) st.times(was);
@@ -530,6 +535,422 @@ template <typename S, int WV> struct PagedSplit {
             u32x2{(uint32_t)e[0] | (uint32_t)e[1] << 16, (uint32_t)e[2] | (uint32_t)e[3] << 16};
       }
       __syncthreads();
+    }
+  }
+};
+
+// ---------------------------------------------------------------- rows of prompts
+// A workgroup has TOKENS rows of the batch and one kv head (of a group of more
+// than 16 query heads, 16 of them): 128 matrix-core rows, 32 a wave.  Its rows'
+// sequences are taken one after another; of each, tiles of 64 tokens are
+// decoded to 16 bits into LDS, keys by token and values by channel, for all
+// four waves, while the tile before is worked on.
+// As above the products are transposed, here 32x32x16: a lane's 16 scores of a K
+// tile of 32 tokens are tokens 16 (i / 8) + 8 (lane / 32) + i % 8 of one row, eight at a
+// time the B operand of the second product as they lie, if row r of the K tile
+// is the token with bits 2 and 3 of r exchanged.
+// The running maximum is only raised, and what is summed only scaled, when a
+// row's new scores exceed it by 2^6: numbers up to that are as good as up to 1.
+template <typename S> struct PagedPrompt {
+  static constexpr int TOKENS = 128 / S::GT, HEADS = S::HK * S::GTILES, KP = S::D + 8, VP = 64 + 8;
+  static constexpr int CHUNKS = 4 * S::D, N = (CHUNKS + 255) / 256; // 16-byte pieces of a tile's keys, a thread
+  static constexpr int QF = S::D / 16, OT = S::D / 32;
+  struct Lds {
+    __attribute__((aligned(16))) uint16_t k[2][64 * KP], v[2][S::D * VP];
+  };
+
+  template <int EL> __device__ static __forceinline__ v16f mfma(v4i a, v4i b, v16f c) {
+    if constexpr (EL == EL_BF16) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+  }
+  // The order of PRODUCTS products and their reads from LDS: eight reads ahead
+  // (the compiler's own order has two, and waits for most of them), `more` with
+  // other work between them.  8192 rows of 4 prompts: 412 us, 370 so; and with
+  // the waves at their products before those at their scores 360.
+  template <int PRODUCTS, bool MORE> __device__ static __forceinline__ void ahead() {
+    constexpr int AHEAD = PRODUCTS < 8 ? PRODUCTS : 8;
+    __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0); // LDS reads
+#pragma unroll
+    for (int c = 0; c < PRODUCTS - AHEAD; ++c) {
+      __builtin_amdgcn_sched_group_barrier(0x8, 1, 0); // matrix core
+      if (MORE) __builtin_amdgcn_sched_group_barrier(0x2, 4, 0); // other arithmetic
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x8, AHEAD, 0);
+  }
+  // a tile's four groups of 16 tokens, group lane % 4 in a lane
+  struct Groups {
+    int block;      // of the cache, -1 for none
+    uint32_t ks, vs; // scale bytes
+  };
+  // what the workgroup does with a tile's values: scaled to the reference, or
+  // (f16, of blocks further apart than its range) as they are, with p scaled.
+  // bf16 has the range for all but values 2^100 below the largest block's.
+  struct Mode {
+    uint32_t ref;
+    bool plain;
+  };
+
+  const PagedArgs &a;
+  Lds &lds;
+  const int seq, h, lo, hi;
+  u32x4 kx[N], vx[N];
+
+  __device__ __forceinline__ int block(int tile) const {
+    const int i = (64 * tile + 16 * (int)(threadIdx.x % 4)) / S::BLOCK;
+    const int b = i < S::PER ? a.table[(int64_t)seq * S::PER + i] : -1;
+    return b >= 0 && b < S::NBLK ? b : -1;
+  }
+  __device__ __forceinline__ Groups groups(int b) const {
+    const int64_t at = (int64_t)(b < 0 ? 0 : b) * S::HK + h;
+    return Groups{b, a.ks[at], a.vs[at]};
+  }
+  __device__ __forceinline__ void load(const Groups &gr, int tile) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const int c = (int)threadIdx.x + 256 * e;
+      if (CHUNKS % 256 != 0 && c >= CHUNKS) break;
+      const int tok = c / (S::D / 16), part = c % (S::D / 16), d = c / 4, g = c % 4;
+      if constexpr (S::BLOCK >= 64) { // (one block: its place is a scalar)
+        const int b = __builtin_amdgcn_readfirstlane(gr.block), off = 64 * tile % S::BLOCK;
+        const int64_t at = ((int64_t)(b < 0 ? 0 : b) * S::HK + h) * (S::BLOCK * S::D);
+        kx[e] = *reinterpret_cast<const u32x4_any *>(a.k + at + off * S::D + (tok * S::D + 16 * part));
+        vx[e] = *reinterpret_cast<const u32x4_any *>(a.v + at + off + (d * S::BLOCK + 16 * g));
+      } else {
+        const int bk = __shfl(gr.block, tok / 16), bv = __shfl(gr.block, g); // (lane i of the first four holds group i)
+        const uint8_t *kp = a.k + ((int64_t)(bk < 0 ? 0 : bk) * S::HK + h) * (S::BLOCK * S::D), *vp = a.v + ((int64_t)(bv < 0 ? 0 : bv) * S::HK + h) * (S::BLOCK * S::D);
+        kx[e] = *reinterpret_cast<const u32x4_any *>(kp + (64 * tile + tok) % S::BLOCK * S::D + 16 * part);
+        vx[e] = *reinterpret_cast<const u32x4_any *>(vp + d * S::BLOCK + (64 * tile + 16 * g) % S::BLOCK);
+      }
+    }
+  }
+  __device__ __forceinline__ Mode mode(const Groups &gr, int tile, uint32_t ref) const {
+    auto quad = [](uint32_t v) {
+      v = max_u32(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true));
+      return (uint32_t)__builtin_amdgcn_readfirstlane((int)max_u32(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true)));
+    };
+    const bool read = gr.block >= 0 && gr.vs != 255 && 64 * tile + 16 * (int)(threadIdx.x % 4) <= hi;
+    const uint32_t now = max_u32(ref, quad(read ? gr.vs : 0));
+    if constexpr (S::EL == EL_BF16) return Mode{now, false};
+    return Mode{now, quad(read ? now - gr.vs : 0) > 8};
+  }
+  __device__ __forceinline__ void stage(const Groups &gr, const Mode &mo, int tile, int buf) {
+    const bool whole = 64 * tile + 63 <= hi && __all(gr.block >= 0);
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const int c = (int)threadIdx.x + 256 * e;
+      if (CHUNKS % 256 != 0 && c >= CHUNKS) break;
+      const int tok = c / (S::D / 16), part = c % (S::D / 16), d = c / 4, g = c % 4;
+      v4i *kd = reinterpret_cast<v4i *>(&lds.k[buf][tok * KP + 16 * part]), *vd = reinterpret_cast<v4i *>(&lds.v[buf][d * VP + 16 * g]);
+      kd[0] = attn_decode8<S::EL, S::FMT>(kx[e].x, kx[e].y, 1.0f), kd[1] = attn_decode8<S::EL, S::FMT>(kx[e].z, kx[e].w, 1.0f);
+      const uint32_t vs = S::BLOCK >= 64 ? (uint32_t)__builtin_amdgcn_readfirstlane((int)gr.vs) : (uint32_t)__shfl((int)gr.vs, g);
+      bool used = true;
+      if (!whole) {
+        // (behind the last position, and where there is no block, zeros)
+        const int n = __shfl(gr.block, g) >= 0 ? hi + 1 - (64 * tile + 16 * g) : 0;
+        used = n > 0;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) vx[e][w] &= n >= 4 * w + 4 ? 0xFFFFFFFFu : n <= 4 * w ? 0u : 0xFFFFFFFFu >> (8 * (4 * w + 4 - n));
+      }
+      const uint32_t down = mo.ref - vs < 126u ? mo.ref - vs : 126u;
+      const float by = mo.plain || !used || vs == 255 ? 1.0f : u2f((127 - down) << 23);
+      if (S::EL != EL_BF16 && mo.plain) {
+        vd[0] = wx_decode8<S::FMT>(vx[e].x, vx[e].y, 1.0f), vd[1] = wx_decode8<S::FMT>(vx[e].z, vx[e].w, 1.0f);
+      } else {
+        vd[0] = attn_decode8<S::EL, S::FMT>(vx[e].x, vx[e].y, by), vd[1] = attn_decode8<S::EL, S::FMT>(vx[e].z, vx[e].w, by);
+      }
+    }
+  }
+
+  v16f o[OT];
+  float m, sum;
+  uint32_t ref;
+  v4i q[QF];
+
+  __device__ __forceinline__ void times(float by) {
+#pragma unroll
+    for (int i = 0; i < OT; ++i) o[i] *= by;
+  }
+  // tile from LDS; pos: the lane's row's position (-1: no row), first and last:
+  // the wave's rows'
+  __device__ __forceinline__ void step(const Groups &gr, const Mode &mo, int tile, int buf, int pos, int first, int last) {
+    const int lane = threadIdx.x % 64, r = lane % 32, half = lane / 32, key = (r & 0x13) | (r & 4) << 1 | (r & 8) >> 1;
+    if (mo.ref != ref) {
+      times(mo.ref - ref > 126 ? 0.0f : u2f((127 - (mo.ref - ref)) << 23));
+      ref = mo.ref;
+    }
+    v16f s[2] = {};
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int c = 0; c < QF; ++c)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        s[u] = mfma<S::EL>(*reinterpret_cast<const v4i *>(&lds.k[buf][(32 * u + key) * KP + 16 * c + 8 * half]), q[c], s[u]);
+    ahead<2 * QF, false>();
+    __builtin_amdgcn_s_setprio(0);
+    constexpr int GS = S::BLOCK >= 64 ? 1 : 4; // groups of tokens whose blocks may differ
+    float f[GS];
+    uint32_t there = 0;
+#pragma unroll
+    for (int g = 0; g < GS; ++g) {
+      // (a block of values that are NaN makes NaN of the rows that see it: by their scores)
+      const uint32_t ks = (uint32_t)__builtin_amdgcn_readlane((int)gr.ks, g), vs = (uint32_t)__builtin_amdgcn_readlane((int)gr.vs, g);
+      f[g] = __builtin_fabsf(a.scale) * mx_scale(vs == 255 ? 255 : ks);
+      there |= (uint32_t)(__builtin_amdgcn_readlane(gr.block, g) >= 0) << g;
+    }
+    const bool whole = there == (1u << GS) - 1 && 64 * tile + 63 <= first && (S::WINDOW == 0 || 64 * tile > last - S::WINDOW);
+    // (tokens by their distance from the lane's first: compares with constants)
+    const int to = pos - (64 * tile + 8 * half), from = to - S::WINDOW;
+    auto sees = [&](int u, int i) {
+      const int at = 32 * u + i / 8 * 16 + i % 8;
+      return (there >> ((2 * u + i / 8) * GS / 4) & 1) && at <= to && (S::WINDOW == 0 || at > from);
+    };
+    if (!whole) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[u][i] = sees(u, i) ? s[u][i] : -__builtin_inff();
+    }
+    float top = -__builtin_inff();
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        float t = s[u][8 * g];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) t = __builtin_fmaxf(t, s[u][8 * g + i]);
+        top = __builtin_fmaxf(top, t * f[(2 * u + g) * GS / 4]); // (f is not negative)
+      }
+    top = with_lane<32>(top, max2);
+    if (__any(top > m + 6.0f)) {
+      const float now = __builtin_fmaxf(m, top), was = m == now ? 1.0f : __builtin_amdgcn_exp2f(m - now);
+      m = now;
+      sum *= was;
+      times(was);
+    }
+    const float mu = m == -__builtin_inff() ? 0.0f : m; // (a row that has seen nothing)
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[u][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], f[(2 * u + i / 8) * GS / 4], -mu));
+    if (!whole) { // (a scale may be zero, or NaN)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[u][i] = sees(u, i) ? s[u][i] : 0.0f;
+    }
+    float part[4] = {0, 0, 0, 0}; // (no long chain of additions)
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) part[i % 4] += s[u][i];
+    sum += (part[0] + part[1]) + (part[2] + part[3]);
+    auto product = [&](auto el) {
+      constexpr int EL = decltype(el)::value;
+      __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float p[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[i] = s[k / 2][8 * (k % 2) + i];
+        const v4i pf = attn_round8<EL>(p);
+#pragma unroll
+        for (int dt = 0; dt < OT; ++dt)
+          o[dt] = mfma<EL>(*reinterpret_cast<const v4i *>(&lds.v[buf][(32 * dt + r) * VP + 16 * k + 8 * half]), pf, o[dt]);
+      }
+      ahead<4 * OT, true>();
+      __builtin_amdgcn_s_setprio(0);
+    };
+    if (S::EL == EL_BF16 || !mo.plain) {
+      product(std::integral_constant<int, S::EL>{});
+      return;
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const uint32_t vs = (uint32_t)__builtin_amdgcn_readlane((int)gr.vs, 2 * u + i / 8);
+        s[u][i] *= vs > ref || ref - vs > 126u ? 0.0f : u2f((127 + vs - ref) << 23); // (above it: not read)
+      }
+#pragma unroll 1
+    for (int part = 0; part < 2; ++part) {
+      product(std::integral_constant<int, EL_BF16>{});
+      // what the rounding left
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[u][i] -= bf16_to_f32(f32_to_bf16_rne(s[u][i]));
+    }
+  }
+
+  // Rows t .. t + n - 1, of a sequence's positions lo .. hi; t0: the tile's first
+  // row.  PARTS: piece `piece` of `pieces` of their tiles, at least CUT tiles
+  // long, to part and stats.
+  template <bool PARTS> __device__ __forceinline__ void run(int64_t t0, int64_t t, int n, int gt, int piece, int pieces, float *part, float *stats) {
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, r = lane % 32, half = lane / 32;
+    const int row = 32 * wave + r, tok = row / S::GT, head = gt * 16 + row % S::GT, skip = (int)(t - t0);
+    const bool ok = tok >= skip && tok < skip + n && head < S::G && row < TOKENS * S::GT;
+    const int pos = ok ? lo + tok - skip : -1;
+    int begin = PagedUnits<S>::first(lo), end = hi / 64 + 1;
+    bool alone = true; // one piece has all of them: the result, and the mark DONE for a sum
+    if constexpr (PARTS) {
+      int cut = (end - begin + pieces - 1) / pieces;
+      cut = cut < CUT ? CUT : cut;
+      alone = end - begin <= cut;
+      begin += piece * cut;
+      end = begin + cut < end ? begin + cut : end;
+      if (begin >= end) {
+        if (ok && half == 0) stats[2 * row] = -__builtin_inff(), stats[2 * row + 1] = 0;
+        return;
+      }
+    }
+    // the wave's rows' positions
+    const int a0 = 32 * wave / S::GT, a1 = (32 * wave + 31) / S::GT;
+    const int first = lo + (a0 > skip ? a0 - skip : 0), last = a1 < skip ? -1 : lo + (a1 - skip < n ? a1 - skip : n - 1);
+    const int seen = a0 >= skip + n ? -1 : last; // (-1: the wave has no rows)
+    const uint16_t *qp = a.q + ((t0 + (ok ? tok : skip)) * S::HQ + h * S::G + (ok ? head : 0)) * S::D + 8 * half;
+#pragma unroll
+    for (int c = 0; c < QF; ++c) {
+      const u32x4 w = *reinterpret_cast<const u32x4_any *>(qp + 16 * c);
+      // (a negative scale's sign goes to the queries: a maximum is one before and after)
+      const int turn = a.scale < 0 ? (int)0x80008000u : 0;
+      q[c] = ok ? v4i{(int)w.x ^ turn, (int)w.y ^ turn, (int)w.z ^ turn, (int)w.w ^ turn} : v4i{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int i = 0; i < OT; ++i) o[i] = v16f{};
+    m = -__builtin_inff(), sum = 0, ref = 0;
+    Groups gr = groups(block(begin));
+    load(gr, begin);
+    Mode mo = mode(gr, begin, 0);
+    int next = block(begin + 1);
+    stage(gr, mo, begin, begin & 1);
+    __syncthreads();
+    for (int i = begin; i < end; ++i) {
+      Groups gn = gr;
+      if (i + 1 < end) {
+        gn = groups(next);
+        load(gn, i + 1);
+        next = block(i + 2);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if (64 * i <= seen && (S::WINDOW == 0 || 64 * i + 63 > first - S::WINDOW)) step(gr, mo, i, i & 1, pos, first, last);
+      if (i + 1 < end) {
+        mo = mode(gn, i + 1, mo.ref);
+        stage(gn, mo, i + 1, (i + 1) & 1);
+        gr = gn;
+      }
+      __syncthreads();
+    }
+    times(mx_scale(ref));
+    sum = with_lane<32>(sum, [](float x, float y) { return x + y; });
+    if (!ok) return;
+    if (PARTS && alone && half == 0) stats[2 * row + 1] = DONE;
+    if (PARTS && !alone) {
+      if (half == 0) stats[2 * row] = m, stats[2 * row + 1] = sum;
+      float *dst = part + row * S::D + 4 * half;
+#pragma unroll
+      for (int dt = 0; dt < OT; ++dt)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          *reinterpret_cast<v4f *>(dst + 32 * dt + 8 * k) = v4f{o[dt][4 * k], o[dt][4 * k + 1], o[dt][4 * k + 2], o[dt][4 * k + 3]};
+      return;
+    }
+    const float by = sum == 0 ? 0.0f : 1.0f / sum;
+    uint16_t *dst = a.out + ((t0 + tok) * (int64_t)S::HQ + h * S::G + head) * S::D + 4 * half;
+#pragma unroll
+    for (int dt = 0; dt < OT; ++dt)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        uint16_t e[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float v = o[dt][4 * k + j] * by;
+          e[j] = S::EL == EL_BF16 ? f32_to_bf16_rne(v) : __builtin_bit_cast(uint16_t, (_Float16)v);
+        }
+        *reinterpret_cast<u32x2_any *>(dst + 32 * dt + 8 * k) = u32x2{(uint32_t)e[0] | (uint32_t)e[1] << 16, (uint32_t)e[2] | (uint32_t)e[3] << 16};
+      }
+  }
+
+  __device__ static __forceinline__ int64_t tiles(int64_t T) { return (T + TOKENS - 1) / TOKENS; }
+  // The units of a tile and a head in `pieces` pieces each, first all units'
+  // first ones: few units leave most of the chip idle, and those of a prompt's
+  // last rows take longest.  us of a call, whole and in pieces of at least 16
+  // tiles: 512 rows behind 7000 positions 226 and 105, 64 behind 8000 244 and 55; a
+  // prompt of 512 rows, whose tiles stay whole, 20.5 and 23.5, of 2048 73.5 and 70;
+  // pieces of at least 4, 8 and 12 tiles, 1001 rows over a window of 4096: 63, 61,
+  // 64, of 16 53.
+  // ws: the pieces' statistics (two of each of 128 rows), then their rows.
+  static constexpr int PIECES = 1024, CUT = 16;
+  static constexpr float DONE = -1; // (no sum is negative)
+  __device__ static __forceinline__ int pieces(int64_t T) {
+    const int64_t n = PIECES / (tiles(T) * HEADS);
+    return n > 16 ? 16 : n < 1 ? 1 : (int)n;
+  }
+  __device__ static __forceinline__ float *stats_of(char *ws, int64_t piece) { return reinterpret_cast<float *>(ws) + piece * 256; }
+  __device__ static __forceinline__ float *part_of(char *ws, int64_t piece) { return reinterpret_cast<float *>(ws) + PIECES * 256 + piece * (128 * S::D); }
+
+  // grid: tiles(T) * HEADS, PARTS: PIECES; the last rows, which see most, first
+  template <bool PARTS> __device__ static __forceinline__ void rows(const PagedArgs &a, int64_t T, char *ws) {
+    __shared__ Lds lds;
+    const int cuts = PARTS ? pieces(T) : 1, units = (int)tiles(T) * HEADS, piece = PARTS ? (int)blockIdx.x / units : 0;
+    if (piece >= cuts) return;
+    const int64_t t0 = (tiles(T) - 1 - (blockIdx.x - piece * units) / HEADS) * TOKENS;
+    const int hh = (int)(blockIdx.x - piece * units) % HEADS, h = hh / S::GTILES, gt = hh % S::GTILES, lane = threadIdx.x % 64;
+    const int tokens = (int)(T - t0 < TOKENS ? T - t0 : TOKENS);
+    for (int at = 0; at < tokens;) {
+      const int64_t t = t0 + at;
+      const int s = a.seq[t], p = a.pos[t];
+      if (!S::inside(s, p)) {
+        ++at;
+        continue;
+      }
+      // the rows that follow it
+      int n = 0;
+#pragma unroll
+      for (int k = 0; k < TOKENS; k += 64) {
+        const int i = k + lane;
+        const uint64_t other = __ballot(!(i < tokens - at && p + i < S::FAR && a.seq[t + i] == s && a.pos[t + i] == p + i));
+        if (n == k) n += other ? __builtin_ctzll(other) : 64;
+      }
+      PagedPrompt{a, lds, s, h, p, p + n - 1}.template run<PARTS>(t0, t, n, gt, piece, cuts, PARTS ? part_of(ws, blockIdx.x) : nullptr,
+                                                                 PARTS ? stats_of(ws, blockIdx.x) : nullptr);
+      at += n;
+    }
+  }
+
+  // The rows' pieces added in order, eight lanes a row: grid PIECES / 2 * 4, a
+  // quarter of a unit's rows each.
+  __device__ static __forceinline__ void join(const PagedArgs &a, int64_t T, const char *ws_) {
+    char *ws = const_cast<char *>(ws_);
+    const int cuts = pieces(T), unit = blockIdx.x / 4, hh = unit % HEADS, h = hh / S::GTILES, gt = hh % S::GTILES;
+    const int64_t t0 = (tiles(T) - 1 - unit / HEADS) * TOKENS, units = tiles(T) * HEADS;
+    if (t0 < 0) return;
+    const int row = blockIdx.x % 4 * 32 + threadIdx.x / 8, tok = row / S::GT, head = gt * 16 + row % S::GT;
+    if (row >= TOKENS * S::GT || t0 + tok >= T || head >= S::G || !S::inside(a.seq[t0 + tok], a.pos[t0 + tok])) return;
+    auto piece = [&](int i) { return i * units + unit; };
+    if (stats_of(ws, piece(0))[2 * row + 1] == DONE) return;
+    float m = -__builtin_inff(), l = 0, by[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (i < cuts) m = __builtin_fmaxf(m, by[i] = stats_of(ws, piece(i))[2 * row]);
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (i < cuts) {
+        const float sum = stats_of(ws, piece(i))[2 * row + 1];
+        by[i] = sum == 0 ? 0.0f : by[i] == m ? 1.0f : __builtin_amdgcn_exp2f(by[i] - m);
+        l += sum * by[i];
+      }
+    const float over = l == 0 ? 0.0f : 1.0f / l;
+    for (int d = threadIdx.x % 8 * 4; d < S::D; d += 32) {
+      v4f o = {0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < 16; ++i) // (what saw nothing may not have been written)
+        if (i < cuts && by[i] != 0) o += *reinterpret_cast<const v4f *>(part_of(ws, piece(i)) + row * S::D + d) * by[i];
+      uint16_t e[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) e[k] = S::EL == EL_BF16 ? f32_to_bf16_rne(o[k] * over) : __builtin_bit_cast(uint16_t, (_Float16)(o[k] * over));
+      *reinterpret_cast<u32x2_any *>(a.out + ((t0 + tok) * (int64_t)S::HQ + h * S::G + head) * S::D + d) =
+          u32x2{(uint32_t)e[0] | (uint32_t)e[1] << 16, (uint32_t)e[2] | (uint32_t)e[3] << 16};
     }
   }
 };

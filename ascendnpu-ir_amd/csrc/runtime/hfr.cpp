@@ -41,7 +41,8 @@ struct PreLaunch {
   std::string kernel;
   hipFunction_t fn = nullptr;
   hfr_launch_cfg cfg{};
-  int64_t perRow = 0; // at launch-time rows: blocks a row, besides the grid's own
+  int64_t perRow = 0;   // at launch-time rows: blocks a row, besides the grid's own
+  uint64_t wsBytes = 0; // what a launch behind this one alone needs of the workspace (0: all)
   std::vector<Karg> kargs;
 };
 
@@ -54,6 +55,7 @@ struct RowAlt {
   int64_t maxRows = 0, rowsB = 1, rowsC = 1;
   unsigned block = 0;
   bool pre = false; // after the group's pre kernels
+  int only = -1;    // ... after this one of them
 };
 
 // Workspaces that a handle owns for launches without a caller's: one a
@@ -195,8 +197,13 @@ int parseBlock(const std::vector<std::string> &lines, hfr_group &g) {
       if (is.fail() || n <= 0 || g.pre.empty() || !g.rowsDyn) return fail(HFR_ERR_MANIFEST, "bad pre_rows line: " + ln);
       g.pre.back().perRow = n;
     }
+    else if (key == "pre_workspace") {
+      // pre_workspace <bytes>: of a launch behind the pre kernel before it alone
+      is >> (g.pre.empty() ? g.wsBytes : g.pre.back().wsBytes);
+      if (is.fail() || g.pre.empty() || g.pre.back().wsBytes > g.wsBytes) return fail(HFR_ERR_MANIFEST, "bad pre_workspace line: " + ln);
+    }
     else if (key == "alt") {
-      // alt <kernel> <max rows> <rows per block row> <blocks per block row> <threads> [pre]
+      // alt <kernel> <max rows> <rows per block row> <blocks per block row> <threads> [pre [n]]
       RowAlt ra;
       is >> ra.kernel >> ra.maxRows >> ra.rowsB >> ra.rowsC >> ra.block;
       if (is.fail()) return fail(HFR_ERR_MANIFEST, "malformed manifest line: " + ln);
@@ -204,6 +211,8 @@ int parseBlock(const std::vector<std::string> &lines, hfr_group &g) {
       if (is >> more) {
         if (more != "pre") return fail(HFR_ERR_MANIFEST, "bad alt line: " + ln);
         ra.pre = true;
+        if (is >> ra.only && (ra.only < 0 || ra.only >= (int)g.pre.size())) return fail(HFR_ERR_MANIFEST, "bad alt line: " + ln);
+        if (is.fail()) ra.only = -1;
       }
       is.clear();
       if (ra.maxRows <= 0 || ra.rowsB <= 0 || ra.rowsC <= 0 || !ra.block || (!g.alts.empty() && g.alts.back().maxRows >= ra.maxRows))
@@ -355,6 +364,7 @@ const RowAlt *altFor(const hfr_group *g, int64_t rows) {
 uint64_t workspaceOf(const hfr_group *g, int64_t rows) {
   if (g->rowsDyn && rows == 0 && !g->rowsZero) return 0;
   const RowAlt *alt = altFor(g, rows);
+  if (alt && alt->only >= 0 && g->pre[alt->only].wsBytes) return g->pre[alt->only].wsBytes;
   return alt && !alt->pre ? 0 : g->wsBytes;
 }
 
@@ -385,8 +395,9 @@ int launchGroup(const hfr_group *g, const uint64_t *params, void *const *results
     }
     return launchRaw(fn, cfg, args, n, stream);
   };
-  auto runPre = [&]() {
-    for (auto &pl : g->pre) {
+  auto runPre = [&](int only) {
+    for (const PreLaunch &pl : g->pre) {
+      if (only >= 0 && &pl != &g->pre[only]) continue;
       hfr_launch_cfg cfg = pl.cfg;
       if (pl.perRow) cfg.grid[0] += (unsigned)(rows * pl.perRow);
       const int rc = launch(pl.fn, cfg, pl.kargs);
@@ -396,14 +407,14 @@ int launchGroup(const hfr_group *g, const uint64_t *params, void *const *results
   };
   if (const RowAlt *alt = altFor(g, rows)) {
     if (alt->pre)
-      if (const int rc = runPre()) return rc;
+      if (const int rc = runPre(alt->only)) return rc;
     hfr_launch_cfg cfg{};
     cfg.grid[0] = (unsigned)((std::max<int64_t>(rows, 1) + alt->rowsB - 1) / alt->rowsB * alt->rowsC); // (no rows only with rows_zero)
     cfg.grid[1] = cfg.grid[2] = cfg.block[1] = cfg.block[2] = 1;
     cfg.block[0] = alt->block;
     return launch(alt->fn, cfg, g->kargs);
   }
-  if (const int rc = runPre()) return rc;
+  if (const int rc = runPre(-1)) return rc;
   return launch(g->fn, rowsCfg(g->cfg), g->kargs);
 }
 

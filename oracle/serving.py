@@ -105,25 +105,32 @@ def paged_attention(q, k, ks, v, vs, seq, pos, table, out, fmt, scale, window):
     size, reach = np.zeros_like(out), np.zeros(out.shape[:2])
     blocks, kv, block, dim = k.shape
     heads = q.shape[1]
-    values = bs.code_values(fmt)
+    codes = bs.code_values(fmt)
+    held = {}
+
+    def cache(s, g, n):
+        """Keys and values of the first n positions of a sequence (of blocks that it has not: of some block)."""
+        if (s, g) not in held or len(held[s, g][0]) < n:
+            j = np.arange(max([n] + [int(p) + 1 for s2, p in zip(seq, pos) if s2 == s and p < table.shape[1] * block]))
+            b = np.clip(table[s, j // block], 0, blocks - 1)
+            held[s, g] = (codes[k[b, g, j % block]] * bs.scale_values(ks[b, g])[:, None], codes[v[b, g, :, j % block]] * bs.scale_values(vs[b, g])[:, None])
+        return held[s, g]
     for t in range(len(seq)):
         s, p = int(seq[t]), int(pos[t])
         if not (0 <= s < table.shape[0] and 0 <= p < table.shape[1] * block):
             continue
         j = visible(p, s, table, blocks, block, window)
-        b, o = table[s, j // block], j % block
-        for h in range(heads):
-            g = h // (heads // kv)
-            if not len(j):
-                out[t, h] = 0
-                continue
-            key = values[k[b, g, o]] * bs.scale_values(ks[b, g])[:, None]
-            val = values[v[b, g, :, o]] * bs.scale_values(vs[b, g])[:, None]
+        if not len(j):
+            out[t] = 0
+            continue
+        for g in range(kv):
+            key, val = (a[j] for a in cache(s, g, p + 1))
+            h = slice(g * heads // kv, (g + 1) * heads // kv)
             with np.errstate(invalid="ignore"):
-                x = key @ q[t, h] * scale
-                w = np.exp(x - x.max())
-                w /= w.sum()
+                x = q[t, h] @ key.T * scale
+                w = np.exp(x - x.max(axis=1, keepdims=True))
+                w /= w.sum(axis=1, keepdims=True)
                 out[t, h] = w @ val
                 size[t, h] = w @ np.abs(val)
-                reach[t, h] = (np.abs(key) @ np.abs(q[t, h])).max() * abs(scale)
+                reach[t, h] = (np.abs(q[t, h]) @ np.abs(key).T).max(axis=1) * abs(scale)
     return out, size, reach

@@ -16,10 +16,10 @@ NORM = [
 APPEND = {
     "group4": (8, 2, 64, 16, 5, 160, 40, "bf16", "e4m3"), "alone": (4, 4, 32, 16, 3, 64, 13, "f32", "e5m2"),
     "group3": (6, 2, 96, 32, 4, 320, 30, "f16", "e4m3"), "wide": (4, 1, 256, 128, 3, 512, 11, "bf16", "e5m2"),
-    "usual": (32, 8, 128, 64, 6, 640, 40, "bf16", "e4m3"),
+    "usual": (32, 8, 128, 64, 6, 640, 40, "bf16", "e4m3"), "many": (2, 1, 32, 16, 700, 64, 2900, "bf16", "e4m3"),
 }
 # rotated channels, neighbouring pairs
-TURN = {"group4": (64, 0), "alone": (32, 1), "group3": (48, 0), "wide": (128, 1), "usual": (128, 0)}
+TURN = {"group4": (64, 0), "alone": (32, 1), "group3": (48, 0), "wide": (128, 1), "usual": (128, 0), "many": (32, 0)}
 # the same for the attention, and its window
 ATTEND = {
     "group4": (8, 2, 64, 16, 5, 160, 40, "bf16", "e4m3", 0), "alone": (4, 4, 32, 16, 5, 160, 47, "f16", "e5m2", 0),
@@ -27,6 +27,9 @@ ATTEND = {
     "group20": (20, 1, 64, 32, 5, 320, 40, "bf16", "e5m2", 0), "wide": (4, 1, 256, 128, 5, 512, 20, "bf16", "e5m2", 0),
     "window": (8, 2, 64, 32, 5, 640, 90, "bf16", "e4m3", 50), "window_f16": (4, 2, 128, 16, 5, 320, 90, "f16", "e4m3", 7),
     "usual": (32, 8, 128, 64, 6, 4096, 90, "bf16", "e4m3", 0), "far": (8, 2, 128, 16, 3, 8192, 600, "bf16", "e4m3", 0),
+    "far_f16": (6, 2, 96, 32, 3, 4096, 300, "f16", "e4m3", 0), "far_group20": (20, 1, 64, 64, 3, 4096, 150, "bf16", "e5m2", 0),
+    "far_window": (8, 2, 64, 16, 3, 4096, 600, "bf16", "e4m3", 1500), "far_wide": (4, 1, 256, 128, 3, 4096, 80, "f16", "e5m2", 0),
+    "far_alone": (3, 3, 32, 32, 3, 4096, 300, "bf16", "e4m3", 0), "many": (2, 1, 32, 16, 150, 4096, 2900, "bf16", "e4m3", 0),
 }
 # rows of the groups that are compiled for one row count
 STATIC = {"append": ("usual", 70), "attend": ("usual", 70)}

@@ -302,6 +302,10 @@ def paged_table(rng, slots, room, block, blocks, used):
 
 def append_batches(c):
     hq, hk, d, block, slots, room, blocks, el, fmt = c
+    if slots > 100:  # row counts of every tile
+        yield [(s, 5 + s % 40, 1) for s in range(300)], 2
+        yield [(s, s % 50, 2) for s in range(600)], 0
+        return
     yield [(0, 0, 1)], 0
     yield [(1, block - 1, 2), (0, block, 1), (2, 3, 5)], 3
     yield [(slots - 1, room - block - 1, block + 1), (0, block // 2, block + 3)], 0
@@ -395,6 +399,11 @@ def cache_of(rng, c, wide=False):
 
 def attend_batches(c):
     hq, hk, d, block, slots, room, blocks, el, fmt, window = c
+    if slots > 100:  # groups of tokens whose tiles each thread has several of
+        yield [(s, (s * 37) % 190, 1 + s % 6) for s in range(slots)], 3, {}
+        yield [(s, (s * 37) % 190, 7) for s in range(slots)], 0, {}
+        yield [(s, 1 + s % 20, 1) for s in range(slots - 1)] + [(slots - 1, 4000, 3)], 0, {}
+        return
     far = min(room, 5000)
     yield [(0, 0, 1)], 0, {}
     yield [(1, far - 1, 1), (0, 63, 1), (2, 64, 1)], 3, {}
@@ -402,6 +411,10 @@ def attend_batches(c):
     yield [(1, far - 70, 70), (0, 0, 33)], 5, {}
     yield [(2, 3 * block - 2, 6), (0, 40, 4), (1, 20, 1)], 1, dict(holes=True)
     yield [(s, 11 * s + 2, 3) for s in range(slots)], 2, dict(nan=True)
+    # rows of prompts: tiles of several sequences, ends inside a tile
+    yield [(0, far - 130, 129), (1, 10, 31), (2, 1, 90)], 3, dict(wide=True)
+    yield [(0, 0, 17), (2, far - 61, 60), (1, 2 * block, 40)], 0, dict(holes=True)
+    yield [(1, far // 2, 75), (0, 3, 64), (2, 0, 1)], 2, dict(nan=True)
 
 
 def check_attention(c, outs, q, cache, seq, pos, table, before, scale=None):
@@ -439,7 +452,7 @@ def attend_case(rng, c, parts, pad, wide=False, holes=False, nan=False):
     for b in free:
         k[b], v[b], ks[b], vs[b] = 0xFF, 0x7F, 255, 255
     for s, n in enumerate(used):  # stale entries that name them
-        if free and -(-n // block) < table.shape[1]:
+        if n and free and -(-n // block) < table.shape[1]:
             table[s, -(-n // block)] = free[0]
     if holes:
         table[parts[0][0], 1] = -1
