@@ -559,8 +559,8 @@ template <typename S> struct PagedPrompt {
     __attribute__((aligned(16))) uint16_t k[2][64 * KP], v[2][S::D * VP];
   };
 
-  template <int EL> __device__ static __forceinline__ v16f mfma(v4i a, v4i b, v16f c) {
-    if constexpr (EL == EL_BF16) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
+  __device__ static __forceinline__ v16f mfma(v4i a, v4i b, v16f c) {
+    if constexpr (S::EL == EL_BF16) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
     else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
   }
   // The order of PRODUCTS products and their reads from LDS: eight reads ahead
@@ -583,13 +583,15 @@ template <typename S> struct PagedPrompt {
     int block;      // of the cache, -1 for none
     uint32_t ks, vs; // scale bytes
   };
-  // what the workgroup does with a tile's values: scaled to the reference, or
-  // (f16, of blocks further apart than its range) as they are, with p scaled.
-  // bf16 has the range for all but values 2^100 below the largest block's.
+  // What the tile's values are scaled to: o is in units of 2^(ref - 127), of
+  // about the largest block that is read.  bf16 has the range for blocks 2^100
+  // below it; f16 for 2^8 (DOWN), and what is below that scales p (`more`), which
+  // keeps its 11 bits down to 2^-14 and is 2^-25 off below.
   struct Mode {
     uint32_t ref;
-    bool plain;
+    bool more;
   };
+  static constexpr uint32_t DOWN = S::EL == EL_BF16 ? 126 : 8;
 
   const PagedArgs &a;
   Lds &lds;
@@ -630,9 +632,8 @@ template <typename S> struct PagedPrompt {
       return (uint32_t)__builtin_amdgcn_readfirstlane((int)max_u32(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true)));
     };
     const bool read = gr.block >= 0 && gr.vs != 255 && 64 * tile + 16 * (int)(threadIdx.x % 4) <= hi;
-    const uint32_t now = max_u32(ref, quad(read ? gr.vs : 0));
-    if constexpr (S::EL == EL_BF16) return Mode{now, false};
-    return Mode{now, quad(read ? now - gr.vs : 0) > 8};
+    const uint32_t big = quad(read ? gr.vs : 0), now = big > ref || (big && big + 4 < ref) ? big : ref;
+    return Mode{now, S::EL != EL_BF16 && quad(read ? now - gr.vs : 0) > DOWN};
   }
   __device__ __forceinline__ void stage(const Groups &gr, const Mode &mo, int tile, int buf) {
     const bool whole = 64 * tile + 63 <= hi && __all(gr.block >= 0);
@@ -652,13 +653,9 @@ template <typename S> struct PagedPrompt {
 #pragma unroll
         for (int w = 0; w < 4; ++w) vx[e][w] &= n >= 4 * w + 4 ? 0xFFFFFFFFu : n <= 4 * w ? 0u : 0xFFFFFFFFu >> (8 * (4 * w + 4 - n));
       }
-      const uint32_t down = mo.ref - vs < 126u ? mo.ref - vs : 126u;
-      const float by = mo.plain || !used || vs == 255 ? 1.0f : u2f((127 - down) << 23);
-      if (S::EL != EL_BF16 && mo.plain) {
-        vd[0] = wx_decode8<S::FMT>(vx[e].x, vx[e].y, 1.0f), vd[1] = wx_decode8<S::FMT>(vx[e].z, vx[e].w, 1.0f);
-      } else {
-        vd[0] = attn_decode8<S::EL, S::FMT>(vx[e].x, vx[e].y, by), vd[1] = attn_decode8<S::EL, S::FMT>(vx[e].z, vx[e].w, by);
-      }
+      const uint32_t down = mo.ref - vs < DOWN ? mo.ref - vs : DOWN;
+      const float by = !used || vs == 255 ? 1.0f : u2f((127 - down) << 23);
+      vd[0] = attn_decode8<S::EL, S::FMT>(vx[e].x, vx[e].y, by), vd[1] = attn_decode8<S::EL, S::FMT>(vx[e].z, vx[e].w, by);
     }
   }
 
@@ -676,7 +673,8 @@ template <typename S> struct PagedPrompt {
   __device__ __forceinline__ void step(const Groups &gr, const Mode &mo, int tile, int buf, int pos, int first, int last) {
     const int lane = threadIdx.x % 64, r = lane % 32, half = lane / 32, key = (r & 0x13) | (r & 4) << 1 | (r & 8) >> 1;
     if (mo.ref != ref) {
-      times(mo.ref - ref > 126 ? 0.0f : u2f((127 - (mo.ref - ref)) << 23));
+      const int by = (int)ref - (int)mo.ref;
+      times(u2f((uint32_t)(127 + (by < -126 ? -126 : by > 127 ? 127 : by)) << 23));
       ref = mo.ref;
     }
     v16f s[2] = {};
@@ -685,7 +683,7 @@ template <typename S> struct PagedPrompt {
     for (int c = 0; c < QF; ++c)
 #pragma unroll
       for (int u = 0; u < 2; ++u)
-        s[u] = mfma<S::EL>(*reinterpret_cast<const v4i *>(&lds.k[buf][(32 * u + key) * KP + 16 * c + 8 * half]), q[c], s[u]);
+        s[u] = mfma(*reinterpret_cast<const v4i *>(&lds.k[buf][(32 * u + key) * KP + 16 * c + 8 * half]), q[c], s[u]);
     ahead<2 * QF, false>();
     __builtin_amdgcn_s_setprio(0);
     constexpr int GS = S::BLOCK >= 64 ? 1 : 4; // groups of tokens whose blocks may differ
@@ -745,42 +743,30 @@ template <typename S> struct PagedPrompt {
 #pragma unroll
       for (int i = 0; i < 16; ++i) part[i % 4] += s[u][i];
     sum += (part[0] + part[1]) + (part[2] + part[3]);
-    auto product = [&](auto el) {
-      constexpr int EL = decltype(el)::value;
-      __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float p[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) p[i] = s[k / 2][8 * (k % 2) + i];
-        const v4i pf = attn_round8<EL>(p);
-#pragma unroll
-        for (int dt = 0; dt < OT; ++dt)
-          o[dt] = mfma<EL>(*reinterpret_cast<const v4i *>(&lds.v[buf][(32 * dt + r) * VP + 16 * k + 8 * half]), pf, o[dt]);
-      }
-      ahead<4 * OT, true>();
-      __builtin_amdgcn_s_setprio(0);
-    };
-    if (S::EL == EL_BF16 || !mo.plain) {
-      product(std::integral_constant<int, S::EL>{});
-      return;
-    }
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const uint32_t vs = (uint32_t)__builtin_amdgcn_readlane((int)gr.vs, 2 * u + i / 8);
-        s[u][i] *= vs > ref || ref - vs > 126u ? 0.0f : u2f((127 + vs - ref) << 23); // (above it: not read)
-      }
-#pragma unroll 1
-    for (int part = 0; part < 2; ++part) {
-      product(std::integral_constant<int, EL_BF16>{});
-      // what the rounding left
+    if (mo.more) {
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[u][i] -= bf16_to_f32(f32_to_bf16_rne(s[u][i]));
+        for (int g = 0; g < 2; ++g) {
+          const uint32_t vs = (uint32_t)__builtin_amdgcn_readlane((int)gr.vs, 2 * u + g), down = ref - vs;
+          // (not read: p is zero)
+          const float by = vs > ref || down <= DOWN ? 1.0f : down > DOWN + 100 ? 0.0f : u2f((127 + DOWN - down) << 23);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) s[u][8 * g + i] *= by;
+        }
     }
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float p[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) p[i] = s[k / 2][8 * (k % 2) + i];
+      const v4i pf = attn_round8<S::EL>(p);
+#pragma unroll
+      for (int dt = 0; dt < OT; ++dt) o[dt] = mfma(*reinterpret_cast<const v4i *>(&lds.v[buf][(32 * dt + r) * VP + 16 * k + 8 * half]), pf, o[dt]);
+    }
+    ahead<4 * OT, true>();
+    __builtin_amdgcn_s_setprio(0);
   }
 
   // Rows t .. t + n - 1, of a sequence's positions lo .. hi; t0: the tile's first
