@@ -4,7 +4,8 @@
 `bench.py` on a GPU machine load prebuilt code objects: the headline
 workloads of `groups.CONFIGS` at their full sizes, the bf16 and [K, N]-layout
 contractions, the block-scaled fp8 contraction, the transpose+cast group, the layer norm,
-block-scaled codes and weight product of a 4096-wide layer, and the reduced
+block-scaled codes and weight product of a 4096-wide layer, the same layer's
+norm, cache and attention in serving, and the reduced
 RMSNorm+quant group the smoke check runs.  The parity cases the tests compile (ragged sizes,
 every op family of the generic lowering, dynamic dims) live beside the tests.
 """
@@ -37,6 +38,14 @@ def entries():
     e["dequantize_mx_weight"] = g.dequantize_mx(4096, 4096, fmt="e2m1", axis=0)
     # the linear layer with a 4-bit weight, any row count
     e["linear_mx_rt"] = _any_rows(g.linear_mx, n=4096, k=4096, bias=True)
+    # the attention half of a decoder layer in serving: the residual's norm into
+    # int8 codes, rotation and append to an 8-bit cache of 64 sequences, and the
+    # attention over it, any row count
+    cache = dict(heads=32, kv_heads=8, dim=128, slots=64, room=8192, blocks=4096, block=64)
+    e["rms_norm"] = g.rms_norm(8192, 4096)
+    e["rms_norm_rt"] = _any_rows(g.rms_norm, cols=4096)
+    e["append_kv_rt"] = _any_rows(g.append_kv, **cache)
+    e["paged_attention_rt"] = _any_rows(g.paged_attention, **cache)
     return e
 
 

@@ -812,3 +812,42 @@ def paged_attention(rows, heads, kv_heads, dim, slots, room, blocks, block=64, e
     more = f", window = {window} : i32" if window else ""
     return _group_text("paged_attention", "hfusion.paged_attention", f"format = {_MX_CODE[fmt]} : i32, scale = {scale:.9e} : f32{more}",
                        ins, [("out", t["q"])])
+
+
+def decoder_attention(rows, cols, heads, kv_heads, dim, slots, room, blocks, block=64, fmt="e4m3", eps=1e-6, window=0):
+    """An un-fused host function: the attention half of a decoder layer for a
+    batch of `rows` tokens.  The residual stream [rows, cols] gets the last
+    layer's output added and is normalised into block-scaled codes (rms_norm),
+    the block-scaled product with a weight [cols, (heads + 2 kv_heads) dim]
+    (quantize_mx with axis 0 makes it) makes queries, keys and values,
+    append_kv rotates and appends them, paged_attention answers.  A program of
+    these launches; residual sum, result and cache are arguments."""
+    n = (heads + 2 * kv_heads) * dim
+    t = _paged_types(rows, heads, kv_heads, dim, slots, room, blocks, block, "bf16", fmt)
+    ins, outs, code = _rms_operands(rows, cols, "bf16", None, "e4m3", True)
+    (X, G), (Q, S) = (ins[0][1], ins[2][1]), (outs[1][1], outs[2][1])
+    (W, SW), R, C, O = _mx_types(cols, n, "e4m3", 0), _t([room, dim], "f32"), _t([rows, n], "f32"), _t([rows, n], "bf16")
+    caches = ["k", "ks", "v", "vs"]
+    args = [("x", X), ("residual", X), ("gamma", G), ("w", W), ("sw", SW), ("rot", R)] + [(m, t[m]) for m in ("seq", "pos", "table")]
+    args += [("sum", X)] + [(m, t[m]) for m in caches] + [("out", t["q"])]
+    sig = ", ".join(f"%{m}: {ty}" for m, ty in args)
+    cache_tys = ", ".join(t[m] for m in caches)
+    batch, batch_tys = "%seq, %pos, %table", f'{t["seq"]}, {t["pos"]}, {t["table"]}'
+    form, more = f"format = {_MX_CODE[fmt]} : i32", f", window = {window} : i32" if window else ""
+    return f"""module {{
+  func.func @decoder_attention({sig}) -> ({t["q"]}, {X}, {cache_tys})
+      {_HOST} {{
+    %e0 = tensor.empty() : {Q}
+    %e1 = tensor.empty() : {S}
+    %n:3 = hfusion.rms_norm {{eps = {eps:.17e} : f64{code}}} ins(%x, %residual, %gamma : {X}, {X}, {G}) outs(%sum, %e0, %e1 : {X}, {Q}, {S}) -> {X}, {Q}, {S}
+    %e2 = tensor.empty() : {C}
+    %c = hfusion.matmul_mx ins(%n#1, %w, %n#2, %sw : {Q}, {W}, {S}, {SW}) outs(%e2 : {C}) -> {C}
+    %e3 = tensor.empty() : {O}
+    %qkv = hfusion.cast {{round_mode = #hfusion.round_mode<rint>}} ins(%c : {C}) outs(%e3 : {O}) -> {O}
+    %e4 = tensor.empty() : {t["q"]}
+    %a:5 = hfusion.append_kv {{{form}, pairs = 0 : i32}} ins(%qkv, %rot, {batch} : {O}, {R}, {batch_tys}) outs(%e4, %k, %ks, %v, %vs : {t["q"]}, {cache_tys}) -> {t["q"]}, {cache_tys}
+    %o = hfusion.paged_attention {{{form}, scale = {dim ** -0.5:.9e} : f32{more}}} ins(%a#0, %a#1, %a#2, %a#3, %a#4, {batch} : {t["q"]}, {cache_tys}, {batch_tys}) outs(%out : {t["q"]}) -> {t["q"]}
+    return %o, %n#0, %a#1, %a#2, %a#3, %a#4 : {t["q"]}, {X}, {cache_tys}
+  }}
+}}
+"""

@@ -34,6 +34,10 @@ ATTEND = {
 # rows of the groups that are compiled for one row count
 STATIC = {"append": ("usual", 70), "attend": ("usual", 70)}
 # a decoder layer's attention: columns of the residual stream, its cache
+# the un-fused layer as a program
+PROGRAM = dict(rows=20, cols=512, heads=8, kv_heads=2, dim=64, slots=4, room=4096, blocks=300, block=32)
+# a cache whose last blocks lie past byte 2^31, and a small one
+BIG = dict(rows=130, heads=8, kv_heads=8, dim=128, slots=2, room=192, blocks=33000, block=64, few=8)
 LAYER = dict(cols=512, heads=8, kv_heads=2, dim=64, slots=4, room=256, blocks=24, block=32)
 
 
@@ -81,4 +85,18 @@ def entries():
     e["layer_qkv_rt"] = rt(g.w8a8_dequant(_ANY, (LAYER["heads"] + 2 * LAYER["kv_heads"]) * LAYER["dim"], LAYER["cols"]))
     e["layer_append_rt"] = rt(g.append_kv(_ANY, **layer))
     e["layer_attend_rt"] = rt(g.paged_attention(_ANY, **layer))
+    size = {k: v for k, v in PROGRAM.items() if k not in ("rows", "cols")}
+    rows, cols = PROGRAM["rows"], PROGRAM["cols"]
+    e["prog_decoder_attention"] = g.decoder_attention(**PROGRAM)
+    e["part_norm"] = g.rms_norm(rows, cols, out="e4m3")
+    e["part_product"] = g.matmul_mx(rows, (size["heads"] + 2 * size["kv_heads"]) * size["dim"], cols, out="bf16")
+    e["part_append"], e["part_attend"] = g.append_kv(rows, **size), g.paged_attention(rows, **size)
+    big = {k: v for k, v in BIG.items() if k not in ("rows", "few")}
+    for name, blocks in (("big", BIG["blocks"]), ("small", BIG["few"])):
+        e[f"appendkv_{name}"] = g.append_kv(BIG["rows"], **{**big, "blocks": blocks})
+        e[f"pagedattn_{name}"] = g.paged_attention(BIG["rows"], **{**big, "blocks": blocks})
+    for name, scale in (("negative", -0.2), ("zero", 0.0), ("large", 3.0)):
+        e[f"pagedattn_{name}_rt"] = rt(g.paged_attention(_ANY, scale=scale, **_sizes(ATTEND["group4"])))
+    from norm_mx_catalog import untied
+    e["pagedattn_untied"], e["rmsnorm_untied"] = untied(attend("usual", 70)), untied(g.rms_norm(33, 512))
     return e
