@@ -4,10 +4,9 @@
 //   j in (pos - WINDOW, pos] of the row's sequence whose blocks the table has
 // in one pass with the running maximum and sum (f32); a row that sees nothing
 // is zeros.  The matrix core takes 16-bit operands and sums in f32; codes are
-// exact in both types.  Of bf16 queries, p_j times its block's value scale is
-// rounded to bf16.  f16 has not the range for that: p_j is rounded by itself and
-// the codes are scaled to a running reference exponent, exactly; a tile with
-// blocks that lie further apart takes p_j as the sum of two bf16 numbers.
+// exact in both types.  A probability is rounded once to the queries' type, which
+// costs a result some half of a step of its own; its sum takes it unrounded.  Of
+// f16, which has not the range for values' scales, see where they are applied.
 //
 // Transposed products, so that nothing moves between lanes: S^T = K Q^T leaves
 // a lane with four tokens' scores of one row, and these are the B operand of
@@ -250,7 +249,9 @@ template <typename S> __device__ __forceinline__ void paged_step(PagedState<S> &
     }
     return;
   }
-  // the exponents of the blocks that are read
+  // f16: p by itself, and the codes scaled to a running reference exponent; where
+  // a block lies further below it than f16 reaches, p times its scale as the sum
+  // of two bf16 numbers
   const bool read = t.there && at <= hi;
   const bool bad = __any(read && t.vs == 255);
   uint32_t big = read && t.vs != 255 ? t.vs : 0, small = read ? t.vs : 255;
@@ -584,11 +585,12 @@ template <typename S> struct PagedPrompt {
     uint32_t ks, vs; // scale bytes
   };
   // What the tile's values are scaled to: o is in units of 2^(ref - 127), of
-  // about the largest block that is read.  bf16 has the range for blocks 2^100
-  // below it; f16 for 2^8 (DOWN), and what is below that scales p (`more`), which
-  // keeps its 11 bits down to 2^-14 and is 2^-25 off below.
+  // about the largest block of the tile, but no less than 2^-60 of the largest
+  // so far (`peak`; o would pass f32's range).  bf16 has the range for blocks
+  // 2^126 below it; f16 for 2^8 (DOWN), and what is below that scales p (`more`),
+  // which keeps its 11 bits down to 2^-14 and is 2^-25 off below.
   struct Mode {
-    uint32_t ref;
+    uint32_t ref, peak;
     bool more;
   };
   static constexpr uint32_t DOWN = S::EL == EL_BF16 ? 126 : 8;
@@ -626,14 +628,16 @@ template <typename S> struct PagedPrompt {
       }
     }
   }
-  __device__ __forceinline__ Mode mode(const Groups &gr, int tile, uint32_t ref) const {
+  __device__ __forceinline__ Mode mode(const Groups &gr, int tile, const Mode &was) const {
     auto quad = [](uint32_t v) {
       v = max_u32(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true));
       return (uint32_t)__builtin_amdgcn_readfirstlane((int)max_u32(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true)));
     };
     const bool read = gr.block >= 0 && gr.vs != 255 && 64 * tile + 16 * (int)(threadIdx.x % 4) <= hi;
-    const uint32_t big = quad(read ? gr.vs : 0), now = big > ref || (big && big + 4 < ref) ? big : ref;
-    return Mode{now, S::EL != EL_BF16 && quad(read ? now - gr.vs : 0) > DOWN};
+    const uint32_t big = quad(read ? gr.vs : 0), peak = max_u32(was.peak, big);
+    uint32_t now = big > was.ref || (big && big + 4 < was.ref) ? big : was.ref; // (a little lower is near enough)
+    now = now + 60 < peak ? peak - 60 : now;
+    return Mode{now, peak, S::EL != EL_BF16 && quad(read ? now - gr.vs : 0) > DOWN};
   }
   __device__ __forceinline__ void stage(const Groups &gr, const Mode &mo, int tile, int buf) {
     const bool whole = 64 * tile + 63 <= hi && __all(gr.block >= 0);
@@ -674,7 +678,7 @@ template <typename S> struct PagedPrompt {
     const int lane = threadIdx.x % 64, r = lane % 32, half = lane / 32, key = (r & 0x13) | (r & 4) << 1 | (r & 8) >> 1;
     if (mo.ref != ref) {
       const int by = (int)ref - (int)mo.ref;
-      times(u2f((uint32_t)(127 + (by < -126 ? -126 : by > 127 ? 127 : by)) << 23));
+      times(by < -126 ? 0.0f : u2f((uint32_t)(127 + by) << 23)); // (up to 2^60)
       ref = mo.ref;
     }
     v16f s[2] = {};
@@ -807,7 +811,7 @@ template <typename S> struct PagedPrompt {
     m = -__builtin_inff(), sum = 0, ref = 0;
     Groups gr = groups(block(begin));
     load(gr, begin);
-    Mode mo = mode(gr, begin, 0);
+    Mode mo = mode(gr, begin, Mode{0, 0, false});
     int next = block(begin + 1);
     stage(gr, mo, begin, begin & 1);
     __syncthreads();
@@ -821,7 +825,7 @@ template <typename S> struct PagedPrompt {
       __builtin_amdgcn_sched_barrier(0);
       if (64 * i <= seen && (S::WINDOW == 0 || 64 * i + 63 > first - S::WINDOW)) step(gr, mo, i, i & 1, pos, first, last);
       if (i + 1 < end) {
-        mo = mode(gn, i + 1, mo.ref);
+        mo = mode(gn, i + 1, mo);
         stage(gn, mo, i + 1, (i + 1) & 1);
         gr = gn;
       }

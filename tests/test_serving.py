@@ -415,6 +415,9 @@ def attend_batches(c):
     yield [(0, far - 130, 129), (1, 10, 31), (2, 1, 90)], 3, dict(wide=True)
     yield [(0, 0, 17), (2, far - 61, 60), (1, 2 * block, 40)], 0, dict(holes=True)
     yield [(1, far // 2, 75), (0, 3, 64), (2, 0, 1)], 2, dict(nan=True)
+    for slope in (-3, 3):
+        yield [(0, far - 130, 129), (1, 2 * block, 40)], 0, dict(slope=slope)
+        yield [(0, far - 2, 1), (1, 2 * block, 2)], 0, dict(slope=slope)
 
 
 def check_attention(c, outs, q, cache, seq, pos, table, before, scale=None):
@@ -439,12 +442,18 @@ def check_attention(c, outs, q, cache, seq, pos, table, before, scale=None):
     assert (ok | nan).all(), (np.argwhere(~(ok | nan))[:5], np.nanmax(np.abs(got - want)))
 
 
-def attend_case(rng, c, parts, pad, wide=False, holes=False, nan=False):
+def attend_case(rng, c, parts, pad, wide=False, holes=False, nan=False, slope=0):
     hq, hk, d, block, slots, room, blocks, el, fmt, window = c
     seq, pos = batch(parts, pad, slots)
     used = [max([p + n for s2, p, n in parts if s2 == s] or [0]) for s in range(slots)]
     table, free = paged_table(rng, slots, room, block, blocks, used)
     k, ks, v, vs = cache = cache_of(rng, c, wide)
+    if slope:  # values' scales that fall (or rise) from block to block
+        low = 127 - bs.EMAX[fmt]
+        for s, n in enumerate(used):
+            for i in range(-(-n // block)):
+                step = i if slope < 0 else -(-n // block) - i
+                vs[table[s, i]] = max(1, low - abs(slope) * step)
     # memory that no token has come to: NaN codes behind each end, in blocks of nobody
     for s, n in enumerate(used):
         if n % block:
