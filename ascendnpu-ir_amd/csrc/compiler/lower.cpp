@@ -3561,16 +3561,17 @@ void keepsRest(Analysis &A, const Op *op) {
   for (const Value *o : op->outs)
     if (const int t = tiedArgOf(o); t >= 0) A.params[t].role = "inout";
 }
-// blocks = ceil(rows / rowsB) * rowsC, refused where a static count is past what a launch takes
+// blocks = ceil(rows / rowsB) * rowsC of 256 threads; more rows than a launch
+// takes (2^32 threads, and a kernel's index of a row) are refused
 void tileGrid(const Analysis &A, const Op *op, KernelPlan &p, int64_t T, int64_t rowsB, int64_t rowsC) {
+  const int64_t most = std::min<int64_t>(int64_t(1) << 31, ((int64_t(1) << 24) - 1) / rowsC * rowsB);
   if (A.rowsDyn) {
     p.rowsDyn = true;
-    p.rowsA = 1, p.rowsB = rowsB, p.rowsC = rowsC;
+    p.rowsA = 1, p.rowsB = rowsB, p.rowsC = rowsC, p.maxRows = most;
     return;
   }
-  const int64_t blocks = (T + rowsB - 1) / rowsB * rowsC;
-  if (blocks > (int64_t(1) << 30)) unsupported(op, "more rows than a launch takes");
-  p.grid[0] = (unsigned)blocks;
+  if (T > most) unsupported(op, "more rows than a launch takes (" + std::to_string(most) + ")");
+  p.grid[0] = (unsigned)((T + rowsB - 1) / rowsB * rowsC);
 }
 } // namespace
 
@@ -3710,6 +3711,9 @@ static KernelPlan lowerPagedAttention(Analysis &A, const std::string &kname, con
     all.push_back({"pieces", pieces, promptForm + "rows<true>(a, " + rows + ", (char *)ws)", bounds, kPieces, 0, (uint64_t)(kPieces * 128 * (8 + 4 * z.D)),
                    promptForm + "join(a, " + rows + ", (const char *)ws)", "256", 0, kPieceUnits * 4});
   all.push_back({"prompt", int64_t(1) << 31, "", "", 0, 0, 0, promptForm + "rows<false>(a, " + rows + ", nullptr)", bounds, tile, heads});
+  p.block[0] = 256;
+  tileGrid(A, op, p, z.T, tile, heads);
+  p.rowsA = 0; // (each count has its alternative)
   if (!A.rowsDyn) {
     while (all.front().most < z.T) all.erase(all.begin());
     all.resize(1);
@@ -3717,8 +3721,6 @@ static KernelPlan lowerPagedAttention(Analysis &A, const std::string &kname, con
   uint64_t ws = 0;
   for (const Schedule &s : all) ws = std::max(ws, s.ws);
   p.workspaceBytes = ws;
-  p.rowsDyn = A.rowsDyn;
-  p.block[0] = 256;
   for (const Schedule &s : all) {
     int pre = -1;
     if (s.ws) {
@@ -3740,7 +3742,6 @@ static KernelPlan lowerPagedAttention(Analysis &A, const std::string &kname, con
     p.kargs = kargs;
     if (A.rowsDyn) p.alts.push_back({nm, s.most, s.rowsB ? s.rowsB : s.most, s.rowsC, 256, pre >= 0, pre});
     else p.grid[0] = (unsigned)(s.rowsB ? (z.T + s.rowsB - 1) / s.rowsB * s.rowsC : s.rowsC);
-    if (!A.rowsDyn && s.rowsB && (z.T + s.rowsB - 1) / s.rowsB * s.rowsC > (int64_t(1) << 30)) unsupported(op, "more rows than a launch takes");
     p.variant += (p.variant.empty() ? "" : ", ") + std::string(s.name);
   }
   // (what is read of the cache depends on the positions and is not counted)
@@ -5324,6 +5325,7 @@ std::string emitManifest(const KernelPlan &p, const std::string &hsacoName) {
     << "algo_ops " << (uint64_t)p.algoOps << "\n";
   if (p.rowsDyn) s << "rows_dyn " << p.rowsA << " " << p.rowsB << " " << p.rowsC << " " << p.rowsCap << "\n";
   if (p.rowsZero) s << "rows_zero 1\n";
+  if (p.maxRows) s << "max_rows " << p.maxRows << "\n";
   auto indices = [&](const char *key, const std::vector<int> &v) {
     if (v.empty()) return;
     s << key;

@@ -67,6 +67,7 @@ struct KernelPlan {
   // algoBytes is per row.
   bool rowsDyn = false;
   int64_t rowsA = 0, rowsB = 1, rowsC = 1, rowsCap = 0;
+  int64_t maxRows = 0;   // launch-time rows of one launch (0: any number; more are refused)
   bool rowsZero = false; // a launch of no rows has results to write
   std::vector<int> apart; // arguments that no destination may overlap (refused at launch)
   std::vector<int> inplace; // arguments that a destination may be, but not overlap otherwise

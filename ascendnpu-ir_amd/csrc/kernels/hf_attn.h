@@ -391,7 +391,8 @@ template <typename S, int WV> __device__ __forceinline__ void paged_rows(const P
 template <typename S, int WV> struct PagedSplit {
   using U = PagedUnits<S>;
   static constexpr int MOST = 1024, PIECES = 1024, LEAST = 256, SHARED = 768, THREADS = 64 * WV, PER = (MOST + THREADS - 1) / THREADS;
-  static_assert((S::FAR / 64 + 1) * MOST < (int64_t(1) << 31) && (int64_t)MOST * U::HEADS < (int64_t(1) << 30));
+  // (a unit has at most 2^20 tiles, less than the longest `run`)
+  static_assert(S::FAR <= 1 << 26 && (int64_t)MOST * U::HEADS < (int64_t(1) << 30));
   struct Record { // a token (row t, `token` of its unit) of a unit in parts
     int t, token, hh, part, parts, pad[3];
   };
@@ -451,7 +452,10 @@ template <typename S, int WV> struct PagedSplit {
     const int64_t all = (int64_t)sizes[0] * U::HEADS;
     int want = PIECES - sizes[1] * U::HEADS;
     want = want < LEAST ? LEAST : want > SHARED ? SHARED : want;
-    const int run = ((int)((all + want - 1) / want) + WV - 1) / WV * WV; // (every wave as many)
+    // (every wave as many; a batch of padding alone has none)
+    int64_t few = ((all + want - 1) / want + WV - 1) / WV * WV;
+    few = few < WV ? WV : few > 1 << 24 ? 1 << 24 : few;
+    const int run = (int)few;
     // pieces of `run` tiles, shorter ones, tokens of units in parts, and parts, of the thread's rows
     int count[4] = {0, 0, 0, 0}, counts[4];
     auto add = [&](int i) {

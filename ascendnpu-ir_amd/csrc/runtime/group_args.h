@@ -27,6 +27,7 @@ struct GroupArgs {
   std::string func;
   bool rowsDyn = false; // the row count comes with the launch (-1 in the shapes)
   bool rowsZero = false; // a launch of no rows has results to write (manifest `rows_zero 1`)
+  int64_t maxRows = 0; // launch-time rows that the group takes at most (manifest `max_rows`; 0: any number)
   uint64_t wsBytes = 0;
   bool wsZero = false; // zero when first used, and what a launch leaves there the next one reads
   std::vector<std::string> paramRoles;
@@ -55,6 +56,9 @@ struct GroupArgs {
       int z = 0;
       is >> z;
       rowsZero = z != 0;
+    } else if (key == "max_rows") {
+      is >> maxRows;
+      if (maxRows <= 0) is.setstate(std::ios::failbit);
     } else if (key == "param" || key == "result") {
       int i, tied = -1, rank = 0;
       std::string role;
@@ -123,6 +127,7 @@ struct GroupArgs {
     if (nresults != resultTied.size())
       return "group @" + func + " has " + std::to_string(resultTied.size()) + " results, got " + std::to_string(nresults);
     if (nparams && !params) return "null params array";
+    if (maxRows && rows > maxRows) return "group @" + func + " takes at most " + std::to_string(maxRows) + " rows a launch, got " + std::to_string(rows);
     // (a tensor of no rows has no address)
     auto empty = [&](const std::vector<Buf> &bufs, size_t i) {
       return rows == 0 && i < bufs.size() && std::count(bufs[i].shape.begin(), bufs[i].shape.end(), int64_t(-1)) != 0;

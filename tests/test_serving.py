@@ -132,6 +132,20 @@ def test_destinations_apart(folder):
     assert [p["role"] for p in art.blocks[0]["params"]] == ["in"] * 5 + ["inout"] * 5
 
 
+def test_most_rows(folder):
+    """More rows than a launch has workgroups for are refused, not cut short:
+    16 rows (five workgroups) and 64 rows (two heads) a tile, 2^24 workgroups of
+    256 threads less one."""
+    refuse(g.append_kv(1 << 27, 8, 2, 64, 5, 160, 40), "more rows than a launch takes")
+    refuse(g.paged_attention(1 << 29, 4, 2, 64, 5, 160, 40), "more rows than a launch takes")
+    refuse(g.paged_attention(1 << 33, 4, 2, 64, 5, 160, 40), "more rows than a launch takes")
+    for ir, most in ((g.append_kv(7919, 8, 2, 64, 5, 160, 40), (2 ** 24 - 1) // 5 * 16), (g.paged_attention(7919, 4, 2, 64, 5, 160, 40), (2 ** 24 - 1) // 2 * 64)):
+        c = Checked(g.with_dynamic_rows(ir, 7919), folder, options="dyn=runtime", rows=12)
+        assert c.why() == ""
+        c.rows = most + 1
+        assert f"takes at most {most} rows a launch, got {most + 1}" in c.why()
+
+
 def test_oracle_append_in_parts():
     """Tokens appended one by one leave the scales of one append of all, and
     codes within what the roundings on the way cost: a code is rounded at most

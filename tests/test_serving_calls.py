@@ -374,3 +374,60 @@ def test_append_twice(gpu):
     torch.cuda.synchronize()
     for t, w in zip(cache, want[1:]):
         assert np.array_equal(t.view(torch.uint8).cpu().numpy(), w)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["group4", "far", "usual", "many"])
+def test_batches_of_padding(gpu, name):
+    """Rows that are all padding leave everything as it was, and the call behind
+    them has its rows."""
+    import torch
+    note("padding alone " + name)
+    c = sc.ATTEND[name]
+    grp = load(f"pagedattn_{name}_rt")
+    for rows in (1, 9, 300, 1300):
+        case = attend_case(np.random.default_rng(rows), c, [(1, 7, 1)], rows)
+        args = attend_args(c, case, gpu)
+        pad = [t[1:].clone() if i in (0, 5, 6) else t.clone() for i, t in enumerate(args[:-1])] + [torch.full_like(args[-1][1:], 3.0)]
+        grp(*pad)
+        out = grp(*args)
+        torch.cuda.synchronize()
+        assert (pad[-1] == 3.0).all()
+        check_attention(c, to_host(out, c[7]), case[5], case[3], *case[:3], np.zeros(case[5].shape))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("own", [False, True], ids=["one stream", "streams"])
+def test_two_threads(gpu, own):
+    """Calls of one handle from two threads, on one stream or on one each."""
+    import threading
+
+    import torch
+    note(f"two threads {own}")
+    c = sc.ATTEND["far"]
+    grp = load("pagedattn_far_rt")
+    rng = np.random.default_rng(21)
+    args = [attend_args(c, attend_case(rng, c, parts, 2), gpu) for parts in ([(0, 4990, 3), (2, 3000, 1)], [(1, 4000, 150)])]
+    want = []
+    for a in args:
+        want.append(grp(*a).clone())
+        a[-1].zero_()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in args]
+    bad = []
+
+    def calls(i):
+        try:
+            with torch.cuda.stream(streams[i if own else 0]):
+                for _ in range(20):
+                    grp(*args[i])
+                streams[i if own else 0].synchronize()
+        except Exception as e:  # noqa: BLE001
+            bad.append(e)
+    threads = [threading.Thread(target=calls, args=(i,)) for i in range(len(args))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not bad and all(same(a[-1], w) for a, w in zip(args, want))
