@@ -3644,6 +3644,8 @@ constexpr int64_t kSplitShared = 768, kSplitJoin = 1024;
 constexpr int64_t kWholeFar = 2048;
 // Rows that count as groups of tokens whatever the number of sequences.
 constexpr int64_t kPagedFew = 64;
+// Tiles of a prompt's rows that say whether some come a few at a time (PagedFew::TILES).
+constexpr int64_t kPagedFlags = 4096;
 // Pieces of a prompt's units, units up to which it has some, and their shortest
 // length in tiles (PagedPrompt::PIECES, CUT).
 constexpr int64_t kPieces = 1024, kPieceUnits = 512, kPieceTiles = 16;
@@ -3697,20 +3699,23 @@ static KernelPlan lowerPagedAttention(Analysis &A, const std::string &kname, con
     const char *name;
     int64_t most; // rows
     std::string pre, preBounds;
-    int64_t preGrid, prePerRow;
+    int64_t preB, preC, preMore; // its workgroups: ceil(rows / preB) * preC + preMore
     uint64_t ws;
     std::string call, bounds;
     int64_t rowsB, rowsC; // 0: rowsC workgroups
   };
+  // (of a prompt's rows the second launch has those that come a few at a time)
+  const int64_t few = 1024 / heads * heads, flags = 4 * kPagedFlags;
   std::vector<Schedule> all;
   if (split)
-    all.push_back({"parts", split, splitForm + "rows(a, " + rows + ", (char *)ws)", "256, 2", kSplitShared, heads,
+    all.push_back({"parts", split, splitForm + "rows(a, " + rows + ", (char *)ws)", "256, 2", 1, heads, kSplitShared,
                    (uint64_t)(32 + kSplitShared * (32 * N + 2 * GT * N * (8 + 4 * z.D))), splitForm + "join(a, (const char *)ws)", "256", 0, kSplitJoin});
-  if (tokens > split) all.push_back({"units", tokens, "", "", 0, 0, 0, "hf::paged_rows<S, 4>(a, " + rows + ")", "256, 2", 1, heads});
+  if (tokens > split) all.push_back({"units", tokens, "", "", 0, 0, 0, 0, "hf::paged_rows<S, 4>(a, " + rows + ")", "256, 2", 1, heads});
   if (pieces > tokens)
-    all.push_back({"pieces", pieces, promptForm + "rows<true>(a, " + rows + ", (char *)ws)", bounds, kPieces, 0, (uint64_t)(kPieces * 128 * (8 + 4 * z.D)),
-                   promptForm + "join(a, " + rows + ", (const char *)ws)", "256", 0, kPieceUnits * 4});
-  all.push_back({"prompt", int64_t(1) << 31, "", "", 0, 0, 0, promptForm + "rows<false>(a, " + rows + ", nullptr)", bounds, tile, heads});
+    all.push_back({"pieces", pieces, promptForm + "rows<true>(a, " + rows + ", (char *)ws)", bounds, 0, 0, kPieces, (uint64_t)(flags + kPieces * 128 * (8 + 4 * z.D)),
+                   promptForm + "finish<true>(a, " + rows + ", (const char *)ws)", "256, 2", 0, few + kPieceUnits * 4});
+  all.push_back({"prompt", int64_t(1) << 31, promptForm + "rows<false>(a, " + rows + ", (char *)ws)", bounds, tile, heads, 0, (uint64_t)flags,
+                 promptForm + "finish<false>(a, " + rows + ", (const char *)ws)", "256, 2", 0, few});
   p.block[0] = 256;
   tileGrid(A, op, p, z.T, tile, heads);
   p.rowsA = 0; // (each count has its alternative)
@@ -3723,13 +3728,13 @@ static KernelPlan lowerPagedAttention(Analysis &A, const std::string &kname, con
   p.workspaceBytes = ws;
   for (const Schedule &s : all) {
     int pre = -1;
-    if (s.ws) {
+    if (!s.pre.empty()) {
       KernelPlan::PreKernel pk;
       pk.name = kname + "_" + s.name;
       const std::string params = kernelParamList(A, pk.kargs, true);
-      pk.grid = (unsigned)(s.preGrid + (A.rowsDyn ? 0 : z.T * s.prePerRow));
-      pk.perRow = A.rowsDyn ? s.prePerRow : 0;
-      pk.wsBytes = s.ws;
+      pk.grid = (unsigned)(s.preMore + (A.rowsDyn || !s.preB ? 0 : (z.T + s.preB - 1) / s.preB * s.preC));
+      if (A.rowsDyn) pk.rowsB = s.preB, pk.rowsC = s.preC;
+      pk.wsBytes = (int64_t)s.ws;
       pk.block = 256;
       kernel(pk.name, params, s.preBounds, s.pre);
       pre = (int)p.pre.size();
@@ -5349,8 +5354,8 @@ std::string emitManifest(const KernelPlan &p, const std::string &hsacoName) {
     s << "pre " << pk.name << " " << pk.grid << " 1 1 " << pk.block << " 1 1 " << pk.kargs.size();
     for (auto &k : pk.kargs) s << " " << k;
     s << "\n";
-    if (pk.perRow) s << "pre_rows " << pk.perRow << "\n";
-    if (pk.wsBytes) s << "pre_workspace " << pk.wsBytes << "\n";
+    if (pk.rowsB) s << "pre_rows " << pk.rowsB << " " << pk.rowsC << "\n";
+    if (pk.wsBytes >= 0) s << "pre_workspace " << pk.wsBytes << "\n";
   }
   for (auto &a : p.alts)
     s << "alt " << a.name << " " << a.maxRows << " " << a.rowsB << " " << a.rowsC << " " << a.block << (a.pre ? " pre" : "")

@@ -44,8 +44,8 @@ struct KernelPlan {
     std::string name;
     unsigned grid = 1, block = 256;
     std::vector<std::string> kargs;
-    int64_t perRow = 0;   // launch-time rows: blocks a row, besides `grid`
-    uint64_t wsBytes = 0; // what a launch behind this one alone needs of the workspace (0: all)
+    int64_t rowsB = 0, rowsC = 0; // launch-time rows R: ceil(R / rowsB) * rowsC blocks besides `grid` (0: none)
+    int64_t wsBytes = -1; // what a launch behind this one alone needs of the workspace (-1: all)
   };
   std::vector<PreKernel> pre;
   // other kernels of the group for small runtime row counts, by ascending

@@ -90,6 +90,20 @@ template <int EL_, int FMT_, int HQ_, int HK_, int D_, int BLOCK_, int64_t SLOTS
       if (n == i && t + i < T && (p + i) % N != 0 && p + i < FAR && sn[i] == s && pn[i] == p + i) ++n;
     return n;
   }
+  // whether row t, of sequence s at p, is one of at most FEW that follow each
+  // other in the batch (all rows about it are asked for at once)
+  static constexpr int FEW = N > 4 ? N : 4;
+  __device__ static __forceinline__ bool few(const int *seq, const int *pos, int64_t t, int64_t T, int s, int p) {
+    int before = 0, after = 0;
+#pragma unroll
+    for (int i = 1; i <= FEW; ++i) {
+      const int64_t b = t - i < 0 ? 0 : t - i, e = t + i < T ? t + i : T - 1;
+      const bool up = seq[b] == s && pos[b] == p - i, down = seq[e] == s && pos[e] == p + i;
+      before += before == i - 1 && t - i >= 0 && p - i >= 0 && up;
+      after += after == i - 1 && t + i < T && p + i < FAR && down;
+    }
+    return before + after < FEW;
+  }
 };
 
 struct PagedArgs {
@@ -377,6 +391,44 @@ template <typename S, int WV> __device__ __forceinline__ void paged_rows(const P
   paged_part<S, WV>(a, join, t, n, seq, lo, blockIdx.x % U::HEADS, t0, t0 + U::tiles(lo, n), nullptr, nullptr);
 }
 
+// The rows beside a prompt's that come a few at a time (Paged::few): PagedPrompt
+// would take a tile's sequences one after another, a workgroup here takes one
+// unit.  BLOCKS workgroups, each a head and every STEP-th row of the batch, so
+// that neighbours are different workgroups'.  flags: of the first TILES tiles
+// of PagedPrompt, whether they have such rows (of 10495 rows of prompts alone
+// this launch takes 5 us, 7 where each workgroup reads every row's neighbours).
+// us of a call, tokens of 63 sequences of 100 to 8100 positions beside a prompt
+// of 300, 2000 and 4000 rows: 156, 193, 299; the tokens alone 108, the prompts
+// 20, 76, 159.  512 workgroups: three tokens a sequence beside 1000 rows 289,
+// 237 so.
+template <typename S> struct PagedFew {
+  using U = PagedUnits<S>;
+  static constexpr int STEP = 1024 / U::HEADS, BLOCKS = STEP * U::HEADS, TILES = 4096;
+  static_assert(U::HEADS <= 1024);
+  __device__ static __forceinline__ void rows(const PagedArgs &a, int64_t T, const int *flags, int block) {
+    __shared__ __attribute__((aligned(16))) PagedJoin<S, 4> join;
+    __shared__ uint64_t found[4];
+    const int tid = threadIdx.x, hh = block % U::HEADS;
+    for (int64_t base = block / U::HEADS; base < T; base += 256 * STEP) {
+      const int64_t mine = base + tid * STEP, tile = mine / (128 / S::GT);
+      int seq, lo;
+      bool one = mine < T && (tile >= TILES || flags[tile]);
+      if (!__syncthreads_or(one)) continue;
+      one = one && S::tokens(a.seq, a.pos, mine, T, seq, lo) > 0 && S::few(a.seq, a.pos, mine, T, seq, lo);
+      const uint64_t some = __ballot(one);
+      if (tid % 64 == 0) found[tid / 64] = some;
+      __syncthreads();
+      for (int w = 0; w < 4; ++w)
+        for (uint64_t left = found[w]; left; left &= left - 1) {
+          const int64_t t = base + (64 * w + __builtin_ctzll(left)) * STEP;
+          const int n = S::tokens(a.seq, a.pos, t, T, seq, lo), t0 = U::first(lo);
+          paged_part<S, 4>(a, join, t, n, seq, lo, hh, t0, t0 + U::tiles(lo, n), nullptr, nullptr);
+        }
+      __syncthreads(); // (found is written again)
+    }
+  }
+};
+
 // Units of different lengths: one is cut into pieces of at most `run` tiles, a
 // workgroup a piece, the longest first; units of several pieces leave parts,
 // which join() adds in order.  run makes as many pieces as fill the chip with
@@ -569,9 +621,9 @@ template <typename S> struct PagedPrompt {
     else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
   }
   // The order of PRODUCTS products and their reads from LDS: eight reads ahead
-  // (the compiler's own order has two, and waits for most of them), `more` with
-  // other work between them.  8192 rows of 4 prompts: 412 us, 370 so; and with
-  // the waves at their products before those at their scores 360.
+  // (the compiler's own order has two, and waits for most of them), MORE with
+  // other work between them.  10495 rows of four prompts: 412 us, 370 so; and
+  // with the waves at their products before those at their scores 360.
   template <int PRODUCTS, bool MORE> __device__ static __forceinline__ void ahead() {
     constexpr int AHEAD = PRODUCTS < 8 ? PRODUCTS : 8;
     __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0); // LDS reads
@@ -873,15 +925,16 @@ template <typename S> struct PagedPrompt {
   // prompt of 512 rows, whose tiles stay whole, 20.5 and 23.5, of 2048 73.5 and 70;
   // pieces of at least 4, 8 and 12 tiles, 1001 rows over a window of 4096: 63, 61,
   // 64, of 16 53.
-  // ws: the pieces' statistics (two of each of 128 rows), then their rows.
+  // ws: PagedFew's flags, the pieces' statistics (two of each of 128 rows), then
+  // their rows.
   static constexpr int PIECES = 1024, CUT = 16;
   static constexpr float DONE = -1; // (no sum is negative)
   __device__ static __forceinline__ int pieces(int64_t T) {
     const int64_t n = PIECES / (tiles(T) * HEADS);
     return n > 16 ? 16 : n < 1 ? 1 : (int)n;
   }
-  __device__ static __forceinline__ float *stats_of(char *ws, int64_t piece) { return reinterpret_cast<float *>(ws) + piece * 256; }
-  __device__ static __forceinline__ float *part_of(char *ws, int64_t piece) { return reinterpret_cast<float *>(ws) + PIECES * 256 + piece * (128 * S::D); }
+  __device__ static __forceinline__ float *stats_of(char *ws, int64_t piece) { return reinterpret_cast<float *>(ws) + PagedFew<S>::TILES + piece * 256; }
+  __device__ static __forceinline__ float *part_of(char *ws, int64_t piece) { return stats_of(ws, PIECES) + piece * (128 * S::D); }
 
   // grid: tiles(T) * HEADS, PARTS: PIECES; the last rows, which see most, first
   template <bool PARTS> __device__ static __forceinline__ void rows(const PagedArgs &a, int64_t T, char *ws) {
@@ -891,6 +944,7 @@ template <typename S> struct PagedPrompt {
     const int64_t t0 = (tiles(T) - 1 - (blockIdx.x - piece * units) / HEADS) * TOKENS;
     const int hh = (int)(blockIdx.x - piece * units) % HEADS, h = hh / S::GTILES, gt = hh % S::GTILES, lane = threadIdx.x % 64;
     const int tokens = (int)(T - t0 < TOKENS ? T - t0 : TOKENS);
+    int few = 0;
     for (int at = 0; at < tokens;) {
       const int64_t t = t0 + at;
       const int s = a.seq[t], p = a.pos[t];
@@ -906,20 +960,33 @@ template <typename S> struct PagedPrompt {
         const uint64_t other = __ballot(!(i < tokens - at && p + i < S::FAR && a.seq[t + i] == s && a.pos[t + i] == p + i));
         if (n == k) n += other ? __builtin_ctzll(other) : 64;
       }
+      if (n <= S::FEW && S::few(a.seq, a.pos, t, T, s, p)) { // PagedFew's
+        if (PARTS && piece == 0)
+          for (int i = threadIdx.x; i < n * S::GT; i += 256) stats_of(ws, blockIdx.x)[2 * (at * S::GT + i) + 1] = DONE;
+        at += n, few = 1;
+        continue;
+      }
       PagedPrompt{a, lds, s, h, p, p + n - 1}.template run<PARTS>(t0, t, n, gt, piece, cuts, PARTS ? part_of(ws, blockIdx.x) : nullptr,
                                                                  PARTS ? stats_of(ws, blockIdx.x) : nullptr);
       at += n;
     }
+    if (piece == 0 && hh == 0 && threadIdx.x == 0 && t0 / TOKENS < PagedFew<S>::TILES) reinterpret_cast<int *>(ws)[t0 / TOKENS] = few;
   }
 
-  // The rows' pieces added in order, eight lanes a row: grid PIECES / 2 * 4, a
-  // quarter of a unit's rows each.
-  __device__ static __forceinline__ void join(const PagedArgs &a, int64_t T, const char *ws_) {
+  // The second launch: PagedFew's workgroups, and PARTS behind them PIECES / 2 *
+  // 4 that add the rows' pieces in order, eight lanes a row, a quarter of a
+  // unit's rows each.
+  template <bool PARTS> __device__ static __forceinline__ void finish(const PagedArgs &a, int64_t T, const char *ws_) {
+    const int block = (int)blockIdx.x - PagedFew<S>::BLOCKS;
+    if (block < 0) return PagedFew<S>::rows(a, T, reinterpret_cast<const int *>(ws_), (int)blockIdx.x);
+    if constexpr (PARTS) join(a, T, ws_, block);
+  }
+  __device__ static __forceinline__ void join(const PagedArgs &a, int64_t T, const char *ws_, int block) {
     char *ws = const_cast<char *>(ws_);
-    const int cuts = pieces(T), unit = blockIdx.x / 4, hh = unit % HEADS, h = hh / S::GTILES, gt = hh % S::GTILES;
+    const int cuts = pieces(T), unit = block / 4, hh = unit % HEADS, h = hh / S::GTILES, gt = hh % S::GTILES;
     const int64_t t0 = (tiles(T) - 1 - unit / HEADS) * TOKENS, units = tiles(T) * HEADS;
     if (t0 < 0) return;
-    const int row = blockIdx.x % 4 * 32 + threadIdx.x / 8, tok = row / S::GT, head = gt * 16 + row % S::GT;
+    const int row = block % 4 * 32 + threadIdx.x / 8, tok = row / S::GT, head = gt * 16 + row % S::GT;
     if (row >= TOKENS * S::GT || t0 + tok >= T || head >= S::G || !S::inside(a.seq[t0 + tok], a.pos[t0 + tok])) return;
     auto piece = [&](int i) { return i * units + unit; };
     if (stats_of(ws, piece(0))[2 * row + 1] == DONE) return;

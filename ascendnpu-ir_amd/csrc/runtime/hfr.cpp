@@ -41,8 +41,8 @@ struct PreLaunch {
   std::string kernel;
   hipFunction_t fn = nullptr;
   hfr_launch_cfg cfg{};
-  int64_t perRow = 0;   // at launch-time rows: blocks a row, besides the grid's own
-  uint64_t wsBytes = 0; // what a launch behind this one alone needs of the workspace (0: all)
+  int64_t rowsB = 0, rowsC = 0; // at R launch-time rows ceil(R / rowsB) * rowsC blocks besides the grid's own
+  int64_t wsBytes = -1; // what a launch behind this one alone needs of the workspace (-1: all)
   std::vector<Karg> kargs;
 };
 
@@ -187,20 +187,22 @@ int parseBlock(const std::vector<std::string> &lines, hfr_group &g) {
         if (!parseKarg(k, a)) return fail(HFR_ERR_MANIFEST, "bad karg '" + k + "'");
         pl.kargs.push_back(a);
       }
-      if (!pl.cfg.grid[0] || !pl.cfg.block[0]) return fail(HFR_ERR_MANIFEST, "pre kernel without launch shape");
+      if (!pl.cfg.block[0]) return fail(HFR_ERR_MANIFEST, "pre kernel without launch shape");
       g.pre.push_back(pl);
     }
     else if (key == "pre_rows") {
-      // pre_rows <blocks a row>: of the pre kernel before it, besides its grid
-      int64_t n = 0;
-      is >> n;
-      if (is.fail() || n <= 0 || g.pre.empty() || !g.rowsDyn) return fail(HFR_ERR_MANIFEST, "bad pre_rows line: " + ln);
-      g.pre.back().perRow = n;
+      // pre_rows <rows> <blocks for as many>: of the pre kernel before it, besides its grid
+      int64_t b = 0, c = 0;
+      is >> b >> c;
+      if (is.fail() || b <= 0 || c <= 0 || g.pre.empty() || !g.rowsDyn) return fail(HFR_ERR_MANIFEST, "bad pre_rows line: " + ln);
+      g.pre.back().rowsB = b, g.pre.back().rowsC = c;
     }
     else if (key == "pre_workspace") {
       // pre_workspace <bytes>: of a launch behind the pre kernel before it alone
-      is >> (g.pre.empty() ? g.wsBytes : g.pre.back().wsBytes);
-      if (is.fail() || g.pre.empty() || g.pre.back().wsBytes > g.wsBytes) return fail(HFR_ERR_MANIFEST, "bad pre_workspace line: " + ln);
+      int64_t n = -1;
+      is >> n;
+      if (!g.pre.empty()) g.pre.back().wsBytes = n;
+      if (is.fail() || g.pre.empty() || n < 0 || (uint64_t)n > g.wsBytes) return fail(HFR_ERR_MANIFEST, "bad pre_workspace line: " + ln);
     }
     else if (key == "alt") {
       // alt <kernel> <max rows> <rows per block row> <blocks per block row> <threads> [pre [n]]
@@ -237,8 +239,10 @@ int parseBlock(const std::vector<std::string> &lines, hfr_group &g) {
     return (int)HFR_OK;
   };
   int rc = check(g.kargs);
-  for (auto &pl : g.pre)
+  for (auto &pl : g.pre) {
+    if (!pl.cfg.grid[0] && !pl.rowsC) return fail(HFR_ERR_MANIFEST, "pre kernel without launch shape");
     if (!rc) rc = check(pl.kargs);
+  }
   return rc;
 }
 
@@ -364,7 +368,7 @@ const RowAlt *altFor(const hfr_group *g, int64_t rows) {
 uint64_t workspaceOf(const hfr_group *g, int64_t rows) {
   if (g->rowsDyn && rows == 0 && !g->rowsZero) return 0;
   const RowAlt *alt = altFor(g, rows);
-  if (alt && alt->only >= 0 && g->pre[alt->only].wsBytes) return g->pre[alt->only].wsBytes;
+  if (alt && alt->only >= 0 && g->pre[alt->only].wsBytes >= 0) return (uint64_t)g->pre[alt->only].wsBytes;
   return alt && !alt->pre ? 0 : g->wsBytes;
 }
 
@@ -399,7 +403,7 @@ int launchGroup(const hfr_group *g, const uint64_t *params, void *const *results
     for (const PreLaunch &pl : g->pre) {
       if (only >= 0 && &pl != &g->pre[only]) continue;
       hfr_launch_cfg cfg = pl.cfg;
-      if (pl.perRow) cfg.grid[0] += (unsigned)(rows * pl.perRow);
+      if (pl.rowsB) cfg.grid[0] += (unsigned)((rows + pl.rowsB - 1) / pl.rowsB * pl.rowsC);
       const int rc = launch(pl.fn, cfg, pl.kargs);
       if (rc) return rc;
     }

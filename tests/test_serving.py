@@ -417,6 +417,7 @@ def attend_batches(c):
         yield [(s, (s * 37) % 190, 1 + s % 6) for s in range(slots)], 3, {}
         yield [(s, (s * 37) % 190, 7) for s in range(slots)], 0, {}
         yield [(s, 1 + s % 20, 1) for s in range(slots - 1)] + [(slots - 1, 4000, 3)], 0, {}
+        yield [(s, 1 + s % 190, 1) for s in range(slots - 1)] + [(slots - 1, 900, 1200)], 0, {}
         return
     far = min(room, 5000)
     yield [(0, 0, 1)], 0, {}
@@ -429,6 +430,9 @@ def attend_batches(c):
     yield [(0, far - 130, 129), (1, 10, 31), (2, 1, 90)], 3, dict(wide=True)
     yield [(0, 0, 17), (2, far - 61, 60), (1, 2 * block, 40)], 0, dict(holes=True)
     yield [(1, far // 2, 75), (0, 3, 64), (2, 0, 1)], 2, dict(nan=True)
+    # single tokens and short runs beside prompts, over the tiles' ends
+    yield [(1, 7, 1), (0, 3, 30), (2, far // 4, 4), (1, 9, 3), (0, far - 90, 90), (2, far // 4 + 9, 1)], 2, {}
+    yield [(0, 0, 1), (1, far - 1, 1), (2, 30, 16), (1, 2, 17), (0, far // 8, 5), (2, 1, 59), (1, far // 3, 2)], 0, dict(wide=True)
     for slope in (-3, 3):
         yield [(0, far - 130, 129), (1, 2 * block, 40)], 0, dict(slope=slope)
         yield [(0, far - 2, 1), (1, 2 * block, 2)], 0, dict(slope=slope)

@@ -41,10 +41,11 @@ def test_manifests():
         text = open(hf.compile(cat.get(name), options="dyn=runtime").manifest).read()
         return [ln.split() for ln in text.splitlines() if ln.startswith("alt ")], text
     a, text = alts("pagedattn_usual_rt")
-    assert [(x[1].rsplit("_", 1)[1], x[2], x[6:]) for x in a] == [("parts", "64", ["pre", "0"]), ("pieces", "2048", ["pre", "1"]), ("attention", str(1 << 31), [])]
-    assert text.count("pre_rows 8\n") == 1 and text.count("pre_workspace ") == 2
+    assert [(x[1].rsplit("_", 1)[1], x[2], x[6:]) for x in a] == [("parts", "64", ["pre", "0"]), ("pieces", "2048", ["pre", "1"]), ("attention", str(1 << 31), ["pre", "2"])]
+    # (prompts in whole units leave a word a tile)
+    assert text.count("pre_rows 1 8\n") == text.count("pre_rows 32 8\n") == text.count("pre_workspace 16384\n") == 1 and text.count("pre_workspace ") == 3
     a, text = alts("pagedattn_group4_rt")  # a short context: nothing in pieces
-    assert [x[1].rsplit("_", 1)[1] for x in a] == ["units", "attention"] and "workspace 0 0" in text
+    assert [x[1].rsplit("_", 1)[1] for x in a] == ["units", "attention"] and "workspace 16384 0" in text
     a, _ = alts("pagedattn_many_rt")  # more groups of tokens than are dealt out
     assert [(x[1].rsplit("_", 1)[1], int(x[2])) for x in a][:2] == [("parts", 1024), ("units", 1200)]
     a, _ = alts("appendkv_usual_rt")
