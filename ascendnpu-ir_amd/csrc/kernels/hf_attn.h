@@ -47,6 +47,13 @@ template <int EL> __device__ __forceinline__ v4i attn_round8(const float *p) {
   }
   return o;
 }
+// c and the two 16-bit numbers in w (none: neither)
+template <int EL> __device__ __forceinline__ float attn_sum2(int w, bool none, float c) {
+  using T = std::conditional_t<EL == EL_BF16, __bf16, _Float16>;
+  typedef T t2 __attribute__((ext_vector_type(2)));
+  if constexpr (EL == EL_BF16) return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(t2, w), __builtin_bit_cast(t2, 0x3F803F80), c, false);
+  else return __builtin_amdgcn_fdot2(__builtin_bit_cast(t2, w), __builtin_bit_cast(t2, none ? 0 : 0x3C003C00), c, false);
+}
 // the value of the lane 16 or 32 lanes away, combined with this one's
 template <int BY, typename F> __device__ __forceinline__ float with_lane(float v, F f) {
   typedef unsigned u2 __attribute__((ext_vector_type(2)));
@@ -749,36 +756,40 @@ template <typename S> struct PagedPrompt {
     constexpr int GS = S::BLOCK >= 64 ? 1 : 4; // groups of tokens whose blocks may differ
     float f[GS];
     uint32_t there = 0;
+    bool odd = false; // (a factor that is zero or NaN, with which -inf is no zero)
 #pragma unroll
     for (int g = 0; g < GS; ++g) {
       // (a block of values that are NaN makes NaN of the rows that see it: by their scores)
       const uint32_t ks = (uint32_t)__builtin_amdgcn_readlane((int)gr.ks, g), vs = (uint32_t)__builtin_amdgcn_readlane((int)gr.vs, g);
       f[g] = __builtin_fabsf(a.scale) * mx_scale(vs == 255 ? 255 : ks);
+      odd |= !(f[g] > 0);
       there |= (uint32_t)(__builtin_amdgcn_readlane(gr.block, g) >= 0) << g;
     }
     const bool whole = there == (1u << GS) - 1 && 64 * tile + 63 <= first && (S::WINDOW == 0 || 64 * tile > last - S::WINDOW);
     // (tokens by their distance from the lane's first: compares with constants)
     const int to = pos - (64 * tile + 8 * half), from = to - S::WINDOW;
-    auto sees = [&](int u, int i) {
-      const int at = 32 * u + i / 8 * 16 + i % 8;
-      return (there >> ((2 * u + i / 8) * GS / 4) & 1) && at <= to && (S::WINDOW == 0 || at > from);
-    };
-    if (!whole) {
+    auto hide = [&](float with) {
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[u][i] = sees(u, i) ? s[u][i] : -__builtin_inff();
-    }
+        for (int g = 0; g < 2; ++g) {
+          const int end = there >> ((2 * u + g) * GS / 4) & 1 ? to : -1;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int at = 32 * u + 16 * g + i;
+            s[u][8 * g + i] = at <= end && (S::WINDOW == 0 || at > from) ? s[u][8 * g + i] : with;
+          }
+        }
+    };
+    if (!whole) hide(-__builtin_inff());
     float top = -__builtin_inff();
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int g = 0; g < GS; ++g) {
+      float t = -__builtin_inff();
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        float t = s[u][8 * g];
-#pragma unroll
-        for (int i = 1; i < 8; ++i) t = __builtin_fmaxf(t, s[u][8 * g + i]);
-        top = __builtin_fmaxf(top, t * f[(2 * u + g) * GS / 4]); // (f is not negative)
-      }
+      for (int i = 32 / GS * g; i < 32 / GS * (g + 1); i += 2) t = __builtin_fmaxf(__builtin_fmaxf(t, s[i / 16][i % 16]), s[i / 16][i % 16 + 1]);
+      top = __builtin_fmaxf(top, t * f[g]); // (f is not negative)
+    }
     top = with_lane<32>(top, max2);
     if (__any(top > m + 6.0f)) {
       const float now = __builtin_fmaxf(m, top), was = m == now ? 1.0f : __builtin_amdgcn_exp2f(m - now);
@@ -791,19 +802,14 @@ template <typename S> struct PagedPrompt {
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[u][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], f[(2 * u + i / 8) * GS / 4], -mu));
-    if (!whole) { // (a scale may be zero, or NaN)
+    if (odd && !whole) hide(0.0f);
+    if (mo.more) { // (what is rounded is not p: no sum of the rounded)
+      float part[4] = {0, 0, 0, 0};
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[u][i] = sees(u, i) ? s[u][i] : 0.0f;
-    }
-    float part[4] = {0, 0, 0, 0}; // (no long chain of additions)
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) part[i % 4] += s[u][i];
-    sum += (part[0] + part[1]) + (part[2] + part[3]);
-    if (mo.more) {
+        for (int i = 0; i < 16; ++i) part[i % 4] += s[u][i];
+      sum += (part[0] + part[1]) + (part[2] + part[3]);
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -815,6 +821,9 @@ template <typename S> struct PagedPrompt {
           for (int i = 0; i < 8; ++i) s[u][8 * g + i] *= by;
         }
     }
+    // (the sum of the rounded, what the values are multiplied by: half the
+    // additions, and its rounding and theirs go together)
+    float part[4] = {0, 0, 0, 0};
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -823,10 +832,13 @@ template <typename S> struct PagedPrompt {
       for (int i = 0; i < 8; ++i) p[i] = s[k / 2][8 * (k % 2) + i];
       const v4i pf = attn_round8<S::EL>(p);
 #pragma unroll
+      for (int w = 0; w < 4; ++w) part[w] = attn_sum2<S::EL>(pf[w], mo.more, part[w]);
+#pragma unroll
       for (int dt = 0; dt < OT; ++dt) o[dt] = mfma(*reinterpret_cast<const v4i *>(&lds.v[buf][(32 * dt + r) * VP + 16 * k + 8 * half]), pf, o[dt]);
     }
     ahead<4 * OT, true>();
     __builtin_amdgcn_s_setprio(0);
+    sum += (part[0] + part[1]) + (part[2] + part[3]);
   }
 
   // Rows t .. t + n - 1, of a sequence's positions lo .. hi; t0: the tile's first
