@@ -615,6 +615,17 @@ template <typename S, int WV> struct PagedSplit {
 // is the token with bits 2 and 3 of r exchanged.
 // The running maximum is only raised, and what is summed only scaled, when a
 // row's new scores exceed it by 2^6: numbers up to that are as good as up to 1.
+//
+// A tile's two halves of 32 tokens go through in turn, so that a half's
+// exponentials have products of the other beside them, and each product's
+// operand is read one stage ahead: scores of the first half; those of the
+// second beside the first's exponentials; the first's values beside the
+// second's exponentials; the second's values.  10495 rows of four prompts (276
+// Gflop) take 342 us, 805 Tflop/s; both halves at once 355, reads ordered by
+// the compiler 412.  A large library product of bf16 reaches 1215 on this card.
+// A SIMD's two waves have some 250 vector instructions for each 32 products,
+// which issue half the time, the matrix core 35 to 40 %; a third of a wave's
+// time goes to waits and barriers.
 template <typename S> struct PagedPrompt {
   static constexpr int TOKENS = 128 / S::GT, HEADS = S::HK * S::GTILES, KP = S::D + 8, VP = 64 + 8;
   static constexpr int CHUNKS = 4 * S::D, N = (CHUNKS + 255) / 256; // 16-byte pieces of a tile's keys, a thread
@@ -626,21 +637,6 @@ template <typename S> struct PagedPrompt {
   __device__ static __forceinline__ v16f mfma(v4i a, v4i b, v16f c) {
     if constexpr (S::EL == EL_BF16) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
     else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
-  }
-  // The order of PRODUCTS products and their reads from LDS: eight reads ahead
-  // (the compiler's own order has two, and waits for most of them), MORE with
-  // other work between them.  10495 rows of four prompts: 412 us, 370 so; and
-  // with the waves at their products before those at their scores 360.
-  template <int PRODUCTS, bool MORE> __device__ static __forceinline__ void ahead() {
-    constexpr int AHEAD = PRODUCTS < 8 ? PRODUCTS : 8;
-    __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0); // LDS reads
-#pragma unroll
-    for (int c = 0; c < PRODUCTS - AHEAD; ++c) {
-      __builtin_amdgcn_sched_group_barrier(0x8, 1, 0); // matrix core
-      if (MORE) __builtin_amdgcn_sched_group_barrier(0x2, 4, 0); // other arithmetic
-      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-    }
-    __builtin_amdgcn_sched_group_barrier(0x8, AHEAD, 0);
   }
   // a tile's four groups of 16 tokens, group lane % 4 in a lane
   struct Groups {
@@ -744,15 +740,6 @@ template <typename S> struct PagedPrompt {
       times(by < -126 ? 0.0f : u2f((uint32_t)(127 + by) << 23)); // (up to 2^60)
       ref = mo.ref;
     }
-    v16f s[2] = {};
-    __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-    for (int c = 0; c < QF; ++c)
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-        s[u] = mfma(*reinterpret_cast<const v4i *>(&lds.k[buf][(32 * u + key) * KP + 16 * c + 8 * half]), q[c], s[u]);
-    ahead<2 * QF, false>();
-    __builtin_amdgcn_s_setprio(0);
     constexpr int GS = S::BLOCK >= 64 ? 1 : 4; // groups of tokens whose blocks may differ
     float f[GS];
     uint32_t there = 0;
@@ -768,50 +755,51 @@ template <typename S> struct PagedPrompt {
     const bool whole = there == (1u << GS) - 1 && 64 * tile + 63 <= first && (S::WINDOW == 0 || 64 * tile > last - S::WINDOW);
     // (tokens by their distance from the lane's first: compares with constants)
     const int to = pos - (64 * tile + 8 * half), from = to - S::WINDOW;
-    auto hide = [&](float with) {
+    v16f s[2] = {};
+    auto hide = [&](int u, float with) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int g = 0; g < 2; ++g) {
+        const int end = there >> ((2 * u + g) * GS / 4) & 1 ? to : -1;
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          const int end = there >> ((2 * u + g) * GS / 4) & 1 ? to : -1;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int at = 32 * u + 16 * g + i;
-            s[u][8 * g + i] = at <= end && (S::WINDOW == 0 || at > from) ? s[u][8 * g + i] : with;
-          }
+        for (int i = 0; i < 8; ++i) {
+          const int at = 32 * u + 16 * g + i;
+          s[u][8 * g + i] = at <= end && (S::WINDOW == 0 || at > from) ? s[u][8 * g + i] : with;
         }
+      }
     };
-    if (!whole) hide(-__builtin_inff());
-    float top = -__builtin_inff();
+    // scores of half u: hidden, and the maximum raised where it has to be
+    auto scored = [&](int u) {
+      if (!whole) hide(u, -__builtin_inff());
+      float top = -__builtin_inff();
 #pragma unroll
-    for (int g = 0; g < GS; ++g) {
-      float t = -__builtin_inff();
+      for (int g = 0; g < (GS + 1) / 2; ++g) {
+        constexpr int W = GS == 1 ? 16 : 8;
+        float t = -__builtin_inff();
 #pragma unroll
-      for (int i = 32 / GS * g; i < 32 / GS * (g + 1); i += 2) t = __builtin_fmaxf(__builtin_fmaxf(t, s[i / 16][i % 16]), s[i / 16][i % 16 + 1]);
-      top = __builtin_fmaxf(top, t * f[g]); // (f is not negative)
-    }
-    top = with_lane<32>(top, max2);
-    if (__any(top > m + 6.0f)) {
-      const float now = __builtin_fmaxf(m, top), was = m == now ? 1.0f : __builtin_amdgcn_exp2f(m - now);
-      m = now;
-      sum *= was;
-      times(was);
-    }
-    const float mu = m == -__builtin_inff() ? 0.0f : m; // (a row that has seen nothing)
+        for (int i = W * g; i < W * (g + 1); i += 2) t = __builtin_fmaxf(__builtin_fmaxf(t, s[u][i]), s[u][i + 1]);
+        top = __builtin_fmaxf(top, t * f[GS == 1 ? 0 : 2 * u + g]); // (f is not negative)
+      }
+      top = with_lane<32>(top, max2);
+      if (__any(top > m + 6.0f)) {
+        const float now = __builtin_fmaxf(m, top), was = m == now ? 1.0f : __builtin_amdgcn_exp2f(m - now);
+        m = now;
+        sum *= was;
+        times(was);
+        if (u == 1) s[0] *= was; // (probabilities by now)
+      }
+    };
+    float part[4] = {0, 0, 0, 0};
+    // probabilities of half u, a share of them; then what the values are multiplied by
+    float mu = 0;
+    auto exps = [&](int u, int c) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[u][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], f[(2 * u + i / 8) * GS / 4], -mu));
-    if (odd && !whole) hide(0.0f);
-    if (mo.more) { // (what is rounded is not p: no sum of the rounded)
-      float part[4] = {0, 0, 0, 0};
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int i = 16 * c / QF; i < 16 * (c + 1) / QF; ++i) s[u][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], f[GS == 1 ? 0 : 2 * u + i / 8], -mu));
+    };
+    auto rounded = [&](int u, v4i (&pf)[2]) {
+      if (odd && !whole) hide(u, 0.0f);
+      if (mo.more) { // (what is rounded is not p: no sum of the rounded)
 #pragma unroll
         for (int i = 0; i < 16; ++i) part[i % 4] += s[u][i];
-      sum += (part[0] + part[1]) + (part[2] + part[3]);
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
           const uint32_t vs = (uint32_t)__builtin_amdgcn_readlane((int)gr.vs, 2 * u + g), down = ref - vs;
@@ -820,23 +808,57 @@ template <typename S> struct PagedPrompt {
 #pragma unroll
           for (int i = 0; i < 8; ++i) s[u][8 * g + i] *= by;
         }
-    }
-    // (the sum of the rounded, what the values are multiplied by: half the
-    // additions, and its rounding and theirs go together)
-    float part[4] = {0, 0, 0, 0};
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        float p[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[i] = s[u][8 * k + i];
+        pf[k] = attn_round8<S::EL>(p);
+        // (the sum of the rounded: half the additions, and its rounding and that
+        // of what the values are multiplied by go together)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) part[w] = attn_sum2<S::EL>(pf[k][w], mo.more, part[w]);
+      }
+    };
+    auto keys = [&](int u, int c) { return *reinterpret_cast<const v4i *>(&lds.k[buf][(32 * u + key) * KP + 16 * c + 8 * half]); };
+    auto values = [&](int u, int c) { return *reinterpret_cast<const v4i *>(&lds.v[buf][(32 * (c % OT) + r) * VP + 32 * u + 16 * (c / OT) + 8 * half]); };
+    auto limit = [] { __builtin_amdgcn_sched_barrier(0); };
+    v4i w[QF], pf[2];
+#pragma unroll
+    for (int c = 0; c < QF; ++c) w[c] = keys(0, c);
+    limit();
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      float p[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) p[i] = s[k / 2][8 * (k % 2) + i];
-      const v4i pf = attn_round8<S::EL>(p);
-#pragma unroll
-      for (int w = 0; w < 4; ++w) part[w] = attn_sum2<S::EL>(pf[w], mo.more, part[w]);
-#pragma unroll
-      for (int dt = 0; dt < OT; ++dt) o[dt] = mfma(*reinterpret_cast<const v4i *>(&lds.v[buf][(32 * dt + r) * VP + 16 * k + 8 * half]), pf, o[dt]);
+    for (int c = 0; c < QF; ++c) {
+      s[0] = mfma(w[c], q[c], s[0]);
+      w[c] = keys(1, c);
+      limit();
     }
-    ahead<4 * OT, true>();
+    __builtin_amdgcn_s_setprio(0);
+    scored(0);
+    mu = m == -__builtin_inff() ? 0.0f : m; // (a row that has seen nothing)
+#pragma unroll
+    for (int c = 0; c < QF; ++c) {
+      s[1] = mfma(w[c], q[c], s[1]);
+      w[c] = values(0, c);
+      exps(0, c);
+      limit();
+    }
+    scored(1);
+    mu = m == -__builtin_inff() ? 0.0f : m;
+    rounded(0, pf);
+#pragma unroll
+    for (int c = 0; c < QF; ++c) {
+      o[c % OT] = mfma(w[c], pf[c / OT], o[c % OT]);
+      w[c] = values(1, c);
+      exps(1, c);
+      limit();
+    }
+    rounded(1, pf);
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int c = 0; c < QF; ++c) o[c % OT] = mfma(w[c], pf[c / OT], o[c % OT]);
     __builtin_amdgcn_s_setprio(0);
     sum += (part[0] + part[1]) + (part[2] + part[3]);
   }
@@ -932,17 +954,18 @@ template <typename S> struct PagedPrompt {
   __device__ static __forceinline__ int64_t tiles(int64_t T) { return (T + TOKENS - 1) / TOKENS; }
   // The units of a tile and a head in `pieces` pieces each, first all units'
   // first ones: few units leave most of the chip idle, and those of a prompt's
-  // last rows take longest.  us of a call, whole and in pieces of at least 16
-  // tiles: 512 rows behind 7000 positions 226 and 105, 64 behind 8000 244 and 55; a
-  // prompt of 512 rows, whose tiles stay whole, 20.5 and 23.5, of 2048 73.5 and 70;
-  // pieces of at least 4, 8 and 12 tiles, 1001 rows over a window of 4096: 63, 61,
-  // 64, of 16 53.
+  // last rows take longest.  us of a call: 512 rows behind 7000 positions whole
+  // 226, in eight pieces 107, in four, which all run at once, 92; two times 900
+  // rows behind 4000 and 7000 whole 336, in two pieces 300; a prompt of 2048 whole
+  // 73.5, in two 70; 1001 rows over a window of 4096 in pieces of at least 4, 8 and
+  // 12 tiles 63, 61, 64, of 16 53.
   // ws: PagedFew's flags, the pieces' statistics (two of each of 128 rows), then
   // their rows.
   static constexpr int PIECES = 1024, CUT = 16;
   static constexpr float DONE = -1; // (no sum is negative)
   __device__ static __forceinline__ int pieces(int64_t T) {
-    const int64_t n = PIECES / (tiles(T) * HEADS);
+    // (four and more that all run at once, or twice as many workgroups as do)
+    const int64_t units = tiles(T) * HEADS, once = PIECES / 2 / units, n = once >= 4 ? once : PIECES / units;
     return n > 16 ? 16 : n < 1 ? 1 : (int)n;
   }
   __device__ static __forceinline__ float *stats_of(char *ws, int64_t piece) { return reinterpret_cast<float *>(ws) + PagedFew<S>::TILES + piece * 256; }
