@@ -5,8 +5,13 @@
 // in one pass with the running maximum and sum (f32); a row that sees nothing
 // is zeros.  The matrix core takes 16-bit operands and sums in f32; codes are
 // exact in both types.  A probability is rounded once to the queries' type, which
-// costs a result some half of a step of its own; its sum takes it unrounded.  Of
-// f16, which has not the range for values' scales, see where they are applied.
+// costs a result some half of a step of its own; the sum of a few tokens' row takes
+// it unrounded, of a prompt's rounded.  Of f16, which has not the range for
+// values' scales, see where they are applied.
+//
+// Which kernel by the row count (the compiler has the bounds and both sides'
+// times): up to a group of tokens a sequence, rows of a few tokens, whose cost is
+// the cache's bytes; more of them a prompt's rows, whose cost is arithmetic.
 //
 // Transposed products, so that nothing moves between lanes: S^T = K Q^T leaves
 // a lane with four tokens' scores of one row, and these are the B operand of
@@ -313,7 +318,12 @@ template <typename S> __device__ __forceinline__ void paged_step(PagedState<S> &
 // ---------------------------------------------------------------- rows of a few tokens
 // A unit is the rows of one group of tokens and one kv head (of a group of more
 // than 16 query heads, 16 of them); its tiles are those that hold a visible
-// position.
+// position.  16-row products: a kv head's query heads share its codes, and the
+// tokens of a sequence that follow each other.  Memory bounds long caches: one
+// row over 32768 positions 19.9 us (67 MB; 16.9 of it the pieces at 4.0 TB/s, 4
+// the join), 48 rows over up to 8100 85.7 (405 MB, 4.7 TB/s).  Eight sequences of
+// four tokens over up to 500 positions take 7.4: positions, table, codes and
+// eight tiles in a row for the longest, each waiting for the one before.
 template <typename S> struct PagedUnits {
   static constexpr int HEADS = S::HK * S::GTILES, ROWS = S::GT * S::N, CH = S::D / 8;
   __device__ static __forceinline__ int first(int lo) { return S::WINDOW && lo >= S::WINDOW ? (lo - S::WINDOW + 1) / 64 : 0; }

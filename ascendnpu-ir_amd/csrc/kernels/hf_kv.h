@@ -112,6 +112,16 @@ template <int FMT> __device__ __forceinline__ u32x2 kv_rescale(u32x2 w, uint32_t
 // tile's other QB workgroups its queries, HB heads a thread that turn alike.
 // Rows with a sequence or position out of range, and blocks out of range, are
 // left alone.
+// A block's rows are read once, kept in registers until its largest magnitude is
+// known, and written as codes (values turned around in LDS, so that a channel's
+// tokens leave together); codes that are there already are read again only where
+// the scale grows.  No atomics: a block has one owner.  Memory bounds long
+// batches: three prompts, 8561 rows of 32 heads over 8 of 128 channels, 40.1 us
+// (226 MB, of which 32 are rotations that each XCD reads, 5.6 TB/s; with a tile's
+// workgroups on one XCD 45.9); a decoding step of 64 rows takes 5.6 us on the device, the
+// chain of positions, table, scale, rows, and the block rounded again.
+// Two rows of one place, or a sequence in two pieces that share a block, leave
+// one or the other there: nothing else is touched, but which is not defined.
 template <int EL, int FMT, int HQ, int HK, int D, int ROT, bool PAIRS, int BLOCK, int64_t SLOTS, int64_t PER, int64_t FAR, int64_t NBLK, int C, int QB, int HB>
 __device__ __forceinline__ void kv_append(const void *__restrict__ qkv, const float *__restrict__ rot, const int *__restrict__ seq,
                                           const int *__restrict__ pos, const int *__restrict__ table, void *__restrict__ q,

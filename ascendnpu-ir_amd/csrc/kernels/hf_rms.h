@@ -11,7 +11,12 @@
 // serial program, and each row's do not depend on how many rows a launch has.
 //
 // Rows, accesses and workgroups are the layer norm's (hf_ln.h): a row group of
-// T threads keeps a row in registers and loads the next one ahead.
+// T threads keeps a row in registers and loads the next one ahead.  Each row is
+// read once and its sum, codes and scale written once, so memory bounds it: bf16
+// [8192, 4096] with a residual to int8 43.5 us (235 MB, 5.4 TB/s; a copy of that
+// size 5.1), f16 [2003, 8192] to e4m3 21.4 (5.4), f32 [777, 5003] without to e5m2
+// 6.9, whose rows end off 16 bytes.  16 rows of 4096 take 3.4 us on the device:
+// one load, two reductions and one store, each waiting for the one before.
 #pragma once
 #include "hf_ln.h"
 
