@@ -799,12 +799,13 @@ def paged_attention(rows, heads, kv_heads, dim, slots, room, blocks, block=64, e
     last `window` of them.  out [rows, heads, dim] = softmax(scale q k) v,
     `scale` 1 / sqrt(dim) by default; query head h reads kv head h / (heads /
     kv_heads).  Sums and softmax statistics are f32, a probability is rounded
-    to bf16 before it multiplies its value.
+    to the queries' type before it multiplies its value.
 
     Positions whose block is not in [0, blocks) are not seen, a row that sees
     none is zeros, and rows whose position is negative or past the table, or
     whose sequence is not in it, are left as they are.  Tokens of a sequence
-    that follow each other are read together.  Codes are finite, as append_kv
+    that follow each other are read together; prompts and single tokens may share
+    a batch.  Codes are finite, as append_kv
     writes them; what lies behind a sequence's last row may be anything."""
     t = _paged_types(rows, heads, kv_heads, dim, slots, room, blocks, block, elem, fmt)
     scale = dim ** -0.5 if scale is None else scale
