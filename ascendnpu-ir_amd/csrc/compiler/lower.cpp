@@ -3640,7 +3640,8 @@ static KernelPlan lowerAppendKv(Analysis &A, const std::string &kname, const Op 
 constexpr int64_t kSplitRows = 1024;
 // ... and units, at most, that leave parts (SHARED), workgroups that add them (BLOCKS).
 constexpr int64_t kSplitShared = 768, kSplitJoin = 1024;
-// Positions of a sequence up to which its groups of tokens are never in pieces.
+// Visible positions of a sequence up to which its groups of tokens are never in
+// pieces, of heads of up to 128 channels (of longer ones as many channels).
 constexpr int64_t kWholeFar = 2048;
 // Rows that count as groups of tokens whatever the number of sequences.
 constexpr int64_t kPagedFew = 64;
@@ -3689,12 +3690,16 @@ static KernelPlan lowerPagedAttention(Analysis &A, const std::string &kname, con
   // Groups of tokens in pieces where some may be long: the second launch and the
   // sums before the first cost some 4 us (18 rows over up to 500 positions 11.6 and
   // 7.6 us, 64 over up to 2000 38.7 and 34.5; 48 over up to 8100 80 and 114, 4 over up to
-  // 4000 14.1 and 30)
-  const int64_t split = far > kWholeFar ? std::min(tokens, kSplitRows) : 0;
+  // 4000 14.1 and 30).  Heads of 256 channels, 8 rows over up to 1200: 13.4 and
+  // 19.2, 64 of them 26.7 and 25.1; one row over a window of 358: 13.2 and 10.0.
+  auto seen = [&](int64_t n) { return window ? std::min(far, window + n) : far; }; // (n tokens')
+  const int64_t split = seen(N) * std::max<int64_t>(z.D, 128) > kWholeFar * 128 ? std::min(tokens, kSplitRows) : 0;
   // Prompt's rows in pieces while they do not fill the chip (PagedPrompt), of
   // contexts that may be longer than the shortest piece
-  const int64_t pieces = far > kPieceTiles * 64 ? kPieceUnits / heads * tile : 0;
+  const int64_t pieces = seen(tile) > kPieceTiles * 64 ? kPieceUnits / heads * tile : 0;
   const std::string splitForm = "hf::PagedSplit<S, 4>::", promptForm = "hf::PagedPrompt<S>::", bounds = z.D > 128 ? "256" : "256, 2";
+  // (f16 of more than 128 channels, two waves a SIMD: 30 to 190 registers spilled)
+  const std::string fewBounds = z.D > 128 && q->type.elem == Elem::F16 ? "256, 1" : "256, 2";
   struct Schedule {
     const char *name;
     int64_t most; // rows
@@ -3708,14 +3713,14 @@ static KernelPlan lowerPagedAttention(Analysis &A, const std::string &kname, con
   const int64_t few = 1024 / heads * heads, flags = 4 * kPagedFlags;
   std::vector<Schedule> all;
   if (split)
-    all.push_back({"parts", split, splitForm + "rows(a, " + rows + ", (char *)ws)", "256, 2", 1, heads, kSplitShared,
+    all.push_back({"parts", split, splitForm + "rows(a, " + rows + ", (char *)ws)", fewBounds, 1, heads, kSplitShared,
                    (uint64_t)(32 + kSplitShared * (32 * N + 2 * GT * N * (8 + 4 * z.D))), splitForm + "join(a, (const char *)ws)", "256", 0, kSplitJoin});
-  if (tokens > split) all.push_back({"units", tokens, "", "", 0, 0, 0, 0, "hf::paged_rows<S, 4>(a, " + rows + ")", "256, 2", 1, heads});
+  if (tokens > split) all.push_back({"units", tokens, "", "", 0, 0, 0, 0, "hf::paged_rows<S, 4>(a, " + rows + ")", fewBounds, 1, heads});
   if (pieces > tokens)
     all.push_back({"pieces", pieces, promptForm + "rows<true>(a, " + rows + ", (char *)ws)", bounds, 0, 0, kPieces, (uint64_t)(flags + kPieces * 128 * (8 + 4 * z.D)),
-                   promptForm + "finish<true>(a, " + rows + ", (const char *)ws)", "256, 2", 0, few + kPieceUnits * 4});
+                   promptForm + "finish<true>(a, " + rows + ", (const char *)ws)", fewBounds, 0, few + kPieceUnits * 4});
   all.push_back({"prompt", int64_t(1) << 31, promptForm + "rows<false>(a, " + rows + ", (char *)ws)", bounds, tile, heads, 0, (uint64_t)flags,
-                 promptForm + "finish<false>(a, " + rows + ", (const char *)ws)", "256, 2", 0, few});
+                 promptForm + "finish<false>(a, " + rows + ", (const char *)ws)", fewBounds, 0, few});
   p.block[0] = 256;
   tileGrid(A, op, p, z.T, tile, heads);
   p.rowsA = 0; // (each count has its alternative)

@@ -30,6 +30,7 @@ ATTEND = {
     "far_f16": (6, 2, 96, 32, 3, 4096, 300, "f16", "e4m3", 0), "far_group20": (20, 1, 64, 64, 3, 4096, 150, "bf16", "e5m2", 0),
     "far_window": (8, 2, 64, 16, 3, 4096, 600, "bf16", "e4m3", 1500), "far_wide": (4, 1, 256, 128, 3, 4096, 80, "f16", "e5m2", 0),
     "far_alone": (3, 3, 32, 32, 3, 4096, 300, "bf16", "e4m3", 0), "many": (2, 1, 32, 16, 150, 4096, 2900, "bf16", "e4m3", 0),
+    "far_longer": (8, 2, 64, 16, 3, 4096, 600, "f16", "e4m3", 2500), "wide_f16": (4, 2, 192, 32, 3, 2048, 300, "f16", "e4m3", 0),
 }
 # rows of the groups that are compiled for one row count
 STATIC = {"append": ("usual", 70), "attend": ("usual", 70)}
