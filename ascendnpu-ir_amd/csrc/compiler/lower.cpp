@@ -3641,7 +3641,8 @@ constexpr int64_t kSplitRows = 1024;
 // ... and units, at most, that leave parts (SHARED), workgroups that add them (BLOCKS).
 constexpr int64_t kSplitShared = 768, kSplitJoin = 1024;
 // Visible positions of a sequence up to which its groups of tokens are never in
-// pieces, of heads of up to 128 channels (of longer ones as many channels).
+// pieces, of heads of up to 128 channels; of 256 a quarter (twice the bytes a
+// position, and half as many waves).
 constexpr int64_t kWholeFar = 2048;
 // Rows that count as groups of tokens whatever the number of sequences.
 constexpr int64_t kPagedFew = 64;
@@ -3691,9 +3692,9 @@ static KernelPlan lowerPagedAttention(Analysis &A, const std::string &kname, con
   // sums before the first cost some 4 us (18 rows over up to 500 positions 11.6 and
   // 7.6 us, 64 over up to 2000 38.7 and 34.5; 48 over up to 8100 80 and 114, 4 over up to
   // 4000 14.1 and 30).  Heads of 256 channels, 8 rows over up to 1200: 13.4 and
-  // 19.2, 64 of them 26.7 and 25.1; one row over a window of 358: 13.2 and 10.0.
+  // 19.2, 64 of them 26.7 and 25.1, 5 over up to 867 12.3 and 17.2; one row over a window of 358: 13.2 and 10.0.
   auto seen = [&](int64_t n) { return window ? std::min(far, window + n) : far; }; // (n tokens')
-  const int64_t split = seen(N) * std::max<int64_t>(z.D, 128) > kWholeFar * 128 ? std::min(tokens, kSplitRows) : 0;
+  const int64_t wide = std::max<int64_t>(z.D, 128), split = seen(N) * wide * wide > kWholeFar * 128 * 128 ? std::min(tokens, kSplitRows) : 0;
   // Prompt's rows in pieces while they do not fill the chip (PagedPrompt), of
   // contexts that may be longer than the shortest piece
   const int64_t pieces = seen(tile) > kPieceTiles * 64 ? kPieceUnits / heads * tile : 0;
