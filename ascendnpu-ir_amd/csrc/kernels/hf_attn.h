@@ -52,12 +52,12 @@ template <int EL> __device__ __forceinline__ v4i attn_round8(const float *p) {
   }
   return o;
 }
-// c and the two 16-bit numbers in w (none: neither)
-template <int EL> __device__ __forceinline__ float attn_sum2(int w, bool none, float c) {
+// c and the two 16-bit numbers in w
+template <int EL> __device__ __forceinline__ float attn_sum2(int w, float c) {
   using T = std::conditional_t<EL == EL_BF16, __bf16, _Float16>;
   typedef T t2 __attribute__((ext_vector_type(2)));
   if constexpr (EL == EL_BF16) return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(t2, w), __builtin_bit_cast(t2, 0x3F803F80), c, false);
-  else return __builtin_amdgcn_fdot2(__builtin_bit_cast(t2, w), __builtin_bit_cast(t2, none ? 0 : 0x3C003C00), c, false);
+  else return __builtin_amdgcn_fdot2(__builtin_bit_cast(t2, w), __builtin_bit_cast(t2, 0x3C003C00), c, false);
 }
 // the value of the lane 16 or 32 lanes away, combined with this one's
 template <int BY, typename F> __device__ __forceinline__ float with_lane(float v, F f) {
@@ -640,8 +640,11 @@ template <typename S> struct PagedPrompt {
   static constexpr int TOKENS = 128 / S::GT, HEADS = S::HK * S::GTILES, KP = S::D + 8, VP = 64 + 8;
   static constexpr int CHUNKS = 4 * S::D, N = (CHUNKS + 255) / 256; // 16-byte pieces of a tile's keys, a thread
   static constexpr int QF = S::D / 16, OT = S::D / 32;
-  struct Lds {
-    __attribute__((aligned(16))) uint16_t k[2][64 * KP], v[2][S::D * VP];
+  union Lds {
+    struct {
+      __attribute__((aligned(16))) uint16_t k[2][64 * KP], v[2][S::D * VP];
+    };
+    PagedJoin<S, 4> join;
   };
 
   __device__ static __forceinline__ v16f mfma(v4i a, v4i b, v16f c) {
@@ -656,11 +659,12 @@ template <typename S> struct PagedPrompt {
   // What the tile's values are scaled to: o is in units of 2^(ref - 127), of
   // about the largest block of the tile, but no less than 2^-60 of the largest
   // so far (`peak`; o would pass f32's range).  bf16 has the range for blocks
-  // 2^126 below it; f16 for 2^8 (DOWN), and what is below that scales p (`more`),
-  // which keeps its 11 bits down to 2^-14 and is 2^-25 off below.
+  // 2^126 below it, f16 for 2^8 (DOWN).  Blocks further apart cannot share a
+  // product (`apart`), and a row may see the small ones alone: rows that meet
+  // such a tile go by paged_part, which splits p.
   struct Mode {
     uint32_t ref, peak;
-    bool more;
+    bool apart;
   };
   static constexpr uint32_t DOWN = S::EL == EL_BF16 ? 126 : 8;
 
@@ -807,18 +811,6 @@ template <typename S> struct PagedPrompt {
     };
     auto rounded = [&](int u, v4i (&pf)[2]) {
       if (odd && !whole) hide(u, 0.0f);
-      if (mo.more) { // (what is rounded is not p: no sum of the rounded)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) part[i % 4] += s[u][i];
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          const uint32_t vs = (uint32_t)__builtin_amdgcn_readlane((int)gr.vs, 2 * u + g), down = ref - vs;
-          // (not read: p is zero)
-          const float by = vs > ref || down <= DOWN ? 1.0f : down > DOWN + 100 ? 0.0f : u2f((127 + DOWN - down) << 23);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) s[u][8 * g + i] *= by;
-        }
-      }
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         float p[8];
@@ -828,7 +820,7 @@ template <typename S> struct PagedPrompt {
         // (the sum of the rounded: half the additions, and its rounding and that
         // of what the values are multiplied by go together)
 #pragma unroll
-        for (int w = 0; w < 4; ++w) part[w] = attn_sum2<S::EL>(pf[k][w], mo.more, part[w]);
+        for (int w = 0; w < 4; ++w) part[w] = attn_sum2<S::EL>(pf[k][w], part[w]);
       }
     };
     auto keys = [&](int u, int c) { return *reinterpret_cast<const v4i *>(&lds.k[buf][(32 * u + key) * KP + 16 * c + 8 * half]); };
@@ -873,26 +865,32 @@ template <typename S> struct PagedPrompt {
     sum += (part[0] + part[1]) + (part[2] + part[3]);
   }
 
+  // The tiles of a piece of the rows; whether it has all of them.
+  template <bool PARTS> __device__ __forceinline__ bool range(int piece, int pieces, int &begin, int &end) const {
+    begin = PagedUnits<S>::first(lo), end = hi / 64 + 1;
+    if constexpr (!PARTS) return true;
+    int cut = (end - begin + pieces - 1) / pieces;
+    cut = cut < CUT ? CUT : cut;
+    const bool alone = end - begin <= cut;
+    begin += piece * cut;
+    end = begin + cut < end ? begin + cut : end;
+    return alone;
+  }
   // Rows t .. t + n - 1, of a sequence's positions lo .. hi; t0: the tile's first
   // row.  PARTS: piece `piece` of `pieces` of their tiles, at least CUT tiles
   // long, to part and stats.
-  template <bool PARTS> __device__ __forceinline__ void run(int64_t t0, int64_t t, int n, int gt, int piece, int pieces, float *part, float *stats) {
+  // (false: a tile's blocks are too far apart, and split() has these rows to do)
+  template <bool PARTS> __device__ __forceinline__ bool run(int64_t t0, int64_t t, int n, int gt, int piece, int pieces, float *part, float *stats) {
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, r = lane % 32, half = lane / 32;
     const int row = 32 * wave + r, tok = row / S::GT, head = gt * 16 + row % S::GT, skip = (int)(t - t0);
     const bool ok = tok >= skip && tok < skip + n && head < S::G && row < TOKENS * S::GT;
     const int pos = ok ? lo + tok - skip : -1;
-    int begin = PagedUnits<S>::first(lo), end = hi / 64 + 1;
-    bool alone = true; // one piece has all of them: the result, and the mark DONE for a sum
-    if constexpr (PARTS) {
-      int cut = (end - begin + pieces - 1) / pieces;
-      cut = cut < CUT ? CUT : cut;
-      alone = end - begin <= cut;
-      begin += piece * cut;
-      end = begin + cut < end ? begin + cut : end;
-      if (begin >= end) {
-        if (ok && half == 0) stats[2 * row] = -__builtin_inff(), stats[2 * row + 1] = 0;
-        return;
-      }
+    int begin, end;
+    // one piece has all of them: the result, and the mark DONE for a sum
+    const bool alone = range<PARTS>(piece, pieces, begin, end);
+    if (PARTS && begin >= end) {
+      if (ok && half == 0) stats[2 * row] = -__builtin_inff(), stats[2 * row + 1] = 0;
+      return true;
     }
     // the wave's rows' positions
     const int a0 = 32 * wave / S::GT, a1 = (32 * wave + 31) / S::GT;
@@ -913,9 +911,9 @@ template <typename S> struct PagedPrompt {
     load(gr, begin);
     Mode mo = mode(gr, begin, Mode{0, 0, false});
     int next = block(begin + 1);
-    stage(gr, mo, begin, begin & 1);
+    if (!mo.apart) stage(gr, mo, begin, begin & 1);
     __syncthreads();
-    for (int i = begin; i < end; ++i) {
+    for (int i = begin; i < end && !mo.apart; ++i) {
       Groups gn = gr;
       if (i + 1 < end) {
         gn = groups(next);
@@ -926,14 +924,15 @@ template <typename S> struct PagedPrompt {
       if (64 * i <= seen && (S::WINDOW == 0 || 64 * i + 63 > first - S::WINDOW)) step(gr, mo, i, i & 1, pos, first, last);
       if (i + 1 < end) {
         mo = mode(gn, i + 1, mo);
-        stage(gn, mo, i + 1, (i + 1) & 1);
+        if (!mo.apart) stage(gn, mo, i + 1, (i + 1) & 1);
         gr = gn;
       }
       __syncthreads();
     }
+    if (mo.apart) return false;
     times(mx_scale(ref));
     sum = with_lane<32>(sum, [](float x, float y) { return x + y; });
-    if (!ok) return;
+    if (!ok) return true;
     if (PARTS && alone && half == 0) stats[2 * row + 1] = DONE;
     if (PARTS && !alone) {
       if (half == 0) stats[2 * row] = m, stats[2 * row + 1] = sum;
@@ -943,7 +942,7 @@ template <typename S> struct PagedPrompt {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
           *reinterpret_cast<v4f *>(dst + 32 * dt + 8 * k) = v4f{o[dt][4 * k], o[dt][4 * k + 1], o[dt][4 * k + 2], o[dt][4 * k + 3]};
-      return;
+      return true;
     }
     const float by = sum == 0 ? 0.0f : 1.0f / sum;
     uint16_t *dst = a.out + ((t0 + tok) * (int64_t)S::HQ + h * S::G + head) * S::D + 4 * half;
@@ -959,6 +958,19 @@ template <typename S> struct PagedPrompt {
         }
         *reinterpret_cast<u32x2_any *>(dst + 32 * dt + 8 * k) = u32x2{(uint32_t)e[0] | (uint32_t)e[1] << 16, (uint32_t)e[2] | (uint32_t)e[3] << 16};
       }
+    return true;
+  }
+  // The same rows and piece, N tokens at a time, by paged_part, which takes
+  // blocks any distance apart.
+  template <bool PARTS> __device__ __forceinline__ void split(int64_t t0, int64_t t, int n, int gt, int piece, int pieces, float *part, float *stats) {
+    int begin, end;
+    const bool alone = range<PARTS>(piece, pieces, begin, end);
+    for (int i = 0; i < n; i += S::N) {
+      const int k = n - i < S::N ? n - i : S::N, row = (int)(t - t0 + i) * S::GT, b = PagedUnits<S>::first(lo + i), e = (lo + i + k - 1) / 64 + 1;
+      paged_part<S, 4>(a, lds.join, t + i, k, seq, lo + i, h * S::GTILES + gt, b < begin ? begin : b, e < end ? e : end,
+                       alone ? nullptr : part + row * S::D, alone ? nullptr : stats + 2 * row);
+      if (PARTS && alone && (int)threadIdx.x < k * S::GT) stats[2 * (row + threadIdx.x) + 1] = DONE;
+    }
   }
 
   __device__ static __forceinline__ int64_t tiles(int64_t T) { return (T + TOKENS - 1) / TOKENS; }
@@ -989,15 +1001,10 @@ template <typename S> struct PagedPrompt {
     const int64_t t0 = (tiles(T) - 1 - (blockIdx.x - piece * units) / HEADS) * TOKENS;
     const int hh = (int)(blockIdx.x - piece * units) % HEADS, h = hh / S::GTILES, gt = hh % S::GTILES, lane = threadIdx.x % 64;
     const int tokens = (int)(T - t0 < TOKENS ? T - t0 : TOKENS);
-    int few = 0;
-    for (int at = 0; at < tokens;) {
+    float *const part = PARTS ? part_of(ws, blockIdx.x) : nullptr, *const stats = PARTS ? stats_of(ws, blockIdx.x) : nullptr;
+    // a row and those that follow it
+    auto follow = [&](int at, int s, int p) {
       const int64_t t = t0 + at;
-      const int s = a.seq[t], p = a.pos[t];
-      if (!S::inside(s, p)) {
-        ++at;
-        continue;
-      }
-      // the rows that follow it
       int n = 0;
 #pragma unroll
       for (int k = 0; k < TOKENS; k += 64) {
@@ -1005,16 +1012,34 @@ template <typename S> struct PagedPrompt {
         const uint64_t other = __ballot(!(i < tokens - at && p + i < S::FAR && a.seq[t + i] == s && a.pos[t + i] == p + i));
         if (n == k) n += other ? __builtin_ctzll(other) : 64;
       }
+      return n;
+    };
+    int few = 0;
+    uint64_t apart[2] = {0, 0}; // rows that run() has left
+    for (int at = 0; at < tokens;) {
+      const int64_t t = t0 + at;
+      const int s = a.seq[t], p = a.pos[t];
+      if (!S::inside(s, p)) {
+        ++at;
+        continue;
+      }
+      const int n = follow(at, s, p);
       if (n <= S::FEW && S::few(a.seq, a.pos, t, T, s, p)) { // PagedFew's
         if (PARTS && piece == 0)
-          for (int i = threadIdx.x; i < n * S::GT; i += 256) stats_of(ws, blockIdx.x)[2 * (at * S::GT + i) + 1] = DONE;
+          for (int i = threadIdx.x; i < n * S::GT; i += 256) stats[2 * (at * S::GT + i) + 1] = DONE;
         at += n, few = 1;
         continue;
       }
-      PagedPrompt{a, lds, s, h, p, p + n - 1}.template run<PARTS>(t0, t, n, gt, piece, cuts, PARTS ? part_of(ws, blockIdx.x) : nullptr,
-                                                                 PARTS ? stats_of(ws, blockIdx.x) : nullptr);
+      if (!PagedPrompt{a, lds, s, h, p, p + n - 1}.template run<PARTS>(t0, t, n, gt, piece, cuts, part, stats)) (at < 64 ? apart[0] : apart[1]) |= 1ull << at % 64;
       at += n;
     }
+    // (behind the others: what this computes ahead would take their registers)
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+      for (uint64_t left = apart[w]; left; left &= left - 1) {
+        const int at = 64 * w + __builtin_ctzll(left), s = a.seq[t0 + at], p = a.pos[t0 + at], n = follow(at, s, p);
+        PagedPrompt{a, lds, s, h, p, p + n - 1}.template split<PARTS>(t0, t0 + at, n, gt, piece, cuts, part, stats);
+      }
     if (piece == 0 && hh == 0 && threadIdx.x == 0 && t0 / TOKENS < PagedFew<S>::TILES) reinterpret_cast<int *>(ws)[t0 / TOKENS] = few;
   }
 

@@ -1,0 +1,104 @@
+"""Attention over caches whose blocks hold values of very different sizes, and
+over tables that name what a window has left behind: a row's result follows the
+positions that it sees, whatever the blocks beside them in its tile hold.
+
+Tolerance of a value, with N positions seen, D channels, P = sum p |v| and the
+largest |v|, all over the positions that the row sees (of its own kv head):
+  scores: D + 8 f32 roundings of at most sum |q k| scale, in the numerator and
+    the denominator                        2 (D + 8) 2^-23 sum |q k| P
+  exp2 of the hardware (1 ulp) and its argument's rounding       2^-20 P
+  N f32 additions in both sums             2 N 2^-23 P
+  p to 16 bits (half a step), of a prompt also in the denominator
+                                           2 2^-8 P, of f16 queries 2 2^-11 P and
+                                           2^-25 |v| for each position
+  the result's own rounding (half a step)"""
+import numpy as np
+import pytest
+
+import serving_catalog as sc
+from helpers import to_dev, to_host
+from oracle import blockscaled as bs
+from oracle import serving as sv
+from test_norm_mx import TINY, U, note, stored, value
+from test_serving import batch, cache_of, load
+
+TOP16 = 65504.0
+
+
+def largest(cache, seq, pos, table, window, heads, fmt):
+    """The largest |v| that each row and query head sees, and how many positions."""
+    _, _, v, vs = cache
+    blocks, kv, _, block = v.shape
+    with np.errstate(invalid="ignore"):
+        size = np.abs(bs.code_values(fmt)[v]).max(axis=2) * bs.scale_values(vs)[:, :, None]  # [block, head, token]
+    out, n = np.zeros((len(seq), heads)), np.zeros(len(seq))
+    for t in range(len(seq)):
+        if 0 <= seq[t] < table.shape[0] and 0 <= pos[t] < table.shape[1] * block:
+            j = sv.visible(pos[t], seq[t], table, blocks, block, window)
+            n[t] = len(j)
+            if len(j):
+                out[t] = np.repeat(size[table[seq[t], j // block], :, j % block].max(axis=0), heads // kv)
+    return out, n
+
+
+def check_rows(c, outs, q, cache, seq, pos, table, before):
+    hq, hk, d, block, slots, room, blocks, el, fmt, window = c
+    want, size, reach = sv.paged_attention(q, *cache, seq, pos, table, before, fmt, float(np.float32(d ** -0.5)), window)
+    vmax, n = largest(cache, seq, pos, table, window, hq, fmt)
+    n = n[:, None, None]
+    tol = size * (2 * U[el] + 2.0 ** -20 + 2 * (d + 8) * 2.0 ** -23 * reach[:, :, None] + 2 * n * 2.0 ** -23)
+    if el == "f16":
+        tol = tol + 2.0 ** -25 * n * vmax[:, :, None]
+    got = value(outs, el)
+    assert np.array_equal(np.isnan(got), np.isnan(want)), np.argwhere(np.isnan(got) != np.isnan(want))[:5]
+    # (what may round to an infinity of f16 has no value to compare)
+    far = np.abs(want) + tol + U[el] * (np.abs(want) + tol) > TOP16 if el == "f16" else np.zeros(want.shape, bool)
+    with np.errstate(invalid="ignore"):
+        ok = np.abs(got - want) <= tol + U[el] * (np.abs(want) + tol) + TINY[el]
+    assert (ok | far | np.isnan(want)).all(), [(i.tolist(), got[tuple(i)], want[tuple(i)]) for i in np.argwhere(~(ok | far | np.isnan(want)))[:5]]
+    return far
+
+
+def run(grp, c, gpu, seq, pos, table, cache, qs, qv):
+    import torch
+    before = np.full(qv.shape, 3.0)
+    args = [qs, cache[0], cache[1].view(np.int8), cache[2], cache[3].view(np.int8), seq, pos, table, stored(before, c[7])[0]]
+    out = grp(*[to_dev(a, p["elem"], gpu) for a, p in zip(args, grp.meta["params"])])
+    torch.cuda.synchronize()
+    return check_rows(c, to_host(out, c[7]), qv, cache, seq, pos, table, before)
+
+
+def case_of(rng, c, parts, byte, pad=0):
+    """A batch over sequences whose block i has the value scale byte(i) in
+    every head; blocks in any order, none behind a sequence's last row."""
+    hq, hk, d, block, slots, room, blocks, el, fmt, window = c
+    seq, pos = batch(parts, pad, slots)
+    cache = cache_of(rng, c)
+    order = list(rng.permutation(blocks))
+    table = np.full((slots, -(-room // block)), -1, np.int32)
+    for s in {s for s, _, _ in parts}:
+        for i in range(-(-max(p + n for s2, p, n in parts if s2 == s) // block)):
+            table[s, i] = order.pop()
+            cache[3][table[s, i]] = byte(i)
+    qs, qv = stored(rng.normal(size=(len(seq), hq, d)), el)
+    return seq, pos, table, cache, qs, qv
+
+
+# ---------------------------------------------------------------- blocks far apart
+@pytest.mark.gpu
+@pytest.mark.parametrize("down", [9, 20, 25, 31])
+@pytest.mark.parametrize("name", ["group3", "alone", "far_f16"])
+def test_f16_prompt_beside_larger_blocks(gpu, name, down):
+    """Rows of f16 prompts that see small values alone, and later blocks of
+    the same tile 2^down larger, that the later rows see; and the other way
+    round, where the large values have small weights or large ones."""
+    c = sc.ATTEND[name]
+    fmt, block, far = c[8], c[3], min(c[5], 2000)
+    grp = load(f"pagedattn_{name}_rt")
+    # (the largest values are some 2^14 times 1.75)
+    big = 127 + 14 - bs.EMAX[fmt]
+    for k, byte in enumerate((lambda i: big if i % 2 else big - down, lambda i: big - down if i % 2 else big,
+                              lambda i: big - down if i < 3 else big - down // 2 if i < 5 else big)):
+        note(f"{name} down {down} order {k}")
+        rng = np.random.default_rng(down + k)
+        run(grp, c, gpu, *case_of(rng, c, [(0, 0, 3 * block + 5), (2, far - 70, 70)], byte, 1))
