@@ -658,15 +658,15 @@ template <typename S> struct PagedPrompt {
   };
   // What the tile's values are scaled to: o is in units of 2^(ref - 127), of
   // about the largest block of the tile, but no less than 2^-60 of the largest
-  // so far (`peak`; o would pass f32's range).  bf16 has the range for blocks
-  // 2^126 below it, f16 for 2^8 (DOWN).  Blocks further apart cannot share a
+  // so far (`peak`; o would pass f32's range).  bf16 has the range for codes
+  // 2^100 below it, f16 for 2^8 (DOWN).  Blocks further apart cannot share a
   // product (`apart`), and a row may see the small ones alone: rows that meet
   // such a tile go by paged_part, which splits p.
   struct Mode {
     uint32_t ref, peak;
     bool apart;
   };
-  static constexpr uint32_t DOWN = S::EL == EL_BF16 ? 126 : 8;
+  static constexpr uint32_t DOWN = S::EL == EL_BF16 ? 100 : 8;
 
   const PagedArgs &a;
   Lds &lds;
@@ -710,7 +710,7 @@ template <typename S> struct PagedPrompt {
     const uint32_t big = quad(read ? gr.vs : 0), peak = max_u32(was.peak, big);
     uint32_t now = big > was.ref || (big && big + 4 < was.ref) ? big : was.ref; // (a little lower is near enough)
     now = now + 60 < peak ? peak - 60 : now;
-    return Mode{now, peak, S::EL != EL_BF16 && quad(read ? now - gr.vs : 0) > DOWN};
+    return Mode{now, peak, quad(read ? now - gr.vs : 0) > DOWN};
   }
   __device__ __forceinline__ void stage(const Groups &gr, const Mode &mo, int tile, int buf) {
     const bool whole = 64 * tile + 63 <= hi && __all(gr.block >= 0);

@@ -102,3 +102,20 @@ def test_f16_prompt_beside_larger_blocks(gpu, name, down):
         note(f"{name} down {down} order {k}")
         rng = np.random.default_rng(down + k)
         run(grp, c, gpu, *case_of(rng, c, [(0, 0, 3 * block + 5), (2, far - 70, 70)], byte, 1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("down", [60, 99, 101, 112, 126, 127, 133, 150])
+@pytest.mark.parametrize("name", ["group4", "group20", "far_alone"])
+def test_bf16_prompt_beside_larger_blocks(gpu, name, down):
+    """The same of bf16, whose exponents are f32's: no block's values are
+    taken for larger ones, and none are lost that a row sees alone."""
+    c = sc.ATTEND[name]
+    block, far = c[3], min(c[5], 2000)
+    grp = load(f"pagedattn_{name}_rt")
+    big = 60 + down  # (small values are some 2^-60)
+    for k, byte in enumerate((lambda i: big if i % 2 else big - down, lambda i: big - down if i % 2 else big,
+                              lambda i: big - down if i < 3 else big - down // 2 if i < 5 else big)):
+        note(f"{name} down {down} order {k}")
+        rng = np.random.default_rng(down + k)
+        run(grp, c, gpu, *case_of(rng, c, [(0, 0, 3 * block + 5), (2, far - 70, 70)], byte, 1))
