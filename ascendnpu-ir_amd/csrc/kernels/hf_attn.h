@@ -198,6 +198,21 @@ template <typename S> __device__ __forceinline__ void paged_query(const PagedArg
   }
 }
 
+// Whether rows at lo .. hi see some of the sixteen positions from `at` on.
+// Elsewhere, behind the last row's position and before the first one's window,
+// the cache may hold anything, NaN and any scale.
+template <typename S> __device__ __forceinline__ bool some_seen(int at, int lo, int hi) { return at <= hi && (S::WINDOW == 0 || at + 15 > lo - S::WINDOW); }
+// the codes in word w of the sixteen that they see
+template <typename S> __device__ __forceinline__ uint32_t kept_codes(int w, int at, int lo, int hi) {
+  const int n = hi + 1 - at - 4 * w; // those up to the last row's
+  uint32_t keep = n >= 4 ? 0xFFFFFFFFu : n <= 0 ? 0u : 0xFFFFFFFFu >> (8 * (4 - n));
+  if constexpr (S::WINDOW != 0) {
+    const int gone = lo - S::WINDOW + 1 - at - 4 * w; // those before the window
+    keep &= gone <= 0 ? 0xFFFFFFFFu : gone >= 4 ? 0u : 0xFFFFFFFFu << (8 * gone);
+  }
+  return keep;
+}
+
 // One tile of 64 tokens from b0 on.  pos: the lane's row's position (-1: no
 // row), lo and hi: the first and last of the tile's rows.
 template <typename S> __device__ __forceinline__ void paged_step(PagedState<S> &st, PagedTile<S> &t, const v4i (&q)[S::KS], const PagedArgs &a, int b0,
@@ -229,11 +244,9 @@ template <typename S> __device__ __forceinline__ void paged_step(PagedState<S> &
     for (int u = 0; u < 4; ++u)
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[u][i] = sees(4 * u + i) ? s[u][i] : -__builtin_inff();
-    // (behind the last position the cache may hold anything, NaN too)
-    const int n = t.there ? hi + 1 - at : 0;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const uint32_t keep = n >= 4 * w + 4 ? 0xFFFFFFFFu : n <= 4 * w ? 0u : 0xFFFFFFFFu >> (8 * (4 * w + 4 - n));
+      const uint32_t keep = t.there ? kept_codes<S>(w, at, lo, hi) : 0u;
 #pragma unroll
       for (int dt = 0; dt < S::DT; ++dt) t.v[dt][w] &= keep;
     }
@@ -278,7 +291,7 @@ template <typename S> __device__ __forceinline__ void paged_step(PagedState<S> &
   // f16: p by itself, and the codes scaled to a running reference exponent; where
   // a block lies further below it than f16 reaches, p times its scale as the sum
   // of two bf16 numbers
-  const bool read = t.there && at <= hi;
+  const bool read = t.there && some_seen<S>(at, lo, hi);
   const bool bad = __any(read && t.vs == 255);
   uint32_t big = read && t.vs != 255 ? t.vs : 0, small = read ? t.vs : 255;
   if constexpr (S::BLOCK < 64) {
@@ -706,14 +719,14 @@ template <typename S> struct PagedPrompt {
       v = max_u32(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true));
       return (uint32_t)__builtin_amdgcn_readfirstlane((int)max_u32(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true)));
     };
-    const bool read = gr.block >= 0 && gr.vs != 255 && 64 * tile + 16 * (int)(threadIdx.x % 4) <= hi;
+    const bool read = gr.block >= 0 && gr.vs != 255 && some_seen<S>(64 * tile + 16 * (int)(threadIdx.x % 4), lo, hi);
     const uint32_t big = quad(read ? gr.vs : 0), peak = max_u32(was.peak, big);
     uint32_t now = big > was.ref || (big && big + 4 < was.ref) ? big : was.ref; // (a little lower is near enough)
     now = now + 60 < peak ? peak - 60 : now;
     return Mode{now, peak, quad(read ? now - gr.vs : 0) > DOWN};
   }
   __device__ __forceinline__ void stage(const Groups &gr, const Mode &mo, int tile, int buf) {
-    const bool whole = 64 * tile + 63 <= hi && __all(gr.block >= 0);
+    const bool whole = 64 * tile + 63 <= hi && (S::WINDOW == 0 || 64 * tile > lo - S::WINDOW) && __all(gr.block >= 0);
 #pragma unroll
     for (int e = 0; e < N; ++e) {
       const int c = (int)threadIdx.x + 256 * e;
@@ -724,11 +737,11 @@ template <typename S> struct PagedPrompt {
       const uint32_t vs = S::BLOCK >= 64 ? (uint32_t)__builtin_amdgcn_readfirstlane((int)gr.vs) : (uint32_t)__shfl((int)gr.vs, g);
       bool used = true;
       if (!whole) {
-        // (behind the last position, and where there is no block, zeros)
-        const int n = __shfl(gr.block, g) >= 0 ? hi + 1 - (64 * tile + 16 * g) : 0;
-        used = n > 0;
+        // (what no row sees, and where there is no block, zeros)
+        const int at = 64 * tile + 16 * g;
+        used = __shfl(gr.block, g) >= 0 && some_seen<S>(at, lo, hi);
 #pragma unroll
-        for (int w = 0; w < 4; ++w) vx[e][w] &= n >= 4 * w + 4 ? 0xFFFFFFFFu : n <= 4 * w ? 0u : 0xFFFFFFFFu >> (8 * (4 * w + 4 - n));
+        for (int w = 0; w < 4; ++w) vx[e][w] &= used ? kept_codes<S>(w, at, lo, hi) : 0u;
       }
       const uint32_t down = mo.ref - vs < DOWN ? mo.ref - vs : DOWN;
       const float by = !used || vs == 255 ? 1.0f : u2f((127 - down) << 23);

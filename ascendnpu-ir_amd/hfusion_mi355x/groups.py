@@ -805,8 +805,9 @@ def paged_attention(rows, heads, kv_heads, dim, slots, room, blocks, block=64, e
     none is zeros, and rows whose position is negative or past the table, or
     whose sequence is not in it, are left as they are.  Tokens of a sequence
     that follow each other are read together; prompts and single tokens may share
-    a batch.  Codes are finite, as append_kv
-    writes them; what lies behind a sequence's last row may be anything."""
+    a batch.  Codes are finite, as append_kv writes them; what lies behind a
+    sequence's last row, or before the window of its first row in the batch, may
+    be anything."""
     t = _paged_types(rows, heads, kv_heads, dim, slots, room, blocks, block, elem, fmt)
     scale = dim ** -0.5 if scale is None else scale
     ins = [(n, t[n]) for n in ("q", "k", "ks", "v", "vs", "seq", "pos", "table")]

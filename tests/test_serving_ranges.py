@@ -119,3 +119,41 @@ def test_bf16_prompt_beside_larger_blocks(gpu, name, down):
         note(f"{name} down {down} order {k}")
         rng = np.random.default_rng(down + k)
         run(grp, c, gpu, *case_of(rng, c, [(0, 0, 3 * block + 5), (2, far - 70, 70)], byte, 1))
+
+
+# ---------------------------------------------------------------- windows
+def placeholder(rng, c, case, scale):
+    """Names one block of NaN codes in the place of all that lie before the
+    window of a sequence's first row."""
+    seq, pos, table, (k, ks, v, vs), qs, qv = case
+    block, window, fmt = c[3], c[9], c[8]
+    free = [b for b in range(len(k)) if b not in table]
+    k[free[0]], v[free[0]], ks[free[0]], vs[free[0]] = 0xFF, 0x7F, scale, scale
+    gone = 0
+    for s in set(seq[(seq >= 0) & (seq < len(table)) & (pos >= 0)].tolist()):
+        first = pos[(seq == s) & (pos >= 0)].min()
+        n = max(0, (first - window + 1) // block)
+        table[s, :n] = free[0]
+        gone += n
+    return gone
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [0, 127, 200, 254, 255])
+@pytest.mark.parametrize("name", ["window", "window_f16", "far_window", "far_longer"])
+def test_blocks_before_the_window(gpu, name, scale):
+    """What lies before the window of a sequence's first row may be anything:
+    a placeholder of NaN codes, whatever its scale.  Single tokens and a few at
+    a time, rows of prompts, and both in one batch."""
+    c = sc.ATTEND[name]
+    slots, room, window = c[4], c[5], c[9]
+    rng = np.random.default_rng(scale + len(name))
+    low = 127 - bs.EMAX[c[8]]
+    grp = load(f"pagedattn_{name}_rt")
+    near = min(room, window + 200)
+    for i, parts in enumerate(([(0, near - 3, 1), (1, window + 20, 1), (2, window + 33, 1)], [(0, near - 7, 6), (2, window + 61, 3)],
+                               [(1, near - 90, 90), (0, window + 7, 33)], [(1, window + 17, 100), (0, near - 4, 3), (2, near - 1, 1)])):
+        note(f"{name} scale {scale} batch {i}")
+        case = case_of(rng, c, parts, lambda i: low - i % 3)
+        assert placeholder(rng, c, case, scale) > 0
+        run(grp, c, gpu, *case)
