@@ -198,6 +198,10 @@ template <typename S> __device__ __forceinline__ void paged_query(const PagedArg
   }
 }
 
+// The largest scale byte, 2^16, whose unit a row's sums are held in while it may
+// see small values alone: those keep their bits down to 2^-110.
+constexpr uint32_t kTopScale = 143;
+
 // Whether rows at lo .. hi see some of the sixteen positions from `at` on.
 // Elsewhere, behind the last row's position and before the first one's window,
 // the cache may hold anything, NaN and any scale.
@@ -288,9 +292,10 @@ template <typename S> __device__ __forceinline__ void paged_step(PagedState<S> &
     }
     return;
   }
-  // f16: p by itself, and the codes scaled to a running reference exponent; where
-  // a block lies further below it than f16 reaches, p times its scale as the sum
-  // of two bf16 numbers
+  // f16: p by itself, and the codes scaled to a running reference exponent, that
+  // of the largest block up to kTopScale (a row may see small ones alone); where
+  // a block lies above it, or further below than f16 reaches, p times its scale as
+  // the sum of two bf16 numbers
   const bool read = t.there && some_seen<S>(at, lo, hi);
   const bool bad = __any(read && t.vs == 255);
   uint32_t big = read && t.vs != 255 ? t.vs : 0, small = read ? t.vs : 255;
@@ -299,11 +304,11 @@ template <typename S> __device__ __forceinline__ void paged_step(PagedState<S> &
     for (int k = 16; k < 64; k *= 2) big = max_u32(big, (uint32_t)__shfl_xor((int)big, k)), small = 255 - max_u32(255 - small, 255 - (uint32_t)__shfl_xor((int)small, k));
   }
   big = __builtin_amdgcn_readfirstlane(big), small = __builtin_amdgcn_readfirstlane(small);
-  const uint32_t ref = max_u32(st.ref, big);
+  const uint32_t ref = max_u32(st.ref, big < kTopScale ? big : kTopScale);
   const float by = ref - st.ref > 126 ? 0.0f : u2f((127 - (ref - st.ref)) << 23);
   st.ref = ref;
   if (!__all(was * by == 1.0f)) st.times(was * by);
-  if (!bad && (int)(ref - small) <= 8) {
+  if (!bad && big <= ref && (int)(ref - small) <= 8) {
     const float vs = read ? u2f((127 - (ref - t.vs)) << 23) : 1.0f;
     const v4i p0 = attn_round8<EL_F16>(p), p1 = attn_round8<EL_F16>(p + 8);
 #pragma unroll
@@ -673,8 +678,8 @@ template <typename S> struct PagedPrompt {
   // about the largest block of the tile, but no less than 2^-60 of the largest
   // so far (`peak`; o would pass f32's range).  bf16 has the range for codes
   // 2^100 below it, f16 for 2^8 (DOWN).  Blocks further apart cannot share a
-  // product (`apart`), and a row may see the small ones alone: rows that meet
-  // such a tile go by paged_part, which splits p.
+  // product, and one above kTopScale not the sums (`apart`), since a row may see the
+  // small ones alone: rows that meet such a tile go by paged_part.
   struct Mode {
     uint32_t ref, peak;
     bool apart;
@@ -723,7 +728,7 @@ template <typename S> struct PagedPrompt {
     const uint32_t big = quad(read ? gr.vs : 0), peak = max_u32(was.peak, big);
     uint32_t now = big > was.ref || (big && big + 4 < was.ref) ? big : was.ref; // (a little lower is near enough)
     now = now + 60 < peak ? peak - 60 : now;
-    return Mode{now, peak, quad(read ? now - gr.vs : 0) > DOWN};
+    return Mode{now, peak, now > kTopScale || quad(read ? now - gr.vs : 0) > DOWN};
   }
   __device__ __forceinline__ void stage(const Groups &gr, const Mode &mo, int tile, int buf) {
     const bool whole = 64 * tile + 63 <= hi && (S::WINDOW == 0 || 64 * tile > lo - S::WINDOW) && __all(gr.block >= 0);
@@ -763,8 +768,11 @@ template <typename S> struct PagedPrompt {
   __device__ __forceinline__ void step(const Groups &gr, const Mode &mo, int tile, int buf, int pos, int first, int last) {
     const int lane = threadIdx.x % 64, r = lane % 32, half = lane / 32, key = (r & 0x13) | (r & 4) << 1 | (r & 8) >> 1;
     if (mo.ref != ref) {
-      const int by = (int)ref - (int)mo.ref;
-      times(by < -126 ? 0.0f : u2f((uint32_t)(127 + by) << 23)); // (up to 2^60)
+      const int by = (int)ref - (int)mo.ref; // -143 .. 60
+#pragma unroll
+      for (int i = 0; i < OT; ++i)
+#pragma unroll
+        for (int k = 0; k < 16; ++k) o[i][k] = __builtin_amdgcn_ldexpf(o[i][k], by);
       ref = mo.ref;
     }
     constexpr int GS = S::BLOCK >= 64 ? 1 : 4; // groups of tokens whose blocks may differ

@@ -157,3 +157,22 @@ def test_blocks_before_the_window(gpu, name, scale):
         case = case_of(rng, c, parts, lambda i: low - i % 3)
         assert placeholder(rng, c, case, scale) > 0
         run(grp, c, gpu, *case)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["group3", "alone", "far_f16", "group4", "group20", "far_alone"])
+def test_rows_before_far_larger_values(gpu, name):
+    """Rows that see small values alone, beside rows of the same sequence
+    that see values up to f32's largest, in the next block and in the next tile:
+    a few at a time and as rows of a prompt."""
+    c = sc.ATTEND[name]
+    block, el, slots = c[3], c[7], c[4]
+    grp = load(f"pagedattn_{name}_rt")
+    low = 127 - bs.EMAX[c[8]] - (14 if el == "f16" else 90)
+    for big in (low + 40, 190, 254 - bs.EMAX[c[8]] - 16):
+        for i, (parts, edge) in enumerate((([(0, 0, 140)], block), ([(0, 0, 140)], 64), ([(2, 64 - 2, 4)], 64), ([(1, block - 3, 6), (0, 3 * block - 1, 2)], block))):
+            note(f"{name} big {big} batch {i}")
+            rng = np.random.default_rng(big + i)
+            case = case_of(rng, c, parts, lambda k: big if k * block >= edge else low)
+            far = run(grp, c, gpu, *case)
+            assert not far[case[1] < edge].any()
