@@ -3687,7 +3687,9 @@ static KernelPlan lowerPagedAttention(Analysis &A, const std::string &kname, con
   // The kernels, by the row count.  More rows than the sequences' groups of N
   // tokens are a prompt's, unless they are few: 64 rows behind 8000 positions 44
   // us as groups of tokens, 52 as a prompt's rows, 256 behind 30000 364 and 178.
-  const int64_t tile = 128 / GT, tokens = std::max<int64_t>(kPagedFew, std::min<int64_t>(int64_t(1) << 30, N * z.slots)), far = z.per * z.block;
+  // (no more than a launch has workgroups for, a row and head each)
+  const int64_t tile = 128 / GT, far = z.per * z.block;
+  const int64_t tokens = std::max<int64_t>(kPagedFew, std::min<int64_t>(((int64_t(1) << 24) - 1) / heads, N * z.slots));
   // Groups of tokens in pieces where some may be long: the second launch and the
   // sums before the first cost some 4 us (18 rows over up to 500 positions 11.6 and
   // 7.6 us, 64 over up to 2000 38.7 and 34.5; 48 over up to 8100 80 and 114, 4 over up to

@@ -1,0 +1,41 @@
+"""What the serving ops refuse or launch at the ends of their ranges (no GPU)."""
+import pytest
+
+import hfusion_mi355x as hf
+from hfusion_mi355x import groups as g
+
+
+def manifest(ir, options="dyn=runtime"):
+    return open(hf.compile(ir, options=options).manifest).read().splitlines()
+
+
+@pytest.mark.parametrize("heads,kv,slots", [(32, 8, 64), (32, 32, 65536), (20, 1, 1 << 22), (64, 64, 1 << 20), (1024, 1024, 1 << 20)])
+def test_every_kernel_has_a_launchable_grid(heads, kv, slots):
+    """At the most rows that each of the attention's kernels is taken for, less than
+    2^24 workgroups of 256 threads; in any order of the kernels, every row
+    count up to max_rows has one."""
+    ir = g.with_dynamic_rows(g.paged_attention(7919, heads=heads, kv_heads=kv, dim=32, slots=slots, room=64, blocks=64, block=16), 7919)
+    lines = [ln.split() for ln in manifest(ir)]
+    most = next(int(ln[1]) for ln in lines if ln[0] == "max_rows")
+    pre = []  # (workgroups, rows and workgroups besides)
+    for ln in lines:
+        if ln[0] == "pre":
+            pre.append([int(ln[2]), 1, 0])
+        elif ln[0] == "pre_rows":
+            pre[-1][1:] = int(ln[1]), int(ln[2])
+    alts = [ln for ln in lines if ln[0] == "alt"]
+    bounds = [int(ln[2]) for ln in alts]
+    assert bounds and bounds[-1] >= most and bounds == sorted(bounds)
+    for ln in alts:
+        rows = min(int(ln[2]), most)
+        grids = [-(-rows // int(ln[3])) * int(ln[4])]
+        grids += [n + -(-rows // b) * c for n, b, c in pre[int(ln[7]):][:1]] if "pre" in ln else []
+        assert max(grids) < 1 << 24, (ln, grids)
+
+
+def test_a_static_batch_of_many_slots():
+    """A row count past the decoding kernels' grid is a prompt's."""
+    size = dict(heads=32, kv_heads=32, dim=32, slots=1 << 20, room=64, blocks=64, block=16)
+    for rows, kind in ((1 << 18, "units"), (1 << 21, "prompt")):
+        variant = next(ln for ln in manifest(g.paged_attention(rows, **size), "") if ln.startswith("variant "))
+        assert variant.split()[1].rstrip(",") == kind, (rows, variant)
