@@ -3662,7 +3662,8 @@ static KernelPlan lowerPagedAttention(Analysis &A, const std::string &kname, con
   if (out->type.shape != q->type.shape || out->type.elem != q->type.elem) unsupported(op, "result " + out->type.str() + " beside " + q->type.str());
   float scale = 0;
   try { scale = std::stof(op->attr("scale", "")); } catch (const std::exception &) { unsupported(op, "a missing scale"); }
-  if (!std::isfinite(scale)) unsupported(op, "a scale that is no number");
+  const float scale2 = (float)(scale * 1.4426950408889634); // of the exponents of 2
+  if (!std::isfinite(scale2)) unsupported(op, "a scale that is no number (times log2 e)");
   int64_t window = 0;
   try { window = std::stoll(op->attr("window", "0")); } catch (const std::exception &) { unsupported(op, "window"); }
   if (window < 0 || window > (int64_t(1) << 30)) unsupported(op, "a negative window, or one of more than 2^30 positions");
@@ -3680,7 +3681,7 @@ static KernelPlan lowerPagedAttention(Analysis &A, const std::string &kname, con
       << "  const hf::PagedArgs a{(const uint16_t *)" << in(0);
   for (size_t i = 1; i < 5; ++i) pre << ", (const uint8_t *)" << in(i);
   for (size_t i = 5; i < 8; ++i) pre << ", (const int *)" << in(i);
-  pre << ", (uint16_t *)" << outPtr[0] << ", " << floatLit((float)(scale * 1.4426950408889634)) << "};\n";
+  pre << ", (uint16_t *)" << outPtr[0] << ", " << floatLit(scale2) << "};\n";
   auto kernel = [&](const std::string &name, const std::string &params, const std::string &bounds, const std::string &call) {
     k << "extern \"C\" __global__ __launch_bounds__(" << bounds << ") void " << name << "(" << params << ") {\n" << pre.str() << "  " << call << ";\n}\n";
   };

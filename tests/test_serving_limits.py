@@ -39,3 +39,10 @@ def test_a_static_batch_of_many_slots():
     for rows, kind in ((1 << 18, "units"), (1 << 21, "prompt")):
         variant = next(ln for ln in manifest(g.paged_attention(rows, **size), "") if ln.startswith("variant "))
         assert variant.split()[1].rstrip(",") == kind, (rows, variant)
+
+
+@pytest.mark.parametrize("scale", [2.4e38, -3.4e38, float("inf"), float("nan")])
+def test_refused_scales(scale):
+    """A scale that is no f32 number any more as one of exponents of 2."""
+    with pytest.raises(hf.CompileError, match="a scale that is no number"):
+        hf.compile(g.paged_attention(8, heads=4, kv_heads=2, dim=32, slots=2, room=64, blocks=8, block=16, scale=scale), cache=False)
