@@ -153,21 +153,23 @@ __device__ __forceinline__ void rms_rows(const void *x, const void *residual, co
     uint32_t top = 0;
 #pragma unroll
     for (int j = 0; j < NCH; ++j) {
+      const int n = ln_count<D, V, FULL>(col(j), row < R);
+      // (behind the row's end y is zero, but NaN where r is infinite; a block of
+      // 32 columns that has an infinity has the byte 255 either way)
+      const bool all = OUT >= 0 || (int64_t)(j + 1) * T * V <= D;
       uint32_t most = 0;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float n = pack_get<EL>(s[j], i) * r;
-        y[j][i] = n * gm[j].get(i);
-        most = max_u32(most, f2u(y[j][i]) & 0x7FFFFFFFu);
+        const float u = pack_get<EL>(s[j], i) * r;
+        y[j][i] = u * gm[j].get(i);
+        most = max_u32(most, all || i < n ? f2u(y[j][i]) & 0x7FFFFFFFu : 0u);
       }
-      const int n = ln_count<D, V, FULL>(col(j), row < R);
       if constexpr (RES) {
         char *dst = (char *)sum + (row * D + col(j)) * el_bytes<EL>;
         if (n == V) pack_store<EL>(dst, s[j]);
         else if (!FULL) pack_store_part<EL>(dst, s[j], n);
       }
       if constexpr (OUT < 0) {
-        // (behind the row's end y is zero, or NaN where the whole row is)
         top = max_u32(top, most);
       } else {
         const uint32_t byte = mx_scale_byte<(OUT < 0 ? 0 : OUT)>(block_max<EL>(most));

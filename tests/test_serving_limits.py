@@ -1,8 +1,13 @@
-"""What the serving ops refuse or launch at the ends of their ranges (no GPU)."""
+"""What the serving ops refuse or launch at the ends of their ranges, and what
+they answer there."""
+import numpy as np
 import pytest
 
 import hfusion_mi355x as hf
+from helpers import run_gpu
 from hfusion_mi355x import groups as g
+from test_norm_mx import note, stored
+from test_serving import check_codes
 
 
 def manifest(ir, options="dyn=runtime"):
@@ -46,3 +51,21 @@ def test_refused_scales(scale):
     """A scale that is no f32 number any more as one of exponents of 2."""
     with pytest.raises(hf.CompileError, match="a scale that is no number"):
         hf.compile(g.paged_attention(8, heads=4, kv_heads=2, dim=32, slots=2, room=64, blocks=8, block=16, scale=scale), cache=False)
+
+
+@pytest.mark.gpu
+def test_norm_whose_reciprocal_overflows(gpu):
+    """Rows so small that 1 / sqrt(mean) is infinite in f32 (eps 0): infinite
+    scales, NaN only where a row has a zero."""
+    note("norm of the smallest rows")
+    c = (6, 100, "bf16", "bf16", "i8", True)
+    x = np.full((6, 100), 1e-40)
+    x[1] *= np.where(np.arange(100) % 3, 1, -1)
+    x[2, 50] = 0
+    x[3] = 1.0
+    xs, xv = stored(x, "bf16")
+    gs, gm = stored(np.ones(100), "bf16")
+    zero = np.zeros_like(xs)
+    got = run_gpu("rmsnorm_eps0", [xs, zero, gs, zero, np.zeros((6, 100), np.int8), np.zeros(6, np.float32)], gpu)
+    check_codes(c, got, xv.astype(np.float32), np.zeros((6, 100), np.float32), gm, 0.0)
+    assert np.isinf(got[-1][[0, 1, 4, 5]]).all() and np.isnan(got[-1][2]) and np.isfinite(got[-1][3])
