@@ -206,14 +206,10 @@ constexpr uint32_t kTopScale = 143;
 // Elsewhere, behind the last row's position and before the first one's window,
 // the cache may hold anything, NaN and any scale.
 template <typename S> __device__ __forceinline__ bool some_seen(int at, int lo, int hi) { return at <= hi && (S::WINDOW == 0 || at + 15 > lo - S::WINDOW); }
-// the codes in word w of the sixteen that they see
-template <typename S> __device__ __forceinline__ uint32_t kept_codes(int w, int at, int lo, int hi) {
-  const int n = hi + 1 - at - 4 * w; // those up to the last row's
-  uint32_t keep = n >= 4 ? 0xFFFFFFFFu : n <= 0 ? 0u : 0xFFFFFFFFu >> (8 * (4 - n));
-  if constexpr (S::WINDOW != 0) {
-    const int gone = lo - S::WINDOW + 1 - at - 4 * w; // those before the window
-    keep &= gone <= 0 ? 0xFFFFFFFFu : gone >= 4 ? 0u : 0xFFFFFFFFu << (8 * gone);
-  }
+// the codes in word w of sixteen that are among the first n, less the first `gone`
+template <typename S> __device__ __forceinline__ uint32_t kept_codes(int w, int n, int gone) {
+  uint32_t keep = n >= 4 * w + 4 ? 0xFFFFFFFFu : n <= 4 * w ? 0u : 0xFFFFFFFFu >> (8 * (4 * w + 4 - n));
+  if constexpr (S::WINDOW != 0) keep &= gone <= 4 * w ? 0xFFFFFFFFu : gone >= 4 * w + 4 ? 0u : 0xFFFFFFFFu << (8 * (gone - 4 * w));
   return keep;
 }
 
@@ -248,9 +244,10 @@ template <typename S> __device__ __forceinline__ void paged_step(PagedState<S> &
     for (int u = 0; u < 4; ++u)
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[u][i] = sees(4 * u + i) ? s[u][i] : -__builtin_inff();
+    const int n = t.there ? hi + 1 - at : 0, gone = lo - S::WINDOW + 1 - at;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const uint32_t keep = t.there ? kept_codes<S>(w, at, lo, hi) : 0u;
+      const uint32_t keep = kept_codes<S>(w, n, gone);
 #pragma unroll
       for (int dt = 0; dt < S::DT; ++dt) t.v[dt][w] &= keep;
     }
@@ -720,11 +717,13 @@ template <typename S> struct PagedPrompt {
     }
   }
   __device__ __forceinline__ Mode mode(const Groups &gr, int tile, const Mode &was) const {
+    // (the tile's largest; of blocks of 64 tokens and more it has one)
     auto quad = [](uint32_t v) {
+      if constexpr (S::BLOCK >= 64) return (uint32_t)__builtin_amdgcn_readfirstlane((int)v);
       v = max_u32(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true));
       return (uint32_t)__builtin_amdgcn_readfirstlane((int)max_u32(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true)));
     };
-    const bool read = gr.block >= 0 && gr.vs != 255 && some_seen<S>(64 * tile + 16 * (int)(threadIdx.x % 4), lo, hi);
+    const bool read = gr.block >= 0 && gr.vs != 255 && (S::BLOCK >= 64 || some_seen<S>(64 * tile + 16 * (int)(threadIdx.x % 4), lo, hi));
     const uint32_t big = quad(read ? gr.vs : 0), peak = max_u32(was.peak, big);
     uint32_t now = big > was.ref || (big && big + 4 < was.ref) ? big : was.ref; // (a little lower is near enough)
     now = now + 60 < peak ? peak - 60 : now;
@@ -743,10 +742,10 @@ template <typename S> struct PagedPrompt {
       bool used = true;
       if (!whole) {
         // (what no row sees, and where there is no block, zeros)
-        const int at = 64 * tile + 16 * g;
-        used = __shfl(gr.block, g) >= 0 && some_seen<S>(at, lo, hi);
+        const int at = 64 * tile + 16 * g, n = __shfl(gr.block, g) >= 0 ? hi + 1 - at : 0, gone = lo - S::WINDOW + 1 - at;
+        used = n > 0 && (S::WINDOW == 0 || gone < 16);
 #pragma unroll
-        for (int w = 0; w < 4; ++w) vx[e][w] &= used ? kept_codes<S>(w, at, lo, hi) : 0u;
+        for (int w = 0; w < 4; ++w) vx[e][w] &= kept_codes<S>(w, n, gone);
       }
       const uint32_t down = mo.ref - vs < DOWN ? mo.ref - vs : DOWN;
       const float by = !used || vs == 255 ? 1.0f : u2f((127 - down) << 23);
