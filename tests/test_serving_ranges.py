@@ -176,3 +176,23 @@ def test_rows_before_far_larger_values(gpu, name):
             case = case_of(rng, c, parts, lambda k: big if k * block >= edge else low)
             far = run(grp, c, gpu, *case)
             assert not far[case[1] < edge].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["group3", "alone", "far_f16", "group4", "group20", "far_alone"])
+def test_smallest_codes_beside_larger_blocks(gpu, name):
+    """Values that are the format's smallest numbers, as far below the tile's
+    largest block as one product takes them, and one further: as exact as others."""
+    c = sc.ATTEND[name]
+    block, el, fmt = c[3], c[7], c[8]
+    grp = load(f"pagedattn_{name}_rt")
+    for down in (7, 8, 9) if el == "f16" else (98, 99, 100, 101):
+        for parts in ([(0, 0, 140)], [(0, block - 3, 6)]):
+            note(f"{name} down {down} {parts}")
+            rng = np.random.default_rng(down)
+            big = 141 if el == "f16" else 136
+            seq, pos, table, cache, qs, qv = case_of(rng, c, parts, lambda k: big if k else big - down)
+            v = cache[2][table[0, 0]]
+            v[:] = rng.integers(1, 4, v.shape) | (rng.integers(0, 2, v.shape) << 7)
+            far = run(grp, c, gpu, seq, pos, table, cache, qs, qv)
+            assert not far[pos < block].any()
