@@ -675,11 +675,12 @@ template <typename S> struct PagedPrompt {
   // about the largest block of the tile, but no less than 2^-60 of the largest
   // so far (`peak`; o would pass f32's range).  bf16 has the range for codes
   // 2^100 below it, f16 for 2^8 (DOWN).  Blocks further apart cannot share a
-  // product, and one above kTopScale not the sums (`apart`), since a row may see the
-  // small ones alone: rows that meet such a tile go by paged_part.
+  // product, and one above kTopScale not the sums (`apart`, a peak past all bytes),
+  // since a row may see the small ones alone: what rows that have met such a tile
+  // come to is dropped, and they go by paged_part.
   struct Mode {
     uint32_t ref, peak;
-    bool apart;
+    __device__ __forceinline__ bool apart() const { return peak > 255; }
   };
   static constexpr uint32_t DOWN = S::EL == EL_BF16 ? 100 : 8;
 
@@ -717,17 +718,21 @@ template <typename S> struct PagedPrompt {
     }
   }
   __device__ __forceinline__ Mode mode(const Groups &gr, int tile, const Mode &was) const {
-    // (the tile's largest; of blocks of 64 tokens and more it has one)
-    auto quad = [](uint32_t v) {
-      if constexpr (S::BLOCK >= 64) return (uint32_t)__builtin_amdgcn_readfirstlane((int)v);
-      v = max_u32(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true));
-      return (uint32_t)__builtin_amdgcn_readfirstlane((int)max_u32(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true)));
-    };
+    // the tile's largest scale byte, and 255 less the smallest (a tile has one of
+    // blocks of 64 tokens and more)
+    typedef uint16_t u2 __attribute__((ext_vector_type(2)));
     const bool read = gr.block >= 0 && gr.vs != 255 && (S::BLOCK >= 64 || some_seen<S>(64 * tile + 16 * (int)(threadIdx.x % 4), lo, hi));
-    const uint32_t big = quad(read ? gr.vs : 0), peak = max_u32(was.peak, big);
+    uint32_t both = read ? gr.vs << 16 | (255 - gr.vs) : 0u;
+    if constexpr (S::BLOCK < 64) {
+      auto most = [](uint32_t a, uint32_t b) { return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u2, a), __builtin_bit_cast(u2, b))); };
+      both = most(both, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)both, 0xB1, 0xF, 0xF, true));
+      both = most(both, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)both, 0x4E, 0xF, 0xF, true));
+    }
+    both = (uint32_t)__builtin_amdgcn_readfirstlane((int)both);
+    const uint32_t big = both >> 16, up = both & 0xFFFF, peak = max_u32(was.peak, big);
     uint32_t now = big > was.ref || (big && big + 4 < was.ref) ? big : was.ref; // (a little lower is near enough)
     now = now + 60 < peak ? peak - 60 : now;
-    return Mode{now, peak, now > kTopScale || quad(read ? now - gr.vs : 0) > DOWN};
+    return Mode{now, now > kTopScale || now + up > 255 + DOWN ? 512u : peak};
   }
   __device__ __forceinline__ void stage(const Groups &gr, const Mode &mo, int tile, int buf) {
     const bool whole = 64 * tile + 63 <= hi && (S::WINDOW == 0 || 64 * tile > lo - S::WINDOW) && __all(gr.block >= 0);
@@ -768,10 +773,9 @@ template <typename S> struct PagedPrompt {
     const int lane = threadIdx.x % 64, r = lane % 32, half = lane / 32, key = (r & 0x13) | (r & 4) << 1 | (r & 8) >> 1;
     if (mo.ref != ref) {
       const int by = (int)ref - (int)mo.ref; // -143 .. 60
-#pragma unroll
-      for (int i = 0; i < OT; ++i)
-#pragma unroll
-        for (int k = 0; k < 16; ++k) o[i][k] = __builtin_amdgcn_ldexpf(o[i][k], by);
+      // (a power of two that far below 1 is none of f32)
+      if (by < -120) times(0x1p-40f);
+      times(u2f((uint32_t)(127 + (by < -120 ? by + 40 : by)) << 23));
       ref = mo.ref;
     }
     constexpr int GS = S::BLOCK >= 64 ? 1 : 4; // groups of tokens whose blocks may differ
@@ -929,11 +933,11 @@ template <typename S> struct PagedPrompt {
     m = -__builtin_inff(), sum = 0, ref = 0;
     Groups gr = groups(block(begin));
     load(gr, begin);
-    Mode mo = mode(gr, begin, Mode{0, 0, false});
+    Mode mo = mode(gr, begin, Mode{0, 0});
     int next = block(begin + 1);
-    if (!mo.apart) stage(gr, mo, begin, begin & 1);
+    stage(gr, mo, begin, begin & 1);
     __syncthreads();
-    for (int i = begin; i < end && !mo.apart; ++i) {
+    for (int i = begin; i < end; ++i) {
       Groups gn = gr;
       if (i + 1 < end) {
         gn = groups(next);
@@ -944,12 +948,12 @@ template <typename S> struct PagedPrompt {
       if (64 * i <= seen && (S::WINDOW == 0 || 64 * i + 63 > first - S::WINDOW)) step(gr, mo, i, i & 1, pos, first, last);
       if (i + 1 < end) {
         mo = mode(gn, i + 1, mo);
-        if (!mo.apart) stage(gn, mo, i + 1, (i + 1) & 1);
+        stage(gn, mo, i + 1, (i + 1) & 1);
         gr = gn;
       }
       __syncthreads();
     }
-    if (mo.apart) return false;
+    if (mo.apart()) return false;
     times(mx_scale(ref));
     sum = with_lane<32>(sum, [](float x, float y) { return x + y; });
     if (!ok) return true;
@@ -1021,7 +1025,9 @@ template <typename S> struct PagedPrompt {
     const int64_t t0 = (tiles(T) - 1 - (blockIdx.x - piece * units) / HEADS) * TOKENS;
     const int hh = (int)(blockIdx.x - piece * units) % HEADS, h = hh / S::GTILES, gt = hh % S::GTILES, lane = threadIdx.x % 64;
     const int tokens = (int)(T - t0 < TOKENS ? T - t0 : TOKENS);
-    float *const part = PARTS ? part_of(ws, blockIdx.x) : nullptr, *const stats = PARTS ? stats_of(ws, blockIdx.x) : nullptr;
+    auto uniform = [](uint64_t v) {
+      return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v);
+    };
     // a row and those that follow it
     auto follow = [&](int at, int s, int p) {
       const int64_t t = t0 + at;
@@ -1034,8 +1040,13 @@ template <typename S> struct PagedPrompt {
       }
       return n;
     };
+    auto part = [&]() -> float * { return PARTS ? part_of(ws, blockIdx.x) : nullptr; };
+    auto stats = [&]() -> float * { return PARTS ? stats_of(ws, blockIdx.x) : nullptr; };
     int few = 0;
-    uint64_t apart[2] = {0, 0}; // rows that run() has left
+    // rows that run() has left, done behind all others: beside its loop they would
+    // take registers (f16 heads of 256 channels 12 % slower)
+    __shared__ uint64_t apart[2];
+    if (threadIdx.x < 2) apart[threadIdx.x] = 0;
     for (int at = 0; at < tokens;) {
       const int64_t t = t0 + at;
       const int s = a.seq[t], p = a.pos[t];
@@ -1046,21 +1057,25 @@ template <typename S> struct PagedPrompt {
       const int n = follow(at, s, p);
       if (n <= S::FEW && S::few(a.seq, a.pos, t, T, s, p)) { // PagedFew's
         if (PARTS && piece == 0)
-          for (int i = threadIdx.x; i < n * S::GT; i += 256) stats[2 * (at * S::GT + i) + 1] = DONE;
+          for (int i = threadIdx.x; i < n * S::GT; i += 256) stats()[2 * (at * S::GT + i) + 1] = DONE;
         at += n, few = 1;
         continue;
       }
-      if (!PagedPrompt{a, lds, s, h, p, p + n - 1}.template run<PARTS>(t0, t, n, gt, piece, cuts, part, stats)) (at < 64 ? apart[0] : apart[1]) |= 1ull << at % 64;
+      const bool done = PagedPrompt{a, lds, s, h, p, p + n - 1}.template run<PARTS>(t0, t, n, gt, piece, cuts, part(), stats());
+      if (!done && (int)threadIdx.x == at / 64) apart[at / 64] |= 1ull << at % 64;
       at += n;
     }
-    // (behind the others: what this computes ahead would take their registers)
-#pragma unroll
+    auto end = [&] {
+      if (piece == 0 && hh == 0 && threadIdx.x == 0 && t0 / TOKENS < PagedFew<S>::TILES) reinterpret_cast<int *>(ws)[t0 / TOKENS] = few;
+    };
+    __syncthreads();
+    if (__builtin_expect(uniform(apart[0] | apart[1]) == 0, 1)) return end();
     for (int w = 0; w < 2; ++w)
-      for (uint64_t left = apart[w]; left; left &= left - 1) {
+      for (uint64_t left = uniform(apart[w]); left; left &= left - 1) {
         const int at = 64 * w + __builtin_ctzll(left), s = a.seq[t0 + at], p = a.pos[t0 + at], n = follow(at, s, p);
-        PagedPrompt{a, lds, s, h, p, p + n - 1}.template split<PARTS>(t0, t0 + at, n, gt, piece, cuts, part, stats);
+        PagedPrompt{a, lds, s, h, p, p + n - 1}.template split<PARTS>(t0, t0 + at, n, gt, piece, cuts, part(), stats());
       }
-    if (piece == 0 && hh == 0 && threadIdx.x == 0 && t0 / TOKENS < PagedFew<S>::TILES) reinterpret_cast<int *>(ws)[t0 / TOKENS] = few;
+    end();
   }
 
   // The second launch: PagedFew's workgroups, and PARTS behind them PIECES / 2 *
