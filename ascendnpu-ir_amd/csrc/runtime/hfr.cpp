@@ -63,14 +63,20 @@ struct RowAlt {
 // what its kernels left there from launch to launch and stays the only one.
 struct OwnWorkspace {
   // allocated and zeroed when the handle is loaded, or, where the row count
-  // decides whether a launch uses one, at the first launch that does (a weight
-  // product that only ever has a few rows holds no bf16 copy of its weight)
+  // decides whether a launch uses one or how much of it, at the first launch that
+  // does (a weight product that only ever has a few rows holds no bf16 copy of its
+  // weight, attention of single tokens not what prompts need)
   void *first = nullptr;
+  uint64_t bytes = 0; // of the first
   int device = -1;
   std::mutex mu;
   bool taken = false;
   void *firstStream = nullptr;
-  std::vector<std::pair<void *, void *>> more; // stream, workspace
+  struct More {
+    void *stream, *ws;
+    uint64_t bytes;
+  };
+  std::vector<More> more; // (a stream whose launches need different sizes may have several)
 };
 
 struct hfr_group : GroupArgs {
@@ -293,6 +299,7 @@ int launchRaw(hipFunction_t fn, const hfr_launch_cfg &cfg, const uint64_t *args,
 hipError_t ownWorkspaceInit(OwnWorkspace &o, uint64_t bytes) {
   (void)hipGetDevice(&o.device);
   hipError_t e = hipMalloc(&o.first, bytes);
+  o.bytes = bytes;
   if (e != hipSuccess) o.first = nullptr;
   else if ((e = hipMemset(o.first, 0, bytes)) != hipSuccess) {
     (void)hipFree(o.first);
@@ -307,7 +314,7 @@ hipError_t ownWorkspaceFree(OwnWorkspace &o) {
   (void)hipSetDevice(o.device);
   hipError_t e = hipFree(o.first);
   for (auto &m : o.more) {
-    const hipError_t e2 = hipFree(m.second);
+    const hipError_t e2 = hipFree(m.ws);
     if (e == hipSuccess) e = e2;
   }
   o.first = nullptr;
@@ -316,7 +323,8 @@ hipError_t ownWorkspaceFree(OwnWorkspace &o) {
   return e;
 }
 // The workspace of a launch on `stream`, allocated at the stream's first one
-// that uses it.  The caller holds o.mu until it has enqueued what uses it: a
+// that uses as much of it; a smaller one that the stream has stays, for launches
+// under way and for later ones that need no more.  The caller holds o.mu until it has enqueued what uses it: a
 // launch of another thread on the same stream comes behind, not between a pre
 // kernel and the kernel that reads what it left.
 int ownWorkspaceOf(OwnWorkspace &o, uint64_t bytes, bool zeroed, void *stream, const char *what, void **ws) {
@@ -328,10 +336,10 @@ int ownWorkspaceOf(OwnWorkspace &o, uint64_t bytes, bool zeroed, void *stream, c
     o.firstStream = stream;
   }
   *ws = o.first;
-  if (o.first && (zeroed || stream == o.firstStream)) return HFR_OK;
+  if (o.first && (zeroed || stream == o.firstStream) && bytes <= o.bytes) return HFR_OK;
   for (auto &m : o.more)
-    if (m.first == stream) {
-      *ws = m.second;
+    if (m.stream == stream && bytes <= m.bytes) {
+      *ws = m.ws;
       return HFR_OK;
     }
   // (a stream under capture somewhere does not mind an allocation of this kind)
@@ -341,9 +349,10 @@ int ownWorkspaceOf(OwnWorkspace &o, uint64_t bytes, bool zeroed, void *stream, c
   const hipError_t e = hipMalloc(&p, bytes);
   (void)hipThreadExchangeStreamCaptureMode(&mode);
   if (e != hipSuccess) return hipFail(e, "workspace allocation");
-  if (o.first) o.more.push_back({stream, p});
+  if (o.first) o.more.push_back({stream, p, bytes});
   else {
     o.first = p;
+    o.bytes = bytes;
     o.taken = true;
     o.firstStream = stream;
   }
@@ -438,9 +447,9 @@ int runChecked(hfr_group *g, const uint64_t *params, void *const *results, int64
   if (g->rowsDyn && rows == 0 && !g->rowsZero) return HFR_OK; // nothing to do
   void *ws = workspace;
   std::unique_lock<std::mutex> lock(g->own->mu, std::defer_lock);
-  if (!ws && workspaceOf(g, rows)) {
+  if (const uint64_t bytes = ws ? 0 : workspaceOf(g, rows)) {
     lock.lock();
-    if (const int rc = ownWorkspaceOf(*g->own, g->wsBytes, g->wsZero, stream, "group", &ws)) return rc;
+    if (const int rc = ownWorkspaceOf(*g->own, bytes, g->wsZero, stream, "group", &ws)) return rc;
   }
   return launchGroup(g, params, results, ws, stream, rows);
 }
@@ -528,8 +537,8 @@ int hfr_group_load(const char *manifest_path, const char *func, hfr_group_t *out
   }
   // the group's own workspace lives on the device current at load time, so
   // that launches stay asynchronous
-  bool always = true; // every launch uses the workspace
-  for (const RowAlt &alt : g->alts) always = always && alt.pre;
+  bool always = true; // every launch uses the workspace, and all of it
+  for (const RowAlt &alt : g->alts) always = always && workspaceOf(g.get(), alt.maxRows) == g->wsBytes;
   if (g->wsBytes && !always && !g->wsZero) {
     (void)hipGetDevice(&g->own->device);
   } else if (g->wsBytes) {

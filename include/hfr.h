@@ -16,9 +16,10 @@
  * stream that the handle is launched on has it; every other stream gets one of
  * its own at its first launch of the handle, except where launches rely on what
  * earlier ones left in a zeroed workspace: that one stays the handle's only
- * one.  Where the launch's row count decides whether it uses a workspace
- * (hfr_group_workspace_rows), the first one is allocated at the first launch
- * that does too.  No other launch allocates.  All of them are freed with the
+ * one.  Where the launch's row count decides whether it uses a workspace, or how
+ * much of it (hfr_group_workspace_rows), the first one is allocated at the first
+ * launch that does too, of that size, and a further one where a stream's later
+ * launch needs more.  No other launch allocates.  All of them are freed with the
  * handle, not with their streams.
  * Threading: launches are asynchronous on the given stream; the caller
  * synchronises.  Two in-flight launches that use one workspace must be on the

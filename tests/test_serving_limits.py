@@ -69,3 +69,53 @@ def test_norm_whose_reciprocal_overflows(gpu):
     got = run_gpu("rmsnorm_eps0", [xs, zero, gs, zero, np.zeros((6, 100), np.int8), np.zeros(6, np.float32)], gpu)
     check_codes(c, got, xv.astype(np.float32), np.zeros((6, 100), np.float32), gm, 0.0)
     assert np.isinf(got[-1][[0, 1, 4, 5]]).all() and np.isnan(got[-1][2]) and np.isfinite(got[-1][3])
+
+
+@pytest.mark.gpu
+def test_streams_hold_what_their_launches_need(gpu):
+    """A handle's workspaces by what each stream's launches use: single tokens
+    less than prompts, whose own comes with the first of them; the answers are
+    those of a launch with a caller's workspace of full size."""
+    import torch
+    import serving_catalog as sc
+    from test_serving import attend_case, load
+    from test_serving_calls import attend_args, same
+    note("workspaces by launch")
+    c = sc.ATTEND["usual"]
+    rng = np.random.default_rng(3)
+    few, prompt = (attend_args(c, attend_case(rng, c, parts, 0), gpu) for parts in ([(0, 3000, 1), (1, 900, 2)], [(2, 1500, 150)]))
+    grp = load("pagedattn_usual_rt")
+    full = grp.info.workspace_bytes
+    lib = hf.native.hfr()
+    need = lib.hfr_group_workspace_rows(grp._h, 3)
+    assert need < full // 4 and lib.hfr_group_workspace_rows(grp._h, 150) == full
+    want = []
+    space = torch.zeros(full, dtype=torch.uint8, device=gpu)
+    for a in (few, prompt):
+        grp(*a, workspace=space)
+        torch.cuda.synchronize()
+        want.append(a[-1].clone())
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    for s in streams:  # (what a stream itself holds is there before)
+        with torch.cuda.stream(s):
+            grp(*few, workspace=space)
+        torch.cuda.synchronize()
+    before = torch.cuda.mem_get_info()[0]
+    for s in streams:
+        few[-1].zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            grp(*few)
+        torch.cuda.synchronize()
+        assert same(few[-1], want[0])
+    # (allocations are in whole pages of 2 MiB)
+    assert before - torch.cuda.mem_get_info()[0] <= len(streams) * (need + (4 << 20)) < len(streams) * full // 2
+    for _ in range(2):
+        for s in streams[:2]:
+            for a, w in ((prompt, want[1]), (few, want[0])):
+                a[-1].zero_()
+                torch.cuda.synchronize()
+                with torch.cuda.stream(s):
+                    grp(*a)
+                torch.cuda.synchronize()
+                assert same(a[-1], w)
