@@ -3578,7 +3578,7 @@ void tileGrid(const Analysis &A, const Op *op, KernelPlan &p, int64_t T, int64_t
 // Rows whose blocks a workgroup of append_kv owns: a decoding step's rows are
 // all in blocks of their own, which one workgroup takes one after another; a
 // prompt's rows share theirs, and workgroups that own none are for nothing.  us
-// of a call, tiles of 1, 4, 16 and 64 rows (32 heads over 8, 128 channels, blocks
+// of the kernel (a call of few rows takes some 1.5 more), tiles of 1, 4, 16 and 64 rows (32 heads over 8, 128 channels, blocks
 // of 64): 64 sequences of one token 5.5, 10.3, 32.0, 121; 256 of them 12.4, 14.2,
 // 35.5, 119; 1024 39.5, 36.6, 46.0, 141; 4000 183, 155, 161, 330; a prompt of 256
 // tokens 6.1, 5.4, 5.5, 5.3; 1024 11.9, 7.3, 5.6, 5.7; 8192 87, 37, 34, 34 (5.4 TB/s).
@@ -3688,14 +3688,19 @@ static KernelPlan lowerPagedAttention(Analysis &A, const std::string &kname, con
   // The kernels, by the row count.  More rows than the sequences' groups of N
   // tokens are a prompt's, unless they are few: 64 rows behind 8000 positions 44
   // us as groups of tokens, 52 as a prompt's rows, 256 behind 30000 364 and 178.
+  // (So a prompt's rows are taken for groups of tokens where the table has many
+  // sequences: of 256 sequences instead of 4, 512 rows behind 7000 175 and 99,
+  // 1000 rows 82 and 41, 1000 behind 3000 of 32 heads over 32 531 and 113.)
   // (no more than a launch has workgroups for, a row and head each)
   const int64_t tile = 128 / GT, far = z.per * z.block;
   const int64_t tokens = std::max<int64_t>(kPagedFew, std::min<int64_t>(((int64_t(1) << 24) - 1) / heads, N * z.slots));
   // Groups of tokens in pieces where some may be long: the second launch and the
   // sums before the first cost some 4 us (18 rows over up to 500 positions 11.6 and
-  // 7.6 us, 64 over up to 2000 38.7 and 34.5; 48 over up to 8100 80 and 114, 4 over up to
-  // 4000 14.1 and 30).  Heads of 256 channels, 8 rows over up to 1200: 13.4 and
-  // 19.2, 64 of them 26.7 and 25.1, 5 over up to 867 12.3 and 17.2; one row over a window of 358: 13.2 and 10.0.
+  // 7.4 us; 48 over up to 8100 85 and 114, 4 over up to 4000 14.7 and 30.7).  8 rows over up to
+  // 900, 1800 and 3600 positions, and 48 over up to 1800, in pieces and whole: 64
+  // channels 11.7, 8.0; 12.9, 12.4; 15.9, 20.2; 22.8, 19.1; 128 channels 11.0, 10.7;
+  // 13.9, 17.5; 16.8, 29.5; 28.6, 28.9; 192 channels 11.8, 13.1; 12.7, 25.3; 16.8, 46.0;
+  // 26.6, 27.7; 256 channels 13.3, 18.9; 14.3, 34.8; 19.4, 63.9; 31.6, 37.1.
   auto seen = [&](int64_t n) { return window ? std::min(far, window + n) : far; }; // (n tokens')
   const int64_t wide = std::max<int64_t>(z.D, 128), split = seen(N) * wide * wide > kWholeFar * 128 * 128 ? std::min(tokens, kSplitRows) : 0;
   // Prompt's rows in pieces while they do not fill the chip (PagedPrompt), of

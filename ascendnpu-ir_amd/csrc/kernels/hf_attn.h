@@ -465,9 +465,10 @@ template <typename S> struct PagedFew {
 // workgroup a piece, the longest first; units of several pieces leave parts,
 // which join() adds in order.  run makes as many pieces as fill the chip with
 // the units that stay whole: PIECES less the units, LEAST to SHARED of them.  us of
-// a call, with 512, 768 (taken), 1536 at most: one row over 32768 positions 19.5,
-// 19.6, 23; over 131072 49, 53, 58; 48 rows over up to 8100 90, 80, 87 (5.1 TB/s;
-// a workgroup a unit 114, as long as the longest takes).
+// a call, with 512, 768 (taken), 1536 (of 2048 in all) at most: one row over 32768
+// positions 19.8, 19.8, 24.1; over 131072 49, 53, 57; 48 rows over up to 8100 90, 85,
+// 79 (a workgroup a unit 114, as long as the longest takes); 4 over up to 4000 14.7,
+// 14.8, 14.9 (30.7).
 // Up to MOST rows: every workgroup adds up the units' tiles itself, which takes
 // it some 2 us.
 // ws: the number of records, one a token of a unit in parts; then for each part
@@ -646,8 +647,8 @@ template <typename S, int WV> struct PagedSplit {
 // operand is read one stage ahead: scores of the first half; those of the
 // second beside the first's exponentials; the first's values beside the
 // second's exponentials; the second's values.  10495 rows of four prompts (276
-// Gflop) take 342 us, 805 Tflop/s; both halves at once 355, reads ordered by
-// the compiler 412.  A large library product of bf16 reaches 1215 on this card.
+// Gflop) take 345 to 368 us a call by box, 750 to 800 Tflop/s; beside 342 both
+// halves at once took 355, reads ordered by the compiler 412.  A large library product of bf16 reaches 1215 on this card.
 // A SIMD's two waves have some 250 vector instructions for each 32 products,
 // which issue half the time, the matrix core 35 to 40 %; a third of a wave's
 // time goes to waits and barriers.

@@ -120,8 +120,9 @@ template <int FMT> __device__ __forceinline__ u32x2 kv_rescale(u32x2 w, uint32_t
 // (226 MB, of which 32 are rotations that each XCD reads, 5.6 TB/s; with a tile's
 // workgroups on one XCD 45.9); a decoding step of 64 rows takes 5.6 us on the device, the
 // chain of positions, table, scale, rows, and the block rounded again.
-// Two rows of one place, or a sequence in two pieces that share a block, leave
-// one or the other there: nothing else is touched, but which is not defined.
+// Two rows of one place, or a sequence in two pieces that share a block, write
+// it at once: codes and scale of its tokens, earlier ones too, need not belong
+// together then.  Other blocks are not touched.
 template <int EL, int FMT, int HQ, int HK, int D, int ROT, bool PAIRS, int BLOCK, int64_t SLOTS, int64_t PER, int64_t FAR, int64_t NBLK, int C, int QB, int HB>
 __device__ __forceinline__ void kv_append(const void *__restrict__ qkv, const float *__restrict__ rot, const int *__restrict__ seq,
                                           const int *__restrict__ pos, const int *__restrict__ table, void *__restrict__ q,

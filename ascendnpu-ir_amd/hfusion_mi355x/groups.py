@@ -781,7 +781,10 @@ def append_kv(rows, heads, kv_heads, dim, slots, room, blocks, block=64, rot=Non
     and codes 0.
 
     A sequence's rows lie together with positions that follow each other, and
-    a block that gets tokens is one sequence's alone.  Rows whose position is
+    a block that gets tokens is one sequence's alone; of rows that break this the
+    blocks that they share are undefined.  What a block holds behind its new
+    tokens counts as gone (a sequence may be cut back and go on).  q is of the
+    rows' type; paged_attention takes bf16 and f16.  Rows whose position is
     negative or past `room`, or whose sequence is not in the table, pad the
     batch: nothing of them is written.  Keys and values whose block is not in
     [0, blocks) are dropped."""
@@ -799,7 +802,11 @@ def paged_attention(rows, heads, kv_heads, dim, slots, room, blocks, block=64, e
     last `window` of them.  out [rows, heads, dim] = softmax(scale q k) v,
     `scale` 1 / sqrt(dim) by default; query head h reads kv head h / (heads /
     kv_heads).  Sums and softmax statistics are f32, a probability is rounded
-    to the queries' type before it multiplies its value.
+    to the queries' type before it multiplies its value (below 2^-14 of f16 it is
+    2^-25 off at most), and what the positions that a row does not see hold changes
+    nothing of it.  `slots` decides which batches count as tokens: up to 16 / (heads /
+    kv_heads) rows a slot, so that prompts are answered sooner by a group for few
+    sequences.
 
     Positions whose block is not in [0, blocks) are not seen, a row that sees
     none is zeros, and rows whose position is negative or past the table, or
