@@ -293,7 +293,8 @@ template <typename S> __device__ __forceinline__ void paged_step(PagedState<S> &
   // of the largest block up to kTopScale (a row may see small ones alone); where
   // a block lies above it, or further below than f16 reaches, p times its scale as
   // the sum of two bf16 numbers
-  const bool read = t.there && some_seen<S>(at, lo, hi);
+  // (a tile of one block is read)
+  const bool read = t.there && (S::BLOCK >= 64 || some_seen<S>(at, lo, hi));
   const bool bad = __any(read && t.vs == 255);
   uint32_t big = read && t.vs != 255 ? t.vs : 0, small = read ? t.vs : 255;
   if constexpr (S::BLOCK < 64) {

@@ -1353,6 +1353,8 @@ def entries():
     e.update(norm_mx_catalog.entries())
     import serving_catalog
     e.update(serving_catalog.entries())
+    import serving_range_catalog
+    e.update(serving_range_catalog.entries())
     return e
 
 
