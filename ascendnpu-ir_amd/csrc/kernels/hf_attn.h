@@ -80,6 +80,9 @@ template <int EL_, int FMT_, int HQ_, int HK_, int D_, int BLOCK_, int64_t SLOTS
   static constexpr int64_t SLOTS = SLOTS_, PER = PER_, NBLK = NBLK_, FAR = PER * BLOCK;
   static constexpr int G = HQ / HK, GT = G < 16 ? G : 16, GTILES = (G + 15) / 16, N = 16 / GT;
   static constexpr int KS = D / 32, DT = D / 16;
+  // Probabilities and their sums are in units of 2^-LIFT: a prompt's are up to 2^6,
+  // and f16, which ends at 2^16, has all bits of a number from 2^-14 on
+  static constexpr float LIFT = EL == EL_F16 ? 9 : 0;
   static_assert(HQ % HK == 0 && D % 32 == 0 && D <= 256 && BLOCK % 16 == 0 && BLOCK <= 128 && (BLOCK & (BLOCK - 1)) == 0);
   __device__ static __forceinline__ bool inside(int s, int p) { return s >= 0 && s < SLOTS && p >= 0 && p < FAR; }
   // whether row t begins a group of tokens, and how many follow it there: rows
@@ -267,7 +270,7 @@ template <typename S> __device__ __forceinline__ void paged_step(PagedState<S> &
   for (int u = 0; u < 4; ++u)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      p[4 * u + i] = __builtin_amdgcn_exp2f(s[u][i] - m);
+      p[4 * u + i] = __builtin_amdgcn_exp2f(s[u][i] - (m - S::LIFT));
       sum += p[4 * u + i];
     }
   st.sum = st.sum * was + sum;
@@ -865,7 +868,7 @@ template <typename S> struct PagedPrompt {
     }
     __builtin_amdgcn_s_setprio(0);
     scored(0);
-    mu = m == -__builtin_inff() ? 0.0f : m; // (a row that has seen nothing)
+    mu = (m == -__builtin_inff() ? 0.0f : m) - S::LIFT; // (a row that has seen nothing)
 #pragma unroll
     for (int c = 0; c < QF; ++c) {
       s[1] = mfma(w[c], q[c], s[1]);
@@ -874,7 +877,7 @@ template <typename S> struct PagedPrompt {
       limit();
     }
     scored(1);
-    mu = m == -__builtin_inff() ? 0.0f : m;
+    mu = (m == -__builtin_inff() ? 0.0f : m) - S::LIFT;
     rounded(0, pf);
 #pragma unroll
     for (int c = 0; c < QF; ++c) {

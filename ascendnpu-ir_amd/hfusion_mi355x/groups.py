@@ -802,8 +802,8 @@ def paged_attention(rows, heads, kv_heads, dim, slots, room, blocks, block=64, e
     last `window` of them.  out [rows, heads, dim] = softmax(scale q k) v,
     `scale` 1 / sqrt(dim) by default; query head h reads kv head h / (heads /
     kv_heads).  Sums and softmax statistics are f32, a probability is rounded
-    to the queries' type before it multiplies its value (below 2^-14 of f16 it is
-    2^-25 off at most), and what the positions that a row does not see hold changes
+    to the queries' type before it multiplies its value (below 2^-23 of f16 it is
+    2^-34 off at most), and what the positions that a row does not see hold changes
     nothing of it.  `slots` decides which batches count as tokens: up to 16 / (heads /
     kv_heads) rows a slot, so that prompts are answered sooner by a group for few
     sequences.
